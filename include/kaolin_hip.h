@@ -33,7 +33,8 @@ typedef enum {
   KL_I8 = 4,
   KL_I16 = 5,
   KL_I32 = 6,
-  KL_I64 = 7
+  KL_I64 = 7,
+  KL_BF16 = 8
 } kl_dtype;
 
 enum {
@@ -526,6 +527,43 @@ int kl_inclusive_sum_i32(int64_t num, const int32_t *info, int32_t *out, void *w
  * unordered atomics).  num_out = inclusive_sum[num_feats - 1] in the reference. */
 int kl_sum_reduce(kl_dtype dtype, int64_t num_feats, int64_t feat_dim, const void *feats,
                   const int32_t *inclusive_sum, int64_t num_out, void *out, kl_stream stream);
+
+/* ------------------------------------------- sequence operators over packs
+ * Learned operators along packs, beside the packed ray ops above; the reference has none of them.
+ * boundaries (num_rows): one byte a row, non-zero at each pack's first row (mark_pack_boundaries);
+ * rows before the first pack belong to none.  Nothing is read back: every call can be captured. */
+
+/* The pack arrays that the calls below take: ids (num_rows) int32, the pack of each row (-1 before the
+ * first), and starts (num_rows + 1) int32, the first row of each pack, num_rows past the last one. */
+size_t kl_pack_layout_workspace_bytes(int64_t num_rows);
+int kl_pack_layout(int64_t num_rows, const uint8_t *boundaries, int32_t *ids, int32_t *starts, void *workspace,
+                   size_t workspace_bytes, kl_stream stream);
+
+/* out[i] = sum_j softmax_j(scale * q[i] . k[j]) v[j] over the keys j of the pack of keys that has the number
+ * of i's pack of queries; causal: the last query of a pack sees all its keys, each one before it one key
+ * fewer.  A row that sees no key is 0.  q (num_q, heads, dim), k and v (num_k, kv_heads, dim), heads a
+ * multiple of kv_heads (query head h reads key head h / (heads / kv_heads)), dim a multiple of 8 up to 128;
+ * f16 / bf16 / f32.  strides_host: the row and head strides of q, k, v in elements (q row, q head, k row, k
+ * head, v row, v head); every row of a head starts at a multiple of 16 bytes.  out (num_q, heads, dim) and
+ * lse (num_q, heads) f32 are contiguous; lse (base-2 logarithm of the softmax's sum, what the backward
+ * takes) may be NULL. */
+size_t kl_pack_attention_workspace_bytes(kl_dtype dtype, int64_t num_q, int64_t num_k, int heads, int kv_heads,
+                                         int dim);
+int kl_pack_attention_forward(kl_dtype dtype, int64_t num_q, int64_t num_k, int heads, int kv_heads, int dim,
+                              const void *q, const void *k, const void *v, const int64_t *strides_host,
+                              const int32_t *q_ids, const int32_t *q_starts, const int32_t *k_ids,
+                              const int32_t *k_starts, float scale, int causal, void *out, float *lse,
+                              void *workspace, size_t workspace_bytes, kl_stream stream);
+/* Its gradients: grad_out, out (num_q, heads, dim) contiguous and 16-byte aligned; grad_q as q and grad_k,
+ * grad_v as k and v, contiguous, fully written (grad_q, or grad_k with grad_v, may be NULL).  Every sum has a
+ * fixed order. */
+size_t kl_pack_attention_bwd_workspace_bytes(int64_t num_q, int heads);
+int kl_pack_attention_backward(kl_dtype dtype, int64_t num_q, int64_t num_k, int heads, int kv_heads, int dim,
+                               const void *grad_out, const void *q, const void *k, const void *v,
+                               const int64_t *strides_host, const int32_t *q_ids, const int32_t *q_starts,
+                               const int32_t *k_ids, const int32_t *k_starts, const void *out, const float *lse,
+                               float scale, int causal, void *grad_q, void *grad_k, void *grad_v, void *workspace,
+                               size_t workspace_bytes, kl_stream stream);
 
 /* ------------------------------------------------------------ check_sign */
 

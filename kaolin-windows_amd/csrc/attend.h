@@ -1,0 +1,181 @@
+// attend.h -- the geometry that the attention kernels over packs share (attend.hip, attendgrad.hip).
+#pragma once
+
+#include "seqcommon.h"
+
+namespace kl {
+
+// One attention call.  The query heads g = 0 .. group - 1 of key head m are its heads m * group + g, and
+// the (row, g) of one key head are numbered as virtual rows row * group + g: they share keys and values,
+// so one tile of virtual rows serves a whole group, and a single query row with its group still fills
+// part of a tile.
+struct Attend {
+  Heads q, k, v;
+  const int32_t *qid, *qstart, *kid, *kstart;
+  int nq, nk;         // rows
+  int kv_heads, group, dim, causal;
+  float scale, c;     // c = scale * log2(e): exponentials are base 2
+};
+
+// The keys [lo, hi) that query row `row` sees: those of its pack; causal: the pack's last query sees all,
+// and each query before it one key fewer.  No key: lo = INT_MAX, hi = INT_MIN.
+struct Range {
+  int lo, hi;
+};
+__device__ __forceinline__ Range no_keys() { return {0x7fffffff, (int)0x80000000}; }
+__device__ __forceinline__ Range key_range(const Attend &a, int row) {
+  const int p = a.qid[row];
+  if (p < 0) return no_keys();
+  const int lo = a.kstart[min(p, a.nk)];
+  int hi = a.kstart[min(p + 1, a.nk)];
+  if (a.causal) hi -= a.qstart[p + 1] - 1 - row;
+  return hi > lo ? Range{lo, hi} : no_keys();
+}
+
+// `a`'s pieces of 16 bytes of rows [row0, row0 + ROWS) of one head, for the 256 threads of a workgroup
+template <typename T, int DP, int ROWS>
+struct Stage {
+  static constexpr int CH = DP * (int)sizeof(T) / 16;  // pieces per row
+  static constexpr int PER = ROWS * CH / 256;
+  static constexpr int E = 16 / (int)sizeof(T);        // elements per piece
+  static constexpr int LD = DP + E;                    // LDS row length: one piece of padding
+  static_assert(ROWS * CH % 256 == 0, "whole pieces per thread");
+  u32x4 w[PER];
+
+  // rows at or past `end` and columns at or past `dim` become zeros
+  __device__ __forceinline__ void load(const T *__restrict__ base, int64_t stride, int row0, int end, int dim) {
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+      const int at = threadIdx.x + 256 * i, row = row0 + at / CH, col = at % CH * E;
+      w[i] = u32x4{0, 0, 0, 0};
+      if (row < end && col < dim) w[i] = *reinterpret_cast<const u32x4 *>(base + row * stride + col);
+    }
+  }
+  __device__ __forceinline__ void store(T *tile) const {
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+      const int at = threadIdx.x + 256 * i;
+      *reinterpret_cast<u32x4 *>(tile + at / CH * LD + at % CH * E) = w[i];
+    }
+  }
+  // bit r of bad[r / 32] for every row r that holds an infinity or a NaN
+  __device__ __forceinline__ void mark_bad(uint32_t *bad) const {
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+      const int r = (threadIdx.x + 256 * i) / CH;
+      if (piece_bad<T>(w[i])) atomicOr(&bad[r / 32], 1u << (r % 32));
+    }
+  }
+  // pieces of bad rows as zeros
+  __device__ __forceinline__ void store_good(T *tile, const uint32_t *bad) const {
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+      const int at = threadIdx.x + 256 * i, r = at / CH;
+      const bool b = bad[r / 32] >> (r % 32) & 1;
+      *reinterpret_cast<u32x4 *>(tile + r * LD + at % CH * E) = b ? u32x4{0, 0, 0, 0} : w[i];
+    }
+  }
+};
+
+// The stationary operand: the 32 columns of a wave are 32 rows of a (rows, dim) matrix; element e of
+// fragment s is row[16 * s + 8 * h + e].
+template <typename T>
+__device__ __forceinline__ V8<T> global_frag(const T *row, bool valid, int col, int dim) {
+  union {
+    u32x4 w[sizeof(T) / 2];
+    V8<T> v;
+  } x;
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; i++)
+    x.w[i] = valid && col < dim ? reinterpret_cast<const u32x4 *>(row + col)[i] : u32x4{0, 0, 0, 0};
+  return x.v;
+}
+
+// sum over the dim elements of a column's stationary row (fragments f) times another row in memory
+template <typename T, int DP>
+__device__ __forceinline__ float frag_dot(const V8<T> (&f)[DP / 16], const T *__restrict__ other, int h, int dim) {
+  float s = 0;
+#pragma unroll
+  for (int i = 0; i < DP / 16; i++) {
+    const int col = 16 * i + 8 * h;
+    if (col < dim) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) s = fmaf((float)f[i][e], (float)other[col + e], s);
+    }
+  }
+  return s + half_swap(s);
+}
+
+// acc[db][r] += w * row[32 * db + acc_row(r, h)]: one inner index of the transposed product by itself
+template <typename T, int DP>
+__device__ __forceinline__ void add_row(f32x16 (&acc)[DP / 32], float w, const T *__restrict__ row, int h, int dim) {
+#pragma unroll
+  for (int db = 0; db < DP / 32; db++) {
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+      const int d = 32 * db + acc_row(r, h);
+      if (d < dim) acc[db][r] = fmaf(w, (float)row[d], acc[db][r]);
+    }
+  }
+}
+
+__device__ __forceinline__ int min_over(int v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o));
+  return v;
+}
+__device__ __forceinline__ int max_over(int v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o));
+  return v;
+}
+
+// Rows of the transposed accumulators (columns = rows of the output) to memory, four at a time
+template <typename T, int DP>
+__device__ __forceinline__ void store_cols(T *row, const f32x16 (&acc)[DP / 32], float w, int h, int dim) {
+#pragma unroll
+  for (int db = 0; db < DP / 32; db++) {
+#pragma unroll
+    for (int b = 0; b < 4; b++) {
+      const int d = 32 * db + 8 * b + 4 * h;
+      if (d < dim) {
+        const f32x4 x = {acc[db][4 * b] * w, acc[db][4 * b + 1] * w, acc[db][4 * b + 2] * w, acc[db][4 * b + 3] * w};
+        *reinterpret_cast<V4<T> *>(row + d) = __builtin_convertvector(x, V4<T>);
+      }
+    }
+  }
+}
+
+template <int N>
+__device__ __forceinline__ bool all_finite(const f32x16 (&acc)[N]) {
+  bool ok = true;
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+#pragma unroll
+    for (int r = 0; r < 16; r++) ok = ok && finite(acc[i][r]);
+  }
+  return ok;
+}
+
+template <typename F>
+int with_dim(int dim, F f) {
+  if (dim <= 32) return f(std::integral_constant<int, 32>());
+  if (dim <= 64) return f(std::integral_constant<int, 64>());
+  return f(std::integral_constant<int, 128>());
+}
+template <typename F>
+int with_type(kl_dtype dtype, const char *func, F f) {
+  switch (dtype) {
+    case KL_F32: return f(float());
+    case KL_F16: return f(f16_t());
+    case KL_BF16: return f(bf16_t());
+    default: set_error(std::string(func) + ": expected a Half, BFloat16 or Float tensor"); return KL_E_INVALID;
+  }
+}
+
+// Checks an Attend's sizes and fills it.  dim: a multiple of 8 up to 128, so rows are whole 16-byte pieces.
+int fill_attend(Attend &a, const char *func, int64_t nq, int64_t nk, int heads, int kv_heads, int dim,
+                const int64_t *strides, const int32_t *qid, const int32_t *qstart, const int32_t *kid,
+                const int32_t *kstart, float scale, int causal);
+
+}  // namespace kl

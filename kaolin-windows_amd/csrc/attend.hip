@@ -1,0 +1,321 @@
+// attend.hip -- attention over packs, forward: o[i] = sum_j softmax_j(scale * q[i] . k[j]) v[j] over the
+// keys j of row i's pack, with grouped heads (attend.h).
+//
+// One workgroup of four waves takes 128 virtual rows of one key head and walks the keys that any of them
+// sees, a tile at a time, keeping the running maximum and sum of the softmax in 32 bits.  Scores are
+// computed transposed, S^T = K Q^T, so a lane holds one row's scores: the softmax is lane-local but for one
+// exchange with the other half, and the weights are the second product's operand (O^T = V^T P^T) where
+// they lie, without a trip through LDS (seqcommon.h, acc_frag).
+// Rounding: weights are in [0, 1] and are rounded to the inputs' type for the second product (off by at
+// most half a step each, and averaged over the keys; float stays float); the sum they are divided by is
+// taken before the rounding, in 32 bits.
+//
+// A key outside a row's range has weight 0, but 0 * inf and 0 * NaN would still reach the row through the
+// product.  Nothing in the main walk guards against that: if an accumulator ends up not finite, the
+// workgroup walks its keys again with the rows of k and v that hold such values taken out of the tiles and
+// added one by one to just the rows that see them.
+#include "attend.h"
+
+namespace kl {
+
+template <typename T, int DP>
+struct FwdTile {
+  static constexpr int BM = 128;                         // virtual rows: 32 a wave
+  static constexpr int BN = sizeof(T) == 4 ? 32 : 64;    // keys
+};
+
+struct RowState {
+  float m = -INFINITY, l = 0;
+};
+
+template <typename T, int DP, bool CAREFUL>
+__device__ __forceinline__ void fwd_walk(const Attend &a, const T *__restrict__ k, const T *__restrict__ v, int begin,
+                                         int end, Range mine, int wlo, int whi, int full_lo, int full_hi,
+                                         const V8<T> (&qf)[DP / 16], T *ks, T *vs, uint32_t *bad,
+                                         f32x16 (&acc)[DP / 32], RowState &st) {
+  constexpr int BN = FwdTile<T, DP>::BN;
+  using KV = Stage<T, DP, BN>;
+  constexpr int LD = KV::LD;
+  const int lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
+  KV ka, va;
+  ka.load(k, a.k.row, begin, end, a.dim);
+  va.load(v, a.v.row, begin, end, a.dim);
+  for (int kt = begin; kt < end; kt += BN) {
+    __syncthreads();  // the tile of the round before is read
+    if constexpr (CAREFUL) {
+      if (threadIdx.x < BN / 32) bad[threadIdx.x] = 0;
+      __syncthreads();
+      ka.mark_bad(bad);
+      va.mark_bad(bad);
+      __syncthreads();
+      ka.store_good(ks, bad);
+      va.store_good(vs, bad);
+    } else {
+      ka.store(ks);
+      va.store(vs);
+    }
+    __syncthreads();
+    if (kt + BN < end) {
+      ka.load(k, a.k.row, kt + BN, end, a.dim);
+      va.load(v, a.v.row, kt + BN, end, a.dim);
+    }
+    if (kt >= whi || kt + BN <= wlo) continue;
+    f32x16 s[BN / 32];
+#pragma unroll
+    for (int b = 0; b < BN / 32; b++) {
+      s[b] = f32x16{};
+#pragma unroll
+      for (int i = 0; i < DP / 16; i++) s[b] = mma(row_frag(ks, LD, 32 * b + col, 16 * i + 8 * h), qf[i], s[b]);
+    }
+    const bool whole = !CAREFUL && kt >= full_lo && kt + BN <= full_hi;
+    float top = -INFINITY;
+#pragma unroll
+    for (int b = 0; b < BN / 32; b++) {
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        const int key = kt + 32 * b + acc_row(r, h);
+        bool in = whole || (key >= mine.lo && key < mine.hi);
+        if constexpr (CAREFUL) in = in && !(bad[b] >> acc_row(r, h) & 1);
+        s[b][r] = in ? s[b][r] * a.c : -INFINITY;
+        top = fmaxf(top, s[b][r]);
+      }
+    }
+    top = fmaxf(top, half_swap(top));
+    const float m = fmaxf(st.m, top), base = m == -INFINITY ? 0.f : m;
+    const float keep = exp2_fast(st.m - base);
+    st.m = m;
+    st.l *= keep;
+#pragma unroll
+    for (int db = 0; db < DP / 32; db++) {
+#pragma unroll
+      for (int r = 0; r < 16; r++) acc[db][r] *= keep;
+    }
+#pragma unroll
+    for (int b = 0; b < BN / 32; b++) {
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        s[b][r] = exp2_fast(s[b][r] - base);
+        st.l += s[b][r];
+      }
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const V8<T> p = acc_frag<T>(s[b], i);
+#pragma unroll
+        for (int db = 0; db < DP / 32; db++) acc[db] = mma(col_frag(vs, LD, 32 * b + 16 * i, 32 * db), p, acc[db]);
+      }
+    }
+    if constexpr (CAREFUL) {
+      for (int b = 0; b < BN / 32; b++) {
+        for (uint32_t w = bad[b]; w; w &= w - 1) {
+          const int key = kt + 32 * b + __builtin_ctz(w);
+          if (key >= whi || key < wlo) continue;
+          const float t = frag_dot<T, DP>(qf, k + key * a.k.row, h, a.dim) * a.c;
+          if (key >= mine.lo && key < mine.hi) {
+            const float m1 = fmaxf(st.m, t), base1 = m1 == -INFINITY ? 0.f : m1;
+            const float keep1 = exp2_fast(st.m - base1), p = exp2_fast(t - base1);
+            st.m = m1;
+            st.l = st.l * keep1 + (h == 0 ? p : 0.f);
+            for (int db = 0; db < DP / 32; db++) {
+#pragma unroll
+              for (int r = 0; r < 16; r++) acc[db][r] *= keep1;
+            }
+            add_row<T, DP>(acc, p, v + key * a.v.row, h, a.dim);
+          }
+        }
+      }
+    }
+  }
+}
+
+// grid: (tiles * kv_heads, splits).  part / stat: the splits' unfinished sums (NULL without splits).
+template <typename T, int DP>
+__global__ void __launch_bounds__(256, 2) attend_fwd_kernel(Attend a, const T *__restrict__ q, const T *__restrict__ k,
+                                                         const T *__restrict__ v, T *__restrict__ o,
+                                                         float *__restrict__ lse, float *__restrict__ part,
+                                                         float2 *__restrict__ stat) {
+  constexpr int BM = FwdTile<T, DP>::BM, BN = FwdTile<T, DP>::BN;
+  using KV = Stage<T, DP, BN>;
+  __shared__ T ks[BN * KV::LD], vs[BN * KV::LD];
+  __shared__ uint32_t bad[BN / 32];
+  __shared__ int s_lo[4], s_hi[4], s_redo;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
+  const int head = blockIdx.x % a.kv_heads;
+  const int64_t total = (int64_t)a.nq * a.group;
+  const int64_t tiles = gridDim.x / a.kv_heads;
+  const int64_t m = (tiles - 1 - blockIdx.x / a.kv_heads) * BM + wave * 32 + col;  // the last rows see most keys
+  const bool live = m < total;
+  const int row = live ? (int)(m / a.group) : 0, qhead = head * a.group + (live ? (int)(m % a.group) : 0);
+  const Range mine = live ? key_range(a, row) : no_keys();
+  const int wlo = min_over(mine.lo), whi = max_over(mine.hi);
+  const int full_lo = max_over(mine.lo), full_hi = min_over(mine.hi);
+  if (lane == 0) {
+    s_lo[wave] = wlo;
+    s_hi[wave] = whi;
+  }
+  if (threadIdx.x == 0) s_redo = 0;
+  __syncthreads();
+  int begin = min(min(s_lo[0], s_lo[1]), min(s_lo[2], s_lo[3]));
+  int end = max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3]));
+  if (begin >= end) begin = end = 0;
+  if (part) {  // this split's share of the keys, whole tiles
+    const int tiles_here = (end - begin + BN - 1) / BN, n = (int)gridDim.y;
+    const int share = (tiles_here + n - 1) / n * BN;
+    begin = (int)min((int64_t)end, begin + (int64_t)share * blockIdx.y);
+    end = (int)min((int64_t)end, (int64_t)begin + share);
+  }
+  V8<T> qf[DP / 16];
+  const T *qrow = q + row * a.q.row + qhead * a.q.head;
+#pragma unroll
+  for (int i = 0; i < DP / 16; i++) qf[i] = global_frag(qrow, live, 16 * i + 8 * h, a.dim);
+  const T *kh = k + head * a.k.head, *vh = v + head * a.v.head;
+  f32x16 acc[DP / 32] = {};
+  RowState st;
+  fwd_walk<T, DP, false>(a, kh, vh, begin, end, mine, wlo, whi, full_lo, full_hi, qf, ks, vs, bad, acc, st);
+  if (!(all_finite(acc) && finite(st.l))) s_redo = 1;
+  __syncthreads();
+  if (s_redo) {
+#pragma unroll
+    for (int db = 0; db < DP / 32; db++) acc[db] = f32x16{};
+    st = RowState();
+    fwd_walk<T, DP, true>(a, kh, vh, begin, end, mine, wlo, whi, full_lo, full_hi, qf, ks, vs, bad, acc, st);
+  }
+  const float l = st.l + half_swap(st.l);
+  if (!live) return;
+  if (part) {
+    const int64_t at = ((int64_t)blockIdx.y * a.kv_heads + head) * total + m;
+    if (h == 0) stat[at] = make_float2(st.m, l);
+    if (st.m != -INFINITY || l != 0) store_cols<float, DP>(part + at * a.dim, acc, 1.f, h, a.dim);
+    return;
+  }
+  // a row that sees no key: 0
+  store_cols<T, DP>(o + ((int64_t)row * a.kv_heads * a.group + qhead) * a.dim, acc, l == 0 ? 0.f : 1.f / l, h, a.dim);
+  if (lse && h == 0) lse[(int64_t)row * a.kv_heads * a.group + qhead] = l == 0 ? 0.f : st.m + log2_fast(l);
+}
+
+// The splits of one (key head, virtual row) joined: eight elements a thread.
+template <typename T>
+__global__ void __launch_bounds__(256) attend_join_kernel(Attend a, int splits, const float *__restrict__ part,
+                                                        const float2 *__restrict__ stat, T *__restrict__ o,
+                                                        float *__restrict__ lse) {
+  const int64_t total = (int64_t)a.nq * a.group, rows = total * a.kv_heads;
+  const int per = a.dim / 8;
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t at = t / per;
+  if (at >= rows) return;
+  const int d = (int)(t % per) * 8, head = (int)(at / total);
+  const int64_t m = at % total;
+  float top = -INFINITY;
+  for (int s = 0; s < splits; s++) top = fmaxf(top, stat[s * rows + at].x);
+  const float base = top == -INFINITY ? 0.f : top;
+  float l = 0;
+  f32x8 sum = {};
+  for (int s = 0; s < splits; s++) {
+    const float2 x = stat[s * rows + at];
+    if (x.x == -INFINITY && x.y == 0) continue;  // no key of the row in this split
+    const float w = exp2_fast(x.x - base);
+    l = fmaf(w, x.y, l);
+    const f32x4 *p = reinterpret_cast<const f32x4 *>(part + (s * rows + at) * a.dim + d);
+    const f32x4 u0 = p[0], u1 = p[1];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      sum[e] = fmaf(w, u0[e], sum[e]);
+      sum[4 + e] = fmaf(w, u1[e], sum[4 + e]);
+    }
+  }
+  const int64_t out = m / a.group * a.kv_heads * a.group + head * a.group + m % a.group;
+  const float inv = l == 0 ? 0.f : 1.f / l;
+#pragma unroll
+  for (int e = 0; e < 8; e++) sum[e] *= inv;
+  *reinterpret_cast<V8<T> *>(o + out * a.dim + d) = __builtin_convertvector(sum, V8<T>);
+  if (lse && d == 0) lse[out] = l == 0 ? 0.f : top + log2_fast(l);
+}
+
+// Splits of the keys: enough workgroups for the 256 CUs where the rows alone give few, and at least
+// two tiles of keys for each of them if the rows' packs shared the keys evenly.
+static int attend_splits(int64_t nq, int64_t nk, int kv_heads, int group, int bn) {
+  const int64_t blocks = cdiv(nq * group, 128) * kv_heads;
+  if (blocks >= 512) return 1;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(1024, std::max<int64_t>(blocks, 1)), cdiv(nk, 2 * bn), 128}));
+}
+
+int fill_attend(Attend &a, const char *func, int64_t nq, int64_t nk, int heads, int kv_heads, int dim,
+                const int64_t *strides, const int32_t *qid, const int32_t *qstart, const int32_t *kid,
+                const int32_t *kstart, float scale, int causal) {
+  const std::string f = std::string(func) + ": ";
+  KL_REQUIRE(nq >= 0 && nk >= 0 && nq < (int64_t)1 << 31 && nk < (int64_t)1 << 31, f + "rows out of range");
+  KL_REQUIRE(kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && heads <= 4096,
+             f + "the query heads must be a multiple of the key heads");
+  KL_REQUIRE(dim > 0 && dim <= 128 && dim % 8 == 0, f + "the head size must be a multiple of 8 up to 128");
+  KL_REQUIRE(scale > 0 && scale < INFINITY, f + "the scale must be positive and finite");
+  // virtual rows and workgroups are counted in 31 bits
+  KL_REQUIRE(nq * (heads / kv_heads) <= ((int64_t)1 << 31) - 256 &&
+                 cdiv(std::max(nq * (heads / kv_heads), nk), 128) * kv_heads < (int64_t)1 << 31,
+             f + "too many rows and heads");
+  KL_REQUIRE(nk <= ((int64_t)1 << 31) - 256, f + "rows out of range");
+  a.q = {strides[0], strides[1]};
+  a.k = {strides[2], strides[3]};
+  a.v = {strides[4], strides[5]};
+  a.qid = qid;
+  a.qstart = qstart;
+  a.kid = kid;
+  a.kstart = kstart;
+  a.nq = (int)nq;
+  a.nk = (int)nk;
+  a.kv_heads = kv_heads;
+  a.group = heads / kv_heads;
+  a.dim = dim;
+  a.causal = causal ? 1 : 0;
+  a.scale = scale;
+  a.c = scale * kLog2e;
+  return KL_OK;
+}
+
+template <typename T, int DP>
+static int attend_forward(const Attend &a, const void *q, const void *k, const void *v, void *o, float *lse, void *ws,
+                          hipStream_t st) {
+  const int splits = attend_splits(a.nq, a.nk, a.kv_heads, a.group, FwdTile<T, DP>::BN);
+  const int64_t total = (int64_t)a.nq * a.group, rows = total * a.kv_heads;
+  const unsigned blocks = (unsigned)(cdiv(total, FwdTile<T, DP>::BM) * a.kv_heads);
+  float2 *stat = splits > 1 ? (float2 *)ws : nullptr;
+  float *part = splits > 1 ? (float *)((char *)ws + al256((size_t)splits * rows * 8)) : nullptr;
+  hipLaunchKernelGGL((attend_fwd_kernel<T, DP>), dim3(blocks, splits), dim3(256), 0, st, a, (const T *)q, (const T *)k,
+                     (const T *)v, (T *)o, lse, part, stat);
+  KL_CHECK_LAUNCH();
+  if (splits > 1) {
+    hipLaunchKernelGGL(attend_join_kernel<T>, dim3((unsigned)cdiv(rows * (a.dim / 8), 256)), dim3(256), 0, st, a,
+                       splits, part, stat, (T *)o, lse);
+    KL_CHECK_LAUNCH();
+  }
+  return KL_OK;
+}
+
+}  // namespace kl
+
+using namespace kl;
+
+extern "C" size_t kl_pack_attention_workspace_bytes(kl_dtype dtype, int64_t num_q, int64_t num_k, int heads,
+                                                    int kv_heads, int dim) {
+  if (num_q <= 0 || kv_heads <= 0 || heads % kv_heads) return 256;
+  const int splits = attend_splits(num_q, num_k, kv_heads, heads / kv_heads, dtype == KL_F32 ? 32 : 64);
+  if (splits == 1) return 256;
+  const size_t rows = (size_t)num_q * heads;
+  return al256((size_t)splits * rows * 8) + al256((size_t)splits * rows * dim * 4);
+}
+
+extern "C" int kl_pack_attention_forward(kl_dtype dtype, int64_t num_q, int64_t num_k, int heads, int kv_heads, int dim,
+                                         const void *q, const void *k, const void *v, const int64_t *strides_host,
+                                         const int32_t *q_ids, const int32_t *q_starts, const int32_t *k_ids,
+                                         const int32_t *k_starts, float scale, int causal, void *out, float *lse,
+                                         void *ws, size_t ws_bytes, kl_stream stream) {
+  Attend a;
+  KL_CHECK_RC(fill_attend(a, "pack_attention", num_q, num_k, heads, kv_heads, dim, strides_host, q_ids, q_starts, k_ids,
+                          k_starts, scale, causal));
+  KL_REQUIRE(ws_bytes >= kl_pack_attention_workspace_bytes(dtype, num_q, num_k, heads, kv_heads, dim),
+             "pack_attention: the workspace is too small");
+  if (num_q == 0) return KL_OK;
+  return with_type(dtype, "pack_attention", [&](auto t) {
+    return with_dim(dim, [&](auto dp) {
+      return attend_forward<decltype(t), decltype(dp)::value>(a, q, k, v, out, lse, ws, S(stream));
+    });
+  });
+}

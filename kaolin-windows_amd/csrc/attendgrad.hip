@@ -1,0 +1,456 @@
+// attendgrad.hip -- attention over packs, backward.  With p = softmax, D_i = do[i] . o[i] and
+// ds_ij = p_ij (do[i] . v[j] - D_i):  dq[i] = scale sum_j ds_ij k[j],  dk[j] = scale sum_i ds_ij q[i],
+// dv[j] = sum_i p_ij do[i], the sums of dk and dv over the heads that share the key head as well.
+//
+// Two kernels compute the scores again instead of one with atomics on dq: five products become seven, and
+// every sum has a fixed order.  dq: as the forward, the wave's 32 columns are rows of q.  dk / dv: the
+// columns are keys, and virtual rows stream past (attend.h).  Both feed their second products from the
+// accumulators of the first in place (seqcommon.h, acc_frag); the streamed tiles are read from LDS along
+// rows for the first products and along columns for the second.
+// Rounding: p and ds are rounded to the inputs' type for the second products, half a step each; sums stay
+// in 32 bits.  float16 has no exponents for small gradients: there ds is multiplied by a power of two that
+// puts the largest |do| into [16, 32), and the result by its inverse, both exact.
+// Masked places that hold infinities or NaN: as in attend.hip.
+#include "attend.h"
+
+namespace kl {
+
+constexpr int kMaxParts = 1024;  // workgroups of the first kernel: partial maxima of |do|
+
+struct Grad {
+  const float2 *ld;    // (lse, D) of each (row, head)
+  const int2 *range;   // keys of each row
+  const float *amax;   // partial maxima of |do| (f16)
+  int parts;
+};
+
+// D, the key ranges and the maxima of |do|: 16 lanes per (row, head).
+template <typename T>
+__global__ void __launch_bounds__(256) attend_prep_kernel(Attend a, const T *__restrict__ o, const T *__restrict__ go,
+                                                        const float *__restrict__ lse, float2 *__restrict__ ld,
+                                                        int2 *__restrict__ range, float *__restrict__ amax) {
+  const int heads = a.kv_heads * a.group, E = 16 / (int)sizeof(T), sub = threadIdx.x & 15;
+  const int64_t rows = (int64_t)a.nq * heads;
+  float big = 0;
+  for (int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) / 16; at < rows; at += (int64_t)gridDim.x * 16) {
+    float d = 0;
+    for (int c = sub * E; c < a.dim; c += 16 * E) {
+      union {
+        u32x4 w;
+        T v[16 / sizeof(T)];
+      } x, y;
+      x.w = *reinterpret_cast<const u32x4 *>(o + at * a.dim + c);
+      y.w = *reinterpret_cast<const u32x4 *>(go + at * a.dim + c);
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        d = fmaf((float)x.v[e], (float)y.v[e], d);
+        big = fmaxf(big, fabsf((float)y.v[e]));
+      }
+    }
+#pragma unroll
+    for (int s = 8; s > 0; s >>= 1) d += __shfl_xor(d, s);
+    if (sub == 0) ld[at] = make_float2(lse[at], d);
+    if (sub == 0 && at % heads == 0) {
+      const Range r = key_range(a, (int)(at / heads));
+      range[at / heads] = make_int2(r.lo, r.hi);
+    }
+  }
+  if constexpr (std::is_same<T, f16_t>::value) {
+    __shared__ float s_max[4];
+    big = wave_max(big);
+    if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = big;
+    __syncthreads();
+    if (threadIdx.x == 0) amax[blockIdx.x] = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+  }
+}
+
+// the power of two that puts the largest |do| into [16, 32); 1 where there is none.  Every thread calls it.
+template <typename T>
+__device__ __forceinline__ float grad_scale(const Grad &g, float *s_max) {
+  if constexpr (!std::is_same<T, f16_t>::value) return 1.f;
+  float big = 0;
+  for (int i = threadIdx.x; i < g.parts; i += 256) big = fmaxf(big, g.amax[i]);
+  big = wave_max(big);
+  if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = big;
+  __syncthreads();
+  big = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+  if (!(big > 0) || !finite(big)) return 1.f;
+  return __uint_as_float((uint32_t)(127 + 4 + 127 - (int)(__float_as_uint(big) >> 23)) << 23);
+}
+
+template <typename T, int DP>
+struct DqTile {
+  static constexpr int BN = sizeof(T) == 4 ? 32 : 64;
+};
+
+template <typename T, int DP, bool CAREFUL>
+__device__ __forceinline__ void dq_walk(const Attend &a, const T *__restrict__ k, const T *__restrict__ v, int begin,
+                                        int end, int2 mine, float2 ld, float gs, int wlo, int whi, int full_lo,
+                                        int full_hi, const V8<T> (&qf)[DP / 16], const V8<T> (&gf)[DP / 16], T *ks,
+                                        T *vs, uint32_t *bad, f32x16 (&acc)[DP / 32]) {
+  constexpr int BN = DqTile<T, DP>::BN;
+  using KV = Stage<T, DP, BN>;
+  constexpr int LD = KV::LD;
+  const int lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
+  KV ka, va;
+  ka.load(k, a.k.row, begin, end, a.dim);
+  va.load(v, a.v.row, begin, end, a.dim);
+  for (int kt = begin; kt < end; kt += BN) {
+    __syncthreads();
+    if constexpr (CAREFUL) {
+      if (threadIdx.x < BN / 32) bad[threadIdx.x] = 0;
+      __syncthreads();
+      ka.mark_bad(bad);
+      va.mark_bad(bad);
+      __syncthreads();
+      ka.store_good(ks, bad);
+      va.store_good(vs, bad);
+    } else {
+      ka.store(ks);
+      va.store(vs);
+    }
+    __syncthreads();
+    if (kt + BN < end) {
+      ka.load(k, a.k.row, kt + BN, end, a.dim);
+      va.load(v, a.v.row, kt + BN, end, a.dim);
+    }
+    if (kt >= whi || kt + BN <= wlo) continue;
+    const bool whole = !CAREFUL && kt >= full_lo && kt + BN <= full_hi;
+#pragma unroll
+    for (int b = 0; b < BN / 32; b++) {
+      f32x16 s = {}, dp = {};
+#pragma unroll
+      for (int i = 0; i < DP / 16; i++) {
+        s = mma(row_frag(ks, LD, 32 * b + col, 16 * i + 8 * h), qf[i], s);
+        dp = mma(row_frag(vs, LD, 32 * b + col, 16 * i + 8 * h), gf[i], dp);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        const int key = kt + 32 * b + acc_row(r, h);
+        bool in = whole || (key >= mine.x && key < mine.y);
+        if constexpr (CAREFUL) in = in && !(bad[b] >> acc_row(r, h) & 1);
+        s[r] = in ? exp2_fast(fmaf(s[r], a.c, -ld.x)) * (dp[r] - ld.y) * gs : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const V8<T> ds = acc_frag<T>(s, i);
+#pragma unroll
+        for (int db = 0; db < DP / 32; db++) acc[db] = mma(col_frag(ks, LD, 32 * b + 16 * i, 32 * db), ds, acc[db]);
+      }
+    }
+    if constexpr (CAREFUL) {
+      for (int b = 0; b < BN / 32; b++) {
+        for (uint32_t w = bad[b]; w; w &= w - 1) {
+          const int key = kt + 32 * b + __builtin_ctz(w);
+          if (key >= whi || key < wlo) continue;
+          const float t = frag_dot<T, DP>(qf, k + key * a.k.row, h, a.dim) * a.c;
+          const float dp = frag_dot<T, DP>(gf, v + key * a.v.row, h, a.dim);
+          if (key >= mine.x && key < mine.y)
+            add_row<T, DP>(acc, exp2_fast(t - ld.x) * (dp - ld.y) * gs, k + key * a.k.row, h, a.dim);
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(256, sizeof(T) == 4 && DP == 128 ? 1 : 2)
+    attend_dq_kernel(Attend a, Grad g, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
+                     const T *__restrict__ go, T *__restrict__ dq) {
+  constexpr int BN = DqTile<T, DP>::BN;
+  using KV = Stage<T, DP, BN>;
+  __shared__ T ks[BN * KV::LD], vs[BN * KV::LD];
+  __shared__ uint32_t bad[BN / 32];
+  __shared__ int s_lo[4], s_hi[4], s_redo;
+  __shared__ float s_max[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
+  const int head = blockIdx.x % a.kv_heads, heads = a.kv_heads * a.group;
+  const int64_t total = (int64_t)a.nq * a.group;
+  const int64_t tiles = gridDim.x / a.kv_heads;
+  const int64_t m = (tiles - 1 - blockIdx.x / a.kv_heads) * 128 + wave * 32 + col;
+  const bool live = m < total;
+  const int row = live ? (int)(m / a.group) : 0, qhead = head * a.group + (live ? (int)(m % a.group) : 0);
+  const Range none = no_keys();
+  const int2 mine = live ? g.range[row] : make_int2(none.lo, none.hi);
+  const int64_t at = (int64_t)row * heads + qhead;
+  const float2 ld = live ? g.ld[at] : make_float2(0, 0);
+  const int wlo = min_over(mine.x), whi = max_over(mine.y);
+  const int full_lo = max_over(mine.x), full_hi = min_over(mine.y);
+  if (lane == 0) {
+    s_lo[wave] = wlo;
+    s_hi[wave] = whi;
+  }
+  if (threadIdx.x == 0) s_redo = 0;
+  __syncthreads();
+  int begin = min(min(s_lo[0], s_lo[1]), min(s_lo[2], s_lo[3]));
+  int end = max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3]));
+  if (begin >= end) begin = end = 0;
+  const float gs = grad_scale<T>(g, s_max);
+  V8<T> qf[DP / 16], gf[DP / 16];
+  const T *qrow = q + row * a.q.row + qhead * a.q.head, *grow = go + at * a.dim;
+#pragma unroll
+  for (int i = 0; i < DP / 16; i++) {
+    qf[i] = global_frag(qrow, live, 16 * i + 8 * h, a.dim);
+    gf[i] = global_frag(grow, live, 16 * i + 8 * h, a.dim);
+  }
+  const T *kh = k + head * a.k.head, *vh = v + head * a.v.head;
+  f32x16 acc[DP / 32] = {};
+  dq_walk<T, DP, false>(a, kh, vh, begin, end, mine, ld, gs, wlo, whi, full_lo, full_hi, qf, gf, ks, vs, bad, acc);
+  if (!all_finite(acc)) s_redo = 1;
+  __syncthreads();
+  if (s_redo) {
+#pragma unroll
+    for (int db = 0; db < DP / 32; db++) acc[db] = f32x16{};
+    dq_walk<T, DP, true>(a, kh, vh, begin, end, mine, ld, gs, wlo, whi, full_lo, full_hi, qf, gf, ks, vs, bad, acc);
+  }
+  if (live) store_cols<T, DP>(dq + at * a.dim, acc, a.scale / gs, h, a.dim);
+}
+
+// Virtual rows [m0, m0 + ROWS) of a (rows, heads, dim) tensor, one key head's group (Stage with the
+// addresses of virtual rows)
+template <typename T, int DP, int ROWS>
+struct StageRows : Stage<T, DP, ROWS> {
+  using B = Stage<T, DP, ROWS>;
+  __device__ __forceinline__ void load_rows(const T *__restrict__ base, Heads st, int group, int m0, int end, int dim) {
+#pragma unroll
+    for (int i = 0; i < B::PER; i++) {
+      const int at = threadIdx.x + 256 * i, m = m0 + at / B::CH, col = at % B::CH * B::E;
+      this->w[i] = u32x4{0, 0, 0, 0};
+      if (m < end && col < dim) {
+        const int row = (int)((unsigned)m / (unsigned)group);
+        this->w[i] = *reinterpret_cast<const u32x4 *>(base + row * st.row + (m - row * group) * st.head + col);
+      }
+    }
+  }
+};
+
+template <typename T, int DP>
+struct DkvTile {
+  static constexpr int BQ = sizeof(T) == 4 ? 32 : 64;  // virtual rows per step
+};
+
+template <typename T, int DP, bool CAREFUL>
+__device__ __forceinline__ void dkv_walk(const Attend &a, const Grad &g, const T *__restrict__ q, Heads gst,
+                                         const T *__restrict__ go, int head, int begin, int end, int key0, float gs,
+                                         const V8<T> (&kf)[DP / 16], const V8<T> (&vf)[DP / 16], T *qs, T *os,
+                                         float2 *s_ld, int2 *s_range, uint32_t *bad, f32x16 (&dk)[DP / 32],
+                                         f32x16 (&dv)[DP / 32]) {
+  constexpr int BQ = DkvTile<T, DP>::BQ;
+  using Q = StageRows<T, DP, BQ>;
+  constexpr int LD = Q::B::LD;
+  const int lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
+  const int heads = a.kv_heads * a.group, key = key0 + col;
+  const Range none = no_keys();
+  Q qa, oa;
+  float2 ld = make_float2(0, 0);
+  int2 range = make_int2(none.lo, none.hi);
+  auto load = [&](int mt) {
+    qa.load_rows(q, a.q, a.group, mt, end, a.dim);
+    oa.load_rows(go, gst, a.group, mt, end, a.dim);
+    const int m = mt + (int)threadIdx.x;
+    if (threadIdx.x < BQ) {
+      const bool live = m < end;
+      const int row = live ? (int)((unsigned)m / (unsigned)a.group) : 0;
+      ld = live ? g.ld[(int64_t)row * heads + head * a.group + (m - row * a.group)] : make_float2(0, 0);
+      range = live ? g.range[row] : make_int2(none.lo, none.hi);
+    }
+  };
+  if (begin < end) load(begin);
+  for (int mt = begin; mt < end; mt += BQ) {
+    __syncthreads();
+    if constexpr (CAREFUL) {
+      if (threadIdx.x < BQ / 32) bad[threadIdx.x] = 0;
+      __syncthreads();
+      qa.mark_bad(bad);
+      oa.mark_bad(bad);
+      __syncthreads();
+      qa.store_good(qs, bad);
+      oa.store_good(os, bad);
+    } else {
+      qa.store(qs);
+      oa.store(os);
+    }
+    if (threadIdx.x < BQ) {
+      s_ld[threadIdx.x] = ld;
+      s_range[threadIdx.x] = range;
+    }
+    __syncthreads();
+    if (mt + BQ < end) load(mt + BQ);
+    const int2 mine = s_range[lane % BQ];
+    if (!__any(mine.x < key0 + 32 && mine.y > key0)) continue;
+    const bool whole = !CAREFUL && __all(mine.x <= key0 && mine.y >= key0 + 32);
+#pragma unroll
+    for (int b = 0; b < BQ / 32; b++) {
+      f32x16 s = {}, dp = {};
+#pragma unroll
+      for (int i = 0; i < DP / 16; i++) {
+        s = mma(row_frag(qs, LD, 32 * b + col, 16 * i + 8 * h), kf[i], s);
+        dp = mma(row_frag(os, LD, 32 * b + col, 16 * i + 8 * h), vf[i], dp);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        const int i = 32 * b + acc_row(r, h);
+        const float2 x = s_ld[i];
+        bool in = true;
+        if (!whole) {
+          const int2 kr = s_range[i];
+          in = key >= kr.x && key < kr.y;
+        }
+        if constexpr (CAREFUL) in = in && !(bad[b] >> acc_row(r, h) & 1);
+        const float p = in ? exp2_fast(fmaf(s[r], a.c, -x.x)) : 0.f;
+        s[r] = p;
+        dp[r] = in ? p * (dp[r] - x.y) * gs : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const V8<T> p = acc_frag<T>(s, i), ds = acc_frag<T>(dp, i);
+#pragma unroll
+        for (int db = 0; db < DP / 32; db++) {
+          dv[db] = mma(col_frag(os, LD, 32 * b + 16 * i, 32 * db), p, dv[db]);
+          dk[db] = mma(col_frag(qs, LD, 32 * b + 16 * i, 32 * db), ds, dk[db]);
+        }
+      }
+    }
+    if constexpr (CAREFUL) {
+      for (int b = 0; b < BQ / 32; b++) {
+        for (uint32_t w = bad[b]; w; w &= w - 1) {
+          const int i = 32 * b + __builtin_ctz(w), m = mt + i;
+          const int row = (int)((unsigned)m / (unsigned)a.group), sub = m - row * a.group;
+          const T *qrow = q + row * a.q.row + sub * a.q.head, *grow = go + row * gst.row + sub * gst.head;
+          const float2 x = s_ld[i];
+          const int2 kr = s_range[i];
+          if (kr.x >= key0 + 32 || kr.y <= key0) continue;
+          const float t = frag_dot<T, DP>(kf, qrow, h, a.dim) * a.c, dpx = frag_dot<T, DP>(vf, grow, h, a.dim);
+          if (key >= kr.x && key < kr.y) {
+            const float p = exp2_fast(t - x.x);
+            add_row<T, DP>(dv, p, grow, h, a.dim);
+            add_row<T, DP>(dk, p * (dpx - x.y) * gs, qrow, h, a.dim);
+          }
+        }
+      }
+    }
+  }
+}
+
+// The query rows that see any of keys [j0, j1)
+__device__ __forceinline__ Range row_range(const Attend &a, int j0, int j1) {
+  const int first = a.kid[j0], last = a.kid[j1 - 1];
+  if (last < 0) return {0, 0};
+  int r0 = a.qstart[min(max(first, 0), a.nq)];
+  const int r1 = a.qstart[min(last + 1, a.nq)];
+  if (a.causal && first >= 0) {
+    const int ke = a.kstart[min(first + 1, a.nk)], qe = a.qstart[min(first + 1, a.nq)];
+    r0 = max(r0, j0 - ke + qe);
+  }
+  return {min(r0, r1), r1};
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(256, DP == 128 ? 1 : 2)
+    attend_dkv_kernel(Attend a, Grad g, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
+                      const T *__restrict__ go, T *__restrict__ dk_out, T *__restrict__ dv_out) {
+  constexpr int BQ = DkvTile<T, DP>::BQ;
+  using Q = StageRows<T, DP, BQ>;
+  __shared__ T qs[BQ * Q::B::LD], os[BQ * Q::B::LD];
+  __shared__ float2 s_ld[BQ];
+  __shared__ int2 s_range[BQ];
+  __shared__ uint32_t bad[BQ / 32];
+  __shared__ int s_redo;
+  __shared__ float s_max[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
+  const int head = blockIdx.x % a.kv_heads, heads = a.kv_heads * a.group;
+  const int j0 = blockIdx.x / a.kv_heads * 128, key0 = j0 + wave * 32, key = key0 + col;
+  const bool live = key < a.nk;
+  const Range rows = row_range(a, j0, min(j0 + 128, a.nk));
+  if (threadIdx.x == 0) s_redo = 0;
+  const float gs = grad_scale<T>(g, s_max);
+  __syncthreads();
+  const T *qh = q + (int64_t)head * a.group * a.q.head;
+  const Heads gst = {(int64_t)heads * a.dim, a.dim};
+  const T *gh = go + (int64_t)head * a.group * a.dim;
+  V8<T> kf[DP / 16], vf[DP / 16];
+  const T *krow = k + (live ? key : 0) * a.k.row + head * a.k.head;
+  const T *vrow = v + (live ? key : 0) * a.v.row + head * a.v.head;
+#pragma unroll
+  for (int i = 0; i < DP / 16; i++) {
+    kf[i] = global_frag(krow, live, 16 * i + 8 * h, a.dim);
+    vf[i] = global_frag(vrow, live, 16 * i + 8 * h, a.dim);
+  }
+  f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
+  const int begin = rows.lo * a.group, end = rows.hi * a.group;
+  dkv_walk<T, DP, false>(a, g, qh, gst, gh, head, begin, end, key0, gs, kf, vf, qs, os, s_ld, s_range, bad, dk, dv);
+  if (!(all_finite(dk) && all_finite(dv))) s_redo = 1;
+  __syncthreads();
+  if (s_redo) {
+#pragma unroll
+    for (int db = 0; db < DP / 32; db++) dk[db] = dv[db] = f32x16{};
+    dkv_walk<T, DP, true>(a, g, qh, gst, gh, head, begin, end, key0, gs, kf, vf, qs, os, s_ld, s_range, bad, dk, dv);
+  }
+  if (!live) return;
+  const int64_t at = ((int64_t)key * a.kv_heads + head) * a.dim;
+  store_cols<T, DP>(dk_out + at, dk, a.scale / gs, h, a.dim);
+  store_cols<T, DP>(dv_out + at, dv, 1.f, h, a.dim);
+}
+
+static unsigned prep_blocks(int64_t num_q, int heads) {
+  return (unsigned)std::max<int64_t>(1, std::min<int64_t>(cdiv(num_q * heads, 16), kMaxParts));
+}
+
+template <typename T, int DP>
+static int attend_backward(const Attend &a, const Grad &g, const void *q, const void *k, const void *v, const void *go,
+                           void *dq, void *dk, void *dv, hipStream_t st) {
+  if (a.nq > 0 && dq) {
+    const unsigned blocks = (unsigned)(cdiv((int64_t)a.nq * a.group, 128) * a.kv_heads);
+    hipLaunchKernelGGL((attend_dq_kernel<T, DP>), dim3(blocks), dim3(256), 0, st, a, g, (const T *)q, (const T *)k,
+                       (const T *)v, (const T *)go, (T *)dq);
+    KL_CHECK_LAUNCH();
+  }
+  if (a.nk > 0 && dk) {
+    const unsigned blocks = (unsigned)(cdiv(a.nk, 128) * a.kv_heads);
+    hipLaunchKernelGGL((attend_dkv_kernel<T, DP>), dim3(blocks), dim3(256), 0, st, a, g, (const T *)q, (const T *)k,
+                       (const T *)v, (const T *)go, (T *)dk, (T *)dv);
+    KL_CHECK_LAUNCH();
+  }
+  return KL_OK;
+}
+
+}  // namespace kl
+
+using namespace kl;
+
+extern "C" size_t kl_pack_attention_bwd_workspace_bytes(int64_t num_q, int heads) {
+  if (num_q <= 0 || heads <= 0) return 256;
+  return al256((size_t)num_q * heads * 8) + al256((size_t)num_q * 8) + kMaxParts * 4;
+}
+
+extern "C" int kl_pack_attention_backward(kl_dtype dtype, int64_t num_q, int64_t num_k, int heads, int kv_heads,
+                                          int dim, const void *grad_out, const void *q, const void *k, const void *v,
+                                          const int64_t *strides_host, const int32_t *q_ids, const int32_t *q_starts,
+                                          const int32_t *k_ids, const int32_t *k_starts, const void *out,
+                                          const float *lse, float scale, int causal, void *grad_q, void *grad_k,
+                                          void *grad_v, void *ws, size_t ws_bytes, kl_stream stream) {
+  Attend a;
+  KL_CHECK_RC(fill_attend(a, "pack_attention", num_q, num_k, heads, kv_heads, dim, strides_host, q_ids, q_starts, k_ids,
+                          k_starts, scale, causal));
+  KL_REQUIRE(ws_bytes >= kl_pack_attention_bwd_workspace_bytes(num_q, heads),
+             "pack_attention: the workspace is too small");
+  KL_REQUIRE((grad_k == nullptr) == (grad_v == nullptr), "pack_attention: grad_k and grad_v go together");
+  Grad g = {};
+  g.ld = (float2 *)ws;
+  g.range = (int2 *)((char *)ws + al256((size_t)num_q * heads * 8));
+  g.amax = (float *)((char *)g.range + al256((size_t)num_q * 8));
+  g.parts = (int)prep_blocks(num_q, heads);
+  return with_type(dtype, "pack_attention", [&](auto t) -> int {
+    using T = decltype(t);
+    if (num_q > 0) {
+      hipLaunchKernelGGL(attend_prep_kernel<T>, dim3(g.parts), dim3(256), 0, S(stream), a, (const T *)out,
+                         (const T *)grad_out, lse, (float2 *)g.ld, (int2 *)g.range, (float *)g.amax);
+      KL_CHECK_LAUNCH();
+    } else {
+      g.parts = 0;
+    }
+    return with_dim(dim, [&](auto dp) {
+      return attend_backward<T, decltype(dp)::value>(a, g, q, k, v, grad_out, grad_q, grad_k, grad_v, S(stream));
+    });
+  });
+}

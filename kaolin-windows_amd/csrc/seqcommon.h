@@ -1,0 +1,154 @@
+// seqcommon.h -- what the sequence operators over packs share: element types, vector loads, the
+// 32x32 matrix-core tiles and the pack arrays.
+//
+// Pack arrays of one boundary mask (kl_pack_layout): ids[i] = the pack of row i (-1 before the first
+// pack), starts[p] = the first row of pack p, and starts[p] = num_rows for every p past the last pack
+// up to starts[num_rows]: rows [starts[p], starts[p+1]) are pack p, also where p does not exist (none).
+#pragma once
+
+#include <hip/hip_fp16.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "common.h"
+
+namespace kl {
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef bf16_t bf16x4 __attribute__((ext_vector_type(4)));
+typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
+typedef f16_t f16x4 __attribute__((ext_vector_type(4)));
+typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// the vectors of one element type: V8 is a matrix-core operand fragment, V4 four neighbours
+template <typename T>
+struct Vec;
+template <>
+struct Vec<float> {
+  typedef f32x4 V4;
+  typedef f32x8 V8;
+};
+template <>
+struct Vec<f16_t> {
+  typedef f16x4 V4;
+  typedef f16x8 V8;
+};
+template <>
+struct Vec<bf16_t> {
+  typedef bf16x4 V4;
+  typedef bf16x8 V8;
+};
+template <typename T>
+using V4 = typename Vec<T>::V4;
+template <typename T>
+using V8 = typename Vec<T>::V8;
+
+// acc (32 x 32) += A (32 x 16) * B (16 x 32).  Lane l holds A[l % 32][8 * (l / 32) + e] and
+// B[8 * (l / 32) + e][l % 32], e = 0..7, and of acc the column l % 32 at the rows
+// 8 * (r / 4) + 4 * (l / 32) + r % 4, r = 0..15.  The sum over the 16 inner indices does not depend
+// on their order, so any permutation of them is right where A and B use the same one.
+// float has no 16-deep product: eight 2-deep ones, step e taking the inner indices e and 8 + e.
+__device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 acc) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma(f16x8 a, f16x8 b, f32x16 acc) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, acc, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma(f32x8 a, f32x8 b, f32x16 acc) {
+#pragma unroll
+  for (int e = 0; e < 8; e++) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], acc, 0, 0, 0);
+  return acc;
+}
+
+// the row of accumulator register r in lane half h, and the inner index that a fragment made of the
+// eight accumulator registers 8 * s .. 8 * s + 7 holds at element e: the same permutation
+__device__ __forceinline__ constexpr int acc_row(int r, int h) { return 8 * (r / 4) + 4 * h + r % 4; }
+
+// An accumulator half (registers 8 * s .. 8 * s + 7) as an operand: rows 16 * s .. 16 * s + 15 of acc
+// become the 16 inner indices, in the order of acc_row, with no exchange between lanes.
+template <typename T>
+__device__ __forceinline__ V8<T> acc_frag(const f32x16 &acc, int s) {
+  f32x8 v;
+#pragma unroll
+  for (int e = 0; e < 8; e++) v[e] = acc[8 * s + e];
+  return __builtin_convertvector(v, V8<T>);
+}
+
+// Row fragment of a row-major LDS tile: element e = tile[row][col + e].
+template <typename T>
+__device__ __forceinline__ V8<T> row_frag(const T *tile, int ld, int row, int col) {
+  if constexpr (sizeof(T) == 4) {
+    const f32x4 a = *reinterpret_cast<const f32x4 *>(tile + row * ld + col);
+    const f32x4 b = *reinterpret_cast<const f32x4 *>(tile + row * ld + col + 4);
+    return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+  } else {
+    return *reinterpret_cast<const V8<T> *>(tile + row * ld + col);
+  }
+}
+
+// Column fragment: element e = tile[row0 + acc_row(e, h)][col0 + l % 32], the A operand of the
+// transposed tile whose inner indices are in the order of acc_frag.  16-bit types: the transposed LDS
+// read gives lane i of 16 the column i of a 4 x 16 block whose rows four lanes each address, which is
+// just the run of four rows that acc_row holds together.
+template <typename T>
+__device__ __forceinline__ V8<T> col_frag(T *tile, int ld, int row0, int col0) {
+  const int l = threadIdx.x & 63, h = l >> 5;
+  if constexpr (sizeof(T) == 4) {
+    f32x8 v;
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = tile[(row0 + acc_row(e, h)) * ld + col0 + (l & 31)];
+    return v;
+  } else {
+    const int i = l & 15;
+    T *p = tile + (row0 + 4 * h + i / 4) * ld + col0 + (l & 16) + (i & 3) * 4;
+    typedef __attribute__((address_space(3))) i16x4 lds4;
+    union {
+      i16x4 u[2];
+      V8<T> v;
+    } x;
+    x.u[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(p));
+    x.u[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(p + 8 * ld));
+    return x.v;
+  }
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float log2_fast(float x) { return __builtin_amdgcn_logf(x); }
+constexpr float kLog2e = 1.44269504088896340736f;
+
+__device__ __forceinline__ bool finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
+
+// the other half's value of the same column: lanes l and l ^ 32
+__device__ __forceinline__ float half_swap(float v) { return __shfl_xor(v, 32); }
+
+// Strided heads: element (row, head, i) of a (rows, heads, dim) tensor lies at row * row_stride +
+// head * head_stride + i.
+struct Heads {
+  int64_t row, head;
+};
+
+// any element of a 16-byte piece that is an infinity or a NaN
+template <typename T>
+__device__ __forceinline__ bool piece_bad(u32x4 w) {
+  uint32_t bad = 0;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    if constexpr (sizeof(T) == 4) {
+      bad |= (w[i] & 0x7f800000u) == 0x7f800000u;
+    } else {
+      constexpr uint32_t m = std::is_same<T, bf16_t>::value ? 0x7f80u : 0x7c00u;
+      bad |= (w[i] & m) == m;
+      bad |= (w[i] & (m << 16)) == (m << 16);
+    }
+  }
+  return bad != 0;
+}
+
+}  // namespace kl

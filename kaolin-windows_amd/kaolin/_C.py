@@ -13,6 +13,7 @@ import types
 import torch
 
 from . import _native as N
+from . import _sequence
 from ._checks import (Arg, check_all_same_gpu, check_contiguous, check_dim, check_same_size, check_same_type,
                       check_size, check_size_dim)
 
@@ -910,7 +911,9 @@ render.spc = _module('kaolin._C.render.spc', raytrace_cuda=raytrace_cuda, raytra
                      generate_shadow_rays_cuda=generate_shadow_rays_cuda,
                      mark_pack_boundaries_cuda=mark_pack_boundaries_cuda, diff_cuda=diff_cuda,
                      inclusive_sum_cuda=inclusive_sum_cuda, sum_reduce_cuda=sum_reduce_cuda,
-                     cumsum_cuda=cumsum_cuda, cumprod_cuda=cumprod_cuda)
+                     cumsum_cuda=cumsum_cuda, cumprod_cuda=cumprod_cuda, pack_layout_cuda=_sequence.pack_layout_cuda,
+                     pack_attention_forward_cuda=_sequence.pack_attention_forward_cuda,
+                     pack_attention_backward_cuda=_sequence.pack_attention_backward_cuda)
 metrics = _module('kaolin._C.metrics', sided_distance_forward_cuda=sided_distance_forward_cuda,
                   sided_distance_backward_cuda=sided_distance_backward_cuda,
                   unbatched_triangle_distance_forward_cuda=unbatched_triangle_distance_forward_cuda,

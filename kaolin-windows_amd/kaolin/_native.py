@@ -16,7 +16,7 @@ LIB_PATH = os.environ.get('KAOLIN_HIP_LIB') or os.path.join(_LIB_DIR, 'libkaolin
 
 ABI_VERSION = 4  # include/kaolin_hip.h KL_ABI_VERSION: the signatures below
 
-KL_F32, KL_F64, KL_F16, KL_U8, KL_I8, KL_I16, KL_I32, KL_I64 = range(8)
+KL_F32, KL_F64, KL_F16, KL_U8, KL_I8, KL_I16, KL_I32, KL_I64, KL_BF16 = range(9)
 _DTYPES = {
     torch.float32: KL_F32, torch.float64: KL_F64, torch.float16: KL_F16, torch.uint8: KL_U8,
     torch.int8: KL_I8, torch.int16: KL_I16, torch.int32: KL_I32, torch.int64: KL_I64,
@@ -111,6 +111,14 @@ _SIGS = {
     'kl_inclusive_sum_workspace_bytes': (_SZ, [_I64]),
     'kl_inclusive_sum_i32': (_I, [_I64, _P, _P, _P, _SZ, _P]),
     'kl_sum_reduce': (_I, [_I, _I64, _I64, _P, _P, _I64, _P, _P]),
+    'kl_pack_layout_workspace_bytes': (_SZ, [_I64]),
+    'kl_pack_layout': (_I, [_I64, _P, _P, _P, _P, _SZ, _P]),
+    'kl_pack_attention_workspace_bytes': (_SZ, [_I, _I64, _I64, _I, _I, _I]),
+    'kl_pack_attention_forward': (_I, [_I, _I64, _I64, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _F, _I, _P, _P, _P,
+                                       _SZ, _P]),
+    'kl_pack_attention_bwd_workspace_bytes': (_SZ, [_I64, _I]),
+    'kl_pack_attention_backward': (_I, [_I, _I64, _I64, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _F, _I,
+                                        _P, _P, _P, _P, _SZ, _P]),
     'kl_deftet_workspace_bytes': (_SZ, [_I64, _I64]),
     'kl_deftet_sparse_render_forward': (_I, [_I, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P, _F, _P, _P, _P, _P,
                                              _P, _SZ, ALLOC_FN, _P, _P]),
