@@ -565,6 +565,41 @@ int kl_pack_attention_backward(kl_dtype dtype, int64_t num_q, int64_t num_k, int
                                float scale, int causal, void *grad_q, void *grad_k, void *grad_v, void *workspace,
                                size_t workspace_bytes, kl_stream stream);
 
+/* RMS norm of each head of q (num_rows, q_heads, dim) and k (num_rows, k_heads, dim), then the rotation of the
+ * first `turn` elements of each by angle positions[row] * freqs[pair] (freqs: turn / 2 doubles; pairs (2 i,
+ * 2 i + 1) if interleaved, else (i, i + turn / 2)).  f16 / bf16 / f32; dim a multiple of 8 up to 256; strides_host:
+ * the row and head strides of q and of k, in elements; every row of a head starts at a multiple of 16 bytes.
+ * Weights (dim), in the dtype or, with weight_f32, float; NULL: ones.  pos_kind: 0 the row's place in its pack
+ * (ids, starts: kl_pack_layout; 0 for rows of no pack), 1 / 2 / 3 positions (num_rows) int32 / int64 / float.
+ * Outputs and gradients are contiguous and fully written; a weight's gradient may be NULL. */
+int kl_norm_rotary_forward(kl_dtype dtype, int64_t num_rows, int q_heads, int k_heads, int dim, int turn,
+                           int interleaved, const void *q, const void *k, const int64_t *strides_host,
+                           const void *q_weight, const void *k_weight, int weight_f32, const double *freqs,
+                           int pos_kind, const void *positions, const int32_t *ids, const int32_t *starts, float eps,
+                           void *out_q, void *out_k, kl_stream stream);
+size_t kl_norm_rotary_bwd_workspace_bytes(int dim);
+int kl_norm_rotary_backward(kl_dtype dtype, int64_t num_rows, int q_heads, int k_heads, int dim, int turn,
+                            int interleaved, const void *grad_q_out, const void *grad_k_out, const void *q,
+                            const void *k, const int64_t *strides_host, const void *q_weight, const void *k_weight,
+                            int weight_f32, const double *freqs, int pos_kind, const void *positions,
+                            const int32_t *ids, const int32_t *starts, float eps, void *grad_q, void *grad_k,
+                            void *grad_q_weight, void *grad_k_weight, void *workspace, size_t workspace_bytes,
+                            kl_stream stream);
+
+/* out[t] = gates[t] * out[t - 1] + feats[t] down each pack and column of (num_rows, dim), f16 / bf16 / f32 / f64;
+ * out before a pack's first row is initial[pack] (num_initial, dim), 0 where initial is NULL or has no such row;
+ * reverse: out[t + 1] and the pack's last row.  Rows of no pack are 0.  The backward takes the forward's out and
+ * writes every element of grad_gates, grad_feats and (with initial) grad_initial (may be NULL). */
+size_t kl_linear_recurrence_workspace_bytes(kl_dtype dtype, int64_t num_rows, int64_t dim);
+int kl_linear_recurrence_forward(kl_dtype dtype, int64_t num_rows, int64_t dim, const void *gates, const void *feats,
+                                 const void *initial, int64_t num_initial, const int32_t *ids, const int32_t *starts,
+                                 int reverse, void *out, void *workspace, size_t workspace_bytes, kl_stream stream);
+int kl_linear_recurrence_backward(kl_dtype dtype, int64_t num_rows, int64_t dim, const void *grad_out,
+                                  const void *gates, const void *out, const void *initial, int64_t num_initial,
+                                  const int32_t *ids, const int32_t *starts, int reverse, void *grad_gates,
+                                  void *grad_feats, void *grad_initial, void *workspace, size_t workspace_bytes,
+                                  kl_stream stream);
+
 /* ------------------------------------------------------------ check_sign */
 
 /* mesh_intersection.cpp:33-68  unbatched_mesh_intersection_cuda (kernel

@@ -163,16 +163,6 @@ int with_dim(int dim, F f) {
   if (dim <= 64) return f(std::integral_constant<int, 64>());
   return f(std::integral_constant<int, 128>());
 }
-template <typename F>
-int with_type(kl_dtype dtype, const char *func, F f) {
-  switch (dtype) {
-    case KL_F32: return f(float());
-    case KL_F16: return f(f16_t());
-    case KL_BF16: return f(bf16_t());
-    default: set_error(std::string(func) + ": expected a Half, BFloat16 or Float tensor"); return KL_E_INVALID;
-  }
-}
-
 // Checks an Attend's sizes and fills it.  dim: a multiple of 8 up to 128, so rows are whole 16-byte pieces.
 int fill_attend(Attend &a, const char *func, int64_t nq, int64_t nk, int heads, int kv_heads, int dim,
                 const int64_t *strides, const int32_t *qid, const int32_t *qstart, const int32_t *kid,

@@ -151,4 +151,15 @@ __device__ __forceinline__ bool piece_bad(u32x4 w) {
   return bad != 0;
 }
 
+// f(T()) for the element type of a tensor
+template <typename F>
+inline int with_type(kl_dtype dtype, const char *func, F f) {
+  switch (dtype) {
+    case KL_F32: return f(float());
+    case KL_F16: return f(f16_t());
+    case KL_BF16: return f(bf16_t());
+    default: set_error(std::string(func) + ": expected a Half, BFloat16 or Float tensor"); return KL_E_INVALID;
+  }
+}
+
 }  // namespace kl

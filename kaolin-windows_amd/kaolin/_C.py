@@ -913,7 +913,11 @@ render.spc = _module('kaolin._C.render.spc', raytrace_cuda=raytrace_cuda, raytra
                      inclusive_sum_cuda=inclusive_sum_cuda, sum_reduce_cuda=sum_reduce_cuda,
                      cumsum_cuda=cumsum_cuda, cumprod_cuda=cumprod_cuda, pack_layout_cuda=_sequence.pack_layout_cuda,
                      pack_attention_forward_cuda=_sequence.pack_attention_forward_cuda,
-                     pack_attention_backward_cuda=_sequence.pack_attention_backward_cuda)
+                     pack_attention_backward_cuda=_sequence.pack_attention_backward_cuda,
+                     norm_rotary_forward_cuda=_sequence.norm_rotary_forward_cuda,
+                     norm_rotary_backward_cuda=_sequence.norm_rotary_backward_cuda,
+                     linear_recurrence_forward_cuda=_sequence.linear_recurrence_forward_cuda,
+                     linear_recurrence_backward_cuda=_sequence.linear_recurrence_backward_cuda)
 metrics = _module('kaolin._C.metrics', sided_distance_forward_cuda=sided_distance_forward_cuda,
                   sided_distance_backward_cuda=sided_distance_backward_cuda,
                   unbatched_triangle_distance_forward_cuda=unbatched_triangle_distance_forward_cuda,

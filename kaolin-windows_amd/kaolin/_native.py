@@ -119,6 +119,14 @@ _SIGS = {
     'kl_pack_attention_bwd_workspace_bytes': (_SZ, [_I64, _I]),
     'kl_pack_attention_backward': (_I, [_I, _I64, _I64, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _F, _I,
                                         _P, _P, _P, _P, _SZ, _P]),
+    'kl_norm_rotary_forward': (_I, [_I, _I64, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _I, _P, _I, _P, _P, _P, _F, _P, _P,
+                                    _P]),
+    'kl_norm_rotary_bwd_workspace_bytes': (_SZ, [_I]),
+    'kl_norm_rotary_backward': (_I, [_I, _I64, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _I, _P, _I, _P, _P, _P, _F,
+                                     _P, _P, _P, _P, _P, _SZ, _P]),
+    'kl_linear_recurrence_workspace_bytes': (_SZ, [_I, _I64, _I64]),
+    'kl_linear_recurrence_forward': (_I, [_I, _I64, _I64, _P, _P, _P, _I64, _P, _P, _I, _P, _P, _SZ, _P]),
+    'kl_linear_recurrence_backward': (_I, [_I, _I64, _I64, _P, _P, _P, _P, _I64, _P, _P, _I, _P, _P, _P, _P, _SZ, _P]),
     'kl_deftet_workspace_bytes': (_SZ, [_I64, _I64]),
     'kl_deftet_sparse_render_forward': (_I, [_I, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P, _F, _P, _P, _P, _P,
                                              _P, _SZ, ALLOC_FN, _P, _P]),

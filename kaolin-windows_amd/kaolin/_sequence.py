@@ -1,5 +1,5 @@
 """``_C.render.spc`` entries of the sequence operators over packs (csrc/packs.hip, attend.hip,
-attendgrad.hip): argument checks, outputs and one library call each.  The reference has none of
+attendgrad.hip, normrotary.hip, recurrence.hip): argument checks, outputs and one library call each.  The reference has none of
 these; they follow its packed ray ops' conventions (rows grouped by a boundary mask)."""
 import ctypes
 import math
@@ -7,7 +7,8 @@ import math
 import torch
 
 from . import _native as N
-from ._checks import Arg, check_all_same_gpu, check_contiguous, check_dim, check_same_size, check_same_type, check_size
+from ._checks import (Arg, check_all_same_gpu, check_contiguous, check_dim, check_same_size, check_same_type,
+                      check_size, check_size_dim)
 
 _NAMES = {torch.float16: 'Half', torch.bfloat16: 'BFloat16', torch.float32: 'Float', torch.float64: 'Double',
           torch.bool: 'Bool', torch.uint8: 'Byte', torch.int32: 'Int', torch.int64: 'Long'}
@@ -139,3 +140,159 @@ def pack_attention_backward_cuda(grad_out, q, k, v, q_layout, k_layout, out, lse
             N.ptr(k_layout[0]), N.ptr(k_layout[1]), N.ptr(out), N.ptr(lse), scale, int(causal), N.ptr(dq), N.ptr(dk),
             N.ptr(dv), N.ptr(ws), ws_bytes, N.stream_of(dev)), func)
     return dq, dk, dv
+
+
+_POSITIONS = {torch.int32: 1, torch.int64: 2, torch.float32: 3}
+
+
+def _norm_args(func, q, k, q_weight, k_weight, freqs, layout, positions, eps):
+    """Checks; returns q, k as the kernels read them and the arguments from the strides to eps."""
+    aq, ak, af = Arg(q, 'q', 1), Arg(k, 'k', 2), Arg(freqs, 'freqs', 5)
+    check_dim(func, aq, 3)
+    check_dim(func, ak, 3)
+    check_all_same_gpu(func, [aq, ak, af])
+    check_type(func, aq, _FLOATS)
+    check_same_type(func, ak, aq)
+    n, dim = q.shape[0], q.shape[2]
+    check_rows(func, n)
+    if k.shape[0] != n or k.shape[2] != dim:
+        raise RuntimeError(f'{func}: q and k must have the same rows and head size; got {tuple(q.shape)} and '
+                           f'{tuple(k.shape)}')
+    if dim % 8 or not 0 < dim <= 256:
+        raise RuntimeError(f'{func}: the head size must be a multiple of 8 up to 256; got {dim}')
+    if q.shape[1] + k.shape[1] > 1 << 16:
+        raise RuntimeError(f'{func}: at most 65536 heads; got {q.shape[1]} and {k.shape[1]}')
+    check_dim(func, af, 1)
+    check_type(func, af, (torch.float64,))
+    check_contiguous(func, [af])
+    if 2 * freqs.shape[0] > dim:
+        raise RuntimeError(f'{func}: {freqs.shape[0]} pairs do not fit a head of {dim}')
+    if not (eps >= 0 and math.isfinite(eps)):
+        raise RuntimeError(f'{func}: eps must not be negative; got {eps}')
+    kinds = set()
+    for i, (w, name) in enumerate(((q_weight, 'q_weight'), (k_weight, 'k_weight'))):
+        if w is not None:
+            a = Arg(w, name, 3 + i)
+            check_size(func, a, (dim,))
+            check_all_same_gpu(func, [aq, a])
+            check_type(func, a, (q.dtype,) if q.dtype == torch.float32 else (q.dtype, torch.float32))
+            check_contiguous(func, [a])
+            kinds.add(w.dtype)
+    if len(kinds) > 1:
+        raise RuntimeError(f'{func}: the weights must have one type')
+    kind, ids, starts = 0, None, None
+    if positions is not None:
+        ap = Arg(positions, 'positions', 7)
+        check_size(func, ap, (n,))
+        check_all_same_gpu(func, [aq, ap])
+        check_type(func, ap, tuple(_POSITIONS))
+        check_contiguous(func, [ap])
+        kind = _POSITIONS[positions.dtype]
+    else:
+        ids, starts = layout
+        for t, name, size in ((ids, 'ids', n), (starts, 'starts', n + 1)):
+            a = Arg(t, name, 6)
+            check_size(func, a, (size,))
+            check_type(func, a, (torch.int32,))
+            check_all_same_gpu(func, [aq, a])
+            check_contiguous(func, [a])
+    q, k = usable_heads(q), usable_heads(k)
+    strides = (ctypes.c_int64 * 4)(q.stride(0), q.stride(1), k.stride(0), k.stride(1))
+    return q, k, (strides, N.ptr(q_weight), N.ptr(k_weight), int(kinds == {torch.float32}), N.ptr(freqs), kind,
+                  N.ptr(positions), N.ptr(ids), N.ptr(starts), eps)
+
+
+def norm_rotary_forward_cuda(q, k, q_weight, k_weight, freqs, layout, positions, eps, interleaved):
+    """The normed and rotated q and k, contiguous."""
+    func = 'norm_rotary_forward_cuda'
+    q, k, rest = _norm_args(func, q, k, q_weight, k_weight, freqs, layout, positions, eps)
+    dev = q.device
+    yq, yk = (torch.empty(x.shape, dtype=x.dtype, device=dev) for x in (q, k))
+    with N.on_device(dev):
+        N.check(N.lib().kl_norm_rotary_forward(
+            _CODES[q.dtype], q.shape[0], q.shape[1], k.shape[1], q.shape[2], 2 * freqs.shape[0], int(interleaved),
+            N.ptr(q), N.ptr(k), *rest, N.ptr(yq), N.ptr(yk), N.stream_of(dev)), func)
+    return yq, yk
+
+
+def norm_rotary_backward_cuda(grad_q_out, grad_k_out, q, k, q_weight, k_weight, freqs, layout, positions, eps,
+                              interleaved, need_weights):
+    """The gradients of q, k and of the weights (None where a weight is None or, without need_weights)."""
+    func = 'norm_rotary_backward_cuda'
+    q, k, rest = _norm_args(func, q, k, q_weight, k_weight, freqs, layout, positions, eps)
+    gq, gk = usable_heads(grad_q_out.contiguous()), usable_heads(grad_k_out.contiguous())
+    for g, x, name in ((gq, q, 'grad_q_out'), (gk, k, 'grad_k_out')):
+        check_same_size(func, Arg(g, name, 0), Arg(x, name[5], 0))
+        check_same_type(func, Arg(g, name, 0), Arg(x, name[5], 0))
+        check_all_same_gpu(func, [Arg(q, 'q', 1), Arg(g, name, 0)])
+    dev = q.device
+    dq, dk = (torch.empty(x.shape, dtype=x.dtype, device=dev) for x in (q, k))
+    dqw, dkw = (torch.empty_like(w) if w is not None and need_weights else None for w in (q_weight, k_weight))
+    with N.on_device(dev):
+        ws_bytes = N.size('kl_norm_rotary_bwd_workspace_bytes', q.shape[2])
+        ws = N.workspace(ws_bytes, dev)
+        N.check(N.lib().kl_norm_rotary_backward(
+            _CODES[q.dtype], q.shape[0], q.shape[1], k.shape[1], q.shape[2], 2 * freqs.shape[0], int(interleaved),
+            N.ptr(gq), N.ptr(gk), N.ptr(q), N.ptr(k), *rest, N.ptr(dq), N.ptr(dk), N.ptr(dqw), N.ptr(dkw), N.ptr(ws),
+            ws_bytes, N.stream_of(dev)), func)
+    return dq, dk, dqw, dkw
+
+
+def _recurrence_args(func, gates, other, name, initial, layout):
+    ag, ao = Arg(gates, 'gates', 1), Arg(other, name, 2)
+    check_dim(func, ag, 2)
+    check_same_size(func, ao, ag)
+    args = [ag, ao]
+    if initial is not None:
+        ai = Arg(initial, 'initial', 4)
+        check_dim(func, ai, 2)
+        check_size_dim(func, ai, 1, gates.shape[1])
+        args.append(ai)
+    check_all_same_gpu(func, args)
+    check_contiguous(func, args)
+    check_type(func, ag, (torch.float16, torch.bfloat16, torch.float32, torch.float64))
+    for a in args[1:]:
+        check_same_type(func, a, ag)
+    n, dim = gates.shape
+    check_rows(func, n)
+    if dim >= 1 << 24 or (initial is not None and initial.shape[0] >= 1 << 31):
+        raise RuntimeError(f'{func}: sizes out of range: {tuple(gates.shape)}')
+    for t, what, size in zip(layout, ('ids', 'starts'), (n, n + 1)):
+        a = Arg(t, what, 3)
+        check_size(func, a, (size,))
+        check_type(func, a, (torch.int32,))
+        check_all_same_gpu(func, [ag, a])
+        check_contiguous(func, [a])
+
+
+def linear_recurrence_forward_cuda(gates, feats, layout, initial, reverse):
+    """h[t] = gates[t] h[t - 1] + feats[t] along each pack."""
+    func = 'linear_recurrence_forward_cuda'
+    _recurrence_args(func, gates, feats, 'feats', initial, layout)
+    dev, (n, dim), code = gates.device, gates.shape, _CODES[gates.dtype]
+    out = torch.empty_like(gates)
+    with N.on_device(dev):
+        ws_bytes = N.size('kl_linear_recurrence_workspace_bytes', code, n, dim)
+        ws = N.workspace(ws_bytes, dev)
+        N.check(N.lib().kl_linear_recurrence_forward(
+            code, n, dim, N.ptr(gates), N.ptr(feats), N.ptr(initial), 0 if initial is None else initial.shape[0],
+            N.ptr(layout[0]), N.ptr(layout[1]), int(reverse), N.ptr(out), N.ptr(ws), ws_bytes, N.stream_of(dev)), func)
+    return out
+
+
+def linear_recurrence_backward_cuda(grad_out, gates, out, layout, initial, reverse):
+    """The gradients of gates, feats and initial (None without it)."""
+    func = 'linear_recurrence_backward_cuda'
+    _recurrence_args(func, gates, grad_out, 'grad_out', initial, layout)
+    _recurrence_args(func, gates, out, 'out', initial, layout)
+    dev, (n, dim), code = gates.device, gates.shape, _CODES[gates.dtype]
+    da, db = torch.empty_like(gates), torch.empty_like(gates)
+    di = torch.empty_like(initial) if initial is not None else None
+    with N.on_device(dev):
+        ws_bytes = N.size('kl_linear_recurrence_workspace_bytes', code, n, dim)
+        ws = N.workspace(ws_bytes, dev)
+        N.check(N.lib().kl_linear_recurrence_backward(
+            code, n, dim, N.ptr(grad_out), N.ptr(gates), N.ptr(out), N.ptr(initial),
+            0 if initial is None else initial.shape[0], N.ptr(layout[0]), N.ptr(layout[1]), int(reverse), N.ptr(da),
+            N.ptr(db), N.ptr(di), N.ptr(ws), ws_bytes, N.stream_of(dev)), func)
+    return da, db, di
