@@ -545,24 +545,25 @@ int kl_pack_layout(int64_t num_rows, const uint8_t *boundaries, int32_t *ids, in
  * multiple of kv_heads (query head h reads key head h / (heads / kv_heads)), dim a multiple of 8 up to 128;
  * f16 / bf16 / f32.  strides_host: the row and head strides of q, k, v in elements (q row, q head, k row, k
  * head, v row, v head); every row of a head starts at a multiple of 16 bytes.  out (num_q, heads, dim) and
- * lse (num_q, heads) f32 are contiguous; lse (base-2 logarithm of the softmax's sum, what the backward
- * takes) may be NULL. */
+ * lse (num_q, heads) f32 are contiguous; lse (base-2 logarithm of the softmax's sum) and out_low (as
+ * out: what its rounding left out; f16 and bf16) are for the backward, and may be NULL. */
 size_t kl_pack_attention_workspace_bytes(kl_dtype dtype, int64_t num_q, int64_t num_k, int heads, int kv_heads,
                                          int dim);
 int kl_pack_attention_forward(kl_dtype dtype, int64_t num_q, int64_t num_k, int heads, int kv_heads, int dim,
                               const void *q, const void *k, const void *v, const int64_t *strides_host,
                               const int32_t *q_ids, const int32_t *q_starts, const int32_t *k_ids,
-                              const int32_t *k_starts, float scale, int causal, void *out, float *lse,
-                              void *workspace, size_t workspace_bytes, kl_stream stream);
-/* Its gradients: grad_out, out (num_q, heads, dim) contiguous and 16-byte aligned; grad_q as q and grad_k,
+                              const int32_t *k_starts, float scale, int causal, void *out, void *out_low,
+                              float *lse, void *workspace, size_t workspace_bytes, kl_stream stream);
+/* Its gradients: grad_out, out, out_low (num_q, heads, dim; out_low may be NULL) contiguous and 16-byte aligned; grad_q as q and grad_k,
  * grad_v as k and v, contiguous, fully written (grad_q, or grad_k with grad_v, may be NULL).  Every sum has a
  * fixed order. */
-size_t kl_pack_attention_bwd_workspace_bytes(int64_t num_q, int heads);
+size_t kl_pack_attention_bwd_workspace_bytes(kl_dtype dtype, int64_t num_q, int64_t num_k, int heads, int kv_heads,
+                                             int dim);
 int kl_pack_attention_backward(kl_dtype dtype, int64_t num_q, int64_t num_k, int heads, int kv_heads, int dim,
                                const void *grad_out, const void *q, const void *k, const void *v,
                                const int64_t *strides_host, const int32_t *q_ids, const int32_t *q_starts,
-                               const int32_t *k_ids, const int32_t *k_starts, const void *out, const float *lse,
-                               float scale, int causal, void *grad_q, void *grad_k, void *grad_v, void *workspace,
+                               const int32_t *k_ids, const int32_t *k_starts, const void *out, const void *out_low,
+                               const float *lse, float scale, int causal, void *grad_q, void *grad_k, void *grad_v, void *workspace,
                                size_t workspace_bytes, kl_stream stream);
 
 /* RMS norm of each head of q (num_rows, q_heads, dim) and k (num_rows, k_heads, dim), then the rotation of the

@@ -6,6 +6,8 @@
 // computed transposed, S^T = K Q^T, so a lane holds one row's scores: the softmax is lane-local but for one
 // exchange with the other half, and the weights are the second product's operand (O^T = V^T P^T) where
 // they lie, without a trip through LDS (seqcommon.h, acc_frag).
+// low (training, 16-bit types): what the rounding of o left out, so that the backward's sums over do . o,
+// which cancel against other terms, have o to twice its bits.
 // Rounding: weights are in [0, 1] and are rounded to the inputs' type for the second product (off by at
 // most half a step each, and averaged over the keys; float stays float); the sum they are divided by is
 // taken before the rounding, in 32 bits.
@@ -131,7 +133,8 @@ __device__ __forceinline__ void fwd_walk(const Attend &a, const T *__restrict__ 
 template <typename T, int DP>
 __global__ void __launch_bounds__(256, 2) attend_fwd_kernel(Attend a, const T *__restrict__ q, const T *__restrict__ k,
                                                          const T *__restrict__ v, T *__restrict__ o,
-                                                         float *__restrict__ lse, float *__restrict__ part,
+                                                         T *__restrict__ low, float *__restrict__ lse,
+                                                         float *__restrict__ part,
                                                          float2 *__restrict__ stat) {
   constexpr int BM = FwdTile<T, DP>::BM, BN = FwdTile<T, DP>::BN;
   using KV = Stage<T, DP, BN>;
@@ -187,46 +190,91 @@ __global__ void __launch_bounds__(256, 2) attend_fwd_kernel(Attend a, const T *_
     if (st.m != -INFINITY || l != 0) store_cols<float, DP>(part + at * a.dim, acc, 1.f, h, a.dim);
     return;
   }
-  // a row that sees no key: 0
-  store_cols<T, DP>(o + ((int64_t)row * a.kv_heads * a.group + qhead) * a.dim, acc, l == 0 ? 0.f : 1.f / l, h, a.dim);
-  if (lse && h == 0) lse[(int64_t)row * a.kv_heads * a.group + qhead] = l == 0 ? 0.f : st.m + log2_fast(l);
-}
-
-// The splits of one (key head, virtual row) joined: eight elements a thread.
-template <typename T>
-__global__ void __launch_bounds__(256) attend_join_kernel(Attend a, int splits, const float *__restrict__ part,
-                                                        const float2 *__restrict__ stat, T *__restrict__ o,
-                                                        float *__restrict__ lse) {
-  const int64_t total = (int64_t)a.nq * a.group, rows = total * a.kv_heads;
-  const int per = a.dim / 8;
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t at = t / per;
-  if (at >= rows) return;
-  const int d = (int)(t % per) * 8, head = (int)(at / total);
-  const int64_t m = at % total;
-  float top = -INFINITY;
-  for (int s = 0; s < splits; s++) top = fmaxf(top, stat[s * rows + at].x);
-  const float base = top == -INFINITY ? 0.f : top;
-  float l = 0;
-  f32x8 sum = {};
-  for (int s = 0; s < splits; s++) {
-    const float2 x = stat[s * rows + at];
-    if (x.x == -INFINITY && x.y == 0) continue;  // no key of the row in this split
-    const float w = exp2_fast(x.x - base);
-    l = fmaf(w, x.y, l);
-    const f32x4 *p = reinterpret_cast<const f32x4 *>(part + (s * rows + at) * a.dim + d);
-    const f32x4 u0 = p[0], u1 = p[1];
+  const int64_t at = (int64_t)row * a.kv_heads * a.group + qhead;
+  const float w = l == 0 ? 0.f : 1.f / l;  // a row that sees no key: 0
+  store_cols<T, DP>(o + at * a.dim, acc, w, h, a.dim);
+  if constexpr (sizeof(T) == 2) {
+    if (low) {
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-      sum[e] = fmaf(w, u0[e], sum[e]);
-      sum[4 + e] = fmaf(w, u1[e], sum[4 + e]);
+      for (int db = 0; db < DP / 32; db++) {
+#pragma unroll
+        for (int r = 0; r < 16; r++) acc[db][r] = acc[db][r] * w - (float)(T)(acc[db][r] * w);
+      }
+      store_cols<T, DP>(low + at * a.dim, acc, 1.f, h, a.dim);
     }
   }
+  if (lse && h == 0) lse[at] = l == 0 ? 0.f : st.m + log2_fast(l);
+}
+
+// The splits of one (key head, virtual row) joined: `lanes` threads of eight elements (a power of two), and
+// `shares` of them that take every shares-th split, for each of 256 / (lanes * shares) rows.
+constexpr int kMaxSplits = 128;
+template <typename T>
+__global__ void __launch_bounds__(256) attend_join_kernel(Attend a, int splits, int lanes, int shares,
+                                                        const float *__restrict__ part, const float2 *__restrict__ stat,
+                                                        T *__restrict__ o, T *__restrict__ low,
+                                                        float *__restrict__ lse) {
+  __shared__ float s_w[256 + kMaxSplits];  // weights of this workgroup's rows: rows * splits <= 256 or one row
+  __shared__ float s_sum[256 * 8];
+  const int64_t total = (int64_t)a.nq * a.group, rows = total * a.kv_heads;
+  const int per = lanes * shares, here = 256 / per;
+  const int mine = threadIdx.x / per, lane = threadIdx.x % lanes, share = threadIdx.x / lanes % shares;
+  const int64_t at = (int64_t)blockIdx.x * here + mine;
+  const int d = lane * 8;
+  const bool live = at < rows;
+  float top = -INFINITY, l = 0;
+  if (live) {
+    for (int s = threadIdx.x % per; s < splits; s += per) s_w[mine * splits + s] = stat[s * rows + at].x;
+  }
+  __syncthreads();
+  if (live) {
+    for (int s = 0; s < splits; s++) top = fmaxf(top, s_w[mine * splits + s]);
+  }
+  const float base = top == -INFINITY ? 0.f : top;
+  f32x8 sum = {};
+  if (live) {
+    for (int s = share; s < splits; s += shares) {
+      const float2 x = stat[s * rows + at];
+      if (x.x == -INFINITY && x.y == 0) continue;  // no key of the row in this split
+      const float w = exp2_fast(x.x - base);
+      l = fmaf(w, x.y, l);
+      if (d < a.dim) {
+        const f32x4 *p = reinterpret_cast<const f32x4 *>(part + (s * rows + at) * a.dim + d);
+        const f32x4 u0 = p[0], u1 = p[1];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          sum[e] = fmaf(w, u0[e], sum[e]);
+          sum[4 + e] = fmaf(w, u1[e], sum[4 + e]);
+        }
+      }
+    }
+  }
+  // the shares' sums, in their order
+  __syncthreads();
+  s_w[threadIdx.x] = l;
+#pragma unroll
+  for (int e = 0; e < 8; e++) s_sum[e * 256 + threadIdx.x] = sum[e];
+  __syncthreads();
+  if (!live || share > 0) return;
+  for (int s = 1; s < shares; s++) {
+    l += s_w[threadIdx.x + s * lanes];
+#pragma unroll
+    for (int e = 0; e < 8; e++) sum[e] += s_sum[e * 256 + threadIdx.x + s * lanes];
+  }
+  if (d >= a.dim) return;
+  const int head = (int)(at / total);
+  const int64_t m = at % total;
   const int64_t out = m / a.group * a.kv_heads * a.group + head * a.group + m % a.group;
   const float inv = l == 0 ? 0.f : 1.f / l;
 #pragma unroll
   for (int e = 0; e < 8; e++) sum[e] *= inv;
-  *reinterpret_cast<V8<T> *>(o + out * a.dim + d) = __builtin_convertvector(sum, V8<T>);
+  const V8<T> y = __builtin_convertvector(sum, V8<T>);
+  *reinterpret_cast<V8<T> *>(o + out * a.dim + d) = y;
+  if (low) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) sum[e] -= (float)y[e];
+    *reinterpret_cast<V8<T> *>(low + out * a.dim + d) = __builtin_convertvector(sum, V8<T>);
+  }
   if (lse && d == 0) lse[out] = l == 0 ? 0.f : top + log2_fast(l);
 }
 
@@ -235,7 +283,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(Attend a, int splits, 
 static int attend_splits(int64_t nq, int64_t nk, int kv_heads, int group, int bn) {
   const int64_t blocks = cdiv(nq * group, 128) * kv_heads;
   if (blocks >= 512) return 1;
-  return (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(1024, std::max<int64_t>(blocks, 1)), cdiv(nk, 2 * bn), 128}));
+  return (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(1024, std::max<int64_t>(blocks, 1)), cdiv(nk, 2 * bn), kMaxSplits}));
 }
 
 int fill_attend(Attend &a, const char *func, int64_t nq, int64_t nk, int heads, int kv_heads, int dim,
@@ -271,19 +319,22 @@ int fill_attend(Attend &a, const char *func, int64_t nq, int64_t nk, int heads, 
 }
 
 template <typename T, int DP>
-static int attend_forward(const Attend &a, const void *q, const void *k, const void *v, void *o, float *lse, void *ws,
-                          hipStream_t st) {
+static int attend_forward(const Attend &a, const void *q, const void *k, const void *v, void *o, void *low, float *lse,
+                          void *ws, hipStream_t st) {
   const int splits = attend_splits(a.nq, a.nk, a.kv_heads, a.group, FwdTile<T, DP>::BN);
   const int64_t total = (int64_t)a.nq * a.group, rows = total * a.kv_heads;
   const unsigned blocks = (unsigned)(cdiv(total, FwdTile<T, DP>::BM) * a.kv_heads);
   float2 *stat = splits > 1 ? (float2 *)ws : nullptr;
   float *part = splits > 1 ? (float *)((char *)ws + al256((size_t)splits * rows * 8)) : nullptr;
   hipLaunchKernelGGL((attend_fwd_kernel<T, DP>), dim3(blocks, splits), dim3(256), 0, st, a, (const T *)q, (const T *)k,
-                     (const T *)v, (T *)o, lse, part, stat);
+                     (const T *)v, (T *)o, (T *)low, lse, part, stat);
   KL_CHECK_LAUNCH();
   if (splits > 1) {
-    hipLaunchKernelGGL(attend_join_kernel<T>, dim3((unsigned)cdiv(rows * (a.dim / 8), 256)), dim3(256), 0, st, a,
-                       splits, part, stat, (T *)o, lse);
+    int lanes = 1, shares = 1;
+    while (lanes * 8 < a.dim) lanes *= 2;
+    while (shares < splits && lanes * shares < 256) shares *= 2;
+    hipLaunchKernelGGL(attend_join_kernel<T>, dim3((unsigned)cdiv(rows, 256 / (lanes * shares))), dim3(256), 0, st, a,
+                       splits, lanes, shares, part, stat, (T *)o, (T *)low, lse);
     KL_CHECK_LAUNCH();
   }
   return KL_OK;
@@ -305,8 +356,8 @@ extern "C" size_t kl_pack_attention_workspace_bytes(kl_dtype dtype, int64_t num_
 extern "C" int kl_pack_attention_forward(kl_dtype dtype, int64_t num_q, int64_t num_k, int heads, int kv_heads, int dim,
                                          const void *q, const void *k, const void *v, const int64_t *strides_host,
                                          const int32_t *q_ids, const int32_t *q_starts, const int32_t *k_ids,
-                                         const int32_t *k_starts, float scale, int causal, void *out, float *lse,
-                                         void *ws, size_t ws_bytes, kl_stream stream) {
+                                         const int32_t *k_starts, float scale, int causal, void *out, void *out_low,
+                                         float *lse, void *ws, size_t ws_bytes, kl_stream stream) {
   Attend a;
   KL_CHECK_RC(fill_attend(a, "pack_attention", num_q, num_k, heads, kv_heads, dim, strides_host, q_ids, q_starts, k_ids,
                           k_starts, scale, causal));
@@ -315,7 +366,8 @@ extern "C" int kl_pack_attention_forward(kl_dtype dtype, int64_t num_q, int64_t 
   if (num_q == 0) return KL_OK;
   return with_type(dtype, "pack_attention", [&](auto t) {
     return with_dim(dim, [&](auto dp) {
-      return attend_forward<decltype(t), decltype(dp)::value>(a, q, k, v, out, lse, ws, S(stream));
+      return attend_forward<decltype(t), decltype(dp)::value>(a, q, k, v, out, sizeof(t) == 2 ? out_low : nullptr, lse, ws,
+                                                              S(stream));
     });
   });
 }

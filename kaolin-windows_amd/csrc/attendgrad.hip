@@ -24,36 +24,52 @@ struct Grad {
   int parts;
 };
 
-// D, the key ranges and the maxima of |do|: 16 lanes per (row, head).
-template <typename T>
-__global__ void __launch_bounds__(256) attend_prep_kernel(Attend a, const T *__restrict__ o, const T *__restrict__ go,
-                                                        const float *__restrict__ lse, float2 *__restrict__ ld,
-                                                        int2 *__restrict__ range, float *__restrict__ amax) {
-  const int heads = a.kv_heads * a.group, E = 16 / (int)sizeof(T), sub = threadIdx.x & 15;
-  const int64_t rows = (int64_t)a.nq * heads;
+// D, the key ranges and the maxima of |do|: LANES lanes per (row, head), kItems of those a group at once.
+constexpr int kItems = 4;
+template <typename T, int LANES>
+__global__ void __launch_bounds__(256) attend_prep_kernel(Attend a, const T *__restrict__ o, const T *__restrict__ low,
+                                                        const T *__restrict__ go, const float *__restrict__ lse,
+                                                        float2 *__restrict__ ld, int2 *__restrict__ range,
+                                                        float *__restrict__ amax) {
+  constexpr int E = 16 / (int)sizeof(T), GROUPS = 256 / LANES;
+  union Piece {
+    u32x4 w;
+    T v[E];
+  };
+  const int64_t rows = (int64_t)a.nq * a.kv_heads * a.group;
+  const int sub = threadIdx.x % LANES, c = sub * E;
   float big = 0;
-  for (int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) / 16; at < rows; at += (int64_t)gridDim.x * 16) {
-    float d = 0;
-    for (int c = sub * E; c < a.dim; c += 16 * E) {
-      union {
-        u32x4 w;
-        T v[16 / sizeof(T)];
-      } x, y;
-      x.w = *reinterpret_cast<const u32x4 *>(o + at * a.dim + c);
-      y.w = *reinterpret_cast<const u32x4 *>(go + at * a.dim + c);
+  for (int64_t at0 = ((int64_t)blockIdx.x * GROUPS + threadIdx.x / LANES) * kItems; at0 < rows;
+       at0 += (int64_t)gridDim.x * GROUPS * kItems) {
+    Piece x[kItems], y[kItems], z[kItems];
+    float ls[kItems];
 #pragma unroll
-      for (int e = 0; e < E; e++) {
-        d = fmaf((float)x.v[e], (float)y.v[e], d);
-        big = fmaxf(big, fabsf((float)y.v[e]));
+    for (int i = 0; i < kItems; i++) {
+      x[i].w = y[i].w = z[i].w = u32x4{0, 0, 0, 0};
+      ls[i] = 0;
+      if (at0 + i < rows && c < a.dim) {
+        x[i].w = *reinterpret_cast<const u32x4 *>(o + (at0 + i) * a.dim + c);
+        y[i].w = *reinterpret_cast<const u32x4 *>(go + (at0 + i) * a.dim + c);
+        if (low) z[i].w = *reinterpret_cast<const u32x4 *>(low + (at0 + i) * a.dim + c);
+        ls[i] = lse[at0 + i];
       }
     }
 #pragma unroll
-    for (int s = 8; s > 0; s >>= 1) d += __shfl_xor(d, s);
-    if (sub == 0) ld[at] = make_float2(lse[at], d);
-    if (sub == 0 && at % heads == 0) {
-      const Range r = key_range(a, (int)(at / heads));
-      range[at / heads] = make_int2(r.lo, r.hi);
+    for (int i = 0; i < kItems; i++) {
+      float d = 0;
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        d = fmaf((float)x[i].v[e] + (float)z[i].v[e], (float)y[i].v[e], d);
+        big = fmaxf(big, fabsf((float)y[i].v[e]));
+      }
+#pragma unroll
+      for (int s = LANES / 2; s > 0; s >>= 1) d += __shfl_xor(d, s);
+      if (sub == 0 && at0 + i < rows) ld[at0 + i] = make_float2(ls[i], d);
     }
+  }
+  for (int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x; row < a.nq; row += (int64_t)gridDim.x * 256) {
+    const Range r = key_range(a, (int)row);
+    range[row] = make_int2(r.lo, r.hi);
   }
   if constexpr (std::is_same<T, f16_t>::value) {
     __shared__ float s_max[4];
@@ -345,10 +361,18 @@ __device__ __forceinline__ Range row_range(const Attend &a, int j0, int j1) {
   return {min(r0, r1), r1};
 }
 
+// Virtual rows of each of n splits of `rows`: whole steps
+__device__ __forceinline__ int split_share(int rows, int n, int step) {
+  const int steps = (rows + step - 1) / step;
+  return (steps + n - 1) / n * step;
+}
+
+// grid: (tiles of keys * kv_heads, splits of the virtual rows); part: the splits' sums (NULL without splits)
 template <typename T, int DP>
 __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2)
     attend_dkv_kernel(Attend a, Grad g, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
-                      const T *__restrict__ go, T *__restrict__ dk_out, T *__restrict__ dv_out) {
+                      const T *__restrict__ go, T *__restrict__ dk_out, T *__restrict__ dv_out,
+                      float *__restrict__ part) {
   constexpr int BQ = DkvTile<T, DP>::BQ;
   using Q = StageRows<T, DP, BQ>;
   __shared__ T qs[BQ * Q::B::LD], os[BQ * Q::B::LD];
@@ -377,7 +401,13 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2)
     vf[i] = global_frag(vrow, live, 16 * i + 8 * h, a.dim);
   }
   f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
-  const int begin = rows.lo * a.group, end = rows.hi * a.group;
+  int begin = rows.lo * a.group, end = rows.hi * a.group;
+  if (part) {
+    const int share = split_share(end - begin, (int)gridDim.y, BQ);
+    begin = (int)min((int64_t)end, begin + (int64_t)share * blockIdx.y);
+    end = (int)min((int64_t)end, (int64_t)begin + share);
+    if (begin >= end) return;  // the join does not ask for it
+  }
   dkv_walk<T, DP, false>(a, g, qh, gst, gh, head, begin, end, key0, gs, kf, vf, qs, os, s_ld, s_range, bad, dk, dv);
   if (!(all_finite(dk) && all_finite(dv))) s_redo = 1;
   __syncthreads();
@@ -388,17 +418,67 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2)
   }
   if (!live) return;
   const int64_t at = ((int64_t)key * a.kv_heads + head) * a.dim;
+  if (part) {
+    const int64_t all = (int64_t)a.nk * a.kv_heads * a.dim;
+    store_cols<float, DP>(part + 2 * blockIdx.y * all + at, dk, a.scale / gs, h, a.dim);
+    store_cols<float, DP>(part + (2 * blockIdx.y + 1) * all + at, dv, 1.f, h, a.dim);
+    return;
+  }
   store_cols<T, DP>(dk_out + at, dk, a.scale / gs, h, a.dim);
   store_cols<T, DP>(dv_out + at, dv, 1.f, h, a.dim);
 }
 
-static unsigned prep_blocks(int64_t num_q, int heads) {
-  return (unsigned)std::max<int64_t>(1, std::min<int64_t>(cdiv(num_q * heads, 16), kMaxParts));
+// The splits of dk and dv added in their order: four elements a thread.
+template <typename T>
+__global__ void __launch_bounds__(256) attend_dkv_join_kernel(Attend a, int splits, int step,
+                                                            const float *__restrict__ part, T *__restrict__ dk,
+                                                            T *__restrict__ dv) {
+  const int64_t all = (int64_t)a.nk * a.kv_heads * a.dim;
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (at >= all) return;
+  const int j0 = (int)(at / ((int64_t)a.kv_heads * a.dim)) / 128 * 128;
+  const Range rows = row_range(a, j0, min(j0 + 128, a.nk));
+  const int n = (rows.hi - rows.lo) * a.group, share = split_share(n, splits, step);
+  const int used = n > 0 ? (n + share - 1) / share : 0;
+  f32x4 k = {}, v = {};
+#pragma unroll 4
+  for (int s = 0; s < used; s++) {
+    k += *reinterpret_cast<const f32x4 *>(part + 2 * s * all + at);
+    v += *reinterpret_cast<const f32x4 *>(part + (2 * s + 1) * all + at);
+  }
+  *reinterpret_cast<V4<T> *>(dk + at) = __builtin_convertvector(k, V4<T>);
+  *reinterpret_cast<V4<T> *>(dv + at) = __builtin_convertvector(v, V4<T>);
+}
+
+// Splits of the virtual rows that stream past a tile of keys: four workgroups for each of the 256 CUs
+static int dkv_splits(int64_t nq, int64_t nk, int kv_heads, int group, int step) {
+  const int64_t blocks = cdiv(nk, 128) * kv_heads;
+  if (blocks == 0 || blocks >= 1024) return 1;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(1024, blocks), cdiv(nq * group, 2 * step), 16}));
+}
+static int dkv_step(kl_dtype dtype) { return dtype == KL_F32 ? 32 : 64; }
+
+// lanes per (row, head) of the first kernel: 16 bytes each
+static int prep_lanes(kl_dtype dtype, int dim) { return dim * (dtype == KL_F32 ? 4 : 2) / 16; }
+
+// Its workgroups: one per kItems * groups (row, head)s; f16: at most kMaxParts partial maxima
+static unsigned prep_blocks(kl_dtype dtype, int64_t num_q, int heads, int dim) {
+  const int lanes = prep_lanes(dtype, dim), pow2 = lanes <= 4 ? 4 : lanes <= 8 ? 8 : lanes <= 16 ? 16 : 32;
+  const int64_t blocks = cdiv(num_q * heads, (int64_t)kItems * (256 / pow2));
+  return (unsigned)std::max<int64_t>(1, dtype == KL_F16 ? std::min<int64_t>(blocks, kMaxParts) : blocks);
+}
+
+template <typename F>
+static int with_prep_lanes(int lanes, F f) {
+  if (lanes <= 4) return f(std::integral_constant<int, 4>());
+  if (lanes <= 8) return f(std::integral_constant<int, 8>());
+  if (lanes <= 16) return f(std::integral_constant<int, 16>());
+  return f(std::integral_constant<int, 32>());
 }
 
 template <typename T, int DP>
 static int attend_backward(const Attend &a, const Grad &g, const void *q, const void *k, const void *v, const void *go,
-                           void *dq, void *dk, void *dv, hipStream_t st) {
+                           void *dq, void *dk, void *dv, float *part, hipStream_t st) {
   if (a.nq > 0 && dq) {
     const unsigned blocks = (unsigned)(cdiv((int64_t)a.nq * a.group, 128) * a.kv_heads);
     hipLaunchKernelGGL((attend_dq_kernel<T, DP>), dim3(blocks), dim3(256), 0, st, a, g, (const T *)q, (const T *)k,
@@ -407,9 +487,16 @@ static int attend_backward(const Attend &a, const Grad &g, const void *q, const 
   }
   if (a.nk > 0 && dk) {
     const unsigned blocks = (unsigned)(cdiv(a.nk, 128) * a.kv_heads);
-    hipLaunchKernelGGL((attend_dkv_kernel<T, DP>), dim3(blocks), dim3(256), 0, st, a, g, (const T *)q, (const T *)k,
-                       (const T *)v, (const T *)go, (T *)dk, (T *)dv);
+    const int step = DkvTile<T, DP>::BQ, splits = dkv_splits(a.nq, a.nk, a.kv_heads, a.group, step);
+    hipLaunchKernelGGL((attend_dkv_kernel<T, DP>), dim3(blocks, splits), dim3(256), 0, st, a, g, (const T *)q,
+                       (const T *)k, (const T *)v, (const T *)go, (T *)dk, (T *)dv, splits > 1 ? part : nullptr);
     KL_CHECK_LAUNCH();
+    if (splits > 1) {
+      const int64_t pieces = (int64_t)a.nk * a.kv_heads * a.dim / 4;
+      hipLaunchKernelGGL(attend_dkv_join_kernel<T>, dim3((unsigned)cdiv(pieces, 256)), dim3(256), 0, st, a, splits, step,
+                         part, (T *)dk, (T *)dv);
+      KL_CHECK_LAUNCH();
+    }
   }
   return KL_OK;
 }
@@ -418,39 +505,44 @@ static int attend_backward(const Attend &a, const Grad &g, const void *q, const 
 
 using namespace kl;
 
-extern "C" size_t kl_pack_attention_bwd_workspace_bytes(int64_t num_q, int heads) {
-  if (num_q <= 0 || heads <= 0) return 256;
-  return al256((size_t)num_q * heads * 8) + al256((size_t)num_q * 8) + kMaxParts * 4;
+extern "C" size_t kl_pack_attention_bwd_workspace_bytes(kl_dtype dtype, int64_t num_q, int64_t num_k, int heads,
+                                                        int kv_heads, int dim) {
+  if (num_q < 0 || num_k < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || dim <= 0) return 256;
+  const int splits = dkv_splits(num_q, num_k, kv_heads, heads / kv_heads, dkv_step(dtype));
+  return al256((size_t)num_q * heads * 8) + al256((size_t)num_q * 8) + kMaxParts * 4 +
+         (splits > 1 ? (size_t)2 * splits * num_k * kv_heads * dim * 4 : 0);
 }
 
 extern "C" int kl_pack_attention_backward(kl_dtype dtype, int64_t num_q, int64_t num_k, int heads, int kv_heads,
                                           int dim, const void *grad_out, const void *q, const void *k, const void *v,
                                           const int64_t *strides_host, const int32_t *q_ids, const int32_t *q_starts,
                                           const int32_t *k_ids, const int32_t *k_starts, const void *out,
-                                          const float *lse, float scale, int causal, void *grad_q, void *grad_k,
-                                          void *grad_v, void *ws, size_t ws_bytes, kl_stream stream) {
+                                          const void *out_low, const float *lse, float scale, int causal, void *grad_q,
+                                          void *grad_k, void *grad_v, void *ws, size_t ws_bytes, kl_stream stream) {
   Attend a;
   KL_CHECK_RC(fill_attend(a, "pack_attention", num_q, num_k, heads, kv_heads, dim, strides_host, q_ids, q_starts, k_ids,
                           k_starts, scale, causal));
-  KL_REQUIRE(ws_bytes >= kl_pack_attention_bwd_workspace_bytes(num_q, heads),
+  KL_REQUIRE(ws_bytes >= kl_pack_attention_bwd_workspace_bytes(dtype, num_q, num_k, heads, kv_heads, dim),
              "pack_attention: the workspace is too small");
   KL_REQUIRE((grad_k == nullptr) == (grad_v == nullptr), "pack_attention: grad_k and grad_v go together");
-  Grad g = {};
-  g.ld = (float2 *)ws;
-  g.range = (int2 *)((char *)ws + al256((size_t)num_q * heads * 8));
-  g.amax = (float *)((char *)g.range + al256((size_t)num_q * 8));
-  g.parts = (int)prep_blocks(num_q, heads);
+  float2 *ld = (float2 *)ws;
+  int2 *range = (int2 *)((char *)ws + al256((size_t)num_q * heads * 8));
+  float *amax = (float *)((char *)range + al256((size_t)num_q * 8));
+  const Grad g = {ld, range, amax, num_q > 0 ? (int)prep_blocks(dtype, num_q, heads, dim) : 0};
   return with_type(dtype, "pack_attention", [&](auto t) -> int {
     using T = decltype(t);
     if (num_q > 0) {
-      hipLaunchKernelGGL(attend_prep_kernel<T>, dim3(g.parts), dim3(256), 0, S(stream), a, (const T *)out,
-                         (const T *)grad_out, lse, (float2 *)g.ld, (int2 *)g.range, (float *)g.amax);
-      KL_CHECK_LAUNCH();
-    } else {
-      g.parts = 0;
+      KL_CHECK_RC(with_prep_lanes(prep_lanes(dtype, dim), [&](auto lanes) -> int {
+        hipLaunchKernelGGL((attend_prep_kernel<T, decltype(lanes)::value>), dim3(g.parts), dim3(256), 0, S(stream), a,
+                           (const T *)out, sizeof(T) == 2 ? (const T *)out_low : (const T *)nullptr,
+                           (const T *)grad_out, lse, ld, range, amax);
+        KL_CHECK_LAUNCH();
+        return KL_OK;
+      }));
     }
     return with_dim(dim, [&](auto dp) {
-      return attend_backward<T, decltype(dp)::value>(a, g, q, k, v, grad_out, grad_q, grad_k, grad_v, S(stream));
+      return attend_backward<T, decltype(dp)::value>(a, g, q, k, v, grad_out, grad_q, grad_k, grad_v, amax + kMaxParts,
+                                                     S(stream));
     });
   });
 }

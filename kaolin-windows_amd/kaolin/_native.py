@@ -115,10 +115,10 @@ _SIGS = {
     'kl_pack_layout': (_I, [_I64, _P, _P, _P, _P, _SZ, _P]),
     'kl_pack_attention_workspace_bytes': (_SZ, [_I, _I64, _I64, _I, _I, _I]),
     'kl_pack_attention_forward': (_I, [_I, _I64, _I64, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _F, _I, _P, _P, _P,
-                                       _SZ, _P]),
-    'kl_pack_attention_bwd_workspace_bytes': (_SZ, [_I64, _I]),
-    'kl_pack_attention_backward': (_I, [_I, _I64, _I64, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _F, _I,
-                                        _P, _P, _P, _P, _SZ, _P]),
+                                       _P, _SZ, _P]),
+    'kl_pack_attention_bwd_workspace_bytes': (_SZ, [_I, _I64, _I64, _I, _I, _I]),
+    'kl_pack_attention_backward': (_I, [_I, _I64, _I64, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _F,
+                                        _I, _P, _P, _P, _P, _SZ, _P]),
     'kl_norm_rotary_forward': (_I, [_I, _I64, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _I, _P, _I, _P, _P, _P, _F, _P, _P,
                                     _P]),
     'kl_norm_rotary_bwd_workspace_bytes': (_SZ, [_I]),

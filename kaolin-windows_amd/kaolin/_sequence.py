@@ -93,14 +93,16 @@ def _strides(q, k, v):
     return (ctypes.c_int64 * 6)(q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1))
 
 
-def pack_attention_forward_cuda(q, k, v, q_layout, k_layout, scale, causal, with_lse):
+def pack_attention_forward_cuda(q, k, v, q_layout, k_layout, scale, causal, for_backward):
     """Attention of the rows of q over the rows of k, v of the pack with the same number.  Returns the
-    output (num_q, heads, dim) and, with_lse, the base-2 logarithms of the softmax sums (num_q, heads)."""
+    output (num_q, heads, dim) and, for_backward, the base-2 logarithms of the softmax sums (num_q, heads) and
+    (f16, bf16) what the output's rounding left out, as the output; else None."""
     func = 'pack_attention_forward_cuda'
     q, k, v = _attention_args(func, q, k, v, q_layout, k_layout, scale)
     dev = q.device
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev) if with_lse else None
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev) if for_backward else None
+    low = torch.empty_like(out) if for_backward and q.dtype != torch.float32 else None
     code = _CODES[q.dtype]
     with N.on_device(dev):
         ws_bytes = N.size('kl_pack_attention_workspace_bytes', code, q.shape[0], k.shape[0], q.shape[1], k.shape[1],
@@ -109,11 +111,11 @@ def pack_attention_forward_cuda(q, k, v, q_layout, k_layout, scale, causal, with
         N.check(N.lib().kl_pack_attention_forward(
             code, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2], N.ptr(q), N.ptr(k), N.ptr(v),
             _strides(q, k, v), N.ptr(q_layout[0]), N.ptr(q_layout[1]), N.ptr(k_layout[0]), N.ptr(k_layout[1]),
-            scale, int(causal), N.ptr(out), N.ptr(lse), N.ptr(ws), ws_bytes, N.stream_of(dev)), func)
-    return out, lse
+            scale, int(causal), N.ptr(out), N.ptr(low), N.ptr(lse), N.ptr(ws), ws_bytes, N.stream_of(dev)), func)
+    return out, lse, low
 
 
-def pack_attention_backward_cuda(grad_out, q, k, v, q_layout, k_layout, out, lse, scale, causal, need_q, need_kv):
+def pack_attention_backward_cuda(grad_out, q, k, v, q_layout, k_layout, out, lse, low, scale, causal, need_q, need_kv):
     """The gradients of q and of (k, v), None where not needed."""
     func = 'pack_attention_backward_cuda'
     q, k, v = _attention_args(func, q, k, v, q_layout, k_layout, scale)
@@ -126,18 +128,24 @@ def pack_attention_backward_cuda(grad_out, q, k, v, q_layout, k_layout, out, lse
     check_size(func, Arg(lse, 'lse', 0), q.shape[:2])
     check_type(func, Arg(lse, 'lse', 0), (torch.float32,))
     check_contiguous(func, [ao, Arg(lse, 'lse', 0)])
+    if low is not None:
+        check_same_size(func, Arg(low, 'low', 0), ao)
+        check_same_type(func, Arg(low, 'low', 0), ao)
+        check_contiguous(func, [Arg(low, 'low', 0)])
+        check_all_same_gpu(func, [ao, Arg(low, 'low', 0)])
     check_all_same_gpu(func, [Arg(q, 'q', 1), ag, ao, Arg(lse, 'lse', 0)])
     dev = q.device
     dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if need_q else None
     dk = torch.empty(k.shape, dtype=k.dtype, device=dev) if need_kv else None
     dv = torch.empty(k.shape, dtype=k.dtype, device=dev) if need_kv else None
     with N.on_device(dev):
-        ws_bytes = N.size('kl_pack_attention_bwd_workspace_bytes', q.shape[0], q.shape[1])
+        ws_bytes = N.size('kl_pack_attention_bwd_workspace_bytes', _CODES[q.dtype], q.shape[0], k.shape[0], q.shape[1],
+                          k.shape[1], q.shape[2])
         ws = N.workspace(ws_bytes, dev)
         N.check(N.lib().kl_pack_attention_backward(
             _CODES[q.dtype], q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2], N.ptr(grad_out),
             N.ptr(q), N.ptr(k), N.ptr(v), _strides(q, k, v), N.ptr(q_layout[0]), N.ptr(q_layout[1]),
-            N.ptr(k_layout[0]), N.ptr(k_layout[1]), N.ptr(out), N.ptr(lse), scale, int(causal), N.ptr(dq), N.ptr(dk),
+            N.ptr(k_layout[0]), N.ptr(k_layout[1]), N.ptr(out), N.ptr(low), N.ptr(lse), scale, int(causal), N.ptr(dq), N.ptr(dk),
             N.ptr(dv), N.ptr(ws), ws_bytes, N.stream_of(dev)), func)
     return dq, dk, dv
 

@@ -15,18 +15,18 @@ class PackAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, q_layout, k_layout, scale, causal):
         needs = any(ctx.needs_input_grad[:3])
-        out, lse = _C.render.spc.pack_attention_forward_cuda(q, k, v, q_layout, k_layout, scale, causal, needs)
+        out, lse, low = _C.render.spc.pack_attention_forward_cuda(q, k, v, q_layout, k_layout, scale, causal, needs)
         if needs:
-            ctx.save_for_backward(q, k, v, out, lse, *q_layout, *k_layout)
+            ctx.save_for_backward(q, k, v, out, lse, low, *q_layout, *k_layout)
             ctx.scale, ctx.causal = scale, causal
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
-        q, k, v, out, lse, qi, qs, ki, ks = ctx.saved_tensors
+        q, k, v, out, lse, low, qi, qs, ki, ks = ctx.saved_tensors
         dq, dk, dv = _C.render.spc.pack_attention_backward_cuda(
-            grad_out, q, k, v, (qi, qs), (ki, ks), out, lse, ctx.scale, ctx.causal, ctx.needs_input_grad[0],
+            grad_out, q, k, v, (qi, qs), (ki, ks), out, lse, low, ctx.scale, ctx.causal, ctx.needs_input_grad[0],
             ctx.needs_input_grad[1] or ctx.needs_input_grad[2])
         return (dq, dk if ctx.needs_input_grad[1] else None, dv if ctx.needs_input_grad[2] else None, None, None, None,
                 None)

@@ -129,7 +129,7 @@ def test_library_refusals_without_gpu():
 
     def attend(dtype=0, nq=1, nk=1, heads=1, kv=1, dim=8, scale=1.0, ws=1 << 30):
         return lib.kl_pack_attention_forward(dtype, nq, nk, heads, kv, dim, None, None, None, st, None, None, None, None,
-                                             scale, 0, None, None, None, ws, None), lib.kl_last_error()
+                                             scale, 0, None, None, None, None, ws, None), lib.kl_last_error()
     for kw, what in ((dict(dim=12), b'multiple of 8'), (dict(dim=136), b'multiple of 8'), (dict(heads=3, kv=2), b'heads'),
                      (dict(scale=0.0), b'scale'), (dict(scale=float('nan')), b'scale'), (dict(nq=-1), b'rows'),
                      (dict(nq=1 << 31), b'rows'), (dict(nk=(1 << 31) - 1), b'rows'), (dict(ws=0), b'workspace'),
@@ -137,7 +137,7 @@ def test_library_refusals_without_gpu():
         rc, msg = attend(**kw)
         assert rc == -1 and what in msg, (kw, msg)
     rc = lib.kl_pack_attention_backward(0, 1, 1, 1, 1, 8, None, None, None, None, st, None, None, None, None, None, None,
-                                        1.0, 0, None, 16, None, None, 1 << 30, None)
+                                        None, 1.0, 0, None, 16, None, None, 1 << 30, None)
     assert rc == -1 and b'go together' in lib.kl_last_error()
     assert lib.kl_pack_layout(1 << 31, None, None, None, None, 1 << 30, None) == -1
     assert lib.kl_pack_layout(70000, None, None, None, None, 0, None) == -1
