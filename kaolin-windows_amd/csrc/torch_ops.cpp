@@ -1,5 +1,6 @@
 // torch_ops.cpp -- the eager host path of dibr_rasterization (and of the tutorial loop's other
-// library ops: prepare_vertices, mask_iou, texture_mapping) as compiled autograd nodes.
+// library ops: prepare_vertices, mask_iou, texture_mapping; and the sequence operators over packs)
+// as compiled autograd nodes.
 //
 // The reference's native layer is a compiled extension (kaolin/csrc/bindings.cpp); its Python
 // front-end (render/mesh/dibr.py:119-209) pays one autograd Function per op.  The ctypes route of
@@ -16,6 +17,9 @@
 // autograd engine runs on the forward's stream.
 #include <torch/extension.h>
 
+#include <c10/core/DeviceGuard.h>
+
+#include <cmath>
 #include <map>
 #include <mutex>
 #include <string>
@@ -452,6 +456,332 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> dibr_rasterization(int64_t height
   return {r[0], r[1], r[2]};
 }
 
+// ---- The sequence operators over packs (kaolin/render/spc/sequence.py, which holds the same nodes in
+// Python).  Each function takes the plain case -- types, sizes and strides that the kernels read as they
+// are -- and returns nothing for any other call, which the Python route then copies or refuses with its
+// message.
+
+kl_dtype seq_code(at::ScalarType t) {
+  return t == at::kFloat ? KL_F32 : t == at::kHalf ? KL_F16 : t == at::kBFloat16 ? KL_BF16 : KL_F64;
+}
+
+bool seq_float(const at::Tensor &t) {
+  return t.scalar_type() == at::kFloat || t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16;
+}
+
+constexpr int64_t kMaxRows = ((int64_t)1 << 31) - 256;
+
+bool plain_mask(const at::Tensor &b, int64_t rows, const at::Device &dev) {
+  return b.dim() == 1 && b.size(0) == rows && rows < kMaxRows && b.device() == dev && b.is_contiguous() &&
+         (b.scalar_type() == at::kBool || b.scalar_type() == at::kByte);
+}
+
+// (rows, heads, dim) with whole 16-byte pieces in every row of a head
+bool plain_heads(const at::Tensor &t) {
+  const int64_t e = 16 / t.element_size();
+  return t.dim() == 3 && (t.numel() == 0 || (t.stride(2) == 1 && t.stride(0) % e == 0 && t.stride(1) % e == 0 &&
+                                             (uintptr_t)t.data_ptr() % 16 == 0));
+}
+
+bool any_grad(std::initializer_list<const at::Tensor *> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const at::Tensor *t : ts)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+
+at::Tensor contiguous16(const at::Tensor &t) {
+  const at::Tensor c = t.contiguous();
+  return c.numel() && (uintptr_t)c.data_ptr() % 16 ? c.clone() : c;
+}
+
+// The pack arrays of a mask (kl_pack_layout): ids (n) and starts (n + 1) in one tensor
+struct Layout {
+  at::Tensor held;
+  int32_t *ids() const { return held.data_ptr<int32_t>(); }
+  int32_t *starts() const { return held.data_ptr<int32_t>() + (held.numel() - 1) / 2; }
+};
+
+Layout make_layout(const at::Tensor &boundaries, int64_t stream) {
+  const int64_t n = boundaries.size(0);
+  Layout l{at::empty({2 * n + 1}, boundaries.options().dtype(at::kInt))};
+  const size_t bytes = kl_pack_layout_workspace_bytes(n);
+  at::Tensor ws = workspace(bytes, boundaries.device(), stream);
+  check(kl_pack_layout(n, (const uint8_t *)boundaries.data_ptr(), l.ids(), l.starts(), ws.data_ptr(), bytes,
+                       (kl_stream)stream),
+        "pack_layout");
+  return l;
+}
+
+struct HeadStrides {
+  int64_t v[6];
+  HeadStrides(const at::Tensor &q, const at::Tensor &k, const at::Tensor &w)
+      : v{q.stride(0), q.stride(1), k.stride(0), k.stride(1), w.stride(0), w.stride(1)} {}
+};
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_forward(const at::Tensor &q, const at::Tensor &k,
+                                                                 const at::Tensor &v, const Layout &lq,
+                                                                 const Layout &lk, double scale, bool causal,
+                                                                 bool for_backward, int64_t stream) {
+  const kl_dtype code = seq_code(q.scalar_type());
+  at::Tensor out = at::empty(q.sizes(), q.options()), lse, low;
+  if (for_backward) {
+    lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
+    if (code != KL_F32) low = at::empty(q.sizes(), q.options());
+  }
+  const int heads = (int)q.size(1), kv = (int)k.size(1), dim = (int)q.size(2);
+  const size_t bytes = kl_pack_attention_workspace_bytes(code, q.size(0), k.size(0), heads, kv, dim);
+  at::Tensor ws = workspace(bytes, q.device(), stream);
+  const HeadStrides st(q, k, v);
+  check(kl_pack_attention_forward(code, q.size(0), k.size(0), heads, kv, dim, ptr(q), ptr(k), ptr(v), st.v, lq.ids(),
+                                  lq.starts(), lk.ids(), lk.starts(), (float)scale, causal, ptr(out), ptr(low),
+                                  (float *)ptr(lse), ptr(ws), bytes, (kl_stream)stream),
+        "pack_attention");
+  return {out, lse, low};
+}
+
+struct PackAttention : public torch::autograd::Function<PackAttention> {
+  static variable_list forward(AutogradContext *ctx, at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor lq,
+                               at::Tensor lk, double scale, bool causal, int64_t stream) {
+    auto r = attention_forward(q, k, v, Layout{lq}, Layout{lk}, scale, causal, true, stream);
+    ctx->save_for_backward({q, k, v, std::get<0>(r), std::get<1>(r), std::get<2>(r), lq, lk});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["causal"] = causal;
+    ctx->saved_data["stream"] = stream;
+    return {std::get<0>(r)};
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    no_double_backward("pack_attention");
+    variable_list outs(8);
+    if (!grads[0].defined()) return outs;
+    const auto s = ctx->get_saved_variables();
+    const at::Tensor &q = s[0], &k = s[1], &v = s[2];
+    const c10::DeviceGuard guard(q.device());
+    const bool need_q = ctx->needs_input_grad(0), need_kv = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
+    const int64_t stream = ctx->saved_data["stream"].toInt();
+    const at::Tensor g = contiguous16(grads[0]);
+    at::Tensor dq = need_q ? at::empty(q.sizes(), q.options()) : at::Tensor();
+    at::Tensor dk = need_kv ? at::empty(k.sizes(), k.options()) : at::Tensor();
+    at::Tensor dv = need_kv ? at::empty(v.sizes(), v.options()) : at::Tensor();
+    const kl_dtype code = seq_code(q.scalar_type());
+    const int heads = (int)q.size(1), kv = (int)k.size(1), dim = (int)q.size(2);
+    const size_t bytes = kl_pack_attention_bwd_workspace_bytes(code, q.size(0), k.size(0), heads, kv, dim);
+    at::Tensor ws = workspace(bytes, q.device(), stream);
+    const HeadStrides st(q, k, v);
+    const Layout lq{s[6]}, lk{s[7]};
+    check(kl_pack_attention_backward(code, q.size(0), k.size(0), heads, kv, dim, ptr(g), ptr(q), ptr(k), ptr(v), st.v,
+                                     lq.ids(), lq.starts(), lk.ids(), lk.starts(), ptr(s[3]), ptr(s[5]),
+                                     (const float *)ptr(s[4]), (float)ctx->saved_data["scale"].toDouble(),
+                                     ctx->saved_data["causal"].toBool(), ptr(dq), ptr(dk), ptr(dv), ptr(ws), bytes,
+                                     (kl_stream)stream),
+          "pack_attention backward");
+    outs[0] = dq;
+    if (ctx->needs_input_grad(1)) outs[1] = dk;
+    if (ctx->needs_input_grad(2)) outs[2] = dv;
+    return outs;
+  }
+};
+
+c10::optional<at::Tensor> pack_attention(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor boundaries,
+                                         c10::optional<at::Tensor> q_boundaries, bool causal, double scale,
+                                         int64_t stream) {
+  const at::Device dev = q.device();
+  const at::Tensor &qb = q_boundaries ? *q_boundaries : boundaries;
+  if (!q.is_cuda() || k.device() != dev || v.device() != dev || !seq_float(q) || k.scalar_type() != q.scalar_type() ||
+      v.scalar_type() != q.scalar_type() || !plain_heads(q) || !plain_heads(k) || !plain_heads(v) ||
+      k.sizes() != v.sizes() || k.size(2) != q.size(2) || q.size(2) % 8 || q.size(2) < 8 || q.size(2) > 128 ||
+      k.size(1) == 0 || q.size(1) == 0 || q.size(1) % k.size(1) || q.size(1) > 4096 || !(scale > 0) ||
+      !std::isfinite(scale) || !plain_mask(boundaries, k.size(0), dev) || !plain_mask(qb, q.size(0), dev))
+    return c10::nullopt;
+  const c10::DeviceGuard guard(dev);
+  const Layout lk = make_layout(boundaries, stream), lq = q_boundaries ? make_layout(qb, stream) : lk;
+  if (any_grad({&q, &k, &v})) return PackAttention::apply(q, k, v, lq.held, lk.held, scale, causal, stream)[0];
+  return std::get<0>(attention_forward(q, k, v, lq, lk, scale, causal, false, stream));
+}
+
+// norm_rotary's arguments past q and k
+struct NormArgs {
+  at::Tensor wq, wk, freqs, held, positions;  // held: a Layout, where positions is not given
+  double eps;
+  bool interleaved;
+  int64_t stream;
+  int kind() const {
+    if (!positions.defined()) return 0;
+    return positions.scalar_type() == at::kInt ? 1 : positions.scalar_type() == at::kLong ? 2 : 3;
+  }
+  int weight_f32() const { return ((wq.defined() ? wq : wk).defined() &&
+                                   (wq.defined() ? wq : wk).scalar_type() == at::kFloat); }
+  const int32_t *ids() const { return held.defined() ? Layout{held}.ids() : nullptr; }
+  const int32_t *starts() const { return held.defined() ? Layout{held}.starts() : nullptr; }
+};
+
+std::pair<at::Tensor, at::Tensor> norm_forward(const at::Tensor &q, const at::Tensor &k, const NormArgs &a) {
+  at::Tensor yq = at::empty(q.sizes(), q.options()), yk = at::empty(k.sizes(), k.options());
+  const HeadStrides st(q, k, k);
+  check(kl_norm_rotary_forward(seq_code(q.scalar_type()), q.size(0), (int)q.size(1), (int)k.size(1), (int)q.size(2),
+                               2 * (int)a.freqs.size(0), a.interleaved, ptr(q), ptr(k), st.v, ptr(a.wq), ptr(a.wk),
+                               a.weight_f32(), a.freqs.data_ptr<double>(), a.kind(), ptr(a.positions), a.ids(),
+                               a.starts(), (float)a.eps, ptr(yq), ptr(yk), (kl_stream)a.stream),
+        "norm_rotary");
+  return {yq, yk};
+}
+
+struct NormRotary : public torch::autograd::Function<NormRotary> {
+  using Maybe = c10::optional<at::Tensor>;
+  static variable_list forward(AutogradContext *ctx, at::Tensor q, at::Tensor k, Maybe wq_, Maybe wk_, at::Tensor freqs,
+                               Maybe held_, Maybe positions_, double eps, bool interleaved, int64_t stream) {
+    const at::Tensor wq = wq_.value_or(at::Tensor()), wk = wk_.value_or(at::Tensor()),
+                     held = held_.value_or(at::Tensor()), positions = positions_.value_or(at::Tensor());
+    auto r = norm_forward(q, k, {wq, wk, freqs, held, positions, eps, interleaved, stream});
+    ctx->save_for_backward({q, k, wq, wk, freqs, held, positions});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["stream"] = stream;
+    return {r.first, r.second};
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    no_double_backward("norm_rotary");
+    variable_list outs(10);
+    if (!grads[0].defined() && !grads[1].defined()) return outs;
+    const auto s = ctx->get_saved_variables();
+    const at::Tensor &q = s[0], &k = s[1];
+    const c10::DeviceGuard guard(q.device());
+    const NormArgs a{s[2], s[3], s[4], s[5], s[6], ctx->saved_data["eps"].toDouble(),
+                     ctx->saved_data["interleaved"].toBool(), ctx->saved_data["stream"].toInt()};
+    const at::Tensor gq = grads[0].defined() ? contiguous16(grads[0]) : at::zeros(q.sizes(), q.options());
+    const at::Tensor gk = grads[1].defined() ? contiguous16(grads[1]) : at::zeros(k.sizes(), k.options());
+    at::Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options());
+    // the inputs that need a gradient are counted without those that are absent
+    at::Tensor dwq = a.wq.defined() && ctx->needs_input_grad(2) ? at::empty_like(a.wq) : at::Tensor();
+    at::Tensor dwk = a.wk.defined() && ctx->needs_input_grad(a.wq.defined() ? 3 : 2) ? at::empty_like(a.wk)
+                                                                                     : at::Tensor();
+    const size_t bytes = kl_norm_rotary_bwd_workspace_bytes((int)q.size(2));
+    at::Tensor ws = workspace(bytes, q.device(), a.stream);
+    const HeadStrides st(q, k, k);
+    check(kl_norm_rotary_backward(seq_code(q.scalar_type()), q.size(0), (int)q.size(1), (int)k.size(1), (int)q.size(2),
+                                  2 * (int)a.freqs.size(0), a.interleaved, ptr(gq), ptr(gk), ptr(q), ptr(k), st.v,
+                                  ptr(a.wq), ptr(a.wk), a.weight_f32(), a.freqs.data_ptr<double>(), a.kind(),
+                                  ptr(a.positions), a.ids(), a.starts(), (float)a.eps, ptr(dq), ptr(dk), ptr(dwq),
+                                  ptr(dwk), ptr(ws), bytes, (kl_stream)a.stream),
+          "norm_rotary backward");
+    if (ctx->needs_input_grad(0)) outs[0] = dq;
+    if (ctx->needs_input_grad(1)) outs[1] = dk;
+    outs[2] = dwq;
+    outs[3] = dwk;
+    return outs;
+  }
+};
+
+c10::optional<std::tuple<at::Tensor, at::Tensor>> norm_rotary(at::Tensor q, at::Tensor k, c10::optional<at::Tensor> wq_,
+                                                              c10::optional<at::Tensor> wk_, at::Tensor freqs,
+                                                              c10::optional<at::Tensor> boundaries,
+                                                              c10::optional<at::Tensor> positions_, double eps,
+                                                              bool interleaved, int64_t stream) {
+  const at::Device dev = q.device();
+  const at::Tensor wq = wq_.value_or(at::Tensor()), wk = wk_.value_or(at::Tensor()),
+                   positions = positions_.value_or(at::Tensor());
+  auto plain_weight = [&](const at::Tensor &w) {
+    return !w.defined() || (w.device() == dev && w.dim() == 1 && w.size(0) == q.size(2) && w.is_contiguous() &&
+                            (w.scalar_type() == q.scalar_type() || w.scalar_type() == at::kFloat));
+  };
+  if (!q.is_cuda() || k.device() != dev || !seq_float(q) || k.scalar_type() != q.scalar_type() || !plain_heads(q) ||
+      !plain_heads(k) || k.size(0) != q.size(0) || k.size(2) != q.size(2) || q.size(2) % 8 || q.size(2) < 8 ||
+      q.size(2) > 256 || q.size(1) + k.size(1) > 1 << 16 || q.size(0) >= kMaxRows || !plain_weight(wq) ||
+      !plain_weight(wk) || (wq.defined() && wk.defined() && wq.scalar_type() != wk.scalar_type()) ||
+      freqs.device() != dev || freqs.scalar_type() != at::kDouble || freqs.dim() != 1 || !freqs.is_contiguous() ||
+      freqs.requires_grad() || 2 * freqs.size(0) > q.size(2) || !(eps >= 0) || !std::isfinite(eps) ||
+      boundaries.has_value() == positions.defined())
+    return c10::nullopt;
+  if (positions.defined()) {
+    const auto t = positions.scalar_type();
+    if (positions.device() != dev || positions.dim() != 1 || positions.size(0) != q.size(0) ||
+        !positions.is_contiguous() || positions.requires_grad() || (t != at::kInt && t != at::kLong && t != at::kFloat))
+      return c10::nullopt;
+  } else if (!plain_mask(*boundaries, q.size(0), dev)) {
+    return c10::nullopt;
+  }
+  const c10::DeviceGuard guard(dev);
+  c10::optional<at::Tensor> held_;
+  if (!positions.defined()) held_ = make_layout(*boundaries, stream).held;
+  if (any_grad({&q, &k, &wq, &wk})) {
+    auto r = NormRotary::apply(q, k, wq_, wk_, freqs, held_, positions_, eps, interleaved, stream);
+    return std::make_tuple(r[0], r[1]);
+  }
+  const at::Tensor held = held_.value_or(at::Tensor());
+  auto r = norm_forward(q, k, {wq, wk, freqs, held, positions, eps, interleaved, stream});
+  return std::make_tuple(r.first, r.second);
+}
+
+at::Tensor recurrence_forward(const at::Tensor &gates, const at::Tensor &feats, const at::Tensor &initial,
+                              const Layout &l, bool reverse, int64_t stream) {
+  const kl_dtype code = seq_code(gates.scalar_type());
+  const int64_t n = gates.size(0), dim = gates.size(1);
+  at::Tensor out = at::empty(gates.sizes(), gates.options());
+  const size_t bytes = kl_linear_recurrence_workspace_bytes(code, n, dim);
+  at::Tensor ws = workspace(bytes, gates.device(), stream);
+  check(kl_linear_recurrence_forward(code, n, dim, ptr(gates), ptr(feats), ptr(initial),
+                                     initial.defined() ? initial.size(0) : 0, l.ids(), l.starts(), reverse, ptr(out),
+                                     ptr(ws), bytes, (kl_stream)stream),
+        "linear_recurrence");
+  return out;
+}
+
+struct LinearRecurrence : public torch::autograd::Function<LinearRecurrence> {
+  static variable_list forward(AutogradContext *ctx, at::Tensor gates, at::Tensor feats,
+                               c10::optional<at::Tensor> initial_, at::Tensor held, bool reverse, int64_t stream) {
+    const at::Tensor initial = initial_.value_or(at::Tensor());
+    at::Tensor out = recurrence_forward(gates, feats, initial, Layout{held}, reverse, stream);
+    ctx->save_for_backward({gates, out, initial, held});
+    ctx->saved_data["reverse"] = reverse;
+    ctx->saved_data["stream"] = stream;
+    return {out};
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    no_double_backward("linear_recurrence");
+    variable_list outs(6);
+    if (!grads[0].defined()) return outs;
+    const auto s = ctx->get_saved_variables();
+    const at::Tensor &gates = s[0], &initial = s[2];
+    const c10::DeviceGuard guard(gates.device());
+    const Layout l{s[3]};
+    const int64_t stream = ctx->saved_data["stream"].toInt(), n = gates.size(0), dim = gates.size(1);
+    const at::Tensor g = grads[0].contiguous();
+    at::Tensor da = at::empty(gates.sizes(), gates.options()), db = at::empty(gates.sizes(), gates.options());
+    at::Tensor di = initial.defined() ? at::empty(initial.sizes(), initial.options()) : at::Tensor();
+    const kl_dtype code = seq_code(gates.scalar_type());
+    const size_t bytes = kl_linear_recurrence_workspace_bytes(code, n, dim);
+    at::Tensor ws = workspace(bytes, gates.device(), stream);
+    check(kl_linear_recurrence_backward(code, n, dim, ptr(g), ptr(gates), ptr(s[1]), ptr(initial),
+                                        initial.defined() ? initial.size(0) : 0, l.ids(), l.starts(),
+                                        ctx->saved_data["reverse"].toBool(), ptr(da), ptr(db), ptr(di), ptr(ws), bytes,
+                                        (kl_stream)stream),
+          "linear_recurrence backward");
+    if (ctx->needs_input_grad(0)) outs[0] = da;
+    if (ctx->needs_input_grad(1)) outs[1] = db;
+    if (initial.defined() && ctx->needs_input_grad(2)) outs[2] = di;
+    return outs;
+  }
+};
+
+c10::optional<at::Tensor> linear_recurrence(at::Tensor gates, at::Tensor feats, at::Tensor boundaries,
+                                            c10::optional<at::Tensor> initial_, bool reverse, int64_t stream) {
+  const at::Device dev = gates.device();
+  const at::Tensor initial = initial_.value_or(at::Tensor());
+  auto plain = [&](const at::Tensor &t) {
+    return t.device() == dev && t.scalar_type() == gates.scalar_type() && t.dim() == 2 && t.is_contiguous();
+  };
+  if (!gates.is_cuda() || (!seq_float(gates) && gates.scalar_type() != at::kDouble) || !plain(gates) || !plain(feats) ||
+      gates.sizes() != feats.sizes() || gates.size(1) >= 1 << 24 || !plain_mask(boundaries, gates.size(0), dev) ||
+      (initial.defined() && (!plain(initial) || initial.size(1) != gates.size(1) ||
+                             initial.size(0) >= (int64_t)1 << 31)))
+    return c10::nullopt;
+  const c10::DeviceGuard guard(dev);
+  const Layout l = make_layout(boundaries, stream);
+  if (any_grad({&gates, &feats, &initial}))
+    return LinearRecurrence::apply(gates, feats, initial_, l.held, reverse, stream)[0];
+  return recurrence_forward(gates, feats, initial, l, reverse, stream);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -462,6 +792,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("mask_iou", &mask_iou, "mask_iou's fused node; see kaolin/metrics/render.py");
   m.def("prepare_vertices", &prepare_vertices, "prepare_vertices' node; see kaolin/render/mesh/utils.py");
   m.def("texture_mapping", &texture_mapping, "texture_mapping's node; see kaolin/render/mesh/utils.py");
+  m.def("pack_attention", &pack_attention, "pack_attention's node, or None; see kaolin/render/spc/sequence.py");
+  m.def("norm_rotary", &norm_rotary, "norm_rotary's node, or None; see kaolin/render/spc/sequence.py");
+  m.def("linear_recurrence", &linear_recurrence, "linear_recurrence's node, or None; see kaolin/render/spc/sequence.py");
   // the double-backward reference chains, exposed for tests (tests/test_cpu_paths.py)
   m.def("_mask_iou_chain", &mask_iou_chain);
   m.def("_prepare_chain", [](at::Tensor v, at::Tensor faces, at::Tensor proj, c10::optional<at::Tensor> rot,

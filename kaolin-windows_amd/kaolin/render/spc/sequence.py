@@ -1,11 +1,16 @@
 """Learned operators along packs: attention, norm with rotation, and the gated linear recurrence.  They take packs as the packed ray ops do (raytrace.py):
-rows grouped by a boundary mask, and read nothing back to the host."""
+rows grouped by a boundary mask, and read nothing back to the host.
+
+A plain call (types, sizes and strides that the kernels read as they are) runs as a compiled autograd node
+(csrc/torch_ops.cpp); the nodes here take every other one, copy what has to be copied, and refuse what is
+wrong.  Both call the same library entries."""
 import math
 
 import torch
 from torch.autograd.function import once_differentiable
 
-from ... import _C
+from ... import _C, _ext
+from ..._native import stream_of
 
 __all__ = ['pack_attention', 'norm_rotary', 'rotary_frequencies', 'linear_recurrence']
 
@@ -60,6 +65,11 @@ def pack_attention(q, k, v, boundaries, q_boundaries=None, causal=False, scale=N
     on every run.  Differentiable once, with respect to q, k and v.
     """
     scale = (max(q.shape[-1], 1) if q.dim() else 1) ** -0.5 if scale is None else float(scale)
+    ext = _ext.get() if q.is_cuda else None
+    if ext is not None:
+        out = ext.pack_attention(q, k, v, boundaries, q_boundaries, bool(causal), scale, stream_of(q.device))
+        if out is not None:
+            return out
     _check_boundaries('pack_attention', 'boundaries', boundaries, k)
     k_layout = _C.render.spc.pack_layout_cuda(boundaries.contiguous())
     if q_boundaries is None:
@@ -114,6 +124,12 @@ def norm_rotary(q, k, q_weight, k_weight, freqs, boundaries=None, positions=None
     respect to q, k and the weights; the sums for the weights have a fixed order.  Strides: as
     :func:`pack_attention`.
     """
+    ext = _ext.get() if q.is_cuda else None
+    if ext is not None:
+        out = ext.norm_rotary(q, k, q_weight, k_weight, freqs, boundaries, positions, float(eps), bool(interleaved),
+                              stream_of(q.device))
+        if out is not None:
+            return out
     for name, t in (('freqs', freqs), ('positions', positions)):
         if t is not None and t.requires_grad:
             raise RuntimeError(f'norm_rotary: {name} cannot take a gradient; detach it')
@@ -186,6 +202,11 @@ def linear_recurrence(gates, feats, boundaries, initial=None, reverse=False):
     values.  Differentiable once, with respect to gates, feats and initial; the gradient of the gates takes the
     states as they were rounded.
     """
+    ext = _ext.get() if gates.is_cuda else None
+    if ext is not None:
+        out = ext.linear_recurrence(gates, feats, boundaries, initial, bool(reverse), stream_of(gates.device))
+        if out is not None:
+            return out
     _check_boundaries('linear_recurrence', 'boundaries', boundaries, gates)
     layout = _C.render.spc.pack_layout_cuda(boundaries.contiguous())
     return LinearRecurrence.apply(gates.contiguous(), feats.contiguous(),

@@ -12,9 +12,15 @@ DEV = 'cuda'
 TYPES = [torch.float32, torch.float16, torch.bfloat16]
 
 
-@pytest.fixture(scope='module')
-def spc():
+@pytest.fixture(params=['compiled', 'python'])
+def spc(request, monkeypatch):
+    """The operators through their compiled nodes and through the Python ones."""
     import kaolin
+    from kaolin import _ext
+    if request.param == 'python':
+        monkeypatch.setattr(_ext, '_mod', None)
+    elif torch.cuda.is_available():
+        assert _ext.get() is not None, 'the compiled nodes are not built'
     return kaolin.render.spc
 
 
@@ -195,10 +201,13 @@ def test_refusals_on_gpu(spc):
 @pytest.mark.gpu
 def test_second_derivatives_are_refused(spc):
     b = torch.ones(3, dtype=torch.bool, device=DEV)
-    x = torch.rand(3, 2, device=DEV, requires_grad=True)
-    g, = torch.autograd.grad(spc.linear_recurrence(x, x, b).sum(), x, create_graph=True)
-    with pytest.raises(RuntimeError, match='once_differentiable|does not require grad'):
-        g.sum().backward()
+    x = torch.rand(3, 2, 8, device=DEV, requires_grad=True)
+    f = torch.rand(4, dtype=torch.float64, device=DEV)
+    for y in (spc.linear_recurrence(x[:, 0].contiguous(), x[:, 1].contiguous(), b), spc.pack_attention(x, x, x, b),
+              spc.norm_rotary(x, x, None, None, f, boundaries=b)[0]):
+        with pytest.raises(RuntimeError, match='once_differentiable|create_graph=True is not supported'):
+            g, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+            g.sum().backward()
 
 
 # ------------------------------------------------------------------------------- the pack arrays
