@@ -32,13 +32,13 @@ __device__ __forceinline__ Range key_range(const Attend &a, int row) {
   return hi > lo ? Range{lo, hi} : no_keys();
 }
 
-// `a`'s pieces of 16 bytes of rows [row0, row0 + ROWS) of one head, for the 256 threads of a workgroup
+// A tile of ROWS rows on its way from memory through the registers of a workgroup's 256 threads to LDS
 template <typename T, int DP, int ROWS>
 struct Stage {
   static constexpr int CH = DP * (int)sizeof(T) / 16;  // pieces per row
   static constexpr int PER = ROWS * CH / 256;
-  static constexpr int E = 16 / (int)sizeof(T);        // elements per piece
-  static constexpr int LD = DP + E;                    // LDS row length: one piece of padding
+  static constexpr int E = 16 / (int)sizeof(T);
+  static constexpr int SIZE = ROWS * DP;
   static_assert(ROWS * CH % 256 == 0, "whole pieces per thread");
   u32x4 w[PER];
 
@@ -51,11 +51,24 @@ struct Stage {
       if (row < end && col < dim) w[i] = *reinterpret_cast<const u32x4 *>(base + row * stride + col);
     }
   }
+  // the same of virtual rows (Attend): row / group of head row % group
+  __device__ __forceinline__ void load_virtual(const T *__restrict__ base, Heads st, int group, int row0, int end,
+                                               int dim) {
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+      const int at = threadIdx.x + 256 * i, m = row0 + at / CH, col = at % CH * E;
+      w[i] = u32x4{0, 0, 0, 0};
+      if (m < end && col < dim) {
+        const int row = (int)((unsigned)m / (unsigned)group);
+        w[i] = *reinterpret_cast<const u32x4 *>(base + row * st.row + (m - row * group) * st.head + col);
+      }
+    }
+  }
   __device__ __forceinline__ void store(T *tile) const {
 #pragma unroll
     for (int i = 0; i < PER; i++) {
       const int at = threadIdx.x + 256 * i;
-      *reinterpret_cast<u32x4 *>(tile + at / CH * LD + at % CH * E) = w[i];
+      *reinterpret_cast<u32x4 *>(tile + Tile<T, DP>::piece(at / CH, at % CH)) = w[i];
     }
   }
   // bit r of bad[r / 32] for every row r that holds an infinity or a NaN
@@ -66,16 +79,68 @@ struct Stage {
       if (piece_bad<T>(w[i])) atomicOr(&bad[r / 32], 1u << (r % 32));
     }
   }
-  // pieces of bad rows as zeros
+  // bad rows as zeros
   __device__ __forceinline__ void store_good(T *tile, const uint32_t *bad) const {
 #pragma unroll
     for (int i = 0; i < PER; i++) {
       const int at = threadIdx.x + 256 * i, r = at / CH;
       const bool b = bad[r / 32] >> (r % 32) & 1;
-      *reinterpret_cast<u32x4 *>(tile + r * LD + at % CH * E) = b ? u32x4{0, 0, 0, 0} : w[i];
+      *reinterpret_cast<u32x4 *>(tile + Tile<T, DP>::piece(r, at % CH)) = b ? u32x4{0, 0, 0, 0} : w[i];
     }
   }
 };
+
+// Two tiles of ROWS rows streaming past a workgroup, x and y, in two LDS buffers each.  While one pair is
+// computed on, the next is on its way from memory to registers; one barrier a step.
+// CAREFUL (rows that hold infinities or NaN are taken out): buffer 0 has the rows with the bad ones as
+// zeros, buffer 1 all of them as they are, `bad` says which.
+// load(x, y, t) starts the loads of step t, commit(buffer) stores what it kept besides the tiles.
+template <typename T, int DP, int ROWS, bool CAREFUL, typename LOAD, typename COMMIT, typename STEP>
+__device__ __forceinline__ void stream(int begin, int end, T *xs, T *ys, uint32_t *bad, LOAD load, COMMIT commit,
+                                       STEP step) {
+  using St = Stage<T, DP, ROWS>;
+  if (begin >= end) return;
+  St x, y;
+  load(x, y, begin);
+  if constexpr (CAREFUL) {
+    for (int t = begin; t < end; t += ROWS) {
+      __syncthreads();  // the step before is done with the buffers
+      if (threadIdx.x < ROWS / 32) bad[threadIdx.x] = 0;
+      __syncthreads();
+      x.mark_bad(bad);
+      y.mark_bad(bad);
+      __syncthreads();
+      x.store_good(xs, bad);
+      y.store_good(ys, bad);
+      x.store(xs + St::SIZE);
+      y.store(ys + St::SIZE);
+      commit(0);
+      __syncthreads();
+      if (t + ROWS < end) load(x, y, t + ROWS);
+      step(t, 0);
+    }
+  } else {
+    __syncthreads();
+    x.store(xs);
+    y.store(ys);
+    commit(0);
+    if (begin + ROWS < end) load(x, y, begin + ROWS);
+    __syncthreads();
+    int buffer = 0;
+    for (int t = begin; t < end; t += ROWS) {
+      const int other = buffer ^ 1;
+      if (t + ROWS < end) {
+        x.store(xs + other * St::SIZE);
+        y.store(ys + other * St::SIZE);
+        commit(other);
+        if (t + 2 * ROWS < end) load(x, y, t + 2 * ROWS);
+      }
+      step(t, buffer);
+      __syncthreads();
+      buffer = other;
+    }
+  }
+}
 
 // The stationary operand: the 32 columns of a wave are 32 rows of a (rows, dim) matrix; element e of
 // fragment s is row[16 * s + 8 * h + e].
@@ -91,30 +156,29 @@ __device__ __forceinline__ V8<T> global_frag(const T *row, bool valid, int col, 
   return x.v;
 }
 
-// sum over the dim elements of a column's stationary row (fragments f) times another row in memory
+// sum over a column's stationary row (fragments f) times row r of a tile
 template <typename T, int DP>
-__device__ __forceinline__ float frag_dot(const V8<T> (&f)[DP / 16], const T *__restrict__ other, int h, int dim) {
+__device__ __forceinline__ float frag_dot(const V8<T> (&f)[DP / 16], const T *tile, int r, int h) {
   float s = 0;
 #pragma unroll
   for (int i = 0; i < DP / 16; i++) {
-    const int col = 16 * i + 8 * h;
-    if (col < dim) {
+    const V8<T> x = Tile<T, DP>::row_frag(tile, r, 16 * i + 8 * h);
 #pragma unroll
-      for (int e = 0; e < 8; e++) s = fmaf((float)f[i][e], (float)other[col + e], s);
-    }
+    for (int e = 0; e < 8; e++) s = fmaf((float)f[i][e], (float)x[e], s);
   }
-  return s + half_swap(s);
+  return half_sum(s);
 }
 
-// acc[db][r] += w * row[32 * db + acc_row(r, h)]: one inner index of the transposed product by itself
+// acc[db][r] += w * tile[row][32 * db + acc_row(r, h)]: one inner index of the transposed product by itself
 template <typename T, int DP>
-__device__ __forceinline__ void add_row(f32x16 (&acc)[DP / 32], float w, const T *__restrict__ row, int h, int dim) {
+__device__ __forceinline__ void add_row(f32x16 (&acc)[DP / 32], float w, const T *tile, int row, int h) {
 #pragma unroll
   for (int db = 0; db < DP / 32; db++) {
 #pragma unroll
-    for (int r = 0; r < 16; r++) {
-      const int d = 32 * db + acc_row(r, h);
-      if (d < dim) acc[db][r] = fmaf(w, (float)row[d], acc[db][r]);
+    for (int b = 0; b < 4; b++) {
+      const V4<T> x = *reinterpret_cast<const V4<T> *>(tile + Tile<T, DP>::at(row, 32 * db + 8 * b + 4 * h));
+#pragma unroll
+      for (int i = 0; i < 4; i++) acc[db][4 * b + i] = fmaf(w, (float)x[i], acc[db][4 * b + i]);
     }
   }
 }

@@ -26,9 +26,26 @@ struct FwdTile {
   static constexpr int BN = sizeof(T) == 4 ? 32 : 64;    // keys
 };
 
+// The running maximum (in the scores' base-2 scale) and sum of a row.  The maximum lags: sums are
+// rescaled only when a score passes it by kLag, for which weights grow to 2^kLag at most (rescaling at every
+// new maximum cost 64 multiplications a tile, a quarter of the arithmetic).
 struct RowState {
   float m = -INFINITY, l = 0;
+  __device__ __forceinline__ float base() const { return m == -INFINITY ? 0.f : m; }
 };
+constexpr float kLag = 8;
+
+template <int N>
+__device__ __forceinline__ void rescale(RowState &st, float m, f32x16 (&acc)[N]) {
+  const float keep = exp2_fast(st.m - (m == -INFINITY ? 0.f : m));
+  st.m = m;
+  st.l *= keep;
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+#pragma unroll
+    for (int r = 0; r < 16; r++) acc[i][r] *= keep;
+  }
+}
 
 template <typename T, int DP, bool CAREFUL>
 __device__ __forceinline__ void fwd_walk(const Attend &a, const T *__restrict__ k, const T *__restrict__ v, int begin,
@@ -36,109 +53,87 @@ __device__ __forceinline__ void fwd_walk(const Attend &a, const T *__restrict__ 
                                          const V8<T> (&qf)[DP / 16], T *ks, T *vs, uint32_t *bad,
                                          f32x16 (&acc)[DP / 32], RowState &st) {
   constexpr int BN = FwdTile<T, DP>::BN;
-  using KV = Stage<T, DP, BN>;
-  constexpr int LD = KV::LD;
+  using L = Tile<T, DP>;
   const int lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
-  KV ka, va;
-  ka.load(k, a.k.row, begin, end, a.dim);
-  va.load(v, a.v.row, begin, end, a.dim);
-  for (int kt = begin; kt < end; kt += BN) {
-    __syncthreads();  // the tile of the round before is read
-    if constexpr (CAREFUL) {
-      if (threadIdx.x < BN / 32) bad[threadIdx.x] = 0;
-      __syncthreads();
-      ka.mark_bad(bad);
-      va.mark_bad(bad);
-      __syncthreads();
-      ka.store_good(ks, bad);
-      va.store_good(vs, bad);
-    } else {
-      ka.store(ks);
-      va.store(vs);
-    }
-    __syncthreads();
-    if (kt + BN < end) {
-      ka.load(k, a.k.row, kt + BN, end, a.dim);
-      va.load(v, a.v.row, kt + BN, end, a.dim);
-    }
-    if (kt >= whi || kt + BN <= wlo) continue;
-    f32x16 s[BN / 32];
+  stream<T, DP, BN, CAREFUL>(
+      begin, end, ks, vs, bad,
+      [&](auto &x, auto &y, int kt) {
+        x.load(k, a.k.row, kt, end, a.dim);
+        y.load(v, a.v.row, kt, end, a.dim);
+      },
+      [](int) {},
+      [&](int kt, int buffer) {
+        if (kt >= whi || kt + BN <= wlo) return;
+        T *kb = ks + buffer * BN * DP, *vb = vs + buffer * BN * DP;
+        f32x16 s[BN / 32];
 #pragma unroll
-    for (int b = 0; b < BN / 32; b++) {
-      s[b] = f32x16{};
+        for (int b = 0; b < BN / 32; b++) s[b] = f32x16{};
 #pragma unroll
-      for (int i = 0; i < DP / 16; i++) s[b] = mma(row_frag(ks, LD, 32 * b + col, 16 * i + 8 * h), qf[i], s[b]);
-    }
-    const bool whole = !CAREFUL && kt >= full_lo && kt + BN <= full_hi;
-    float top = -INFINITY;
+        for (int i = 0; i < DP / 16; i++) {
 #pragma unroll
-    for (int b = 0; b < BN / 32; b++) {
+          for (int b = 0; b < BN / 32; b++) s[b] = mma(L::row_frag(kb, 32 * b + col, 16 * i + 8 * h), qf[i], s[b]);
+        }
+        if (CAREFUL || kt < full_lo || kt + BN > full_hi) {
 #pragma unroll
-      for (int r = 0; r < 16; r++) {
-        const int key = kt + 32 * b + acc_row(r, h);
-        bool in = whole || (key >= mine.lo && key < mine.hi);
-        if constexpr (CAREFUL) in = in && !(bad[b] >> acc_row(r, h) & 1);
-        s[b][r] = in ? s[b][r] * a.c : -INFINITY;
-        top = fmaxf(top, s[b][r]);
-      }
-    }
-    top = fmaxf(top, half_swap(top));
-    const float m = fmaxf(st.m, top), base = m == -INFINITY ? 0.f : m;
-    const float keep = exp2_fast(st.m - base);
-    st.m = m;
-    st.l *= keep;
+          for (int b = 0; b < BN / 32; b++) {
 #pragma unroll
-    for (int db = 0; db < DP / 32; db++) {
-#pragma unroll
-      for (int r = 0; r < 16; r++) acc[db][r] *= keep;
-    }
-#pragma unroll
-    for (int b = 0; b < BN / 32; b++) {
-#pragma unroll
-      for (int r = 0; r < 16; r++) {
-        s[b][r] = exp2_fast(s[b][r] - base);
-        st.l += s[b][r];
-      }
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        const V8<T> p = acc_frag<T>(s[b], i);
-#pragma unroll
-        for (int db = 0; db < DP / 32; db++) acc[db] = mma(col_frag(vs, LD, 32 * b + 16 * i, 32 * db), p, acc[db]);
-      }
-    }
-    if constexpr (CAREFUL) {
-      for (int b = 0; b < BN / 32; b++) {
-        for (uint32_t w = bad[b]; w; w &= w - 1) {
-          const int key = kt + 32 * b + __builtin_ctz(w);
-          if (key >= whi || key < wlo) continue;
-          const float t = frag_dot<T, DP>(qf, k + key * a.k.row, h, a.dim) * a.c;
-          if (key >= mine.lo && key < mine.hi) {
-            const float m1 = fmaxf(st.m, t), base1 = m1 == -INFINITY ? 0.f : m1;
-            const float keep1 = exp2_fast(st.m - base1), p = exp2_fast(t - base1);
-            st.m = m1;
-            st.l = st.l * keep1 + (h == 0 ? p : 0.f);
-            for (int db = 0; db < DP / 32; db++) {
-#pragma unroll
-              for (int r = 0; r < 16; r++) acc[db][r] *= keep1;
+            for (int r = 0; r < 16; r++) {
+              const int key = kt + 32 * b + acc_row(r, h);
+              bool in = (key >= mine.lo) & (key < mine.hi);
+              if constexpr (CAREFUL) in = in & !(bad[b] >> acc_row(r, h) & 1);
+              s[b][r] = in ? s[b][r] : -INFINITY;
             }
-            add_row<T, DP>(acc, p, v + key * a.v.row, h, a.dim);
           }
         }
-      }
-    }
-  }
+        float top = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < BN / 32; b++) {
+#pragma unroll
+          for (int r = 0; r < 16; r++) top = fmaxf(top, s[b][r]);
+        }
+        top = half_max(top) * a.c;
+        if (__any(top > st.m + kLag)) rescale(st, fmaxf(st.m, top), acc);
+        const float base = st.base();
+#pragma unroll
+        for (int b = 0; b < BN / 32; b++) {
+#pragma unroll
+          for (int r = 0; r < 16; r++) {
+            s[b][r] = exp2_fast(fmaf(s[b][r], a.c, -base));
+            st.l += s[b][r];
+          }
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+            const V8<T> p = acc_frag<T>(s[b], i);
+#pragma unroll
+            for (int db = 0; db < DP / 32; db++) acc[db] = mma(L::col_frag(vb, 32 * b + 16 * i, 32 * db), p, acc[db]);
+          }
+        }
+        if constexpr (CAREFUL) {
+          for (int r = 0; r < BN; r++) {
+            const int key = kt + r;
+            if (!(bad[r / 32] >> (r % 32) & 1) || key >= whi || key < wlo) continue;
+            const float t = frag_dot<T, DP>(qf, ks + BN * DP, r, h) * a.c;
+            if (key >= mine.lo && key < mine.hi) {
+              rescale(st, fmaxf(st.m, t), acc);
+              const float p = exp2_fast(t - st.base());
+              st.l += h == 0 ? p : 0.f;
+              add_row<T, DP>(acc, p, vs + BN * DP, r, h);
+            }
+          }
+        }
+      });
 }
 
 // grid: (tiles * kv_heads, splits).  part / stat: the splits' unfinished sums (NULL without splits).
 template <typename T, int DP>
-__global__ void __launch_bounds__(256, 2) attend_fwd_kernel(Attend a, const T *__restrict__ q, const T *__restrict__ k,
+__global__ void __launch_bounds__(256, sizeof(T) == 4 && DP == 128 ? 1 : 2)
+    attend_fwd_kernel(Attend a, const T *__restrict__ q, const T *__restrict__ k,
                                                          const T *__restrict__ v, T *__restrict__ o,
                                                          T *__restrict__ low, float *__restrict__ lse,
                                                          float *__restrict__ part,
                                                          float2 *__restrict__ stat) {
   constexpr int BM = FwdTile<T, DP>::BM, BN = FwdTile<T, DP>::BN;
-  using KV = Stage<T, DP, BN>;
-  __shared__ T ks[BN * KV::LD], vs[BN * KV::LD];
+  __shared__ alignas(16) T ks[2 * BN * DP], vs[2 * BN * DP];
   __shared__ uint32_t bad[BN / 32];
   __shared__ int s_lo[4], s_hi[4], s_redo;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
@@ -182,7 +177,7 @@ __global__ void __launch_bounds__(256, 2) attend_fwd_kernel(Attend a, const T *_
     st = RowState();
     fwd_walk<T, DP, true>(a, kh, vh, begin, end, mine, wlo, whi, full_lo, full_hi, qf, ks, vs, bad, acc, st);
   }
-  const float l = st.l + half_swap(st.l);
+  const float l = half_sum(st.l);
   if (!live) return;
   if (part) {
     const int64_t at = ((int64_t)blockIdx.y * a.kv_heads + head) * total + m;

@@ -105,68 +105,56 @@ __device__ __forceinline__ void dq_walk(const Attend &a, const T *__restrict__ k
                                         int full_hi, const V8<T> (&qf)[DP / 16], const V8<T> (&gf)[DP / 16], T *ks,
                                         T *vs, uint32_t *bad, f32x16 (&acc)[DP / 32]) {
   constexpr int BN = DqTile<T, DP>::BN;
-  using KV = Stage<T, DP, BN>;
-  constexpr int LD = KV::LD;
+  using L = Tile<T, DP>;
   const int lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
-  KV ka, va;
-  ka.load(k, a.k.row, begin, end, a.dim);
-  va.load(v, a.v.row, begin, end, a.dim);
-  for (int kt = begin; kt < end; kt += BN) {
-    __syncthreads();
-    if constexpr (CAREFUL) {
-      if (threadIdx.x < BN / 32) bad[threadIdx.x] = 0;
-      __syncthreads();
-      ka.mark_bad(bad);
-      va.mark_bad(bad);
-      __syncthreads();
-      ka.store_good(ks, bad);
-      va.store_good(vs, bad);
-    } else {
-      ka.store(ks);
-      va.store(vs);
-    }
-    __syncthreads();
-    if (kt + BN < end) {
-      ka.load(k, a.k.row, kt + BN, end, a.dim);
-      va.load(v, a.v.row, kt + BN, end, a.dim);
-    }
-    if (kt >= whi || kt + BN <= wlo) continue;
-    const bool whole = !CAREFUL && kt >= full_lo && kt + BN <= full_hi;
+  stream<T, DP, BN, CAREFUL>(
+      begin, end, ks, vs, bad,
+      [&](auto &x, auto &y, int kt) {
+        x.load(k, a.k.row, kt, end, a.dim);
+        y.load(v, a.v.row, kt, end, a.dim);
+      },
+      [](int) {},
+      [&](int kt, int buffer) {
+        if (kt >= whi || kt + BN <= wlo) return;
+        T *kb = ks + buffer * BN * DP, *vb = vs + buffer * BN * DP;
+        const bool whole = !CAREFUL && kt >= full_lo && kt + BN <= full_hi;
 #pragma unroll
-    for (int b = 0; b < BN / 32; b++) {
-      f32x16 s = {}, dp = {};
+        for (int b = 0; b < BN / 32; b++) {
+          f32x16 s = {}, dp = {};
 #pragma unroll
-      for (int i = 0; i < DP / 16; i++) {
-        s = mma(row_frag(ks, LD, 32 * b + col, 16 * i + 8 * h), qf[i], s);
-        dp = mma(row_frag(vs, LD, 32 * b + col, 16 * i + 8 * h), gf[i], dp);
-      }
+          for (int i = 0; i < DP / 16; i++) {
+            s = mma(L::row_frag(kb, 32 * b + col, 16 * i + 8 * h), qf[i], s);
+            dp = mma(L::row_frag(vb, 32 * b + col, 16 * i + 8 * h), gf[i], dp);
+          }
 #pragma unroll
-      for (int r = 0; r < 16; r++) {
-        const int key = kt + 32 * b + acc_row(r, h);
-        bool in = whole || (key >= mine.x && key < mine.y);
-        if constexpr (CAREFUL) in = in && !(bad[b] >> acc_row(r, h) & 1);
-        s[r] = in ? exp2_fast(fmaf(s[r], a.c, -ld.x)) * (dp[r] - ld.y) * gs : 0.f;
-      }
+          for (int r = 0; r < 16; r++) s[r] = exp2_fast(fmaf(s[r], a.c, -ld.x)) * ((dp[r] - ld.y) * gs);
+          if (!whole) {
 #pragma unroll
-      for (int i = 0; i < 2; i++) {
-        const V8<T> ds = acc_frag<T>(s, i);
+            for (int r = 0; r < 16; r++) {
+              const int key = kt + 32 * b + acc_row(r, h);
+              bool in = (key >= mine.x) & (key < mine.y);
+              if constexpr (CAREFUL) in = in & !(bad[b] >> acc_row(r, h) & 1);
+              s[r] = in ? s[r] : 0.f;
+            }
+          }
 #pragma unroll
-        for (int db = 0; db < DP / 32; db++) acc[db] = mma(col_frag(ks, LD, 32 * b + 16 * i, 32 * db), ds, acc[db]);
-      }
-    }
-    if constexpr (CAREFUL) {
-      for (int b = 0; b < BN / 32; b++) {
-        for (uint32_t w = bad[b]; w; w &= w - 1) {
-          const int key = kt + 32 * b + __builtin_ctz(w);
-          if (key >= whi || key < wlo) continue;
-          const float t = frag_dot<T, DP>(qf, k + key * a.k.row, h, a.dim) * a.c;
-          const float dp = frag_dot<T, DP>(gf, v + key * a.v.row, h, a.dim);
-          if (key >= mine.x && key < mine.y)
-            add_row<T, DP>(acc, exp2_fast(t - ld.x) * (dp - ld.y) * gs, k + key * a.k.row, h, a.dim);
+          for (int i = 0; i < 2; i++) {
+            const V8<T> ds = acc_frag<T>(s, i);
+#pragma unroll
+            for (int db = 0; db < DP / 32; db++) acc[db] = mma(L::col_frag(kb, 32 * b + 16 * i, 32 * db), ds, acc[db]);
+          }
         }
-      }
-    }
-  }
+        if constexpr (CAREFUL) {
+          for (int r = 0; r < BN; r++) {
+            const int key = kt + r;
+            if (!(bad[r / 32] >> (r % 32) & 1) || key >= whi || key < wlo) continue;
+            const float t = frag_dot<T, DP>(qf, ks + BN * DP, r, h) * a.c;
+            const float dp = frag_dot<T, DP>(gf, vs + BN * DP, r, h);
+            if (key >= mine.x && key < mine.y)
+              add_row<T, DP>(acc, exp2_fast(t - ld.x) * (dp - ld.y) * gs, ks + BN * DP, r, h);
+          }
+        }
+      });
 }
 
 template <typename T, int DP>
@@ -174,8 +162,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP == 128 ? 1 : 2)
     attend_dq_kernel(Attend a, Grad g, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
                      const T *__restrict__ go, T *__restrict__ dq) {
   constexpr int BN = DqTile<T, DP>::BN;
-  using KV = Stage<T, DP, BN>;
-  __shared__ T ks[BN * KV::LD], vs[BN * KV::LD];
+  __shared__ alignas(16) T ks[2 * BN * DP], vs[2 * BN * DP];
   __shared__ uint32_t bad[BN / 32];
   __shared__ int s_lo[4], s_hi[4], s_redo;
   __shared__ float s_max[4];
@@ -222,24 +209,6 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP == 128 ? 1 : 2)
   if (live) store_cols<T, DP>(dq + at * a.dim, acc, a.scale / gs, h, a.dim);
 }
 
-// Virtual rows [m0, m0 + ROWS) of a (rows, heads, dim) tensor, one key head's group (Stage with the
-// addresses of virtual rows)
-template <typename T, int DP, int ROWS>
-struct StageRows : Stage<T, DP, ROWS> {
-  using B = Stage<T, DP, ROWS>;
-  __device__ __forceinline__ void load_rows(const T *__restrict__ base, Heads st, int group, int m0, int end, int dim) {
-#pragma unroll
-    for (int i = 0; i < B::PER; i++) {
-      const int at = threadIdx.x + 256 * i, m = m0 + at / B::CH, col = at % B::CH * B::E;
-      this->w[i] = u32x4{0, 0, 0, 0};
-      if (m < end && col < dim) {
-        const int row = (int)((unsigned)m / (unsigned)group);
-        this->w[i] = *reinterpret_cast<const u32x4 *>(base + row * st.row + (m - row * group) * st.head + col);
-      }
-    }
-  }
-};
-
 template <typename T, int DP>
 struct DkvTile {
   static constexpr int BQ = sizeof(T) == 4 ? 32 : 64;  // virtual rows per step
@@ -252,100 +221,85 @@ __device__ __forceinline__ void dkv_walk(const Attend &a, const Grad &g, const T
                                          float2 *s_ld, int2 *s_range, uint32_t *bad, f32x16 (&dk)[DP / 32],
                                          f32x16 (&dv)[DP / 32]) {
   constexpr int BQ = DkvTile<T, DP>::BQ;
-  using Q = StageRows<T, DP, BQ>;
-  constexpr int LD = Q::B::LD;
+  using L = Tile<T, DP>;
   const int lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
   const int heads = a.kv_heads * a.group, key = key0 + col;
   const Range none = no_keys();
-  Q qa, oa;
   float2 ld = make_float2(0, 0);
   int2 range = make_int2(none.lo, none.hi);
-  auto load = [&](int mt) {
-    qa.load_rows(q, a.q, a.group, mt, end, a.dim);
-    oa.load_rows(go, gst, a.group, mt, end, a.dim);
-    const int m = mt + (int)threadIdx.x;
-    if (threadIdx.x < BQ) {
-      const bool live = m < end;
-      const int row = live ? (int)((unsigned)m / (unsigned)a.group) : 0;
-      ld = live ? g.ld[(int64_t)row * heads + head * a.group + (m - row * a.group)] : make_float2(0, 0);
-      range = live ? g.range[row] : make_int2(none.lo, none.hi);
-    }
-  };
-  if (begin < end) load(begin);
-  for (int mt = begin; mt < end; mt += BQ) {
-    __syncthreads();
-    if constexpr (CAREFUL) {
-      if (threadIdx.x < BQ / 32) bad[threadIdx.x] = 0;
-      __syncthreads();
-      qa.mark_bad(bad);
-      oa.mark_bad(bad);
-      __syncthreads();
-      qa.store_good(qs, bad);
-      oa.store_good(os, bad);
-    } else {
-      qa.store(qs);
-      oa.store(os);
-    }
-    if (threadIdx.x < BQ) {
-      s_ld[threadIdx.x] = ld;
-      s_range[threadIdx.x] = range;
-    }
-    __syncthreads();
-    if (mt + BQ < end) load(mt + BQ);
-    const int2 mine = s_range[lane % BQ];
-    if (!__any(mine.x < key0 + 32 && mine.y > key0)) continue;
-    const bool whole = !CAREFUL && __all(mine.x <= key0 && mine.y >= key0 + 32);
-#pragma unroll
-    for (int b = 0; b < BQ / 32; b++) {
-      f32x16 s = {}, dp = {};
-#pragma unroll
-      for (int i = 0; i < DP / 16; i++) {
-        s = mma(row_frag(qs, LD, 32 * b + col, 16 * i + 8 * h), kf[i], s);
-        dp = mma(row_frag(os, LD, 32 * b + col, 16 * i + 8 * h), vf[i], dp);
-      }
-#pragma unroll
-      for (int r = 0; r < 16; r++) {
-        const int i = 32 * b + acc_row(r, h);
-        const float2 x = s_ld[i];
-        bool in = true;
-        if (!whole) {
-          const int2 kr = s_range[i];
-          in = key >= kr.x && key < kr.y;
+  stream<T, DP, BQ, CAREFUL>(
+      begin, end, qs, os, bad,
+      [&](auto &x, auto &y, int mt) {
+        x.load_virtual(q, a.q, a.group, mt, end, a.dim);
+        y.load_virtual(go, gst, a.group, mt, end, a.dim);
+        if (threadIdx.x < BQ) {
+          const int m = mt + (int)threadIdx.x;
+          const bool live = m < end;
+          const int row = live ? (int)((unsigned)m / (unsigned)a.group) : 0;
+          ld = live ? g.ld[(int64_t)row * heads + head * a.group + (m - row * a.group)] : make_float2(0, 0);
+          range = live ? g.range[row] : make_int2(none.lo, none.hi);
         }
-        if constexpr (CAREFUL) in = in && !(bad[b] >> acc_row(r, h) & 1);
-        const float p = in ? exp2_fast(fmaf(s[r], a.c, -x.x)) : 0.f;
-        s[r] = p;
-        dp[r] = in ? p * (dp[r] - x.y) * gs : 0.f;
-      }
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        const V8<T> p = acc_frag<T>(s, i), ds = acc_frag<T>(dp, i);
-#pragma unroll
-        for (int db = 0; db < DP / 32; db++) {
-          dv[db] = mma(col_frag(os, LD, 32 * b + 16 * i, 32 * db), p, dv[db]);
-          dk[db] = mma(col_frag(qs, LD, 32 * b + 16 * i, 32 * db), ds, dk[db]);
+      },
+      [&](int buffer) {
+        if (threadIdx.x < BQ) {
+          s_ld[buffer * BQ + threadIdx.x] = ld;
+          s_range[buffer * BQ + threadIdx.x] = range;
         }
-      }
-    }
-    if constexpr (CAREFUL) {
-      for (int b = 0; b < BQ / 32; b++) {
-        for (uint32_t w = bad[b]; w; w &= w - 1) {
-          const int i = 32 * b + __builtin_ctz(w), m = mt + i;
-          const int row = (int)((unsigned)m / (unsigned)a.group), sub = m - row * a.group;
-          const T *qrow = q + row * a.q.row + sub * a.q.head, *grow = go + row * gst.row + sub * gst.head;
-          const float2 x = s_ld[i];
-          const int2 kr = s_range[i];
-          if (kr.x >= key0 + 32 || kr.y <= key0) continue;
-          const float t = frag_dot<T, DP>(kf, qrow, h, a.dim) * a.c, dpx = frag_dot<T, DP>(vf, grow, h, a.dim);
-          if (key >= kr.x && key < kr.y) {
-            const float p = exp2_fast(t - x.x);
-            add_row<T, DP>(dv, p, grow, h, a.dim);
-            add_row<T, DP>(dk, p * (dpx - x.y) * gs, qrow, h, a.dim);
+      },
+      [&](int mt, int buffer) {
+        const int slot = buffer * BQ;
+        const int2 mine = s_range[slot + lane % BQ];
+        if (!__any(mine.x < key0 + 32 && mine.y > key0)) return;
+        const bool whole = !CAREFUL && __all(mine.x <= key0 && mine.y >= key0 + 32);
+        T *qb = qs + buffer * BQ * DP, *ob = os + buffer * BQ * DP;
+#pragma unroll
+        for (int b = 0; b < BQ / 32; b++) {
+          f32x16 s = {}, dp = {};
+#pragma unroll
+          for (int i = 0; i < DP / 16; i++) {
+            s = mma(L::row_frag(qb, 32 * b + col, 16 * i + 8 * h), kf[i], s);
+            dp = mma(L::row_frag(ob, 32 * b + col, 16 * i + 8 * h), vf[i], dp);
+          }
+#pragma unroll
+          for (int r = 0; r < 16; r++) {
+            const float2 x = s_ld[slot + 32 * b + acc_row(r, h)];
+            s[r] = exp2_fast(fmaf(s[r], a.c, -x.x));
+            dp[r] = s[r] * ((dp[r] - x.y) * gs);
+          }
+          if (!whole) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+              const int2 kr = s_range[slot + 32 * b + acc_row(r, h)];
+              bool in = (key >= kr.x) & (key < kr.y);
+              if constexpr (CAREFUL) in = in & !(bad[b] >> acc_row(r, h) & 1);
+              s[r] = in ? s[r] : 0.f;
+              dp[r] = in ? dp[r] : 0.f;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+            const V8<T> p = acc_frag<T>(s, i), ds = acc_frag<T>(dp, i);
+#pragma unroll
+            for (int db = 0; db < DP / 32; db++) {
+              dv[db] = mma(L::col_frag(ob, 32 * b + 16 * i, 32 * db), p, dv[db]);
+              dk[db] = mma(L::col_frag(qb, 32 * b + 16 * i, 32 * db), ds, dk[db]);
+            }
           }
         }
-      }
-    }
-  }
+        if constexpr (CAREFUL) {
+          for (int r = 0; r < BQ; r++) {
+            const int2 kr = s_range[slot + r];
+            if (!(bad[r / 32] >> (r % 32) & 1) || kr.x >= key0 + 32 || kr.y <= key0) continue;
+            const float2 x = s_ld[slot + r];
+            const float t = frag_dot<T, DP>(kf, qs + BQ * DP, r, h) * a.c, dpx = frag_dot<T, DP>(vf, os + BQ * DP, r, h);
+            if (key >= kr.x && key < kr.y) {
+              const float p = exp2_fast(t - x.x);
+              add_row<T, DP>(dv, p, os + BQ * DP, r, h);
+              add_row<T, DP>(dk, p * (dpx - x.y) * gs, qs + BQ * DP, r, h);
+            }
+          }
+        }
+      });
 }
 
 // The query rows that see any of keys [j0, j1)
@@ -374,10 +328,9 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2)
                       const T *__restrict__ go, T *__restrict__ dk_out, T *__restrict__ dv_out,
                       float *__restrict__ part) {
   constexpr int BQ = DkvTile<T, DP>::BQ;
-  using Q = StageRows<T, DP, BQ>;
-  __shared__ T qs[BQ * Q::B::LD], os[BQ * Q::B::LD];
-  __shared__ float2 s_ld[BQ];
-  __shared__ int2 s_range[BQ];
+  __shared__ alignas(16) T qs[2 * BQ * DP], os[2 * BQ * DP];
+  __shared__ float2 s_ld[2 * BQ];
+  __shared__ int2 s_range[2 * BQ];
   __shared__ uint32_t bad[BQ / 32];
   __shared__ int s_redo;
   __shared__ float s_max[4];

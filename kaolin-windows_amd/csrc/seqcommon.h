@@ -81,43 +81,59 @@ __device__ __forceinline__ V8<T> acc_frag(const f32x16 &acc, int s) {
   return __builtin_convertvector(v, V8<T>);
 }
 
-// Row fragment of a row-major LDS tile: element e = tile[row][col + e].
-template <typename T>
-__device__ __forceinline__ V8<T> row_frag(const T *tile, int ld, int row, int col) {
-  if constexpr (sizeof(T) == 4) {
-    const f32x4 a = *reinterpret_cast<const f32x4 *>(tile + row * ld + col);
-    const f32x4 b = *reinterpret_cast<const f32x4 *>(tile + row * ld + col + 4);
-    return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-  } else {
-    return *reinterpret_cast<const V8<T> *>(tile + row * ld + col);
+// A tile of rows of DP elements in LDS, its 16-byte pieces shuffled within each row so that both ways of
+// reading it spread over the 64 banks: piece p of row r lies at place p ^ swizzle(r).  A row fragment
+// reads one piece of 32 rows (16 at a time: all 16 places of the bank row must differ), a column fragment of a
+// 16-bit type four neighbouring pieces of four rows (again 16 places), of float 32 neighbouring words of
+// two rows four apart.
+template <typename T, int DP>
+struct Tile {
+  static constexpr int E = 16 / (int)sizeof(T);  // elements per piece
+  __device__ static __forceinline__ int swizzle(int r) {
+    if constexpr (sizeof(T) == 4) return DP >= 64 ? (((r >> 2) & 1) << 3) | (((r >> 3) & 1) << 2) | (r & 3) : (r >> 1) & 7;
+    if constexpr (DP == 128) return ((r & 3) << 2) | ((r >> 2) & 3);
+    if constexpr (DP == 64) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+    return (r >> 2) & 3;
   }
-}
+  // the place of piece p of row r
+  __device__ static __forceinline__ int piece(int r, int p) { return r * DP + (p ^ swizzle(r)) * E; }
+  __device__ static __forceinline__ int at(int r, int c) { return piece(r, c / E) + c % E; }
 
-// Column fragment: element e = tile[row0 + acc_row(e, h)][col0 + l % 32], the A operand of the
-// transposed tile whose inner indices are in the order of acc_frag.  16-bit types: the transposed LDS
-// read gives lane i of 16 the column i of a 4 x 16 block whose rows four lanes each address, which is
-// just the run of four rows that acc_row holds together.
-template <typename T>
-__device__ __forceinline__ V8<T> col_frag(T *tile, int ld, int row0, int col0) {
-  const int l = threadIdx.x & 63, h = l >> 5;
-  if constexpr (sizeof(T) == 4) {
-    f32x8 v;
-#pragma unroll
-    for (int e = 0; e < 8; e++) v[e] = tile[(row0 + acc_row(e, h)) * ld + col0 + (l & 31)];
-    return v;
-  } else {
-    const int i = l & 15;
-    T *p = tile + (row0 + 4 * h + i / 4) * ld + col0 + (l & 16) + (i & 3) * 4;
-    typedef __attribute__((address_space(3))) i16x4 lds4;
-    union {
-      i16x4 u[2];
-      V8<T> v;
-    } x;
-    x.u[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(p));
-    x.u[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(p + 8 * ld));
-    return x.v;
+  // Row fragment: element e = tile[row][col + e].
+  __device__ static __forceinline__ V8<T> row_frag(const T *tile, int row, int col) {
+    if constexpr (sizeof(T) == 4) {
+      const f32x4 a = *reinterpret_cast<const f32x4 *>(tile + piece(row, col / 4));
+      const f32x4 b = *reinterpret_cast<const f32x4 *>(tile + piece(row, col / 4 + 1));
+      return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    } else {
+      return *reinterpret_cast<const V8<T> *>(tile + piece(row, col / 8));
+    }
   }
-}
+
+  // Column fragment: element e = tile[row0 + acc_row(e, h)][col0 + l % 32], the A operand of the transposed
+  // tile whose inner indices are in the order of acc_frag.  16-bit types: the transposed LDS read gives lane
+  // i of 16 the column i of a 4 x 16 block whose rows four lanes each address, which is just the run of four
+  // rows that acc_row holds together.
+  __device__ static __forceinline__ V8<T> col_frag(T *tile, int row0, int col0) {
+    const int l = threadIdx.x & 63, h = l >> 5;
+    if constexpr (sizeof(T) == 4) {
+      f32x8 v;
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] = tile[at(row0 + acc_row(e, h), col0 + (l & 31))];
+      return v;
+    } else {
+      const int i = l & 15, r = row0 + 4 * h + i / 4, c = col0 + (l & 16) + (i & 3) * 4;
+      typedef __attribute__((address_space(3))) i16x4 lds4;
+      union {
+        i16x4 u[2];
+        V8<T> v;
+      } x;
+      x.u[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(tile + at(r, c)));
+      x.u[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(tile + at(r + 8, c)));
+      return x.v;
+    }
+  }
+};
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float log2_fast(float x) { return __builtin_amdgcn_logf(x); }
@@ -125,8 +141,15 @@ constexpr float kLog2e = 1.44269504088896340736f;
 
 __device__ __forceinline__ bool finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
 
-// the other half's value of the same column: lanes l and l ^ 32
-__device__ __forceinline__ float half_swap(float v) { return __shfl_xor(v, 32); }
+// sum and maximum over the two halves that hold a column: lanes l and l ^ 32
+__device__ __forceinline__ float half_sum(float v) {
+  const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(x[0]) + __uint_as_float(x[1]);
+}
+__device__ __forceinline__ float half_max(float v) {
+  const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+}
 
 // Strided heads: element (row, head, i) of a (rows, heads, dim) tensor lies at row * row_stride +
 // head * head_stride + i.
