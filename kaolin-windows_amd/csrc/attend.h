@@ -5,6 +5,8 @@
 
 namespace kl {
 
+constexpr int64_t kMaxStride = 1 << 25;  // elements from row to row: 32 rows of floats span under 2^32 bytes
+
 // One attention call.  The query heads g = 0 .. group - 1 of key head m are its heads m * group + g, and
 // the (row, g) of one key head are numbered as virtual rows row * group + g: they share keys and values,
 // so one tile of virtual rows serves a whole group, and a single query row with its group still fills
@@ -16,6 +18,14 @@ struct Attend {
   int kv_heads, group, dim, causal;
   float scale, c;     // c = scale * log2(e): exponentials are base 2
 };
+
+// Whether waves walk by themselves, operands straight from memory (attend32.h): float with small heads, whose
+// registers allow it.  Waves of a workgroup.
+template <typename T, int DP>
+constexpr bool kDirect = sizeof(T) == 4 && DP == 32;
+template <typename T, int DP>
+constexpr int kWaves = kDirect<T, DP> ? 1 : 4;
+inline bool is_direct(kl_dtype dtype, int dim) { return dtype == KL_F32 && dim <= 32; }
 
 // The keys [lo, hi) that query row `row` sees: those of its pack; causal: the pack's last query sees all,
 // and each query before it one key fewer.  No key: lo = INT_MAX, hi = INT_MIN.
@@ -38,7 +48,7 @@ struct Stage {
   static constexpr int CH = DP * (int)sizeof(T) / 16;  // pieces per row
   static constexpr int PER = ROWS * CH / 256;
   static constexpr int E = 16 / (int)sizeof(T);
-  static constexpr int SIZE = ROWS * DP;
+  static constexpr int SIZE = ROWS * Tile<T, DP>::LD;
   static_assert(ROWS * CH % 256 == 0, "whole pieces per thread");
   u32x4 w[PER];
 
@@ -49,19 +59,6 @@ struct Stage {
       const int at = threadIdx.x + 256 * i, row = row0 + at / CH, col = at % CH * E;
       w[i] = u32x4{0, 0, 0, 0};
       if (row < end && col < dim) w[i] = *reinterpret_cast<const u32x4 *>(base + row * stride + col);
-    }
-  }
-  // the same of virtual rows (Attend): row / group of head row % group
-  __device__ __forceinline__ void load_virtual(const T *__restrict__ base, Heads st, int group, int row0, int end,
-                                               int dim) {
-#pragma unroll
-    for (int i = 0; i < PER; i++) {
-      const int at = threadIdx.x + 256 * i, m = row0 + at / CH, col = at % CH * E;
-      w[i] = u32x4{0, 0, 0, 0};
-      if (m < end && col < dim) {
-        const int row = (int)((unsigned)m / (unsigned)group);
-        w[i] = *reinterpret_cast<const u32x4 *>(base + row * st.row + (m - row * group) * st.head + col);
-      }
     }
   }
   __device__ __forceinline__ void store(T *tile) const {
@@ -90,11 +87,11 @@ struct Stage {
   }
 };
 
-// Two tiles of ROWS rows streaming past a workgroup, x and y, in two LDS buffers each.  While one pair is
-// computed on, the next is on its way from memory to registers; one barrier a step.
+// Two tiles of ROWS rows streaming past a workgroup, x and y, in two LDS buffers each, steps [begin, end).
+// While one pair is computed on, the next is on its way from memory to registers; one barrier a step.
+// load(x, y, t) starts the loads of step t, commit(buffer) stores what it kept besides the tiles.
 // CAREFUL (rows that hold infinities or NaN are taken out): buffer 0 has the rows with the bad ones as
 // zeros, buffer 1 all of them as they are, `bad` says which.
-// load(x, y, t) starts the loads of step t, commit(buffer) stores what it kept besides the tiles.
 template <typename T, int DP, int ROWS, bool CAREFUL, typename LOAD, typename COMMIT, typename STEP>
 __device__ __forceinline__ void stream(int begin, int end, T *xs, T *ys, uint32_t *bad, LOAD load, COMMIT commit,
                                        STEP step) {
@@ -103,7 +100,7 @@ __device__ __forceinline__ void stream(int begin, int end, T *xs, T *ys, uint32_
   St x, y;
   load(x, y, begin);
   if constexpr (CAREFUL) {
-    for (int t = begin; t < end; t += ROWS) {
+    for (int t = begin; t < end; t++) {
       __syncthreads();  // the step before is done with the buffers
       if (threadIdx.x < ROWS / 32) bad[threadIdx.x] = 0;
       __syncthreads();
@@ -116,7 +113,7 @@ __device__ __forceinline__ void stream(int begin, int end, T *xs, T *ys, uint32_
       y.store(ys + St::SIZE);
       commit(0);
       __syncthreads();
-      if (t + ROWS < end) load(x, y, t + ROWS);
+      if (t + 1 < end) load(x, y, t + 1);
       step(t, 0);
     }
   } else {
@@ -124,16 +121,16 @@ __device__ __forceinline__ void stream(int begin, int end, T *xs, T *ys, uint32_
     x.store(xs);
     y.store(ys);
     commit(0);
-    if (begin + ROWS < end) load(x, y, begin + ROWS);
+    if (begin + 1 < end) load(x, y, begin + 1);
     __syncthreads();
     int buffer = 0;
-    for (int t = begin; t < end; t += ROWS) {
+    for (int t = begin; t < end; t++) {
       const int other = buffer ^ 1;
-      if (t + ROWS < end) {
+      if (t + 1 < end) {
         x.store(xs + other * St::SIZE);
         y.store(ys + other * St::SIZE);
         commit(other);
-        if (t + 2 * ROWS < end) load(x, y, t + 2 * ROWS);
+        if (t + 2 < end) load(x, y, t + 2);
       }
       step(t, buffer);
       __syncthreads();
@@ -220,6 +217,30 @@ __device__ __forceinline__ bool all_finite(const f32x16 (&acc)[N]) {
   }
   return ok;
 }
+
+// The running maximum (in the scores' base-2 scale) and sum of a row.  The maximum lags: sums are
+// rescaled only when a score passes it by kLag, for which weights grow to 2^kLag at most (rescaling at every
+// new maximum cost 64 multiplications a tile, a quarter of the arithmetic).
+struct RowState {
+  float m = -INFINITY, l = 0;
+  __device__ __forceinline__ float base() const { return m == -INFINITY ? 0.f : m; }
+};
+constexpr float kLag = 8;
+
+template <int N>
+__device__ __forceinline__ void rescale(RowState &st, float m, f32x16 (&acc)[N]) {
+  const float keep = exp2_fast(st.m - (m == -INFINITY ? 0.f : m));
+  st.m = m;
+  st.l *= keep;
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+#pragma unroll
+    for (int r = 0; r < 16; r++) acc[i][r] *= keep;
+  }
+}
+
+// What is the same in every lane, as such: loops and addresses made of it stay in scalar registers
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 template <typename F>
 int with_dim(int dim, F f) {

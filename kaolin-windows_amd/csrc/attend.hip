@@ -2,7 +2,7 @@
 // keys j of row i's pack, with grouped heads (attend.h).
 //
 // One workgroup of four waves takes 128 virtual rows of one key head and walks the keys that any of them
-// sees, a tile at a time, keeping the running maximum and sum of the softmax in 32 bits.  Scores are
+// sees, a tile at a time (float with heads up to 32: attend32.h), keeping the running maximum and sum of the softmax in 32 bits.  Scores are
 // computed transposed, S^T = K Q^T, so a lane holds one row's scores: the softmax is lane-local but for one
 // exchange with the other half, and the weights are the second product's operand (O^T = V^T P^T) where
 // they lie, without a trip through LDS (seqcommon.h, acc_frag).
@@ -16,55 +16,37 @@
 // product.  Nothing in the main walk guards against that: if an accumulator ends up not finite, the
 // workgroup walks its keys again with the rows of k and v that hold such values taken out of the tiles and
 // added one by one to just the rows that see them.
-#include "attend.h"
+#include "attend32.h"
 
 namespace kl {
 
 template <typename T, int DP>
 struct FwdTile {
-  static constexpr int BM = 128;                         // virtual rows: 32 a wave
+  static constexpr int BM = 32 * kWaves<T, DP>;                  // virtual rows
   static constexpr int BN = sizeof(T) == 4 ? 32 : 64;    // keys
 };
 
-// The running maximum (in the scores' base-2 scale) and sum of a row.  The maximum lags: sums are
-// rescaled only when a score passes it by kLag, for which weights grow to 2^kLag at most (rescaling at every
-// new maximum cost 64 multiplications a tile, a quarter of the arithmetic).
-struct RowState {
-  float m = -INFINITY, l = 0;
-  __device__ __forceinline__ float base() const { return m == -INFINITY ? 0.f : m; }
-};
-constexpr float kLag = 8;
-
-template <int N>
-__device__ __forceinline__ void rescale(RowState &st, float m, f32x16 (&acc)[N]) {
-  const float keep = exp2_fast(st.m - (m == -INFINITY ? 0.f : m));
-  st.m = m;
-  st.l *= keep;
-#pragma unroll
-  for (int i = 0; i < N; i++) {
-#pragma unroll
-    for (int r = 0; r < 16; r++) acc[i][r] *= keep;
-  }
-}
-
 template <typename T, int DP, bool CAREFUL>
-__device__ __forceinline__ void fwd_walk(const Attend &a, const T *__restrict__ k, const T *__restrict__ v, int begin,
+__device__ __forceinline__ void fwd_walk(const Attend &a, const T *__restrict__ k, const T *__restrict__ v, int first,
                                          int end, Range mine, int wlo, int whi, int full_lo, int full_hi,
                                          const V8<T> (&qf)[DP / 16], T *ks, T *vs, uint32_t *bad,
                                          f32x16 (&acc)[DP / 32], RowState &st) {
   constexpr int BN = FwdTile<T, DP>::BN;
+  constexpr int SIZE = Stage<T, DP, BN>::SIZE;
   using L = Tile<T, DP>;
   const int lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
   stream<T, DP, BN, CAREFUL>(
-      begin, end, ks, vs, bad,
-      [&](auto &x, auto &y, int kt) {
+      0, end > first ? (end - first + BN - 1) / BN : 0, ks, vs, bad,
+      [&](auto &x, auto &y, int t) {
+        const int kt = first + t * BN;
         x.load(k, a.k.row, kt, end, a.dim);
         y.load(v, a.v.row, kt, end, a.dim);
       },
       [](int) {},
-      [&](int kt, int buffer) {
+      [&](int t, int buffer) {
+        const int kt = first + t * BN;
         if (kt >= whi || kt + BN <= wlo) return;
-        T *kb = ks + buffer * BN * DP, *vb = vs + buffer * BN * DP;
+        T *kb = ks + buffer * SIZE, *vb = vs + buffer * SIZE;
         f32x16 s[BN / 32];
 #pragma unroll
         for (int b = 0; b < BN / 32; b++) s[b] = f32x16{};
@@ -112,30 +94,32 @@ __device__ __forceinline__ void fwd_walk(const Attend &a, const T *__restrict__ 
           for (int r = 0; r < BN; r++) {
             const int key = kt + r;
             if (!(bad[r / 32] >> (r % 32) & 1) || key >= whi || key < wlo) continue;
-            const float t = frag_dot<T, DP>(qf, ks + BN * DP, r, h) * a.c;
+            const float t = frag_dot<T, DP>(qf, ks + SIZE, r, h) * a.c;
             if (key >= mine.lo && key < mine.hi) {
               rescale(st, fmaxf(st.m, t), acc);
               const float p = exp2_fast(t - st.base());
               st.l += h == 0 ? p : 0.f;
-              add_row<T, DP>(acc, p, vs + BN * DP, r, h);
+              add_row<T, DP>(acc, p, vs + SIZE, r, h);
             }
           }
         }
       });
 }
 
+// The part of keys [begin, end) that split `y` of `n` takes, in whole steps
+__device__ __forceinline__ void take_split(int &begin, int &end, int y, int n, int step) {
+  const int steps = (end - begin + step - 1) / step, share = (steps + n - 1) / n * step;
+  begin = (int)min((int64_t)end, begin + (int64_t)share * y);
+  end = (int)min((int64_t)end, (int64_t)begin + share);
+}
+
 // grid: (tiles * kv_heads, splits).  part / stat: the splits' unfinished sums (NULL without splits).
 template <typename T, int DP>
-__global__ void __launch_bounds__(256, sizeof(T) == 4 && DP == 128 ? 1 : 2)
-    attend_fwd_kernel(Attend a, const T *__restrict__ q, const T *__restrict__ k,
-                                                         const T *__restrict__ v, T *__restrict__ o,
-                                                         T *__restrict__ low, float *__restrict__ lse,
-                                                         float *__restrict__ part,
-                                                         float2 *__restrict__ stat) {
+__global__ void __launch_bounds__((64 * kWaves<T, DP>), sizeof(T) == 4 && DP == 128 ? 1 : 2)
+    attend_fwd_kernel(Attend a, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
+                      T *__restrict__ o, T *__restrict__ low, float *__restrict__ lse, float *__restrict__ part,
+                      float2 *__restrict__ stat) {
   constexpr int BM = FwdTile<T, DP>::BM, BN = FwdTile<T, DP>::BN;
-  __shared__ alignas(16) T ks[2 * BN * DP], vs[2 * BN * DP];
-  __shared__ uint32_t bad[BN / 32];
-  __shared__ int s_lo[4], s_hi[4], s_redo;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
   const int head = blockIdx.x % a.kv_heads;
   const int64_t total = (int64_t)a.nq * a.group;
@@ -144,23 +128,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP == 128 ? 1 : 2)
   const bool live = m < total;
   const int row = live ? (int)(m / a.group) : 0, qhead = head * a.group + (live ? (int)(m % a.group) : 0);
   const Range mine = live ? key_range(a, row) : no_keys();
-  const int wlo = min_over(mine.lo), whi = max_over(mine.hi);
-  const int full_lo = max_over(mine.lo), full_hi = min_over(mine.hi);
-  if (lane == 0) {
-    s_lo[wave] = wlo;
-    s_hi[wave] = whi;
-  }
-  if (threadIdx.x == 0) s_redo = 0;
-  __syncthreads();
-  int begin = min(min(s_lo[0], s_lo[1]), min(s_lo[2], s_lo[3]));
-  int end = max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3]));
-  if (begin >= end) begin = end = 0;
-  if (part) {  // this split's share of the keys, whole tiles
-    const int tiles_here = (end - begin + BN - 1) / BN, n = (int)gridDim.y;
-    const int share = (tiles_here + n - 1) / n * BN;
-    begin = (int)min((int64_t)end, begin + (int64_t)share * blockIdx.y);
-    end = (int)min((int64_t)end, (int64_t)begin + share);
-  }
+  const int wlo = uniform(min_over(mine.lo)), whi = uniform(max_over(mine.hi));
+  const int full_lo = uniform(max_over(mine.lo)), full_hi = uniform(min_over(mine.hi));
   V8<T> qf[DP / 16];
   const T *qrow = q + row * a.q.row + qhead * a.q.head;
 #pragma unroll
@@ -168,14 +137,40 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP == 128 ? 1 : 2)
   const T *kh = k + head * a.k.head, *vh = v + head * a.v.head;
   f32x16 acc[DP / 32] = {};
   RowState st;
-  fwd_walk<T, DP, false>(a, kh, vh, begin, end, mine, wlo, whi, full_lo, full_hi, qf, ks, vs, bad, acc, st);
-  if (!(all_finite(acc) && finite(st.l))) s_redo = 1;
-  __syncthreads();
-  if (s_redo) {
+  if constexpr (kDirect<T, DP>) {
+    int begin = wlo, end = whi;
+    if (begin >= end) begin = end = 0;
+    if (part) take_split(begin, end, blockIdx.y, gridDim.y, BN);
+    fwd_walk32<DP, false>(a, kh, vh, begin, end, mine, full_lo, full_hi, qf, acc, st);
+    if (__any(!(all_finite(acc) && finite(st.l)))) {
 #pragma unroll
-    for (int db = 0; db < DP / 32; db++) acc[db] = f32x16{};
-    st = RowState();
-    fwd_walk<T, DP, true>(a, kh, vh, begin, end, mine, wlo, whi, full_lo, full_hi, qf, ks, vs, bad, acc, st);
+      for (int db = 0; db < DP / 32; db++) acc[db] = f32x16{};
+      st = RowState();
+      fwd_walk32<DP, true>(a, kh, vh, begin, end, mine, full_lo, full_hi, qf, acc, st);
+    }
+  } else {
+    __shared__ alignas(16) T ks[2 * Stage<T, DP, BN>::SIZE], vs[2 * Stage<T, DP, BN>::SIZE];
+    __shared__ uint32_t bad[BN / 32];
+    __shared__ int s_lo[4], s_hi[4], s_redo;
+    if (lane == 0) {
+      s_lo[wave] = wlo;
+      s_hi[wave] = whi;
+    }
+    if (threadIdx.x == 0) s_redo = 0;
+    __syncthreads();
+    int begin = uniform(min(min(s_lo[0], s_lo[1]), min(s_lo[2], s_lo[3])));
+    int end = uniform(max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3])));
+    if (begin >= end) begin = end = 0;
+    if (part) take_split(begin, end, blockIdx.y, gridDim.y, BN);
+    fwd_walk<T, DP, false>(a, kh, vh, begin, end, mine, wlo, whi, full_lo, full_hi, qf, ks, vs, bad, acc, st);
+    if (!(all_finite(acc) && finite(st.l))) s_redo = 1;
+    __syncthreads();
+    if (s_redo) {
+#pragma unroll
+      for (int db = 0; db < DP / 32; db++) acc[db] = f32x16{};
+      st = RowState();
+      fwd_walk<T, DP, true>(a, kh, vh, begin, end, mine, wlo, whi, full_lo, full_hi, qf, ks, vs, bad, acc, st);
+    }
   }
   const float l = half_sum(st.l);
   if (!live) return;
@@ -273,12 +268,14 @@ __global__ void __launch_bounds__(256) attend_join_kernel(Attend a, int splits, 
   if (lse && d == 0) lse[out] = l == 0 ? 0.f : top + log2_fast(l);
 }
 
-// Splits of the keys: enough workgroups for the 256 CUs where the rows alone give few, and at least
-// two tiles of keys for each of them if the rows' packs shared the keys evenly.
-static int attend_splits(int64_t nq, int64_t nk, int kv_heads, int group, int bn) {
-  const int64_t blocks = cdiv(nq * group, 128) * kv_heads;
-  if (blocks >= 512) return 1;
-  return (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(1024, std::max<int64_t>(blocks, 1)), cdiv(nk, 2 * bn), kMaxSplits}));
+// Splits of the keys: enough waves for the chip's 1024 SIMDs where the rows alone give few, and at least two
+// tiles of keys for each of them if one pack held all keys.
+static int attend_splits(kl_dtype dtype, int64_t nq, int64_t nk, int kv_heads, int group, int dim) {
+  const int waves = is_direct(dtype, dim) ? 1 : 4, step = dtype == KL_F32 ? 32 : 64;
+  const int64_t blocks = cdiv(nq * group, 32 * waves) * kv_heads;
+  if (blocks * waves >= 2048) return 1;
+  return (int)std::max<int64_t>(
+      1, std::min<int64_t>({cdiv(4096, std::max<int64_t>(blocks * waves, 1)), cdiv(nk, 2 * step), kMaxSplits}));
 }
 
 int fill_attend(Attend &a, const char *func, int64_t nq, int64_t nk, int heads, int kv_heads, int dim,
@@ -292,9 +289,12 @@ int fill_attend(Attend &a, const char *func, int64_t nq, int64_t nk, int heads, 
   KL_REQUIRE(scale > 0 && scale < INFINITY, f + "the scale must be positive and finite");
   // virtual rows and workgroups are counted in 31 bits
   KL_REQUIRE(nq * (heads / kv_heads) <= ((int64_t)1 << 31) - 256 &&
-                 cdiv(std::max(nq * (heads / kv_heads), nk), 128) * kv_heads < (int64_t)1 << 31,
+                 cdiv(std::max(nq * (heads / kv_heads), nk), 32) * kv_heads < (int64_t)1 << 31,
              f + "too many rows and heads");
   KL_REQUIRE(nk <= ((int64_t)1 << 31) - 256, f + "rows out of range");
+  for (int i = 0; i < 6; i++) KL_REQUIRE(strides[i] >= 0, f + "negative stride");
+  for (int i = 0; i < 6; i += 2) KL_REQUIRE(strides[i] < kMaxStride, f + "rows lie too far apart");
+  KL_REQUIRE((int64_t)heads * dim < kMaxStride, f + "rows lie too far apart");
   a.q = {strides[0], strides[1]};
   a.k = {strides[2], strides[3]};
   a.v = {strides[4], strides[5]};
@@ -316,13 +316,13 @@ int fill_attend(Attend &a, const char *func, int64_t nq, int64_t nk, int heads, 
 template <typename T, int DP>
 static int attend_forward(const Attend &a, const void *q, const void *k, const void *v, void *o, void *low, float *lse,
                           void *ws, hipStream_t st) {
-  const int splits = attend_splits(a.nq, a.nk, a.kv_heads, a.group, FwdTile<T, DP>::BN);
+  const int splits = attend_splits(sizeof(T) == 4 ? KL_F32 : KL_F16, a.nq, a.nk, a.kv_heads, a.group, a.dim);
   const int64_t total = (int64_t)a.nq * a.group, rows = total * a.kv_heads;
   const unsigned blocks = (unsigned)(cdiv(total, FwdTile<T, DP>::BM) * a.kv_heads);
   float2 *stat = splits > 1 ? (float2 *)ws : nullptr;
   float *part = splits > 1 ? (float *)((char *)ws + al256((size_t)splits * rows * 8)) : nullptr;
-  hipLaunchKernelGGL((attend_fwd_kernel<T, DP>), dim3(blocks, splits), dim3(256), 0, st, a, (const T *)q, (const T *)k,
-                     (const T *)v, (T *)o, (T *)low, lse, part, stat);
+  hipLaunchKernelGGL((attend_fwd_kernel<T, DP>), dim3(blocks, splits), dim3(64 * kWaves<T, DP>), 0, st, a, (const T *)q,
+                     (const T *)k, (const T *)v, (T *)o, (T *)low, lse, part, stat);
   KL_CHECK_LAUNCH();
   if (splits > 1) {
     int lanes = 1, shares = 1;
@@ -342,7 +342,7 @@ using namespace kl;
 extern "C" size_t kl_pack_attention_workspace_bytes(kl_dtype dtype, int64_t num_q, int64_t num_k, int heads,
                                                     int kv_heads, int dim) {
   if (num_q <= 0 || kv_heads <= 0 || heads % kv_heads) return 256;
-  const int splits = attend_splits(num_q, num_k, kv_heads, heads / kv_heads, dtype == KL_F32 ? 32 : 64);
+  const int splits = attend_splits(dtype, num_q, num_k, kv_heads, heads / kv_heads, dim);
   if (splits == 1) return 256;
   const size_t rows = (size_t)num_q * heads;
   return al256((size_t)splits * rows * 8) + al256((size_t)splits * rows * dim * 4);

@@ -4,14 +4,14 @@
 //
 // Two kernels compute the scores again instead of one with atomics on dq: five products become seven, and
 // every sum has a fixed order.  dq: as the forward, the wave's 32 columns are rows of q.  dk / dv: the
-// columns are keys, and virtual rows stream past (attend.h).  Both feed their second products from the
+// columns are keys, and the rows of the group's heads stream past.  Both feed their second products from the
 // accumulators of the first in place (seqcommon.h, acc_frag); the streamed tiles are read from LDS along
 // rows for the first products and along columns for the second.
 // Rounding: p and ds are rounded to the inputs' type for the second products, half a step each; sums stay
 // in 32 bits.  float16 has no exponents for small gradients: there ds is multiplied by a power of two that
 // puts the largest |do| into [16, 32), and the result by its inverse, both exact.
 // Masked places that hold infinities or NaN: as in attend.hip.
-#include "attend.h"
+#include "attend32.h"
 
 namespace kl {
 
@@ -96,27 +96,30 @@ __device__ __forceinline__ float grad_scale(const Grad &g, float *s_max) {
 
 template <typename T, int DP>
 struct DqTile {
-  static constexpr int BN = sizeof(T) == 4 ? 32 : 64;
+  static constexpr int BN = sizeof(T) == 4 || DP == 128 ? 32 : 64;
 };
 
 template <typename T, int DP, bool CAREFUL>
-__device__ __forceinline__ void dq_walk(const Attend &a, const T *__restrict__ k, const T *__restrict__ v, int begin,
+__device__ __forceinline__ void dq_walk(const Attend &a, const T *__restrict__ k, const T *__restrict__ v, int first,
                                         int end, int2 mine, float2 ld, float gs, int wlo, int whi, int full_lo,
                                         int full_hi, const V8<T> (&qf)[DP / 16], const V8<T> (&gf)[DP / 16], T *ks,
                                         T *vs, uint32_t *bad, f32x16 (&acc)[DP / 32]) {
   constexpr int BN = DqTile<T, DP>::BN;
+  constexpr int SIZE = Stage<T, DP, BN>::SIZE;
   using L = Tile<T, DP>;
   const int lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
   stream<T, DP, BN, CAREFUL>(
-      begin, end, ks, vs, bad,
-      [&](auto &x, auto &y, int kt) {
+      0, end > first ? (end - first + BN - 1) / BN : 0, ks, vs, bad,
+      [&](auto &x, auto &y, int t) {
+        const int kt = first + t * BN;
         x.load(k, a.k.row, kt, end, a.dim);
         y.load(v, a.v.row, kt, end, a.dim);
       },
       [](int) {},
-      [&](int kt, int buffer) {
+      [&](int t, int buffer) {
+        const int kt = first + t * BN;
         if (kt >= whi || kt + BN <= wlo) return;
-        T *kb = ks + buffer * BN * DP, *vb = vs + buffer * BN * DP;
+        T *kb = ks + buffer * SIZE, *vb = vs + buffer * SIZE;
         const bool whole = !CAREFUL && kt >= full_lo && kt + BN <= full_hi;
 #pragma unroll
         for (int b = 0; b < BN / 32; b++) {
@@ -148,47 +151,33 @@ __device__ __forceinline__ void dq_walk(const Attend &a, const T *__restrict__ k
           for (int r = 0; r < BN; r++) {
             const int key = kt + r;
             if (!(bad[r / 32] >> (r % 32) & 1) || key >= whi || key < wlo) continue;
-            const float t = frag_dot<T, DP>(qf, ks + BN * DP, r, h) * a.c;
-            const float dp = frag_dot<T, DP>(gf, vs + BN * DP, r, h);
+            const float t = frag_dot<T, DP>(qf, ks + SIZE, r, h) * a.c;
+            const float dp = frag_dot<T, DP>(gf, vs + SIZE, r, h);
             if (key >= mine.x && key < mine.y)
-              add_row<T, DP>(acc, exp2_fast(t - ld.x) * (dp - ld.y) * gs, ks + BN * DP, r, h);
+              add_row<T, DP>(acc, exp2_fast(t - ld.x) * (dp - ld.y) * gs, ks + SIZE, r, h);
           }
         }
       });
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(256, sizeof(T) == 4 && DP == 128 ? 1 : 2)
+__global__ void __launch_bounds__((64 * kWaves<T, DP>), sizeof(T) == 4 && DP == 128 ? 1 : 2)
     attend_dq_kernel(Attend a, Grad g, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
                      const T *__restrict__ go, T *__restrict__ dq) {
   constexpr int BN = DqTile<T, DP>::BN;
-  __shared__ alignas(16) T ks[2 * BN * DP], vs[2 * BN * DP];
-  __shared__ uint32_t bad[BN / 32];
-  __shared__ int s_lo[4], s_hi[4], s_redo;
-  __shared__ float s_max[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
   const int head = blockIdx.x % a.kv_heads, heads = a.kv_heads * a.group;
   const int64_t total = (int64_t)a.nq * a.group;
   const int64_t tiles = gridDim.x / a.kv_heads;
-  const int64_t m = (tiles - 1 - blockIdx.x / a.kv_heads) * 128 + wave * 32 + col;
+  const int64_t m = (tiles - 1 - blockIdx.x / a.kv_heads) * (32 * kWaves<T, DP>) + wave * 32 + col;
   const bool live = m < total;
   const int row = live ? (int)(m / a.group) : 0, qhead = head * a.group + (live ? (int)(m % a.group) : 0);
   const Range none = no_keys();
   const int2 mine = live ? g.range[row] : make_int2(none.lo, none.hi);
   const int64_t at = (int64_t)row * heads + qhead;
   const float2 ld = live ? g.ld[at] : make_float2(0, 0);
-  const int wlo = min_over(mine.x), whi = max_over(mine.y);
-  const int full_lo = max_over(mine.x), full_hi = min_over(mine.y);
-  if (lane == 0) {
-    s_lo[wave] = wlo;
-    s_hi[wave] = whi;
-  }
-  if (threadIdx.x == 0) s_redo = 0;
-  __syncthreads();
-  int begin = min(min(s_lo[0], s_lo[1]), min(s_lo[2], s_lo[3]));
-  int end = max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3]));
-  if (begin >= end) begin = end = 0;
-  const float gs = grad_scale<T>(g, s_max);
+  const int wlo = uniform(min_over(mine.x)), whi = uniform(max_over(mine.y));
+  const int full_lo = uniform(max_over(mine.x)), full_hi = uniform(min_over(mine.y));
   V8<T> qf[DP / 16], gf[DP / 16];
   const T *qrow = q + row * a.q.row + qhead * a.q.head, *grow = go + at * a.dim;
 #pragma unroll
@@ -198,29 +187,56 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP == 128 ? 1 : 2)
   }
   const T *kh = k + head * a.k.head, *vh = v + head * a.v.head;
   f32x16 acc[DP / 32] = {};
-  dq_walk<T, DP, false>(a, kh, vh, begin, end, mine, ld, gs, wlo, whi, full_lo, full_hi, qf, gf, ks, vs, bad, acc);
-  if (!all_finite(acc)) s_redo = 1;
-  __syncthreads();
-  if (s_redo) {
+  float gs = 1;
+  if constexpr (kDirect<T, DP>) {
+    dq_walk32<DP, false>(a, kh, vh, wlo, whi, mine, ld, full_lo, full_hi, qf, gf, acc);
+    if (__any(!all_finite(acc))) {
 #pragma unroll
-    for (int db = 0; db < DP / 32; db++) acc[db] = f32x16{};
-    dq_walk<T, DP, true>(a, kh, vh, begin, end, mine, ld, gs, wlo, whi, full_lo, full_hi, qf, gf, ks, vs, bad, acc);
+      for (int db = 0; db < DP / 32; db++) acc[db] = f32x16{};
+      dq_walk32<DP, true>(a, kh, vh, wlo, whi, mine, ld, full_lo, full_hi, qf, gf, acc);
+    }
+  } else {
+    __shared__ alignas(16) T ks[2 * Stage<T, DP, BN>::SIZE], vs[2 * Stage<T, DP, BN>::SIZE];
+    __shared__ uint32_t bad[BN / 32];
+    __shared__ int s_lo[4], s_hi[4], s_redo;
+    __shared__ float s_max[4];
+    if (lane == 0) {
+      s_lo[wave] = wlo;
+      s_hi[wave] = whi;
+    }
+    if (threadIdx.x == 0) s_redo = 0;
+    gs = grad_scale<T>(g, s_max);
+    __syncthreads();
+    int begin = uniform(min(min(s_lo[0], s_lo[1]), min(s_lo[2], s_lo[3])));
+    int end = uniform(max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3])));
+    if (begin >= end) begin = end = 0;
+    dq_walk<T, DP, false>(a, kh, vh, begin, end, mine, ld, gs, wlo, whi, full_lo, full_hi, qf, gf, ks, vs, bad, acc);
+    if (!all_finite(acc)) s_redo = 1;
+    __syncthreads();
+    if (s_redo) {
+#pragma unroll
+      for (int db = 0; db < DP / 32; db++) acc[db] = f32x16{};
+      dq_walk<T, DP, true>(a, kh, vh, begin, end, mine, ld, gs, wlo, whi, full_lo, full_hi, qf, gf, ks, vs, bad, acc);
+    }
   }
   if (live) store_cols<T, DP>(dq + at * a.dim, acc, a.scale / gs, h, a.dim);
 }
 
 template <typename T, int DP>
 struct DkvTile {
-  static constexpr int BQ = sizeof(T) == 4 ? 32 : 64;  // virtual rows per step
+  static constexpr int KEYS = 32 * kWaves<T, DP>;
+  static constexpr int BQ = sizeof(T) == 4 || DP == 128 ? 32 : 64;  // virtual rows per step
 };
 
 template <typename T, int DP, bool CAREFUL>
 __device__ __forceinline__ void dkv_walk(const Attend &a, const Grad &g, const T *__restrict__ q, Heads gst,
-                                         const T *__restrict__ go, int head, int begin, int end, int key0, float gs,
+                                         const T *__restrict__ go, int head, int begin, int end, Range rows,
+                                         int tiles, int key0, float gs,
                                          const V8<T> (&kf)[DP / 16], const V8<T> (&vf)[DP / 16], T *qs, T *os,
                                          float2 *s_ld, int2 *s_range, uint32_t *bad, f32x16 (&dk)[DP / 32],
                                          f32x16 (&dv)[DP / 32]) {
   constexpr int BQ = DkvTile<T, DP>::BQ;
+  constexpr int SIZE = Stage<T, DP, BQ>::SIZE;
   using L = Tile<T, DP>;
   const int lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
   const int heads = a.kv_heads * a.group, key = key0 + col;
@@ -229,14 +245,14 @@ __device__ __forceinline__ void dkv_walk(const Attend &a, const Grad &g, const T
   int2 range = make_int2(none.lo, none.hi);
   stream<T, DP, BQ, CAREFUL>(
       begin, end, qs, os, bad,
-      [&](auto &x, auto &y, int mt) {
-        x.load_virtual(q, a.q, a.group, mt, end, a.dim);
-        y.load_virtual(go, gst, a.group, mt, end, a.dim);
+      [&](auto &x, auto &y, int t) {
+        const int sub = t / tiles, row0 = rows.lo + (t - sub * tiles) * BQ;
+        x.load(q + sub * a.q.head, a.q.row, row0, rows.hi, a.dim);
+        y.load(go + sub * gst.head, gst.row, row0, rows.hi, a.dim);
         if (threadIdx.x < BQ) {
-          const int m = mt + (int)threadIdx.x;
-          const bool live = m < end;
-          const int row = live ? (int)((unsigned)m / (unsigned)a.group) : 0;
-          ld = live ? g.ld[(int64_t)row * heads + head * a.group + (m - row * a.group)] : make_float2(0, 0);
+          const int row = row0 + (int)threadIdx.x;
+          const bool live = row < rows.hi;
+          ld = live ? g.ld[(int64_t)row * heads + head * a.group + sub] : make_float2(0, 0);
           range = live ? g.range[row] : make_int2(none.lo, none.hi);
         }
       },
@@ -246,12 +262,12 @@ __device__ __forceinline__ void dkv_walk(const Attend &a, const Grad &g, const T
           s_range[buffer * BQ + threadIdx.x] = range;
         }
       },
-      [&](int mt, int buffer) {
+      [&](int, int buffer) {
         const int slot = buffer * BQ;
         const int2 mine = s_range[slot + lane % BQ];
         if (!__any(mine.x < key0 + 32 && mine.y > key0)) return;
         const bool whole = !CAREFUL && __all(mine.x <= key0 && mine.y >= key0 + 32);
-        T *qb = qs + buffer * BQ * DP, *ob = os + buffer * BQ * DP;
+        T *qb = qs + buffer * SIZE, *ob = os + buffer * SIZE;
 #pragma unroll
         for (int b = 0; b < BQ / 32; b++) {
           f32x16 s = {}, dp = {};
@@ -291,18 +307,19 @@ __device__ __forceinline__ void dkv_walk(const Attend &a, const Grad &g, const T
             const int2 kr = s_range[slot + r];
             if (!(bad[r / 32] >> (r % 32) & 1) || kr.x >= key0 + 32 || kr.y <= key0) continue;
             const float2 x = s_ld[slot + r];
-            const float t = frag_dot<T, DP>(kf, qs + BQ * DP, r, h) * a.c, dpx = frag_dot<T, DP>(vf, os + BQ * DP, r, h);
+            const float t = frag_dot<T, DP>(kf, qs + SIZE, r, h) * a.c, dpx = frag_dot<T, DP>(vf, os + SIZE, r, h);
             if (key >= kr.x && key < kr.y) {
               const float p = exp2_fast(t - x.x);
-              add_row<T, DP>(dv, p, os + BQ * DP, r, h);
-              add_row<T, DP>(dk, p * (dpx - x.y) * gs, qs + BQ * DP, r, h);
+              add_row<T, DP>(dv, p, os + SIZE, r, h);
+              add_row<T, DP>(dk, p * (dpx - x.y) * gs, qs + SIZE, r, h);
             }
           }
         }
       });
 }
 
-// The query rows that see any of keys [j0, j1)
+// The query rows that see any of keys [j0, j1).  They stream past as steps, the rows of the group's first head,
+// then of its second, ...
 __device__ __forceinline__ Range row_range(const Attend &a, int j0, int j1) {
   const int first = a.kid[j0], last = a.kid[j1 - 1];
   if (last < 0) return {0, 0};
@@ -315,33 +332,27 @@ __device__ __forceinline__ Range row_range(const Attend &a, int j0, int j1) {
   return {min(r0, r1), r1};
 }
 
-// Virtual rows of each of n splits of `rows`: whole steps
-__device__ __forceinline__ int split_share(int rows, int n, int step) {
-  const int steps = (rows + step - 1) / step;
-  return (steps + n - 1) / n * step;
-}
-
-// grid: (tiles of keys * kv_heads, splits of the virtual rows); part: the splits' sums (NULL without splits)
+// grid: (tiles of keys * kv_heads, splits of the rows); part: the splits' sums (NULL without splits)
 template <typename T, int DP>
-__global__ void __launch_bounds__(256, DP == 128 ? 1 : 2)
+__global__ void __launch_bounds__((64 * kWaves<T, DP>), DP == 128 ? 1 : 2)
     attend_dkv_kernel(Attend a, Grad g, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
                       const T *__restrict__ go, T *__restrict__ dk_out, T *__restrict__ dv_out,
                       float *__restrict__ part) {
-  constexpr int BQ = DkvTile<T, DP>::BQ;
-  __shared__ alignas(16) T qs[2 * BQ * DP], os[2 * BQ * DP];
-  __shared__ float2 s_ld[2 * BQ];
-  __shared__ int2 s_range[2 * BQ];
-  __shared__ uint32_t bad[BQ / 32];
-  __shared__ int s_redo;
-  __shared__ float s_max[4];
+  constexpr int BQ = DkvTile<T, DP>::BQ, KEYS = DkvTile<T, DP>::KEYS;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
   const int head = blockIdx.x % a.kv_heads, heads = a.kv_heads * a.group;
-  const int j0 = blockIdx.x / a.kv_heads * 128, key0 = j0 + wave * 32, key = key0 + col;
+  const int j0 = blockIdx.x / a.kv_heads * KEYS, key0 = j0 + wave * 32, key = key0 + col;
   const bool live = key < a.nk;
-  const Range rows = row_range(a, j0, min(j0 + 128, a.nk));
-  if (threadIdx.x == 0) s_redo = 0;
-  const float gs = grad_scale<T>(g, s_max);
-  __syncthreads();
+  Range rows = row_range(a, j0, min(j0 + KEYS, a.nk));
+  rows = {uniform(rows.lo), uniform(rows.hi)};
+  const int tiles = max(1, (rows.hi - rows.lo + BQ - 1) / BQ);
+  int begin = 0, end = rows.hi > rows.lo ? tiles * a.group : 0;
+  if (part) {
+    const int share = (end + (int)gridDim.y - 1) / (int)gridDim.y;
+    begin = min(end, share * (int)blockIdx.y);
+    end = min(end, begin + share);
+    if (begin >= end) return;  // the join does not ask for it
+  }
   const T *qh = q + (int64_t)head * a.group * a.q.head;
   const Heads gst = {(int64_t)heads * a.dim, a.dim};
   const T *gh = go + (int64_t)head * a.group * a.dim;
@@ -354,20 +365,34 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2)
     vf[i] = global_frag(vrow, live, 16 * i + 8 * h, a.dim);
   }
   f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
-  int begin = rows.lo * a.group, end = rows.hi * a.group;
-  if (part) {
-    const int share = split_share(end - begin, (int)gridDim.y, BQ);
-    begin = (int)min((int64_t)end, begin + (int64_t)share * blockIdx.y);
-    end = (int)min((int64_t)end, (int64_t)begin + share);
-    if (begin >= end) return;  // the join does not ask for it
-  }
-  dkv_walk<T, DP, false>(a, g, qh, gst, gh, head, begin, end, key0, gs, kf, vf, qs, os, s_ld, s_range, bad, dk, dv);
-  if (!(all_finite(dk) && all_finite(dv))) s_redo = 1;
-  __syncthreads();
-  if (s_redo) {
+  float gs = 1;
+  if constexpr (kDirect<T, DP>) {
+    __shared__ RowSums s_row[32];
+    const float2 *ld = g.ld + head * a.group;
+    dkv_walk32<DP, false>(a, qh, gst, gh, ld, heads, g.range, begin, end, rows, tiles, key0, kf, vf, s_row, dk, dv);
+    if (__any(!(all_finite(dk) && all_finite(dv)))) {
 #pragma unroll
-    for (int db = 0; db < DP / 32; db++) dk[db] = dv[db] = f32x16{};
-    dkv_walk<T, DP, true>(a, g, qh, gst, gh, head, begin, end, key0, gs, kf, vf, qs, os, s_ld, s_range, bad, dk, dv);
+      for (int db = 0; db < DP / 32; db++) dk[db] = dv[db] = f32x16{};
+      dkv_walk32<DP, true>(a, qh, gst, gh, ld, heads, g.range, begin, end, rows, tiles, key0, kf, vf, s_row, dk, dv);
+    }
+  } else {
+    __shared__ alignas(16) T qs[2 * Stage<T, DP, BQ>::SIZE], os[2 * Stage<T, DP, BQ>::SIZE];
+    __shared__ float2 s_ld[2 * BQ];
+    __shared__ int2 s_range[2 * BQ];
+    __shared__ uint32_t bad[BQ / 32];
+    __shared__ int s_redo;
+    __shared__ float s_max[4];
+    if (threadIdx.x == 0) s_redo = 0;
+    gs = grad_scale<T>(g, s_max);
+    __syncthreads();
+    dkv_walk<T, DP, false>(a, g, qh, gst, gh, head, begin, end, rows, tiles, key0, gs, kf, vf, qs, os, s_ld, s_range, bad, dk, dv);
+    if (!(all_finite(dk) && all_finite(dv))) s_redo = 1;
+    __syncthreads();
+    if (s_redo) {
+#pragma unroll
+      for (int db = 0; db < DP / 32; db++) dk[db] = dv[db] = f32x16{};
+      dkv_walk<T, DP, true>(a, g, qh, gst, gh, head, begin, end, rows, tiles, key0, gs, kf, vf, qs, os, s_ld, s_range, bad, dk, dv);
+    }
   }
   if (!live) return;
   const int64_t at = ((int64_t)key * a.kv_heads + head) * a.dim;
@@ -384,15 +409,15 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2)
 // The splits of dk and dv added in their order: four elements a thread.
 template <typename T>
 __global__ void __launch_bounds__(256) attend_dkv_join_kernel(Attend a, int splits, int step,
-                                                            const float *__restrict__ part, T *__restrict__ dk,
+                                                            int keys, const float *__restrict__ part, T *__restrict__ dk,
                                                             T *__restrict__ dv) {
   const int64_t all = (int64_t)a.nk * a.kv_heads * a.dim;
   const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (at >= all) return;
-  const int j0 = (int)(at / ((int64_t)a.kv_heads * a.dim)) / 128 * 128;
-  const Range rows = row_range(a, j0, min(j0 + 128, a.nk));
-  const int n = (rows.hi - rows.lo) * a.group, share = split_share(n, splits, step);
-  const int used = n > 0 ? (n + share - 1) / share : 0;
+  const int j0 = (int)(at / ((int64_t)a.kv_heads * a.dim)) / keys * keys;
+  const Range rows = row_range(a, j0, min(j0 + keys, a.nk));
+  const int steps = rows.hi > rows.lo ? (rows.hi - rows.lo + step - 1) / step * a.group : 0;
+  const int share = max(1, (steps + splits - 1) / splits), used = (steps + share - 1) / share;
   f32x4 k = {}, v = {};
 #pragma unroll 4
   for (int s = 0; s < used; s++) {
@@ -403,13 +428,13 @@ __global__ void __launch_bounds__(256) attend_dkv_join_kernel(Attend a, int spli
   *reinterpret_cast<V4<T> *>(dv + at) = __builtin_convertvector(v, V4<T>);
 }
 
-// Splits of the virtual rows that stream past a tile of keys: four workgroups for each of the 256 CUs
-static int dkv_splits(int64_t nq, int64_t nk, int kv_heads, int group, int step) {
-  const int64_t blocks = cdiv(nk, 128) * kv_heads;
-  if (blocks == 0 || blocks >= 1024) return 1;
-  return (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(1024, blocks), cdiv(nq * group, 2 * step), 16}));
+// Splits of the rows that stream past a tile of keys: four waves for each of the 1024 SIMDs
+static int dkv_splits(kl_dtype dtype, int64_t nq, int64_t nk, int kv_heads, int group, int dim) {
+  const int waves = is_direct(dtype, dim) ? 1 : 4, step = dtype == KL_F32 ? 32 : 64;
+  const int64_t all = cdiv(nk, 32 * waves) * kv_heads * waves;
+  if (all == 0 || all >= 4096) return 1;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(4096, all), cdiv(nq, 2 * step) * group, 16}));
 }
-static int dkv_step(kl_dtype dtype) { return dtype == KL_F32 ? 32 : 64; }
 
 // lanes per (row, head) of the first kernel: 16 bytes each
 static int prep_lanes(kl_dtype dtype, int dim) { return dim * (dtype == KL_F32 ? 4 : 2) / 16; }
@@ -433,21 +458,22 @@ template <typename T, int DP>
 static int attend_backward(const Attend &a, const Grad &g, const void *q, const void *k, const void *v, const void *go,
                            void *dq, void *dk, void *dv, float *part, hipStream_t st) {
   if (a.nq > 0 && dq) {
-    const unsigned blocks = (unsigned)(cdiv((int64_t)a.nq * a.group, 128) * a.kv_heads);
-    hipLaunchKernelGGL((attend_dq_kernel<T, DP>), dim3(blocks), dim3(256), 0, st, a, g, (const T *)q, (const T *)k,
+    const unsigned blocks = (unsigned)(cdiv((int64_t)a.nq * a.group, 32 * kWaves<T, DP>) * a.kv_heads);
+    hipLaunchKernelGGL((attend_dq_kernel<T, DP>), dim3(blocks), dim3(64 * kWaves<T, DP>), 0, st, a, g, (const T *)q, (const T *)k,
                        (const T *)v, (const T *)go, (T *)dq);
     KL_CHECK_LAUNCH();
   }
   if (a.nk > 0 && dk) {
-    const unsigned blocks = (unsigned)(cdiv(a.nk, 128) * a.kv_heads);
-    const int step = DkvTile<T, DP>::BQ, splits = dkv_splits(a.nq, a.nk, a.kv_heads, a.group, step);
-    hipLaunchKernelGGL((attend_dkv_kernel<T, DP>), dim3(blocks, splits), dim3(256), 0, st, a, g, (const T *)q,
+    constexpr int KEYS = DkvTile<T, DP>::KEYS, step = DkvTile<T, DP>::BQ;
+    const unsigned blocks = (unsigned)(cdiv(a.nk, KEYS) * a.kv_heads);
+    const int splits = dkv_splits(sizeof(T) == 4 ? KL_F32 : KL_F16, a.nq, a.nk, a.kv_heads, a.group, a.dim);
+    hipLaunchKernelGGL((attend_dkv_kernel<T, DP>), dim3(blocks, splits), dim3(64 * kWaves<T, DP>), 0, st, a, g, (const T *)q,
                        (const T *)k, (const T *)v, (const T *)go, (T *)dk, (T *)dv, splits > 1 ? part : nullptr);
     KL_CHECK_LAUNCH();
     if (splits > 1) {
       const int64_t pieces = (int64_t)a.nk * a.kv_heads * a.dim / 4;
       hipLaunchKernelGGL(attend_dkv_join_kernel<T>, dim3((unsigned)cdiv(pieces, 256)), dim3(256), 0, st, a, splits, step,
-                         part, (T *)dk, (T *)dv);
+                         KEYS, part, (T *)dk, (T *)dv);
       KL_CHECK_LAUNCH();
     }
   }
@@ -461,7 +487,7 @@ using namespace kl;
 extern "C" size_t kl_pack_attention_bwd_workspace_bytes(kl_dtype dtype, int64_t num_q, int64_t num_k, int heads,
                                                         int kv_heads, int dim) {
   if (num_q < 0 || num_k < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || dim <= 0) return 256;
-  const int splits = dkv_splits(num_q, num_k, kv_heads, heads / kv_heads, dkv_step(dtype));
+  const int splits = dkv_splits(dtype, num_q, num_k, kv_heads, heads / kv_heads, dim);
   return al256((size_t)num_q * heads * 8) + al256((size_t)num_q * 8) + kMaxParts * 4 +
          (splits > 1 ? (size_t)2 * splits * num_k * kv_heads * dim * 4 : 0);
 }

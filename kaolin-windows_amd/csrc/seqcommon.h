@@ -81,22 +81,23 @@ __device__ __forceinline__ V8<T> acc_frag(const f32x16 &acc, int s) {
   return __builtin_convertvector(v, V8<T>);
 }
 
-// A tile of rows of DP elements in LDS, its 16-byte pieces shuffled within each row so that both ways of
-// reading it spread over the 64 banks: piece p of row r lies at place p ^ swizzle(r).  A row fragment
-// reads one piece of 32 rows (16 at a time: all 16 places of the bank row must differ), a column fragment of a
-// 16-bit type four neighbouring pieces of four rows (again 16 places), of float 32 neighbouring words of
-// two rows four apart.
+// A tile of rows of DP elements in LDS, laid out so that both ways of reading it spread over the 64 banks.  A
+// row fragment reads one 16-byte piece of 32 rows (16 rows at a time: 16 different places of the 256 bytes), a
+// column fragment of a 16-bit type four neighbouring pieces of four rows (again 16 places): piece p of row r lies
+// at place p ^ swizzle(r).  float: rows are a piece longer than DP; its column fragments read 32 neighbouring
+// words of two rows, two places in conflict at most, and its products are too slow for that to matter.
 template <typename T, int DP>
 struct Tile {
   static constexpr int E = 16 / (int)sizeof(T);  // elements per piece
+  static constexpr int LD = sizeof(T) == 4 ? DP + E : DP;
   __device__ static __forceinline__ int swizzle(int r) {
-    if constexpr (sizeof(T) == 4) return DP >= 64 ? (((r >> 2) & 1) << 3) | (((r >> 3) & 1) << 2) | (r & 3) : (r >> 1) & 7;
+    if constexpr (sizeof(T) == 4) return 0;
     if constexpr (DP == 128) return ((r & 3) << 2) | ((r >> 2) & 3);
     if constexpr (DP == 64) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
     return (r >> 2) & 3;
   }
   // the place of piece p of row r
-  __device__ static __forceinline__ int piece(int r, int p) { return r * DP + (p ^ swizzle(r)) * E; }
+  __device__ static __forceinline__ int piece(int r, int p) { return r * LD + (p ^ swizzle(r)) * E; }
   __device__ static __forceinline__ int at(int r, int c) { return piece(r, c / E) + c % E; }
 
   // Row fragment: element e = tile[row][col + e].

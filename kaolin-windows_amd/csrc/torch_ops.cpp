@@ -480,7 +480,7 @@ bool plain_mask(const at::Tensor &b, int64_t rows, const at::Device &dev) {
 bool plain_heads(const at::Tensor &t) {
   const int64_t e = 16 / t.element_size();
   return t.dim() == 3 && (t.numel() == 0 || (t.stride(2) == 1 && t.stride(0) % e == 0 && t.stride(1) % e == 0 &&
-                                             (uintptr_t)t.data_ptr() % 16 == 0));
+                                             t.stride(0) < (int64_t)1 << 25 && (uintptr_t)t.data_ptr() % 16 == 0));
 }
 
 bool any_grad(std::initializer_list<const at::Tensor *> ts) {

@@ -53,10 +53,12 @@ def pack_layout_cuda(boundaries):
 
 
 def usable_heads(t):
-    """(rows, heads, dim) as the kernels read it: rows of a head contiguous and 16-byte aligned."""
+    """(rows, heads, dim) as the kernels read it: rows of a head contiguous, 16-byte aligned, and less than 2^25
+    elements apart."""
     e = 16 // t.element_size()
-    if t.numel() == 0 or (t.stride(2) == 1 and t.stride(0) % e == 0 and t.stride(1) % e == 0 and t.stride(0) >= 0
-                          and t.stride(1) >= 0 and t.data_ptr() % 16 == 0):
+    if t.is_contiguous() and t.data_ptr() % 16 == 0 or (
+            t.stride(2) == 1 and t.stride(0) % e == 0 and t.stride(1) % e == 0 and t.stride(0) < 1 << 25
+            and t.data_ptr() % 16 == 0):
         return t
     return t.contiguous() if not t.is_contiguous() else t.clone()
 
