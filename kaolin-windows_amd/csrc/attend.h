@@ -19,7 +19,7 @@ struct Attend {
   float scale, c;     // c = scale * log2(e): exponentials are base 2
 };
 
-// Whether waves walk by themselves, operands straight from memory (attend32.h): float with small heads, whose
+// Whether waves walk by themselves (attend32.h): float with small heads, whose
 // registers allow it.  Waves of a workgroup.
 template <typename T, int DP>
 constexpr bool kDirect = sizeof(T) == 4 && DP == 32;
@@ -180,15 +180,30 @@ __device__ __forceinline__ void add_row(f32x16 (&acc)[DP / 32], float w, const T
   }
 }
 
-__device__ __forceinline__ int min_over(int v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o));
-  return v;
+// Minimum and maximum over the wave (all lanes active), the same in every lane: rows of 16 lanes, then across
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ int dpp_imax(int v) {
+  return max(v, __builtin_amdgcn_update_dpp(v, v, CTRL, ROW_MASK, 0xf, false));
 }
 __device__ __forceinline__ int max_over(int v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o));
-  return v;
+  v = dpp_imax<0x111, 0xf>(v);
+  v = dpp_imax<0x112, 0xf>(v);
+  v = dpp_imax<0x114, 0xf>(v);
+  v = dpp_imax<0x118, 0xf>(v);
+  v = dpp_imax<0x142, 0xa>(v);
+  v = dpp_imax<0x143, 0xc>(v);
+  return __builtin_amdgcn_readlane(v, 63);
+}
+__device__ __forceinline__ int min_over(int v) { return ~max_over(~v); }
+
+// Virtual row m of a key head
+struct Row {
+  int row, sub;
+};
+__device__ __forceinline__ Row virtual_row(const Attend &a, int m) {
+  if (a.group == 1) return {m, 0};
+  const int row = (int)((unsigned)m / (unsigned)a.group);
+  return {row, m - row * a.group};
 }
 
 // Rows of the transposed accumulators (columns = rows of the output) to memory, four at a time

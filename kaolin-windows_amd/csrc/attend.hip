@@ -113,87 +113,101 @@ __device__ __forceinline__ void take_split(int &begin, int &end, int y, int n, i
   end = (int)min((int64_t)end, (int64_t)begin + share);
 }
 
-// grid: (tiles * kv_heads, splits).  part / stat: the splits' unfinished sums (NULL without splits).
+// What a workgroup keeps in LDS
 template <typename T, int DP>
-__global__ void __launch_bounds__((64 * kWaves<T, DP>), sizeof(T) == 4 && DP == 128 ? 1 : 2)
-    attend_fwd_kernel(Attend a, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
-                      T *__restrict__ o, T *__restrict__ low, float *__restrict__ lse, float *__restrict__ part,
-                      float2 *__restrict__ stat) {
+struct FwdLds {
+  static constexpr int BN = FwdTile<T, DP>::BN;
+  alignas(16) T ks[(kDirect<T, DP> ? 1 : 2) * Stage<T, DP, BN>::SIZE];
+  alignas(16) T vs[kDirect<T, DP> ? 1 : 2 * Stage<T, DP, BN>::SIZE];
+  uint32_t bad[2];
+  int lo[4], hi[4], redo;
+};
+
+struct FwdArgs {
+  const void *q, *k, *v;
+  void *o, *low;
+  float *lse, *part;  // part, stat: the splits' unfinished sums (NULL without splits)
+  float2 *stat;
+};
+
+// One workgroup's rows.  True: something was not finite, and nothing was stored.
+template <typename T, int DP, bool CAREFUL>
+__device__ __forceinline__ bool fwd_rows(const Attend &a, const FwdArgs &p, FwdLds<T, DP> &lds) {
   constexpr int BM = FwdTile<T, DP>::BM, BN = FwdTile<T, DP>::BN;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
-  const int head = blockIdx.x % a.kv_heads;
-  const int64_t total = (int64_t)a.nq * a.group;
-  const int64_t tiles = gridDim.x / a.kv_heads;
-  const int64_t m = (tiles - 1 - blockIdx.x / a.kv_heads) * BM + wave * 32 + col;  // the last rows see most keys
+  const int head = (int)blockIdx.x % a.kv_heads;
+  const int total = a.nq * a.group, tiles = (int)gridDim.x / a.kv_heads;  // virtual rows: under 2^31
+  const int m = (tiles - 1 - (int)blockIdx.x / a.kv_heads) * BM + wave * 32 + col;  // the last rows see most keys
   const bool live = m < total;
-  const int row = live ? (int)(m / a.group) : 0, qhead = head * a.group + (live ? (int)(m % a.group) : 0);
+  const Row at_row = virtual_row(a, live ? m : 0);
+  const int row = at_row.row, qhead = head * a.group + at_row.sub;
   const Range mine = live ? key_range(a, row) : no_keys();
-  const int wlo = uniform(min_over(mine.lo)), whi = uniform(max_over(mine.hi));
-  const int full_lo = uniform(max_over(mine.lo)), full_hi = uniform(min_over(mine.hi));
+  const int wlo = min_over(mine.lo), whi = max_over(mine.hi);
+  const int full_lo = max_over(mine.lo), full_hi = min_over(mine.hi);
   V8<T> qf[DP / 16];
-  const T *qrow = q + row * a.q.row + qhead * a.q.head;
+  const T *qrow = (const T *)p.q + row * a.q.row + qhead * a.q.head;
 #pragma unroll
   for (int i = 0; i < DP / 16; i++) qf[i] = global_frag(qrow, live, 16 * i + 8 * h, a.dim);
-  const T *kh = k + head * a.k.head, *vh = v + head * a.v.head;
+  const T *kh = (const T *)p.k + head * a.k.head, *vh = (const T *)p.v + head * a.v.head;
   f32x16 acc[DP / 32] = {};
   RowState st;
   if constexpr (kDirect<T, DP>) {
     int begin = wlo, end = whi;
     if (begin >= end) begin = end = 0;
-    if (part) take_split(begin, end, blockIdx.y, gridDim.y, BN);
-    fwd_walk32<DP, false>(a, kh, vh, begin, end, mine, full_lo, full_hi, qf, acc, st);
-    if (__any(!(all_finite(acc) && finite(st.l)))) {
-#pragma unroll
-      for (int db = 0; db < DP / 32; db++) acc[db] = f32x16{};
-      st = RowState();
-      fwd_walk32<DP, true>(a, kh, vh, begin, end, mine, full_lo, full_hi, qf, acc, st);
-    }
+    if (p.part) take_split(begin, end, blockIdx.y, gridDim.y, BN);
+    fwd_walk32<DP, CAREFUL>(a, kh, vh, begin, end, mine, full_lo, full_hi, qf, lds.ks, acc, st);
+    if (!CAREFUL && __any(!(all_finite(acc) && finite(st.l)))) return true;
   } else {
-    __shared__ alignas(16) T ks[2 * Stage<T, DP, BN>::SIZE], vs[2 * Stage<T, DP, BN>::SIZE];
-    __shared__ uint32_t bad[BN / 32];
-    __shared__ int s_lo[4], s_hi[4], s_redo;
     if (lane == 0) {
-      s_lo[wave] = wlo;
-      s_hi[wave] = whi;
+      lds.lo[wave] = wlo;
+      lds.hi[wave] = whi;
     }
-    if (threadIdx.x == 0) s_redo = 0;
+    if (CAREFUL) __syncthreads();  // everyone has read lds.redo
+    if (threadIdx.x == 0) lds.redo = 0;
     __syncthreads();
-    int begin = uniform(min(min(s_lo[0], s_lo[1]), min(s_lo[2], s_lo[3])));
-    int end = uniform(max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3])));
+    int begin = uniform(min(min(lds.lo[0], lds.lo[1]), min(lds.lo[2], lds.lo[3])));
+    int end = uniform(max(max(lds.hi[0], lds.hi[1]), max(lds.hi[2], lds.hi[3])));
     if (begin >= end) begin = end = 0;
-    if (part) take_split(begin, end, blockIdx.y, gridDim.y, BN);
-    fwd_walk<T, DP, false>(a, kh, vh, begin, end, mine, wlo, whi, full_lo, full_hi, qf, ks, vs, bad, acc, st);
-    if (!(all_finite(acc) && finite(st.l))) s_redo = 1;
-    __syncthreads();
-    if (s_redo) {
-#pragma unroll
-      for (int db = 0; db < DP / 32; db++) acc[db] = f32x16{};
-      st = RowState();
-      fwd_walk<T, DP, true>(a, kh, vh, begin, end, mine, wlo, whi, full_lo, full_hi, qf, ks, vs, bad, acc, st);
+    if (p.part) take_split(begin, end, blockIdx.y, gridDim.y, BN);
+    fwd_walk<T, DP, CAREFUL>(a, kh, vh, begin, end, mine, wlo, whi, full_lo, full_hi, qf, lds.ks, lds.vs, lds.bad, acc,
+                             st);
+    if (!CAREFUL) {
+      if (!(all_finite(acc) && finite(st.l))) lds.redo = 1;
+      __syncthreads();
+      if (lds.redo) return true;
     }
   }
   const float l = half_sum(st.l);
-  if (!live) return;
-  if (part) {
+  if (!live) return false;
+  if (p.part) {
     const int64_t at = ((int64_t)blockIdx.y * a.kv_heads + head) * total + m;
-    if (h == 0) stat[at] = make_float2(st.m, l);
-    if (st.m != -INFINITY || l != 0) store_cols<float, DP>(part + at * a.dim, acc, 1.f, h, a.dim);
-    return;
+    if (h == 0) p.stat[at] = make_float2(st.m, l);
+    if (st.m != -INFINITY || l != 0) store_cols<float, DP>(p.part + at * a.dim, acc, 1.f, h, a.dim);
+    return false;
   }
   const int64_t at = (int64_t)row * a.kv_heads * a.group + qhead;
   const float w = l == 0 ? 0.f : 1.f / l;  // a row that sees no key: 0
-  store_cols<T, DP>(o + at * a.dim, acc, w, h, a.dim);
+  store_cols<T, DP>((T *)p.o + at * a.dim, acc, w, h, a.dim);
   if constexpr (sizeof(T) == 2) {
-    if (low) {
+    if (p.low) {
 #pragma unroll
       for (int db = 0; db < DP / 32; db++) {
 #pragma unroll
         for (int r = 0; r < 16; r++) acc[db][r] = acc[db][r] * w - (float)(T)(acc[db][r] * w);
       }
-      store_cols<T, DP>(low + at * a.dim, acc, 1.f, h, a.dim);
+      store_cols<T, DP>((T *)p.low + at * a.dim, acc, 1.f, h, a.dim);
     }
   }
-  if (lse && h == 0) lse[at] = l == 0 ? 0.f : st.m + log2_fast(l);
+  if (p.lse && h == 0) p.lse[at] = l == 0 ? 0.f : st.m + log2_fast(l);
+  return false;
+}
+
+// grid: (tiles * kv_heads, splits)
+template <typename T, int DP>
+__global__ void __launch_bounds__((64 * kWaves<T, DP>), (kDirect<T, DP> ? 3 : sizeof(T) == 4 && DP == 128 ? 1 : 2))
+    attend_fwd_kernel(Attend a, FwdArgs p) {
+  __shared__ FwdLds<T, DP> lds;
+  if (fwd_rows<T, DP, false>(a, p, lds)) fwd_rows<T, DP, true>(a, p, lds);
 }
 
 // The splits of one (key head, virtual row) joined: `lanes` threads of eight elements (a power of two), and
@@ -272,10 +286,10 @@ __global__ void __launch_bounds__(256) attend_join_kernel(Attend a, int splits, 
 // tiles of keys for each of them if one pack held all keys.
 static int attend_splits(kl_dtype dtype, int64_t nq, int64_t nk, int kv_heads, int group, int dim) {
   const int waves = is_direct(dtype, dim) ? 1 : 4, step = dtype == KL_F32 ? 32 : 64;
-  const int64_t blocks = cdiv(nq * group, 32 * waves) * kv_heads;
-  if (blocks * waves >= 2048) return 1;
+  const int64_t all = cdiv(nq * group, 32 * waves) * kv_heads * waves;
+  if (all >= 2048) return 1;
   return (int)std::max<int64_t>(
-      1, std::min<int64_t>({cdiv(4096, std::max<int64_t>(blocks * waves, 1)), cdiv(nk, 2 * step), kMaxSplits}));
+      1, std::min<int64_t>({cdiv(4096, std::max<int64_t>(all, 1)), cdiv(nk, 2 * step), kMaxSplits}));
 }
 
 int fill_attend(Attend &a, const char *func, int64_t nq, int64_t nk, int heads, int kv_heads, int dim,
@@ -321,8 +335,8 @@ static int attend_forward(const Attend &a, const void *q, const void *k, const v
   const unsigned blocks = (unsigned)(cdiv(total, FwdTile<T, DP>::BM) * a.kv_heads);
   float2 *stat = splits > 1 ? (float2 *)ws : nullptr;
   float *part = splits > 1 ? (float *)((char *)ws + al256((size_t)splits * rows * 8)) : nullptr;
-  hipLaunchKernelGGL((attend_fwd_kernel<T, DP>), dim3(blocks, splits), dim3(64 * kWaves<T, DP>), 0, st, a, (const T *)q,
-                     (const T *)k, (const T *)v, (T *)o, (T *)low, lse, part, stat);
+  hipLaunchKernelGGL((attend_fwd_kernel<T, DP>), dim3(blocks, splits), dim3(64 * kWaves<T, DP>), 0, st, a,
+                     FwdArgs{q, k, v, o, low, lse, part, stat});
   KL_CHECK_LAUNCH();
   if (splits > 1) {
     int lanes = 1, shares = 1;

@@ -1,135 +1,110 @@
 // attend32.h -- the walks of attention over packs for float with heads up to 32 (attend.hip, attendgrad.hip).
 //
 // A 32 x 32 x 16 product of floats takes the matrix cores 16 times as long as one of a 16-bit type, so
-// feeding them is easy and idle waves are what costs.  Every wave walks by itself: 32 virtual rows (or keys)
-// against just the keys (rows) that they see, operands straight from memory to registers.  Along rows, a
-// lane's fragment is 32 bytes of its row; along columns, the 32 lanes of a half read 128 bytes of one row.  No
-// LDS, no barrier: packs of a few dozen rows, where a workgroup's waves see different keys, do not wait for
-// each other.  attend_rays_train's shapes (311,000 rows, 4 heads of 32): forward 354 -> TBD us against tiles in
-// LDS shared by four waves.
+// feeding them is easy and idle waves are what costs.  Every wave walks by itself, without a barrier: 32 virtual
+// rows (or keys) against just the keys (rows) that they see, so that packs of a few dozen rows, where a
+// workgroup's waves see different keys, do not wait for each other.  A tile of 32 rows goes from memory through
+// registers to LDS of the wave's own, 128 bytes of a row by 8 neighbouring lanes (row fragments straight from
+// memory took the L1 cache one line for each lane).
 //
-// Rows past the end and columns past dim are read from the last ones that exist: their scores are masked and
-// their outputs not stored.  Rows with infinities or NaN: as in attend.hip; the careful walk finds a tile's bad
-// rows from the registers, zeroes them and adds them one by one.
+// Rows past the end are copies of the last one: their scores are masked.  Rows with infinities or NaN: as in
+// attend.hip; the careful walk finds a tile's bad rows in its registers, zeroes them and adds them one by one.
 #pragma once
 
 #include "attend.h"
 
 namespace kl {
 
-// A matrix whose rows are `stride` bytes apart (under 2^27, so 32 rows span less than 2^32), read 32 rows at a
-// time: the tile's address is the same for the whole wave, and a lane's offsets into it stay in registers.
-template <int DP>
+// 32 rows of a matrix whose rows are `stride` bytes apart (under 2^27: the rows of a tile span less than 2^32),
+// on their way to LDS: lane l holds the pieces l % 8 of rows l / 8 + 8 i.  base is the same for the whole wave.
 struct Rows32 {
+  static_assert(Tile<float, 32>::E == 4, "8 pieces a row");
   const char *base;
-  uint32_t stride, col[DP / 16];  // col: this lane's fragments within its row, bytes
-  __device__ __forceinline__ Rows32(const float *p, int64_t row_stride, int h, int dim)
-      : base((const char *)p), stride((uint32_t)row_stride * 4) {
+  uint32_t stride;
+  bool in;  // this lane's piece is one of the row's
+  u32x4 w[4];
+  __device__ __forceinline__ Rows32(const float *p, int64_t row_stride, int dim)
+      : base((const char *)p), stride((uint32_t)row_stride * 4), in((int)(threadIdx.x & 7) * 4 < dim) {
 #pragma unroll
-    for (int i = 0; i < DP / 16; i++) col[i] = 4 * min(16 * i + 8 * h, dim - 8);
+    for (int i = 0; i < 4; i++) w[i] = u32x4{0, 0, 0, 0};
   }
-  __device__ __forceinline__ const char *tile(int row0) const { return base + (int64_t)row0 * stride; }
-
-  // along rows: element e of f[i] = M[row0 + l % 32][16 i + 8 h + e]
-  __device__ __forceinline__ void load(f32x8 (&f)[DP / 16], int row0, int end) const {
-    const char *p = tile(row0);
-    const uint32_t row = (uint32_t)min((int)(threadIdx.x & 31), end - 1 - row0) * stride;
+  __device__ __forceinline__ void load(int row0, int end) {
+    const char *p = base + (int64_t)row0 * stride;
+    const uint32_t row = (threadIdx.x & 63) / 8, col = (threadIdx.x & 7) * 16;
+    const uint32_t last = (uint32_t)(end - 1 - row0);
+    if (in) {
 #pragma unroll
-    for (int i = 0; i < DP / 16; i++) {
-      const f32x4 *q = reinterpret_cast<const f32x4 *>(p + (row + col[i]));
-      const f32x4 a = q[0], b = q[1];
-      f[i] = f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+      for (int i = 0; i < 4; i++) w[i] = *reinterpret_cast<const u32x4 *>(p + (min(row + 8 * i, last) * stride + col));
     }
+  }
+  // to LDS, rows of `bad` as zeros
+  __device__ __forceinline__ void store(float *tile, uint32_t bad) const {
+    const int row = (threadIdx.x & 63) / 8, p = threadIdx.x & 7;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      *reinterpret_cast<u32x4 *>(tile + Tile<float, 32>::piece(row + 8 * i, p)) =
+          bad >> (row + 8 * i) & 1 ? u32x4{0, 0, 0, 0} : w[i];
+  }
+  // bit r: row r has an infinity or a NaN
+  __device__ __forceinline__ uint32_t bad_rows() const {
+    uint32_t out = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const uint64_t b = ballot(in && piece_bad<float>(w[i]));
+      for (int r = 0; r < 8; r++) out |= (b >> (8 * r) & 0xff) ? 1u << (8 * i + r) : 0u;
+    }
+    return out;
   }
 };
 
-template <int DP>
+// One wave writes its tile and reads it: LDS keeps the order of a wave's accesses, the compiler has to as well
+__device__ __forceinline__ void own_lds() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// Column fragments straight from memory, where 32 lanes read 128 bytes of a row: element e of f[i] =
+// M[row0 + 16 i + acc_row(e, h)][l % 32]
 struct Cols32 {
-  uint32_t row[8], col[DP / 32];  // this lane's places in the first 16 rows of a tile, bytes
-  __device__ __forceinline__ Cols32(uint32_t stride, int h, int dim) {
+  const char *base;
+  uint32_t stride, row[8], col;  // this lane's places in the first 16 rows of a tile, bytes
+  __device__ __forceinline__ Cols32(const float *p, int64_t row_stride, int h, int dim)
+      : base((const char *)p), stride((uint32_t)row_stride * 4), col(4 * min((int)(threadIdx.x & 31), dim - 1)) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) row[e] = (uint32_t)acc_row(e, h) * stride;
-#pragma unroll
-    for (int db = 0; db < DP / 32; db++) col[db] = 4 * min(32 * db + (int)(threadIdx.x & 31), dim - 1);
+    for (int e = 0; e < 8; e++) row[e] = (uint32_t)acc_row(e, h) * stride + col;
   }
-  // along columns: element e of f[i][db] = M[row0 + 16 i + acc_row(e, h)][32 db + l % 32]
-  __device__ __forceinline__ void load(f32x8 (&f)[2][DP / 32], const Rows32<DP> &m, int row0, int end, int h) const {
-    const char *p = m.tile(row0);
+  __device__ __forceinline__ void load(f32x8 (&f)[2], int row0, int end, int h) const {
+    const char *p = base + (int64_t)row0 * stride;
     if (row0 + 32 <= end) {
 #pragma unroll
       for (int i = 0; i < 2; i++) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-#pragma unroll
-          for (int db = 0; db < DP / 32; db++)
-            f[i][db][e] = *reinterpret_cast<const float *>(p + (int64_t)(16 * i) * m.stride + (row[e] + col[db]));
-        }
+        for (int e = 0; e < 8; e++) f[i][e] = *reinterpret_cast<const float *>(p + (int64_t)(16 * i) * stride + row[e]);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < 2; i++) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const uint32_t r = (uint32_t)min(16 * i + acc_row(e, h), end - 1 - row0) * m.stride;
-#pragma unroll
-          for (int db = 0; db < DP / 32; db++) f[i][db][e] = *reinterpret_cast<const float *>(p + (r + col[db]));
-        }
+        for (int e = 0; e < 8; e++)
+          f[i][e] = *reinterpret_cast<const float *>(
+              p + ((uint32_t)min(16 * i + acc_row(e, h), end - 1 - row0) * stride + col));
       }
     }
   }
+  __device__ static __forceinline__ uint32_t bad_rows(const f32x8 (&f)[2]) {
+    uint32_t out = 0;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const uint64_t b = ballot(!finite(f[i][e]));
+        if ((uint32_t)b) out |= 1u << (16 * i + acc_row(e, 0));
+        if (b >> 32) out |= 1u << (16 * i + acc_row(e, 1));
+      }
+    }
+    return out;
+  }
 };
-
-// bit r: row r of the tile has an infinity or a NaN among its fragments along rows
-template <int DP>
-__device__ __forceinline__ uint32_t bad_rows32(const f32x8 (&f)[DP / 16]) {
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < DP / 16; i++) {
-#pragma unroll
-    for (int e = 0; e < 8; e++) bad |= !finite(f[i][e]);
-  }
-  const uint64_t b = ballot(bad);
-  return (uint32_t)b | (uint32_t)(b >> 32);
-}
-// the same for fragments along columns
-template <int DP>
-__device__ __forceinline__ uint32_t bad_cols32(const f32x8 (&f)[2][DP / 32]) {
-  uint32_t out = 0;
-#pragma unroll
-  for (int i = 0; i < 2; i++) {
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      bool bad = false;
-#pragma unroll
-      for (int db = 0; db < DP / 32; db++) bad |= !finite(f[i][db][e]);
-      const uint64_t b = ballot(bad);
-      if ((uint32_t)b) out |= 1u << (16 * i + acc_row(e, 0));
-      if (b >> 32) out |= 1u << (16 * i + acc_row(e, 1));
-    }
-  }
-  return out;
-}
-template <int DP>
-__device__ __forceinline__ void zero_rows32(f32x8 (&f)[DP / 16], uint32_t bad) {
-  const bool b = bad >> (threadIdx.x & 31) & 1;
-#pragma unroll
-  for (int i = 0; i < DP / 16; i++) {
-#pragma unroll
-    for (int e = 0; e < 8; e++) f[i][e] = b ? 0.f : f[i][e];
-  }
-}
-template <int DP>
-__device__ __forceinline__ void zero_cols32(f32x8 (&f)[2][DP / 32], uint32_t bad, int h) {
-#pragma unroll
-  for (int i = 0; i < 2; i++) {
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      const bool b = bad >> (16 * i + acc_row(e, h)) & 1;
-#pragma unroll
-      for (int db = 0; db < DP / 32; db++) f[i][db][e] = b ? 0.f : f[i][db][e];
-    }
-  }
-}
 
 // sum over dim of this lane's stationary row (fragments f) times another row in memory
 template <int DP>
@@ -156,36 +131,41 @@ __device__ __forceinline__ void add_row32(f32x16 (&acc)[DP / 32], float w, const
   }
 }
 
-__device__ __forceinline__ f32x8 frag32(const f32x16 &acc, int i) {
-  f32x8 v;
-#pragma unroll
-  for (int e = 0; e < 8; e++) v[e] = acc[8 * i + e];
-  return v;
-}
-
 // Forward: the wave's 32 virtual rows against keys [begin, end)
 template <int DP, bool CAREFUL>
 __device__ __forceinline__ void fwd_walk32(const Attend &a, const float *__restrict__ k, const float *__restrict__ v,
                                            int begin, int end, Range mine, int full_lo, int full_hi,
-                                           const f32x8 (&qf)[DP / 16], f32x16 (&acc)[DP / 32], RowState &st) {
-  const int h = threadIdx.x >> 5 & 1;
+                                           const f32x8 (&qf)[DP / 16], float *ks, f32x16 (&acc)[DP / 32],
+                                           RowState &st) {
+  using L = Tile<float, DP>;
+  const int h = threadIdx.x >> 5 & 1, col = threadIdx.x & 31;
   if (begin >= end) return;
-  const Rows32<DP> km(k, a.k.row, h, a.dim), vm(v, a.v.row, h, a.dim);
-  const Cols32<DP> vc(vm.stride, h, a.dim);
-  f32x8 kf[DP / 16], vf[2][DP / 32];
-  km.load(kf, begin, end);
+  Rows32 km(k, a.k.row, a.dim);
+  const Cols32 vm(v, a.v.row, h, a.dim);
+  f32x8 vf[2], next[2];
+  km.load(begin, end);
+  vm.load(next, begin, end, h);
   for (int kt = begin; kt < end; kt += 32) {
-    vc.load(vf, vm, kt, end, h);
+    vf[0] = next[0];
+    vf[1] = next[1];
     uint32_t bad = 0;
     if constexpr (CAREFUL) {
-      bad = bad_rows32<DP>(kf) | bad_cols32<DP>(vf);
-      zero_rows32<DP>(kf, bad);
-      zero_cols32<DP>(vf, bad, h);
+      bad = km.bad_rows() | Cols32::bad_rows(vf);
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) vf[i][e] = bad >> (16 * i + acc_row(e, h)) & 1 ? 0.f : vf[i][e];
+      }
+    }
+    km.store(ks, bad);
+    own_lds();
+    if (kt + 32 < end) {
+      km.load(kt + 32, end);
+      vm.load(next, kt + 32, end, h);
     }
     f32x16 s = {};
 #pragma unroll
-    for (int i = 0; i < DP / 16; i++) s = mma(kf[i], qf[i], s);
-    if (kt + 32 < end) km.load(kf, kt + 32, end);
+    for (int i = 0; i < DP / 16; i++) s = mma(L::row_frag(ks, col, 16 * i + 8 * h), qf[i], s);
     if (CAREFUL || kt < full_lo || kt + 32 > full_hi) {
 #pragma unroll
       for (int r = 0; r < 16; r++) {
@@ -207,11 +187,8 @@ __device__ __forceinline__ void fwd_walk32(const Attend &a, const float *__restr
       st.l += s[r];
     }
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-      const f32x8 p = frag32(s, i);
-#pragma unroll
-      for (int db = 0; db < DP / 32; db++) acc[db] = mma(vf[i][db], p, acc[db]);
-    }
+    for (int i = 0; i < 2; i++) acc[0] = mma(vf[i], acc_frag<float>(s, i), acc[0]);
+    own_lds();
     if constexpr (CAREFUL) {
       for (; bad; bad &= bad - 1) {
         const int key = kt + __builtin_ctz(bad);
@@ -232,33 +209,29 @@ __device__ __forceinline__ void fwd_walk32(const Attend &a, const float *__restr
 template <int DP, bool CAREFUL>
 __device__ __forceinline__ void dq_walk32(const Attend &a, const float *__restrict__ k, const float *__restrict__ v,
                                           int begin, int end, int2 mine, float2 ld, int full_lo, int full_hi,
-                                          const f32x8 (&qf)[DP / 16], const f32x8 (&gf)[DP / 16],
+                                          const f32x8 (&qf)[DP / 16], const f32x8 (&gf)[DP / 16], float *ks, float *vs,
                                           f32x16 (&acc)[DP / 32]) {
-  const int h = threadIdx.x >> 5 & 1;
+  using L = Tile<float, DP>;
+  const int h = threadIdx.x >> 5 & 1, col = threadIdx.x & 31;
   if (begin >= end) return;
-  const Rows32<DP> km(k, a.k.row, h, a.dim), vm(v, a.v.row, h, a.dim);
-  const Cols32<DP> cols(km.stride, h, a.dim);
-  f32x8 kf[DP / 16], vf[DP / 16], kc[2][DP / 32];
-  km.load(kf, begin, end);
-  vm.load(vf, begin, end);
+  Rows32 km(k, a.k.row, a.dim), vm(v, a.v.row, a.dim);
+  km.load(begin, end);
+  vm.load(begin, end);
   for (int kt = begin; kt < end; kt += 32) {
-    cols.load(kc, km, kt, end, h);
     uint32_t bad = 0;
-    if constexpr (CAREFUL) {
-      bad = bad_rows32<DP>(kf) | bad_rows32<DP>(vf);
-      zero_rows32<DP>(kf, bad);
-      zero_rows32<DP>(vf, bad);
-      zero_cols32<DP>(kc, bad, h);
+    if constexpr (CAREFUL) bad = km.bad_rows() | vm.bad_rows();
+    km.store(ks, bad);
+    vm.store(vs, bad);
+    own_lds();
+    if (kt + 32 < end) {
+      km.load(kt + 32, end);
+      vm.load(kt + 32, end);
     }
     f32x16 s = {}, dp = {};
 #pragma unroll
     for (int i = 0; i < DP / 16; i++) {
-      s = mma(kf[i], qf[i], s);
-      dp = mma(vf[i], gf[i], dp);
-    }
-    if (kt + 32 < end) {
-      km.load(kf, kt + 32, end);
-      vm.load(vf, kt + 32, end);
+      s = mma(L::row_frag(ks, col, 16 * i + 8 * h), qf[i], s);
+      dp = mma(L::row_frag(vs, col, 16 * i + 8 * h), gf[i], dp);
     }
 #pragma unroll
     for (int r = 0; r < 16; r++) s[r] = exp2_fast(fmaf(s[r], a.c, -ld.x)) * (dp[r] - ld.y);
@@ -272,11 +245,8 @@ __device__ __forceinline__ void dq_walk32(const Attend &a, const float *__restri
       }
     }
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-      const f32x8 ds = frag32(s, i);
-#pragma unroll
-      for (int db = 0; db < DP / 32; db++) acc[db] = mma(kc[i][db], ds, acc[db]);
-    }
+    for (int i = 0; i < 2; i++) acc[0] = mma(L::col_frag(ks, 16 * i, 0), acc_frag<float>(s, i), acc[0]);
+    own_lds();
     if constexpr (CAREFUL) {
       for (; bad; bad &= bad - 1) {
         const int key = kt + __builtin_ctz(bad);
@@ -292,8 +262,8 @@ __device__ __forceinline__ void dq_walk32(const Attend &a, const float *__restri
 
 // dk, dv: the wave's 32 keys against steps [begin, end) of the query rows that see any of them: step t is the
 // 32 rows from rows.lo + t % tiles * 32 of head t / tiles of the key head's group (rows of one head lie a
-// constant stride apart).  q, go, ld: of the key head's first head.  s_row: LDS of this wave, the sums and
-// ranges of 32 rows.
+// constant stride apart).  q, go, ld: of the key head's first head.  qs, os, s_row: LDS of this wave, the tiles of q
+// and of do and the sums and ranges of their rows.
 struct RowSums {
   float lse, d;
   int lo, hi;
@@ -302,23 +272,19 @@ template <int DP, bool CAREFUL>
 __device__ __forceinline__ void dkv_walk32(const Attend &a, const float *__restrict__ q, Heads gst,
                                            const float *__restrict__ go, const float2 *__restrict__ ld, int ld_row,
                                            const int2 *__restrict__ range, int begin, int end, Range rows, int tiles,
-                                           int key0, const f32x8 (&kf)[DP / 16], const f32x8 (&vf)[DP / 16],
-                                           RowSums *s_row, f32x16 (&dk)[DP / 32], f32x16 (&dv)[DP / 32]) {
+                                           int key0, const f32x8 (&kf)[DP / 16], const f32x8 (&vf)[DP / 16], float *qs,
+                                           float *os, RowSums *s_row, f32x16 (&dk)[DP / 32], f32x16 (&dv)[DP / 32]) {
+  using L = Tile<float, DP>;
   const int lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31, key = key0 + col;
   if (begin >= end) return;
-  Rows32<DP> qm(q, a.q.row, h, a.dim), gm(go, gst.row, h, a.dim);
-  const Cols32<DP> qcols(qm.stride, h, a.dim), gcols(gm.stride, h, a.dim);
-  f32x8 qf[DP / 16], gf[DP / 16], qc[2][DP / 32], gc[2][DP / 32];
+  Rows32 qm(q, a.q.row, a.dim), gm(go, gst.row, a.dim);
   RowSums mine;
   int head = begin / tiles, row0 = rows.lo + begin % tiles * 32;  // of the step whose loads come next
-  auto at_head = [&]() {
+  auto load = [&]() {
     qm.base = (const char *)(q + head * a.q.head);
     gm.base = (const char *)(go + head * gst.head);
-  };
-  at_head();
-  auto load = [&]() {
-    qm.load(qf, row0, rows.hi);
-    gm.load(gf, row0, rows.hi);
+    qm.load(row0, rows.hi);
+    gm.load(row0, rows.hi);
     const int row = min(row0 + col, rows.hi - 1);
     const float2 l = ld[(int64_t)row * ld_row + head];
     const int2 r = range[row];
@@ -328,41 +294,32 @@ __device__ __forceinline__ void dkv_walk32(const Attend &a, const float *__restr
   load();
   for (int t = begin; t < end; t++) {
     const int here = row0;
+    const char *qbase = qm.base, *gbase = gm.base;
     const bool some = __any(mine.lo < key0 + 32 && mine.hi > key0);
     const bool whole = !CAREFUL && __all(mine.lo <= key0 && mine.hi >= key0 + 32);
     uint32_t bad = 0;
-    const char *qbase = qm.base, *gbase = gm.base;
-    f32x16 s = {}, dp = {};
     if (some) {
-      qcols.load(qc, qm, here, rows.hi, h);
-      gcols.load(gc, gm, here, rows.hi, h);
-      if constexpr (CAREFUL) {
-        bad = bad_rows32<DP>(qf) | bad_rows32<DP>(gf);
-        zero_rows32<DP>(qf, bad);
-        zero_rows32<DP>(gf, bad);
-        zero_cols32<DP>(qc, bad, h);
-        zero_cols32<DP>(gc, bad, h);
-      }
-      // this wave alone writes and reads s_row, and LDS keeps its order
+      if constexpr (CAREFUL) bad = qm.bad_rows() | gm.bad_rows();
+      qm.store(qs, bad);
+      gm.store(os, bad);
       if (h == 0) s_row[col] = mine;
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-#pragma unroll
-      for (int i = 0; i < DP / 16; i++) {
-        s = mma(qf[i], kf[i], s);
-        dp = mma(gf[i], vf[i], dp);
-      }
     }
+    own_lds();
     if (t + 1 < end) {
       row0 += 32;
       if (row0 >= rows.hi) {
         row0 = rows.lo;
         head++;
-        at_head();
       }
       load();
     }
     if (!some) continue;
+    f32x16 s = {}, dp = {};
+#pragma unroll
+    for (int i = 0; i < DP / 16; i++) {
+      s = mma(L::row_frag(qs, col, 16 * i + 8 * h), kf[i], s);
+      dp = mma(L::row_frag(os, col, 16 * i + 8 * h), vf[i], dp);
+    }
 #pragma unroll
     for (int r = 0; r < 16; r++) {
       const RowSums x = s_row[acc_row(r, h)];
@@ -377,12 +334,8 @@ __device__ __forceinline__ void dkv_walk32(const Attend &a, const float *__restr
     }
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-      const f32x8 p = frag32(s, i), ds = frag32(dp, i);
-#pragma unroll
-      for (int db = 0; db < DP / 32; db++) {
-        dv[db] = mma(gc[i][db], p, dv[db]);
-        dk[db] = mma(qc[i][db], ds, dk[db]);
-      }
+      dv[0] = mma(L::col_frag(os, 16 * i, 0), acc_frag<float>(s, i), dv[0]);
+      dk[0] = mma(L::col_frag(qs, 16 * i, 0), acc_frag<float>(dp, i), dk[0]);
     }
     if constexpr (CAREFUL) {
       for (; bad; bad &= bad - 1) {
@@ -399,7 +352,7 @@ __device__ __forceinline__ void dkv_walk32(const Attend &a, const float *__restr
         }
       }
     }
-    __builtin_amdgcn_wave_barrier();
+    own_lds();
   }
 }
 

@@ -160,66 +160,80 @@ __device__ __forceinline__ void dq_walk(const Attend &a, const T *__restrict__ k
       });
 }
 
+struct GradArgs {
+  const void *q, *k, *v, *go;
+  void *dq, *dk, *dv;
+  float *part;  // dk, dv: the splits' sums (NULL without splits)
+};
+
 template <typename T, int DP>
-__global__ void __launch_bounds__((64 * kWaves<T, DP>), sizeof(T) == 4 && DP == 128 ? 1 : 2)
-    attend_dq_kernel(Attend a, Grad g, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
-                     const T *__restrict__ go, T *__restrict__ dq) {
-  constexpr int BN = DqTile<T, DP>::BN;
+struct DqLds {
+  static constexpr int N = (kDirect<T, DP> ? 1 : 2) * Stage<T, DP, DqTile<T, DP>::BN>::SIZE;
+  alignas(16) T ks[N];
+  alignas(16) T vs[N];
+  uint32_t bad[2];
+  int lo[4], hi[4], redo;
+  float max[4];
+};
+
+// One workgroup's rows.  True: something was not finite, and nothing was stored.
+template <typename T, int DP, bool CAREFUL>
+__device__ __forceinline__ bool dq_rows(const Attend &a, const Grad &g, const GradArgs &p, DqLds<T, DP> &lds) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
-  const int head = blockIdx.x % a.kv_heads, heads = a.kv_heads * a.group;
-  const int64_t total = (int64_t)a.nq * a.group;
-  const int64_t tiles = gridDim.x / a.kv_heads;
-  const int64_t m = (tiles - 1 - blockIdx.x / a.kv_heads) * (32 * kWaves<T, DP>) + wave * 32 + col;
+  const int head = (int)blockIdx.x % a.kv_heads, heads = a.kv_heads * a.group;
+  const int total = a.nq * a.group, tiles = (int)gridDim.x / a.kv_heads;  // virtual rows: under 2^31
+  const int m = (tiles - 1 - (int)blockIdx.x / a.kv_heads) * (32 * kWaves<T, DP>) + wave * 32 + col;
   const bool live = m < total;
-  const int row = live ? (int)(m / a.group) : 0, qhead = head * a.group + (live ? (int)(m % a.group) : 0);
+  const Row at_row = virtual_row(a, live ? m : 0);
+  const int row = at_row.row, qhead = head * a.group + at_row.sub;
   const Range none = no_keys();
   const int2 mine = live ? g.range[row] : make_int2(none.lo, none.hi);
   const int64_t at = (int64_t)row * heads + qhead;
   const float2 ld = live ? g.ld[at] : make_float2(0, 0);
-  const int wlo = uniform(min_over(mine.x)), whi = uniform(max_over(mine.y));
-  const int full_lo = uniform(max_over(mine.x)), full_hi = uniform(min_over(mine.y));
+  const int wlo = min_over(mine.x), whi = max_over(mine.y);
+  const int full_lo = max_over(mine.x), full_hi = min_over(mine.y);
   V8<T> qf[DP / 16], gf[DP / 16];
-  const T *qrow = q + row * a.q.row + qhead * a.q.head, *grow = go + at * a.dim;
+  const T *qrow = (const T *)p.q + row * a.q.row + qhead * a.q.head, *grow = (const T *)p.go + at * a.dim;
 #pragma unroll
   for (int i = 0; i < DP / 16; i++) {
     qf[i] = global_frag(qrow, live, 16 * i + 8 * h, a.dim);
     gf[i] = global_frag(grow, live, 16 * i + 8 * h, a.dim);
   }
-  const T *kh = k + head * a.k.head, *vh = v + head * a.v.head;
+  const T *kh = (const T *)p.k + head * a.k.head, *vh = (const T *)p.v + head * a.v.head;
   f32x16 acc[DP / 32] = {};
   float gs = 1;
   if constexpr (kDirect<T, DP>) {
-    dq_walk32<DP, false>(a, kh, vh, wlo, whi, mine, ld, full_lo, full_hi, qf, gf, acc);
-    if (__any(!all_finite(acc))) {
-#pragma unroll
-      for (int db = 0; db < DP / 32; db++) acc[db] = f32x16{};
-      dq_walk32<DP, true>(a, kh, vh, wlo, whi, mine, ld, full_lo, full_hi, qf, gf, acc);
-    }
+    dq_walk32<DP, CAREFUL>(a, kh, vh, wlo, whi, mine, ld, full_lo, full_hi, qf, gf, lds.ks, lds.vs, acc);
+    if (!CAREFUL && __any(!all_finite(acc))) return true;
   } else {
-    __shared__ alignas(16) T ks[2 * Stage<T, DP, BN>::SIZE], vs[2 * Stage<T, DP, BN>::SIZE];
-    __shared__ uint32_t bad[BN / 32];
-    __shared__ int s_lo[4], s_hi[4], s_redo;
-    __shared__ float s_max[4];
     if (lane == 0) {
-      s_lo[wave] = wlo;
-      s_hi[wave] = whi;
+      lds.lo[wave] = wlo;
+      lds.hi[wave] = whi;
     }
-    if (threadIdx.x == 0) s_redo = 0;
-    gs = grad_scale<T>(g, s_max);
+    if (CAREFUL) __syncthreads();  // everyone has read lds.redo
+    if (threadIdx.x == 0) lds.redo = 0;
+    gs = grad_scale<T>(g, lds.max);
     __syncthreads();
-    int begin = uniform(min(min(s_lo[0], s_lo[1]), min(s_lo[2], s_lo[3])));
-    int end = uniform(max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3])));
+    int begin = uniform(min(min(lds.lo[0], lds.lo[1]), min(lds.lo[2], lds.lo[3])));
+    int end = uniform(max(max(lds.hi[0], lds.hi[1]), max(lds.hi[2], lds.hi[3])));
     if (begin >= end) begin = end = 0;
-    dq_walk<T, DP, false>(a, kh, vh, begin, end, mine, ld, gs, wlo, whi, full_lo, full_hi, qf, gf, ks, vs, bad, acc);
-    if (!all_finite(acc)) s_redo = 1;
-    __syncthreads();
-    if (s_redo) {
-#pragma unroll
-      for (int db = 0; db < DP / 32; db++) acc[db] = f32x16{};
-      dq_walk<T, DP, true>(a, kh, vh, begin, end, mine, ld, gs, wlo, whi, full_lo, full_hi, qf, gf, ks, vs, bad, acc);
+    dq_walk<T, DP, CAREFUL>(a, kh, vh, begin, end, mine, ld, gs, wlo, whi, full_lo, full_hi, qf, gf, lds.ks, lds.vs,
+                            lds.bad, acc);
+    if (!CAREFUL) {
+      if (!all_finite(acc)) lds.redo = 1;
+      __syncthreads();
+      if (lds.redo) return true;
     }
   }
-  if (live) store_cols<T, DP>(dq + at * a.dim, acc, a.scale / gs, h, a.dim);
+  if (live) store_cols<T, DP>((T *)p.dq + at * a.dim, acc, a.scale / gs, h, a.dim);
+  return false;
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__((64 * kWaves<T, DP>), (kDirect<T, DP> ? 3 : sizeof(T) == 4 && DP == 128 ? 1 : 2))
+    attend_dq_kernel(Attend a, Grad g, GradArgs p) {
+  __shared__ DqLds<T, DP> lds;
+  if (dq_rows<T, DP, false>(a, g, p, lds)) dq_rows<T, DP, true>(a, g, p, lds);
 }
 
 template <typename T, int DP>
@@ -332,33 +346,43 @@ __device__ __forceinline__ Range row_range(const Attend &a, int j0, int j1) {
   return {min(r0, r1), r1};
 }
 
-// grid: (tiles of keys * kv_heads, splits of the rows); part: the splits' sums (NULL without splits)
 template <typename T, int DP>
-__global__ void __launch_bounds__((64 * kWaves<T, DP>), DP == 128 ? 1 : 2)
-    attend_dkv_kernel(Attend a, Grad g, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
-                      const T *__restrict__ go, T *__restrict__ dk_out, T *__restrict__ dv_out,
-                      float *__restrict__ part) {
+struct DkvLds {
+  static constexpr int BQ = DkvTile<T, DP>::BQ, N = (kDirect<T, DP> ? 1 : 2) * Stage<T, DP, BQ>::SIZE;
+  alignas(16) T qs[N];
+  alignas(16) T os[N];
+  RowSums rows[32];                 // kDirect
+  float2 ld[2 * BQ];
+  int2 range[2 * BQ];
+  uint32_t bad[2];
+  int redo;
+  float max[4];
+};
+
+// One workgroup's keys.  True: something was not finite, and nothing was stored.
+template <typename T, int DP, bool CAREFUL>
+__device__ __forceinline__ bool dkv_keys(const Attend &a, const Grad &g, const GradArgs &p, DkvLds<T, DP> &lds) {
   constexpr int BQ = DkvTile<T, DP>::BQ, KEYS = DkvTile<T, DP>::KEYS;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
-  const int head = blockIdx.x % a.kv_heads, heads = a.kv_heads * a.group;
-  const int j0 = blockIdx.x / a.kv_heads * KEYS, key0 = j0 + wave * 32, key = key0 + col;
+  const int head = (int)blockIdx.x % a.kv_heads, heads = a.kv_heads * a.group;
+  const int j0 = (int)blockIdx.x / a.kv_heads * KEYS, key0 = j0 + wave * 32, key = key0 + col;
   const bool live = key < a.nk;
   Range rows = row_range(a, j0, min(j0 + KEYS, a.nk));
   rows = {uniform(rows.lo), uniform(rows.hi)};
   const int tiles = max(1, (rows.hi - rows.lo + BQ - 1) / BQ);
   int begin = 0, end = rows.hi > rows.lo ? tiles * a.group : 0;
-  if (part) {
+  if (p.part) {
     const int share = (end + (int)gridDim.y - 1) / (int)gridDim.y;
     begin = min(end, share * (int)blockIdx.y);
     end = min(end, begin + share);
-    if (begin >= end) return;  // the join does not ask for it
+    if (begin >= end) return false;  // the join does not ask for it
   }
-  const T *qh = q + (int64_t)head * a.group * a.q.head;
+  const T *qh = (const T *)p.q + (int64_t)head * a.group * a.q.head;
   const Heads gst = {(int64_t)heads * a.dim, a.dim};
-  const T *gh = go + (int64_t)head * a.group * a.dim;
+  const T *gh = (const T *)p.go + (int64_t)head * a.group * a.dim;
   V8<T> kf[DP / 16], vf[DP / 16];
-  const T *krow = k + (live ? key : 0) * a.k.row + head * a.k.head;
-  const T *vrow = v + (live ? key : 0) * a.v.row + head * a.v.head;
+  const T *krow = (const T *)p.k + (live ? key : 0) * a.k.row + head * a.k.head;
+  const T *vrow = (const T *)p.v + (live ? key : 0) * a.v.row + head * a.v.head;
 #pragma unroll
   for (int i = 0; i < DP / 16; i++) {
     kf[i] = global_frag(krow, live, 16 * i + 8 * h, a.dim);
@@ -367,43 +391,42 @@ __global__ void __launch_bounds__((64 * kWaves<T, DP>), DP == 128 ? 1 : 2)
   f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
   float gs = 1;
   if constexpr (kDirect<T, DP>) {
-    __shared__ RowSums s_row[32];
     const float2 *ld = g.ld + head * a.group;
-    dkv_walk32<DP, false>(a, qh, gst, gh, ld, heads, g.range, begin, end, rows, tiles, key0, kf, vf, s_row, dk, dv);
-    if (__any(!(all_finite(dk) && all_finite(dv)))) {
-#pragma unroll
-      for (int db = 0; db < DP / 32; db++) dk[db] = dv[db] = f32x16{};
-      dkv_walk32<DP, true>(a, qh, gst, gh, ld, heads, g.range, begin, end, rows, tiles, key0, kf, vf, s_row, dk, dv);
-    }
+    dkv_walk32<DP, CAREFUL>(a, qh, gst, gh, ld, heads, g.range, begin, end, rows, tiles, key0, kf, vf, lds.qs, lds.os,
+                            lds.rows, dk, dv);
+    if (!CAREFUL && __any(!(all_finite(dk) && all_finite(dv)))) return true;
   } else {
-    __shared__ alignas(16) T qs[2 * Stage<T, DP, BQ>::SIZE], os[2 * Stage<T, DP, BQ>::SIZE];
-    __shared__ float2 s_ld[2 * BQ];
-    __shared__ int2 s_range[2 * BQ];
-    __shared__ uint32_t bad[BQ / 32];
-    __shared__ int s_redo;
-    __shared__ float s_max[4];
-    if (threadIdx.x == 0) s_redo = 0;
-    gs = grad_scale<T>(g, s_max);
+    if (CAREFUL) __syncthreads();  // everyone has read lds.redo
+    if (threadIdx.x == 0) lds.redo = 0;
+    gs = grad_scale<T>(g, lds.max);
     __syncthreads();
-    dkv_walk<T, DP, false>(a, g, qh, gst, gh, head, begin, end, rows, tiles, key0, gs, kf, vf, qs, os, s_ld, s_range, bad, dk, dv);
-    if (!(all_finite(dk) && all_finite(dv))) s_redo = 1;
-    __syncthreads();
-    if (s_redo) {
-#pragma unroll
-      for (int db = 0; db < DP / 32; db++) dk[db] = dv[db] = f32x16{};
-      dkv_walk<T, DP, true>(a, g, qh, gst, gh, head, begin, end, rows, tiles, key0, gs, kf, vf, qs, os, s_ld, s_range, bad, dk, dv);
+    dkv_walk<T, DP, CAREFUL>(a, g, qh, gst, gh, head, begin, end, rows, tiles, key0, gs, kf, vf, lds.qs, lds.os, lds.ld,
+                             lds.range, lds.bad, dk, dv);
+    if (!CAREFUL) {
+      if (!(all_finite(dk) && all_finite(dv))) lds.redo = 1;
+      __syncthreads();
+      if (lds.redo) return true;
     }
   }
-  if (!live) return;
+  if (!live) return false;
   const int64_t at = ((int64_t)key * a.kv_heads + head) * a.dim;
-  if (part) {
+  if (p.part) {
     const int64_t all = (int64_t)a.nk * a.kv_heads * a.dim;
-    store_cols<float, DP>(part + 2 * blockIdx.y * all + at, dk, a.scale / gs, h, a.dim);
-    store_cols<float, DP>(part + (2 * blockIdx.y + 1) * all + at, dv, 1.f, h, a.dim);
-    return;
+    store_cols<float, DP>(p.part + 2 * blockIdx.y * all + at, dk, a.scale / gs, h, a.dim);
+    store_cols<float, DP>(p.part + (2 * blockIdx.y + 1) * all + at, dv, 1.f, h, a.dim);
+    return false;
   }
-  store_cols<T, DP>(dk_out + at, dk, a.scale / gs, h, a.dim);
-  store_cols<T, DP>(dv_out + at, dv, 1.f, h, a.dim);
+  store_cols<T, DP>((T *)p.dk + at, dk, a.scale / gs, h, a.dim);
+  store_cols<T, DP>((T *)p.dv + at, dv, 1.f, h, a.dim);
+  return false;
+}
+
+// grid: (tiles of keys * kv_heads, splits of the rows)
+template <typename T, int DP>
+__global__ void __launch_bounds__((64 * kWaves<T, DP>), (DP == 128 ? 1 : 2))
+    attend_dkv_kernel(Attend a, Grad g, GradArgs p) {
+  __shared__ DkvLds<T, DP> lds;
+  if (dkv_keys<T, DP, false>(a, g, p, lds)) dkv_keys<T, DP, true>(a, g, p, lds);
 }
 
 // The splits of dk and dv added in their order: four elements a thread.
@@ -459,16 +482,16 @@ static int attend_backward(const Attend &a, const Grad &g, const void *q, const 
                            void *dq, void *dk, void *dv, float *part, hipStream_t st) {
   if (a.nq > 0 && dq) {
     const unsigned blocks = (unsigned)(cdiv((int64_t)a.nq * a.group, 32 * kWaves<T, DP>) * a.kv_heads);
-    hipLaunchKernelGGL((attend_dq_kernel<T, DP>), dim3(blocks), dim3(64 * kWaves<T, DP>), 0, st, a, g, (const T *)q, (const T *)k,
-                       (const T *)v, (const T *)go, (T *)dq);
+    hipLaunchKernelGGL((attend_dq_kernel<T, DP>), dim3(blocks), dim3(64 * kWaves<T, DP>), 0, st, a, g,
+                       GradArgs{q, k, v, go, dq, nullptr, nullptr, nullptr});
     KL_CHECK_LAUNCH();
   }
   if (a.nk > 0 && dk) {
     constexpr int KEYS = DkvTile<T, DP>::KEYS, step = DkvTile<T, DP>::BQ;
     const unsigned blocks = (unsigned)(cdiv(a.nk, KEYS) * a.kv_heads);
     const int splits = dkv_splits(sizeof(T) == 4 ? KL_F32 : KL_F16, a.nq, a.nk, a.kv_heads, a.group, a.dim);
-    hipLaunchKernelGGL((attend_dkv_kernel<T, DP>), dim3(blocks, splits), dim3(64 * kWaves<T, DP>), 0, st, a, g, (const T *)q,
-                       (const T *)k, (const T *)v, (const T *)go, (T *)dk, (T *)dv, splits > 1 ? part : nullptr);
+    hipLaunchKernelGGL((attend_dkv_kernel<T, DP>), dim3(blocks, splits), dim3(64 * kWaves<T, DP>), 0, st, a, g,
+                       GradArgs{q, k, v, go, nullptr, dk, dv, splits > 1 ? part : nullptr});
     KL_CHECK_LAUNCH();
     if (splits > 1) {
       const int64_t pieces = (int64_t)a.nk * a.kv_heads * a.dim / 4;
