@@ -254,9 +254,6 @@ __device__ __forceinline__ void rescale(RowState &st, float m, f32x16 (&acc)[N])
   }
 }
 
-// What is the same in every lane, as such: loops and addresses made of it stay in scalar registers
-__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-
 template <typename F>
 int with_dim(int dim, F f) {
   if (dim <= 32) return f(std::integral_constant<int, 32>());

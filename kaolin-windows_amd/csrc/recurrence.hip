@@ -1,16 +1,23 @@
 // recurrence.hip -- gated linear recurrence along packs: h[t] = a[t] h[t-1] + b[t] in every column, from
 // `initial` (or 0) at each pack's first row; reverse: from its last row down.
 //
-// Steps compose: rows t0 .. t1 take a state s to A s + B, so the rows are cut into chunks, and
-//   1. every (chunk, columns) thread computes its chunk's (A, B),
-//   2. a scan over the chunks gives each chunk the state before it,
-//   3. every thread walks its chunk again from that state and writes.
-// A pack's first row takes no state: a chunk with one (`reset`) composes to (0, B), and its A is never
-// multiplied with the state before it (which may be infinite in another pack).  Order and rounding are
-// fixed by the sizes alone.  States, A and B are in 32 bits (64 for double); outputs are rounded once.
+// Steps compose: rows t0 .. t1 take a state s to A s + B.  The rows are cut into chunks, one a thread and piece
+// of columns:
+//   1. every chunk's (A, B), from the start of its last pack on: what lies before has no effect past the chunk;
+//   2. within segments of kSegment chunks, the (A, B) of what lies before each chunk, and each segment's own;
+//   3. every chunk's state before it from those, back to the nearest segment with a pack's start; then it is
+//      walked and written.
+// A chunk in which a pack starts (`reset`) has A = 0, and that is never multiplied with the state before it, which
+// may be infinite in another pack.  Order and rounding follow from the sizes alone.
 //
+// Bound by memory: a and b are read 1 + (share of 1) times and h is written once.  Step 3 takes the chunks in the
+// other order, so that it finds what 1 read last in the 256 MB cache.  One pass, with workgroups that publish and
+// await each other's (A, B), measured no faster: it reads less, but waits.
+// recur_rays_train's shapes (311,000 x 64, float, packs of 38): TBD
+//
+// States, A and B are in 32 bits (64 for double); outputs are rounded once.
 // Backward: g[t] = dh[t] + a[t+1] g[t+1] is the same recurrence in the other direction with the gate of the
-// row walked before; db = g, da[t] = g[t] h[t-1], dinitial = a g at the first row.
+// row walked before; db = g, da[t] = g[t] h[t-1] with h as it was rounded, dinitial = a g at the first row.
 #include "seqcommon.h"
 
 namespace kl {
@@ -30,247 +37,330 @@ struct alignas(sizeof(T) * V) Pack {
 };
 
 struct Recur {
-  int n, cols, chunk, chunks, packs;  // cols: threads across; chunk: rows of one; packs: rows of initial
-  int64_t dim;
+  int n, chunk, chunks, packs, down;  // chunk: rows of one; packs: rows of initial; down: rows descend
+  int64_t dim, cols;                  // cols: pieces across
   const int32_t *ids, *starts;
+  // rows are numbered in the order they are walked
+  __device__ __forceinline__ int64_t row(int64_t i) const { return down ? n - 1 - i : i; }
+  __device__ __forceinline__ int id(int64_t i) const { return i >= 0 && i < n ? ids[row(i)] : -2; }
+  // the first row walked of pack p
+  __device__ __forceinline__ int64_t first(int p) const { return down ? n - starts[p + 1] : starts[p]; }
 };
 
-constexpr int kAhead = 4;  // rows whose loads are in flight together
+constexpr int kAhead = 8;       // rows whose loads are in flight together in step 1
+constexpr int kAheadWrite = 4;  // and in step 3, which keeps more of each
+constexpr int kRunChunks = 4;   // chunks of a thread of step 2
+constexpr int kSegment = 64 * kRunChunks;
 
-// One thread's walk over rows first .. last in processing order.  DOWN: rows descend.  GRAD: the backward.
-// AGG: only (A, B) are computed, from state 0.
-template <typename T, int V, bool DOWN, bool GRAD, bool AGG>
-__device__ __forceinline__ void recur_walk(const Recur &r, int64_t first, int64_t last, int64_t col,
-                                           const T *__restrict__ a, const T *__restrict__ x, const T *__restrict__ h,
-                                           const T *__restrict__ init, T *__restrict__ out, T *__restrict__ da,
-                                           T *__restrict__ dinit, typename StateOf<T>::S (&state)[V],
-                                           typename StateOf<T>::S (&gain)[V], bool &reset) {
-  using S = typename StateOf<T>::S;
-  using P = Pack<T, V>;
-  const int64_t n = r.n;
-  auto row = [&](int64_t i) { return DOWN ? n - 1 - i : i; };
-  auto id = [&](int64_t i) { return i >= 0 && i < n ? r.ids[row(i)] : -2; };
-  auto at = [&](const T *p, int64_t t) { return *reinterpret_cast<const P *>(p + t * r.dim + col * V); };
-  int before = id(first - 1), here = id(first);
-  P gate = {};  // GRAD: the gate of the row walked before
-  if (GRAD && before == here && here >= 0) gate = at(a, row(first - 1));
-  for (int64_t i0 = first; i0 < last; i0 += kAhead) {
-    P av[kAhead], xv[kAhead], hv[kAhead];
-    int idv[kAhead];
-#pragma unroll
-    for (int u = 0; u < kAhead; u++) {
-      const int64_t i = i0 + u;
-      av[u] = P{};
-      xv[u] = P{};
-      hv[u] = P{};
-      idv[u] = -2;
-      if (i < last) {
-        av[u] = at(a, row(i));
-        xv[u] = at(x, row(i));
-        idv[u] = id(i + 1);
-        if (GRAD && !AGG && idv[u] != -2) hv[u] = at(h, row(i + 1));
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < kAhead; u++) {
-      const int64_t i = i0 + u;
-      if (i >= last) break;
-      const int next = idv[u];
-      const bool start = here != before, none = here < 0;
-      const int64_t t = row(i) * r.dim + col * V;
-      reset = reset || start;
-      P y, dy;
-      if (GRAD) {
-        // the forward's state before this row: the next row walked, or the pack's initial state
-        const bool end = next != here;
-        P hp = hv[u];
-        if (!AGG && end) {
-          hp = P{};
-          if (init && !none && here < r.packs) hp = at(init, here);
-        }
-#pragma unroll
-        for (int c = 0; c < V; c++) {
-          const S g = none ? (S)0 : start ? (S)xv[u].v[c] : fma((S)gate.v[c], state[c], (S)xv[u].v[c]);
-          if (AGG) gain[c] = start ? (S)0 : gain[c] * (S)gate.v[c];
-          state[c] = g;
-          y.v[c] = (T)g;
-          dy.v[c] = (T)(none ? (S)0 : g * (S)hp.v[c]);
-        }
-        gate = av[u];
-        if (!AGG) {
-          *reinterpret_cast<P *>(out + t) = y;
-          *reinterpret_cast<P *>(da + t) = dy;
-          if (dinit && end && !none && here < r.packs) {
-            P d;
-#pragma unroll
-            for (int c = 0; c < V; c++) d.v[c] = (T)((S)av[u].v[c] * state[c]);
-            *reinterpret_cast<P *>(dinit + (int64_t)here * r.dim + col * V) = d;
-          }
-        }
-      } else {
-        P h0 = {};
-        const bool from = start && init && !none && here < r.packs;
-        if (from) h0 = at(init, here);
-#pragma unroll
-        for (int c = 0; c < V; c++) {
-          const S b = (S)xv[u].v[c];
-          const S g = none ? (S)0 : start && !from ? b : fma((S)av[u].v[c], from ? (S)h0.v[c] : state[c], b);
-          if (AGG) gain[c] = start ? (S)0 : gain[c] * (S)av[u].v[c];
-          state[c] = g;
-          y.v[c] = (T)g;
-        }
-        if (!AGG) *reinterpret_cast<P *>(out + t) = y;
-      }
-      before = here;
-      here = next;
-    }
-  }
-}
+// (A, B) of chunks and segments: a and b (count, dim), resets (count)
+template <typename S>
+struct Composed {
+  S *a, *b;
+  int32_t *resets;
+};
 
-// Step 1.  The chunk of thread t is t / cols, its columns t % cols.
-template <typename T, int V, bool DOWN, bool GRAD>
+// Step 1.  Thread t: the chunk t / cols, the piece t % cols.
+template <typename T, int V, bool GRAD>
 __global__ void __launch_bounds__(256) recur_chunk_kernel(Recur r, const T *__restrict__ a, const T *__restrict__ x,
                                                         const T *__restrict__ init,
-                                                        typename StateOf<T>::S *__restrict__ agg_a,
-                                                        typename StateOf<T>::S *__restrict__ agg_b,
-                                                        int32_t *__restrict__ resets) {
+                                                        Composed<typename StateOf<T>::S> chunks) {
   using S = typename StateOf<T>::S;
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x, c = t / r.cols, col = t % r.cols;
+  using P = Pack<T, V>;
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x, c = t / r.cols, col = (t - c * r.cols) * V;
   if (c >= r.chunks) return;
-  S state[V] = {}, gain[V];
+  auto at = [&](const T *p, int64_t i) { return *reinterpret_cast<const P *>(p + r.row(i) * r.dim + col); };
+  const int64_t begin = c * r.chunk, end = min((int64_t)r.n, begin + r.chunk);
+  const int last = r.id(end - 1);
+  const int64_t start = last < 0 ? end : r.first(last);
+  const bool reset = start >= begin;
+  S gain[V], state[V];
 #pragma unroll
-  for (int i = 0; i < V; i++) gain[i] = 1;
-  bool reset = false;
-  const int64_t first = c * r.chunk;
-  recur_walk<T, V, DOWN, GRAD, true>(r, first, min((int64_t)r.n, first + r.chunk), col, a, x, nullptr, init, nullptr,
-                                     nullptr, nullptr, state, gain, reset);
-  using P = Pack<S, V>;
-  P pa, pb;
-#pragma unroll
-  for (int i = 0; i < V; i++) {
-    pa.v[i] = gain[i];
-    pb.v[i] = state[i];
+  for (int v = 0; v < V; v++) {
+    gain[v] = reset ? 0 : 1;
+    state[v] = 0;
   }
-  *reinterpret_cast<P *>(agg_a + c * r.dim + col * V) = pa;
-  *reinterpret_cast<P *>(agg_b + c * r.dim + col * V) = pb;
-  if (col == 0) resets[c] = reset;
+  int64_t i = max(begin, start);
+  if (reset && i < end) {  // the pack's first row
+    const P x0 = at(x, i);
+#pragma unroll
+    for (int v = 0; v < V; v++) state[v] = (S)x0.v[v];
+    if (!GRAD && init && last < r.packs) {
+      const P a0 = at(a, i), h0 = *reinterpret_cast<const P *>(init + (int64_t)last * r.dim + col);
+#pragma unroll
+      for (int v = 0; v < V; v++) state[v] = fma((S)a0.v[v], (S)h0.v[v], state[v]);
+    }
+    i++;
+  }
+  for (; i < end; i += kAhead) {
+    P av[kAhead], xv[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; u++) {  // past the last row: that row again
+      const int64_t j = min(i + u, end - 1);
+      av[u] = at(a, GRAD ? j - 1 : j);
+      xv[u] = at(x, j);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; u++) {
+      const bool in = i + u < end;
+#pragma unroll
+      for (int v = 0; v < V; v++) {
+        const S g = (S)av[u].v[v], next = fma(g, state[v], (S)xv[u].v[v]);
+        state[v] = in ? next : state[v];
+        gain[v] = in && !reset ? gain[v] * g : gain[v];
+      }
+    }
+  }
+  Pack<S, V> pa, pb;
+#pragma unroll
+  for (int v = 0; v < V; v++) {
+    pa.v[v] = gain[v];
+    pb.v[v] = state[v];
+  }
+  *reinterpret_cast<Pack<S, V> *>(chunks.a + c * r.dim + col) = pa;
+  *reinterpret_cast<Pack<S, V> *>(chunks.b + c * r.dim + col) = pb;
+  if (col == 0) chunks.resets[c] = reset;
 }
 
-// Step 2: 16 columns and 64 runs of chunks a workgroup; the state before each chunk replaces agg_b.
+// Step 2: 16 columns and a segment a workgroup, 64 runs of kRunChunks chunks.  What lies before a chunk in its
+// segment replaces its (A, B); whether a pack starts there goes to `before` (resets is still read by others).
 template <typename S>
-__global__ void __launch_bounds__(1024) recur_carry_kernel(Recur r, const S *__restrict__ agg_a, S *__restrict__ agg_b,
-                                                         const int32_t *__restrict__ resets) {
-  __shared__ S s_a[64][17], s_b[64][17];
-  __shared__ int s_reset[64][17];
-  const int lane = threadIdx.x & 15, run = threadIdx.x >> 4;
-  const int64_t col = (int64_t)blockIdx.x * 16 + lane;
-  const int per = (r.chunks + 63) / 64, begin = min(r.chunks, run * per), end = min(r.chunks, begin + per);
-  S ga = 1, gb = 0;
-  int reset = 0;
-  if (col < r.dim) {
-#pragma unroll 4
-    for (int c = begin; c < end; c++) {
-      const S a = agg_a[c * r.dim + col], b = agg_b[c * r.dim + col];
-      const int z = resets[c];
-      gb = z ? b : fma(a, gb, b);
-      ga = z ? (S)0 : ga * a;
-      reset |= z;
-    }
+__global__ void __launch_bounds__(1024) recur_scan_kernel(Recur r, Composed<S> chunks, int32_t *__restrict__ before,
+                                                        Composed<S> segments) {
+  __shared__ S s_a[1024], s_b[1024];
+  __shared__ int s_reset[1024];
+  const int me = threadIdx.x;
+  const int64_t col = (int64_t)blockIdx.x * 16 + me % 16, at = min(col, r.dim - 1);
+  const int c0 = blockIdx.y * kSegment + me / 16 * kRunChunks;
+  S a[kRunChunks], b[kRunChunks], ga = 1, gb = 0;
+  int z[kRunChunks], reset = 0;
+#pragma unroll
+  for (int k = 0; k < kRunChunks; k++) {
+    const bool in = c0 + k < r.chunks;
+    const int64_t from = (int64_t)(in ? c0 + k : 0) * r.dim + at;
+    a[k] = in ? chunks.a[from] : (S)1;
+    b[k] = in ? chunks.b[from] : (S)0;
+    z[k] = in ? chunks.resets[c0 + k] : 0;
   }
-  s_a[run][lane] = ga;
-  s_b[run][lane] = gb;
-  s_reset[run][lane] = reset;
-  __syncthreads();
-  S state = 0;
-  for (int i = 0; i < run; i++) state = s_reset[i][lane] ? s_b[i][lane] : fma(s_a[i][lane], state, s_b[i][lane]);
-  if (col < r.dim) {
-#pragma unroll 4
-    for (int c = begin; c < end; c++) {
-      const S a = agg_a[c * r.dim + col], b = agg_b[c * r.dim + col];
-      agg_b[c * r.dim + col] = state;
-      state = resets[c] ? b : fma(a, state, b);
+#pragma unroll
+  for (int k = 0; k < kRunChunks; k++) {
+    gb = z[k] ? b[k] : fma(a[k], gb, b[k]);
+    ga = z[k] ? (S)0 : ga * a[k];
+    reset |= z[k];
+  }
+  // inclusive over the runs in doubling steps
+  for (int off = 16; off < 1024; off *= 2) {
+    s_a[me] = ga;
+    s_b[me] = gb;
+    s_reset[me] = reset;
+    __syncthreads();
+    if (me >= off && !reset) {
+      gb = fma(ga, s_b[me - off], gb);
+      reset = s_reset[me - off];
+      ga = reset ? (S)0 : ga * s_a[me - off];
     }
+    __syncthreads();
+  }
+  s_a[me] = ga;
+  s_b[me] = gb;
+  s_reset[me] = reset;
+  __syncthreads();
+  if (col < r.dim && me >= 1008) {
+    segments.a[(int64_t)blockIdx.y * r.dim + col] = ga;
+    segments.b[(int64_t)blockIdx.y * r.dim + col] = gb;
+    if (col == 0) segments.resets[blockIdx.y] = reset;
+  }
+  ga = me >= 16 ? s_a[me - 16] : (S)1;
+  gb = me >= 16 ? s_b[me - 16] : (S)0;
+  reset = me >= 16 ? s_reset[me - 16] : 0;
+  if (col >= r.dim) return;
+#pragma unroll
+  for (int k = 0; k < kRunChunks; k++) {
+    if (c0 + k >= r.chunks) break;
+    const int64_t to = (int64_t)(c0 + k) * r.dim + col;
+    chunks.a[to] = ga;
+    chunks.b[to] = gb;
+    if (col == 0) before[c0 + k] = reset;
+    gb = z[k] ? b[k] : fma(a[k], gb, b[k]);
+    ga = z[k] ? (S)0 : ga * a[k];
+    reset |= z[k];
   }
 }
 
-// Step 3.  carry: the state before each chunk (NULL with one chunk).  Threads past the chunks write the
-// gradients of initial states that no pack has.
-template <typename T, int V, bool DOWN, bool GRAD>
+// Step 3.  Threads past the chunks write the gradients of initial states that no pack has.
+template <typename T, int V, bool GRAD>
 __global__ void __launch_bounds__(256) recur_write_kernel(Recur r, const T *__restrict__ a, const T *__restrict__ x,
                                                         const T *__restrict__ h, const T *__restrict__ init,
-                                                        const typename StateOf<T>::S *__restrict__ carry,
+                                                        Composed<const typename StateOf<T>::S> chunks,
+                                                        const int32_t *__restrict__ chunk_before,
+                                                        Composed<const typename StateOf<T>::S> segments,
                                                         T *__restrict__ out, T *__restrict__ da,
                                                         T *__restrict__ dinit) {
   using S = typename StateOf<T>::S;
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x, c = t / r.cols, col = t % r.cols;
-  if (c >= r.chunks) {
-    const int64_t p = c - r.chunks;
+  using P = Pack<T, V>;
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x, place = t / r.cols, col = (t - place * r.cols) * V;
+  const int64_t c = r.chunks - 1 - place;
+  if (c < 0) {
+    const int64_t p = -1 - c;
     if (dinit && p < r.packs && (p >= r.n || r.starts[p] >= r.n))
-      *reinterpret_cast<Pack<T, V> *>(dinit + p * r.dim + col * V) = Pack<T, V>{};
+      *reinterpret_cast<P *>(dinit + p * r.dim + col) = P{};
     return;
   }
-  S state[V] = {}, gain[V];
-  bool reset = false;
-  if (carry) {
-    const Pack<S, V> s = *reinterpret_cast<const Pack<S, V> *>(carry + c * r.dim + col * V);
+  auto at = [&](const T *p, int64_t i) { return *reinterpret_cast<const P *>(p + r.row(i) * r.dim + col); };
+  const int64_t begin = c * r.chunk, end = min((int64_t)r.n, begin + r.chunk), n = r.n;
+  int ids[kAheadWrite + 2];  // of the rows before, of and after a batch
 #pragma unroll
-    for (int i = 0; i < V; i++) state[i] = s.v[i];
+  for (int u = 0; u < kAheadWrite + 2; u++) ids[u] = r.id(begin - 1 + u);
+  const bool carried = ids[0] == ids[1] && ids[1] >= 0;
+  S state[V];
+#pragma unroll
+  for (int v = 0; v < V; v++) state[v] = 0;
+  if (carried) {
+    auto step = [&](const Composed<const S> &m, int64_t k, bool reset) {
+      const Pack<S, V> ka = *reinterpret_cast<const Pack<S, V> *>(m.a + k * r.dim + col);
+      const Pack<S, V> kb = *reinterpret_cast<const Pack<S, V> *>(m.b + k * r.dim + col);
+#pragma unroll
+      for (int v = 0; v < V; v++) state[v] = reset ? kb.v[v] : fma(ka.v[v], state[v], kb.v[v]);
+    };
+    const bool here = chunk_before[c] != 0;
+    if (!here) {
+      int64_t k = c / kSegment - 1;
+      while (k > 0 && !segments.resets[k]) k--;
+      for (; k >= 0 && k < c / kSegment; k++) step(segments, k, segments.resets[k] != 0);
+    }
+    step(chunks, c, here);
   }
-  const int64_t first = c * r.chunk;
-  recur_walk<T, V, DOWN, GRAD, false>(r, first, min((int64_t)r.n, first + r.chunk), col, a, x, h, init, out, da, dinit,
-                                      state, gain, reset);
+  P gate = {};  // GRAD: the gate of the row walked before
+  if (GRAD && carried) gate = at(a, begin - 1);
+  for (int64_t i0 = begin; i0 < end; i0 += kAheadWrite) {
+    P av[kAheadWrite], xv[kAheadWrite], hv[kAheadWrite];
+    int next_ids[kAheadWrite + 2];
+#pragma unroll
+    for (int u = 0; u < kAheadWrite; u++) {  // past the last row: that row again
+      const int64_t i = min(i0 + u, end - 1);
+      av[u] = at(a, i);
+      xv[u] = at(x, i);
+      // the state on the far side of a pack's border is its initial one; GRAD: elsewhere the forward's before
+      // this row, which is that of the next row walked
+      const bool none = ids[u + 1] < 0, border = GRAD ? ids[u + 2] != ids[u + 1] : ids[u + 1] != ids[u];
+      hv[u] = P{};
+      if (border) {
+        if (init && !none && ids[u + 1] < r.packs && i0 + u < end)
+          hv[u] = *reinterpret_cast<const P *>(init + (int64_t)ids[u + 1] * r.dim + col);
+      } else if (GRAD) {
+        hv[u] = at(h, min(i + 1, n - 1));
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kAheadWrite + 2; u++) next_ids[u] = r.id(i0 + kAheadWrite - 1 + u);
+#pragma unroll
+    for (int u = 0; u < kAheadWrite; u++) {
+      const int64_t i = i0 + u;
+      if (i >= end) continue;
+      const bool none = ids[u + 1] < 0, start = none || ids[u + 1] != ids[u], last = ids[u + 2] != ids[u + 1];
+      const bool from = init && !none && ids[u + 1] < r.packs;
+      const int64_t to = r.row(i) * r.dim + col;
+      P y;
+      if (GRAD) {
+        P dy;
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+          const S b = (S)xv[u].v[v], with = fma((S)gate.v[v], state[v], b);
+          state[v] = none ? (S)0 : start ? b : with;
+          y.v[v] = (T)state[v];
+          dy.v[v] = (T)(none ? (S)0 : state[v] * (S)hv[u].v[v]);
+        }
+        gate = av[u];
+        *reinterpret_cast<P *>(da + to) = dy;
+        if (dinit && last && from) {
+          P d;
+#pragma unroll
+          for (int v = 0; v < V; v++) d.v[v] = (T)((S)av[u].v[v] * state[v]);
+          *reinterpret_cast<P *>(dinit + (int64_t)ids[u + 1] * r.dim + col) = d;
+        }
+      } else {
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+          const S b = (S)xv[u].v[v], h0 = (S)hv[u].v[v], prev = start ? h0 : state[v];
+          const S with = fma((S)av[u].v[v], prev, b);
+          state[v] = none ? (S)0 : start && !from ? b : with;
+          y.v[v] = (T)state[v];
+        }
+      }
+      *reinterpret_cast<P *>(out + to) = y;
+    }
+#pragma unroll
+    for (int u = 0; u < kAheadWrite + 2; u++) ids[u] = next_ids[u];
+  }
 }
 
-// Rows of a chunk: 2^18 threads fill the chip, and longer chunks save carries from there on.
-static int recur_chunk_rows(int64_t n, int64_t dim) {
-  const int64_t v = dim % 4 == 0 ? 4 : 1;
-  return (int)std::min<int64_t>(256, std::max<int64_t>(16, cdiv(n * (dim / v), 1 << 18)));
+// Elements of a thread's piece: 16 bytes where rows are whole numbers of such pieces, else one element.
+static int recur_piece(int64_t dim, size_t esize) { return dim % (16 / esize) == 0 ? (int)(16 / esize) : 1; }
+
+// Rows of a chunk: 2^17 threads keep the memory busy; longer chunks from there on, for fewer (A, B)
+static int recur_chunk_rows(kl_dtype dtype, int64_t n, int64_t dim) {
+  const int64_t cols = dim / recur_piece(dim, dtype == KL_F64 ? 8 : dtype == KL_F32 ? 4 : 2);
+  return (int)std::min<int64_t>(64, std::max<int64_t>(8, cdiv(n * cols, 1 << 17)));
 }
 
-template <typename T, int V, bool DOWN, bool GRAD>
+// The workspace: (A, B) of chunks and of segments
+template <typename S>
+struct RecurSpace {
+  Composed<S> chunks = {}, segments = {};
+  int32_t *before = nullptr;
+  size_t bytes = 0;
+  RecurSpace(char *ws, int64_t num_chunks, int64_t dim) {
+    auto take = [&](size_t n) {
+      char *p = ws ? ws + bytes : nullptr;
+      bytes += al256(n);
+      return p;
+    };
+    const int64_t num = cdiv(num_chunks, kSegment);
+    chunks.a = (S *)take(num_chunks * dim * sizeof(S));
+    chunks.b = (S *)take(num_chunks * dim * sizeof(S));
+    segments.a = (S *)take(num * dim * sizeof(S));
+    segments.b = (S *)take(num * dim * sizeof(S));
+    chunks.resets = (int32_t *)take(num_chunks * 4);
+    before = (int32_t *)take(num_chunks * 4);
+    segments.resets = (int32_t *)take(num * 4);
+  }
+};
+
+template <typename T, int V, bool GRAD>
 static int recur_run(Recur r, const void *a, const void *x, const void *h, const void *init, void *out, void *da,
                      void *dinit, void *ws, hipStream_t st) {
   using S = typename StateOf<T>::S;
-  r.cols = (int)(r.dim / V);
-  S *agg_a = (S *)ws, *agg_b = (S *)((char *)ws + al256((size_t)r.chunks * r.dim * sizeof(S)));
-  int32_t *resets = (int32_t *)((char *)agg_b + al256((size_t)r.chunks * r.dim * sizeof(S)));
-  const unsigned blocks = (unsigned)cdiv((int64_t)r.chunks * r.cols, 256);
+  r.cols = r.dim / V;
+  const RecurSpace<S> m((char *)ws, r.chunks, r.dim);
   if (r.chunks > 1) {
-    hipLaunchKernelGGL((recur_chunk_kernel<T, V, DOWN, GRAD>), dim3(blocks), dim3(256), 0, st, r, (const T *)a,
-                       (const T *)x, (const T *)init, agg_a, agg_b, resets);
+    hipLaunchKernelGGL((recur_chunk_kernel<T, V, GRAD>), dim3((unsigned)cdiv(r.chunks * r.cols, 256)), dim3(256), 0, st,
+                       r, (const T *)a, (const T *)x, (const T *)init, m.chunks);
     KL_CHECK_LAUNCH();
-    hipLaunchKernelGGL(recur_carry_kernel<S>, dim3((unsigned)cdiv(r.dim, 16)), dim3(1024), 0, st, r, agg_a, agg_b,
-                       resets);
+    hipLaunchKernelGGL(recur_scan_kernel<S>, dim3((unsigned)cdiv(r.dim, 16), (unsigned)cdiv(r.chunks, kSegment)),
+                       dim3(1024), 0, st, r, m.chunks, m.before, m.segments);
     KL_CHECK_LAUNCH();
   }
-  const unsigned all = (unsigned)cdiv((r.chunks + (dinit ? (int64_t)r.packs : 0)) * r.cols, 256);
-  hipLaunchKernelGGL((recur_write_kernel<T, V, DOWN, GRAD>), dim3(all), dim3(256), 0, st, r, (const T *)a,
-                     (const T *)x, (const T *)h, (const T *)init, r.chunks > 1 ? agg_b : (S *)nullptr, (T *)out,
-                     (T *)da, (T *)dinit);
+  const dim3 grid((unsigned)cdiv((r.chunks + (dinit ? (int64_t)r.packs : 0)) * r.cols, 256));
+  hipLaunchKernelGGL((recur_write_kernel<T, V, GRAD>), grid, dim3(256), 0, st, r, (const T *)a, (const T *)x,
+                     (const T *)h, (const T *)init, Composed<const S>{m.chunks.a, m.chunks.b, m.chunks.resets},
+                     m.before, Composed<const S>{m.segments.a, m.segments.b, m.segments.resets}, (T *)out, (T *)da,
+                     (T *)dinit);
   KL_CHECK_LAUNCH();
   return KL_OK;
 }
 
-template <typename T, int V>
-static int recur_direction(const Recur &r, bool down, bool grad, const void *a, const void *x, const void *h,
-                           const void *init, void *out, void *da, void *dinit, void *ws, hipStream_t st) {
-  if (grad) {
-    return down ? recur_run<T, V, true, true>(r, a, x, h, init, out, da, dinit, ws, st)
-                : recur_run<T, V, false, true>(r, a, x, h, init, out, da, dinit, ws, st);
-  }
-  return down ? recur_run<T, V, true, false>(r, a, x, h, init, out, da, dinit, ws, st)
-              : recur_run<T, V, false, false>(r, a, x, h, init, out, da, dinit, ws, st);
-}
-
-// Columns per thread: four (loads of 8 to 32 bytes) where every row is aligned to that, else one
 template <typename T>
-static int recur_type(const Recur &r, bool down, bool grad, const void *a, const void *x, const void *h,
-                      const void *init, void *out, void *da, void *dinit, void *ws, hipStream_t st) {
+static int recur_type(const Recur &r, bool grad, const void *a, const void *x, const void *h, const void *init,
+                      void *out, void *da, void *dinit, void *ws, hipStream_t st) {
   const uintptr_t all = (uintptr_t)a | (uintptr_t)x | (uintptr_t)h | (uintptr_t)init | (uintptr_t)out |
                         (uintptr_t)da | (uintptr_t)dinit;
-  if (r.dim % 4 == 0 && all % (4 * sizeof(T)) == 0)
-    return recur_direction<T, 4>(r, down, grad, a, x, h, init, out, da, dinit, ws, st);
-  return recur_direction<T, 1>(r, down, grad, a, x, h, init, out, da, dinit, ws, st);
+  constexpr int V = 16 / (int)sizeof(T);
+  const bool pieces = recur_piece(r.dim, sizeof(T)) == V && all % 16 == 0;
+  if (grad) {
+    return pieces ? recur_run<T, V, true>(r, a, x, h, init, out, da, dinit, ws, st)
+                  : recur_run<T, 1, true>(r, a, x, h, init, out, da, dinit, ws, st);
+  }
+  return pieces ? recur_run<T, V, false>(r, a, x, h, init, out, da, dinit, ws, st)
+                : recur_run<T, 1, false>(r, a, x, h, init, out, da, dinit, ws, st);
 }
 
 static int recurrence(kl_dtype dtype, bool down, bool grad, int64_t n, int64_t dim, int64_t packs, const void *a,
@@ -279,23 +369,26 @@ static int recurrence(kl_dtype dtype, bool down, bool grad, int64_t n, int64_t d
   KL_REQUIRE(n >= 0 && n < ((int64_t)1 << 31) - 256 && dim >= 0 && dim < (int64_t)1 << 24 && packs >= 0 &&
                  packs < (int64_t)1 << 31,
              "linear_recurrence: sizes out of range");
+  KL_REQUIRE(cdiv((cdiv(n, 8) + packs) * dim, 256) < (int64_t)1 << 31 &&
+                 cdiv(n, recur_chunk_rows(dtype, n, dim)) <= (int64_t)kSegment * 65535,
+             "linear_recurrence: too many elements");
   KL_REQUIRE(ws_bytes >= kl_linear_recurrence_workspace_bytes(dtype, n, dim),
              "linear_recurrence: the workspace is too small");
   if (dim == 0 || (n == 0 && !(dinit && packs))) return KL_OK;
-  Recur r;
+  Recur r = {};
   r.n = (int)n;
   r.dim = dim;
-  r.chunk = recur_chunk_rows(n, dim);
+  r.chunk = recur_chunk_rows(dtype, n, dim);
   r.chunks = (int)cdiv(n, r.chunk);
+  r.down = down ? 1 : 0;
   r.packs = init ? (int)packs : 0;
   r.ids = ids;
   r.starts = starts;
-  KL_REQUIRE(cdiv(((int64_t)r.chunks + packs) * dim, 256) < (int64_t)1 << 31, "linear_recurrence: too many elements");
   switch (dtype) {
-    case KL_F32: return recur_type<float>(r, down, grad, a, x, h, init, out, da, dinit, ws, st);
-    case KL_F64: return recur_type<double>(r, down, grad, a, x, h, init, out, da, dinit, ws, st);
-    case KL_F16: return recur_type<f16_t>(r, down, grad, a, x, h, init, out, da, dinit, ws, st);
-    case KL_BF16: return recur_type<bf16_t>(r, down, grad, a, x, h, init, out, da, dinit, ws, st);
+    case KL_F32: return recur_type<float>(r, grad, a, x, h, init, out, da, dinit, ws, st);
+    case KL_F64: return recur_type<double>(r, grad, a, x, h, init, out, da, dinit, ws, st);
+    case KL_F16: return recur_type<f16_t>(r, grad, a, x, h, init, out, da, dinit, ws, st);
+    case KL_BF16: return recur_type<bf16_t>(r, grad, a, x, h, init, out, da, dinit, ws, st);
     default: set_error("linear_recurrence: expected a Half, BFloat16, Float or Double tensor"); return KL_E_INVALID;
   }
 }
@@ -306,9 +399,8 @@ using namespace kl;
 
 extern "C" size_t kl_linear_recurrence_workspace_bytes(kl_dtype dtype, int64_t num_rows, int64_t dim) {
   if (num_rows <= 0 || dim <= 0) return 256;
-  const size_t chunks = (size_t)cdiv(num_rows, recur_chunk_rows(num_rows, dim));
-  if (chunks <= 1) return 256;
-  return 2 * al256(chunks * dim * (dtype == KL_F64 ? 8 : 4)) + al256(chunks * 4);
+  const size_t chunks = (size_t)cdiv(num_rows, recur_chunk_rows(dtype, num_rows, dim));
+  return dtype == KL_F64 ? RecurSpace<double>(nullptr, chunks, dim).bytes : RecurSpace<float>(nullptr, chunks, dim).bytes;
 }
 
 extern "C" int kl_linear_recurrence_forward(kl_dtype dtype, int64_t num_rows, int64_t dim, const void *gates,

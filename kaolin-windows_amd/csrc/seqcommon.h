@@ -175,6 +175,9 @@ __device__ __forceinline__ bool piece_bad(u32x4 w) {
   return bad != 0;
 }
 
+// What is the same in every lane, as such: loops and addresses made of it stay in scalar registers
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 // f(T()) for the element type of a tensor
 template <typename F>
 inline int with_type(kl_dtype dtype, const char *func, F f) {
