@@ -4,8 +4,13 @@
 //
 // Bound by memory: every element is read once and written once.  A workgroup first writes the cosines and
 // sines of its rows to LDS, one thread a (row, pair), and all heads of both tensors use them; then groups of
-// `lanes` lanes take one head each, 16 bytes a lane.  Angles are formed in 64 bits (a position of 10^6 in 32
-// bits leaves an angle only 4 digits) and reduced to a quarter turn before they become floats.
+// LANES lanes take one head each, 16 bytes a lane, as many heads of a row side by side as there are groups for
+// (a lane keeps its row's cosines and sines in registers over them), then rows.  Sums and partners go between
+// lanes without LDS where they lie 1, 2, 4 or 8 apart: through LDS, with the table read for each head and the
+// weights chosen for each element, the arithmetic was what bound it (16385 rows of 32 + 8 heads of 128, bf16,
+// 336 MB: 102 us, now 81, 4.1 TB/s; a copy of as many bytes takes 67).
+// Angles are formed in 64 bits (a position of 10^6 in 32 bits leaves an angle only 4 digits) and reduced to a
+// quarter turn before they become floats.
 // Norms, products and the sums over rows of the weights' gradients are in 32 bits; the outputs are rounded
 // once.  Backward: g = the gradient rotated back; dw = sum over rows and heads of g x r;
 // dx = r (g w - x r mean(g w x r)).
@@ -14,11 +19,14 @@
 namespace kl {
 
 enum { POS_PACK = 0, POS_I32 = 1, POS_I64 = 2, POS_F32 = 3 };
+// Where an element's partner is: in its own lane (interleaved pairs); at the same place of a lane 8, 4 or any number
+// away; anywhere (through LDS)
+enum Partner { OWN, AWAY_8, AWAY_4, AWAY, ANYWHERE };
 
 struct NormRot {
   Heads q, k;
   int64_t n;
-  int hq, hk, dim, half, interleaved, rows;  // half: pairs; rows: rows of a workgroup's table
+  int hq, hk, dim, half, rows, partner;  // half: pairs; rows: rows of a workgroup's table; partner: a Partner
   float eps;
   const double *freqs;
   int pos_kind;
@@ -58,12 +66,12 @@ __device__ __forceinline__ float2 unit(double angle) {
 template <typename T, int VE>
 struct HeadPiece {
   float v[VE];
-  __device__ __forceinline__ void load(const T *p) {
+  __device__ __forceinline__ void set(u32x4 w) {
     union {
       u32x4 w;
       T t[VE];
     } x;
-    x.w = *reinterpret_cast<const u32x4 *>(p);
+    x.w = w;
 #pragma unroll
     for (int e = 0; e < VE; e++) v[e] = (float)x.t[e];
   }
@@ -87,68 +95,114 @@ __device__ __forceinline__ void load_weight(const NormRot &a, const void *w, int
   }
 }
 
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+
+// Sum over each LANES neighbouring lanes, in every one of them
 template <int LANES>
 __device__ __forceinline__ float lanes_sum(float v) {
-#pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  v += dpp<0xb1>(v);   // lanes 1 away
+  v += dpp<0x4e>(v);   // 2 away
+  v += dpp<0x141>(v);  // the other half of 8
+  if constexpr (LANES >= 16) v += dpp<0x140>(v);  // of 16
+  if constexpr (LANES >= 32) v += __shfl_xor(v, 16);
+  if constexpr (LANES >= 64) v = half_sum(v);
   return v;
 }
 
-// Rotates a head held by LANES lanes, VE elements each; dir -1: back.  cs: the row's table.  spare: LDS of
-// this head, LANES * VE floats, for the half layout where partners lie at other places of their lanes.
-template <int VE, int LANES>
-__device__ __forceinline__ void rotate(const NormRot &a, const float2 *cs, float dir, int sub, float *spare,
-                                       float (&v)[VE]) {
-  const int col = sub * VE;
-  if (a.interleaved) {
-    if (col < 2 * a.half) {
-#pragma unroll
-      for (int e = 0; e < VE; e += 2) {
-        if (col + e < 2 * a.half) {
-          const float2 t = cs[(col + e) / 2];
-          const float s = dir * t.y, x = v[e], y = v[e + 1];
-          v[e] = x * t.x - y * s;
-          v[e + 1] = x * s + y * t.x;
-        }
-      }
-    }
-    return;
-  }
-  if (a.half % VE == 0) {  // partners sit at the same place of a lane half / VE away
-    const bool first = col < a.half, second = !first && col < 2 * a.half;
-    const int other = (int)(threadIdx.x & 63) + (first ? a.half / VE : second ? -(a.half / VE) : 0);
-#pragma unroll
-    for (int e = 0; e < VE; e++) {
-      const float y = __shfl(v[e], other);
-      if (first || second) {
-        const float2 t = cs[first ? col + e : col + e - a.half];
-        v[e] = v[e] * t.x + (first ? -dir : dir) * t.y * y;
-      }
-    }
-    return;
-  }
-#pragma unroll
-  for (int e = 0; e < VE; e++) spare[col + e] = v[e];
-  __builtin_amdgcn_wave_barrier();  // one wave writes and reads; LDS keeps its order
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+// What a lane keeps of its row: element e becomes v[e] c[e] + partner[e] s[e]
+template <int VE>
+struct Turn {
+  float c[VE], s[VE];
+};
+
+template <int VE>
+__device__ __forceinline__ Turn<VE> row_turn(const NormRot &a, const float2 *table, int r, int sub, float dir) {
+  Turn<VE> t;
 #pragma unroll
   for (int e = 0; e < VE; e++) {
-    const int i = col + e;
-    if (i < 2 * a.half) {
-      const bool first = i < a.half;
-      const int j = first ? i : i - a.half;
-      const float2 t = cs[j];
-      v[e] = v[e] * t.x + (first ? -dir : dir) * t.y * spare[first ? i + a.half : j];
+    const int i = sub * VE + e;
+    const bool in = i < 2 * a.half, first = a.partner == OWN ? (e & 1) == 0 : i < a.half;
+    const int pair = a.partner == OWN ? i / 2 : first ? i : i - a.half;
+    const float2 u = in ? table[r * a.half + pair] : make_float2(1, 0);
+    t.c[e] = u.x;
+    t.s[e] = first ? -dir * u.y : dir * u.y;
+  }
+  return t;
+}
+
+// spare: LDS of this head, LANES * VE floats
+template <int VE>
+__device__ __forceinline__ void rotate(const NormRot &a, const Turn<VE> &t, int sub, float *spare, float (&v)[VE]) {
+  float other[VE];
+  switch (a.partner) {
+    case OWN:
+#pragma unroll
+      for (int e = 0; e < VE; e++) other[e] = v[e ^ 1];
+      break;
+    case AWAY_8:
+#pragma unroll
+      for (int e = 0; e < VE; e++) other[e] = dpp<0x128>(v[e]);  // rows of 16 lanes, turned by 8
+      break;
+    case AWAY_4: {
+      const bool first = (sub & 7) < 4;
+#pragma unroll
+      for (int e = 0; e < VE; e++) {
+        const float up = dpp<0x104>(v[e]), down = dpp<0x114>(v[e]);  // from 4 lanes on, from 4 lanes back
+        other[e] = first ? up : down;
+      }
+      break;
+    }
+    case AWAY: {
+      const int h = a.half / VE, lane = threadIdx.x & 63, from = sub < h ? lane + h : sub < 2 * h ? lane - h : lane;
+#pragma unroll
+      for (int e = 0; e < VE; e++) other[e] = __shfl(v[e], from);
+      break;
+    }
+    default: {
+      // one wave writes and reads; LDS keeps its order
+#pragma unroll
+      for (int e = 0; e < VE; e++) spare[sub * VE + e] = v[e];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int e = 0; e < VE; e++) {
+        const int i = sub * VE + e;
+        other[e] = i < a.half ? spare[i + a.half] : i < 2 * a.half ? spare[i - a.half] : 0.f;
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
     }
   }
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
+  if (2 * a.half < a.dim) {  // elements past the rotated ones have no partner, not even an infinite one times 0
+#pragma unroll
+    for (int e = 0; e < VE; e++) other[e] = sub * VE + e < 2 * a.half ? other[e] : 0.f;
+  }
+#pragma unroll
+  for (int e = 0; e < VE; e++) v[e] = fmaf(other[e], t.s[e], v[e] * t.c[e]);
 }
 
 __device__ __forceinline__ void fill_table(const NormRot &a, int64_t row0, int rows, float2 *table) {
   for (int i = threadIdx.x; i < rows * a.half; i += 256) {
     const int r = i / a.half, p = i - r * a.half;
     table[i] = unit(position(a, row0 + r) * a.freqs[p]);
+  }
+}
+
+// Calls f(row, head, live, turn) for the (row, head)s of one tensor that a group of lanes takes: `side` groups
+// side by side along the heads, the others along the rows.  Every lane of a wave makes every call.
+template <int GROUPS, int VE, typename F>
+__device__ __forceinline__ void each_head(const NormRot &a, int heads, int rows, int group, int sub, float dir,
+                                          const float2 *table, F f) {
+  int side = 1;
+  while (side < GROUPS && side < heads) side *= 2;
+  const int h0 = group & (side - 1), r0 = group / side, step = GROUPS / side;
+  for (int rb = 0; rb < rows; rb += step) {
+    const int r = rb + r0;
+    const Turn<VE> t = row_turn<VE>(a, table, min(r, rows - 1), sub, dir);
+    for (int hb = 0; hb < heads; hb += side) f(r, hb + h0, r < rows && hb + h0 < heads, t);
   }
 }
 
@@ -159,34 +213,32 @@ __global__ void __launch_bounds__(256) norm_rotary_kernel(NormRot a, const T *__
   __shared__ float2 table[kTable];
   __shared__ float spare[256 * VE];
   const int64_t row0 = (int64_t)blockIdx.x * a.rows;
-  const int rows = (int)min((int64_t)a.rows, a.n - row0), heads = a.hq + a.hk;
-  const int sub = threadIdx.x % LANES, col = sub * VE;
+  const int rows = (int)min((int64_t)a.rows, a.n - row0);
+  const int sub = threadIdx.x % LANES, col = sub * VE, group = threadIdx.x / LANES;
   const bool in = col < a.dim;
+  const float inv_dim = 1.f / (float)a.dim;
   fill_table(a, row0, rows, table);
-  float wq[VE], wk[VE];
-  load_weight<T, VE>(a, a.wq, col, wq);
-  load_weight<T, VE>(a, a.wk, col, wk);
   __syncthreads();
-  // every lane of a wave makes every round: the exchanges take whole waves
-  for (int i0 = 0; i0 < rows * heads; i0 += GROUPS) {
-    const int i = i0 + threadIdx.x / LANES;
-    const bool live = in && i < rows * heads;
-    const int r = i < rows * heads ? i / heads : 0, hd = i < rows * heads ? i - r * heads : 0;
-    const bool is_q = hd < a.hq;
-    const int64_t row = row0 + r;
-    HeadPiece<T, VE> x;
+  auto side = [&](const T *x, Heads st, int heads, const void *weight, T *y) {
+    float w[VE];
+    load_weight<T, VE>(a, weight, col, w);
+    each_head<GROUPS, VE>(a, heads, rows, group, sub, 1.f, table, [&](int r, int hd, bool live, const Turn<VE> &t) {
+      const int64_t row = row0 + r;
+      live = live && in;
+      HeadPiece<T, VE> v;
+      v.set(live ? *reinterpret_cast<const u32x4 *>(x + row * st.row + hd * st.head + col) : u32x4{0, 0, 0, 0});
+      float ss = 0;
 #pragma unroll
-    for (int e = 0; e < VE; e++) x.v[e] = 0;
-    if (live) x.load(is_q ? q + row * a.q.row + hd * a.q.head + col : k + row * a.k.row + (hd - a.hq) * a.k.head + col);
-    float ss = 0;
+      for (int e = 0; e < VE; e++) ss = fmaf(v.v[e], v.v[e], ss);
+      const float inv = rsqrtf(fmaf(lanes_sum<LANES>(ss), inv_dim, a.eps));
 #pragma unroll
-    for (int e = 0; e < VE; e++) ss = fmaf(x.v[e], x.v[e], ss);
-    const float inv = rsqrtf(lanes_sum<LANES>(ss) / (float)a.dim + a.eps);
-#pragma unroll
-    for (int e = 0; e < VE; e++) x.v[e] *= inv * (is_q ? wq[e] : wk[e]);
-    rotate<VE, LANES>(a, table + r * a.half, 1.f, sub, spare + threadIdx.x / LANES * (LANES * VE), x.v);
-    if (live) x.store(is_q ? yq + (row * a.hq + hd) * a.dim + col : yk + (row * a.hk + hd - a.hq) * a.dim + col);
-  }
+      for (int e = 0; e < VE; e++) v.v[e] *= inv * w[e];
+      rotate<VE>(a, t, sub, spare + group * (LANES * VE), v.v);
+      if (live) v.store(y + (row * heads + hd) * a.dim + col);
+    });
+  };
+  side(q, a.q, a.hq, a.wq, yq);
+  side(k, a.k, a.hk, a.wk, yk);
 }
 
 // part: (workgroups, 2, dim) partial sums of the weights' gradients (NULL: none wanted)
@@ -198,11 +250,10 @@ __global__ void __launch_bounds__(256) norm_rotary_bwd_kernel(NormRot a, const T
   constexpr int VE = 16 / (int)sizeof(T), GROUPS = 256 / LANES;
   __shared__ float2 table[kTable];
   __shared__ float spare[256 * VE];
-  const int heads = a.hq + a.hk, sub = threadIdx.x % LANES, col = sub * VE, group = threadIdx.x / LANES;
+  const int sub = threadIdx.x % LANES, col = sub * VE, group = threadIdx.x / LANES;
   const bool in = col < a.dim;
-  float wq[VE], wk[VE], sq[VE], sk[VE];
-  load_weight<T, VE>(a, a.wq, col, wq);
-  load_weight<T, VE>(a, a.wk, col, wk);
+  const float inv_dim = 1.f / (float)a.dim;
+  float sq[VE], sk[VE];
 #pragma unroll
   for (int e = 0; e < VE; e++) sq[e] = sk[e] = 0;
   for (int64_t row0 = (int64_t)blockIdx.x * a.rows; row0 < a.n; row0 += (int64_t)gridDim.x * a.rows) {
@@ -210,40 +261,38 @@ __global__ void __launch_bounds__(256) norm_rotary_bwd_kernel(NormRot a, const T
     __syncthreads();
     fill_table(a, row0, rows, table);
     __syncthreads();
-    for (int i0 = 0; i0 < rows * heads; i0 += GROUPS) {
-      const int i = i0 + group;
-      const bool live = in && i < rows * heads;
-      const int r = i < rows * heads ? i / heads : 0, hd = i < rows * heads ? i - r * heads : 0;
-      const bool is_q = hd < a.hq;
-      const int64_t row = row0 + r;
-      HeadPiece<T, VE> x, g;
+    auto side = [&](const T *x, Heads st, const T *gy, int heads, const void *weight, T *dx, float (&sum)[VE]) {
+      float w[VE];
+      load_weight<T, VE>(a, weight, col, w);
+      each_head<GROUPS, VE>(a, heads, rows, group, sub, -1.f, table, [&](int r, int hd, bool live, const Turn<VE> &t) {
+        const int64_t row = row0 + r, at = (row * heads + hd) * a.dim + col;
+        live = live && in;
+        HeadPiece<T, VE> v, g;
+        const u32x4 none = {0, 0, 0, 0};
+        v.set(live ? *reinterpret_cast<const u32x4 *>(x + row * st.row + hd * st.head + col) : none);
+        g.set(live ? *reinterpret_cast<const u32x4 *>(gy + at) : none);
+        rotate<VE>(a, t, sub, spare + group * (LANES * VE), g.v);
+        float ss = 0;
 #pragma unroll
-      for (int e = 0; e < VE; e++) x.v[e] = g.v[e] = 0;
-      const int64_t at = is_q ? (row * a.hq + hd) * a.dim + col : (row * a.hk + hd - a.hq) * a.dim + col;
-      if (live) {
-        x.load(is_q ? q + row * a.q.row + hd * a.q.head + col : k + row * a.k.row + (hd - a.hq) * a.k.head + col);
-        g.load((is_q ? gq : gk) + at);
-      }
-      rotate<VE, LANES>(a, table + r * a.half, -1.f, sub, spare + group * (LANES * VE), g.v);
-      float ss = 0;
+        for (int e = 0; e < VE; e++) ss = fmaf(v.v[e], v.v[e], ss);
+        const float inv = rsqrtf(fmaf(lanes_sum<LANES>(ss), inv_dim, a.eps));
+        float dot = 0;
 #pragma unroll
-      for (int e = 0; e < VE; e++) ss = fmaf(x.v[e], x.v[e], ss);
-      const float inv = rsqrtf(lanes_sum<LANES>(ss) / (float)a.dim + a.eps);
-      float dot = 0;
+        for (int e = 0; e < VE; e++) {
+          v.v[e] *= inv;
+          const float t1 = g.v[e] * v.v[e];
+          sum[e] += live ? t1 : 0.f;
+          g.v[e] *= w[e];
+          dot = fmaf(g.v[e], v.v[e], dot);
+        }
+        const float mean = lanes_sum<LANES>(dot) * inv_dim;
 #pragma unroll
-      for (int e = 0; e < VE; e++) {
-        x.v[e] *= inv;
-        const float t = g.v[e] * x.v[e];
-        sq[e] += is_q && live ? t : 0.f;
-        sk[e] += is_q || !live ? 0.f : t;
-        g.v[e] *= is_q ? wq[e] : wk[e];
-        dot = fmaf(g.v[e], x.v[e], dot);
-      }
-      const float mean = lanes_sum<LANES>(dot) / (float)a.dim;
-#pragma unroll
-      for (int e = 0; e < VE; e++) g.v[e] = inv * (g.v[e] - x.v[e] * mean);
-      if (live) g.store((is_q ? dq : dk) + at);
-    }
+        for (int e = 0; e < VE; e++) g.v[e] = inv * (g.v[e] - v.v[e] * mean);
+        if (live) g.store(dx + at);
+      });
+    };
+    side(q, a.q, gq, a.hq, a.wq, dq, sq);
+    side(k, a.k, gk, a.hk, a.wk, dk, sk);
   }
   if (!part) return;
   // the groups' sums, added in their order
@@ -279,10 +328,10 @@ __global__ void __launch_bounds__(256) norm_weight_grad_kernel(int dim, int part
   if (type == KL_BF16) ((bf16_t *)out)[d] = (bf16_t)(float)s;
 }
 
-// Rows of a workgroup: its table holds them, and each group of lanes gets some four heads, unless that leaves
-// too few workgroups for the chip.
+// Rows of a workgroup: its table holds them, and each group of lanes gets some 32 heads (at the size above 4 take
+// 110 us, 8 take 93 and 32 take 81: the table and its barrier come first), unless that leaves too few workgroups.
 static int norm_rows(int64_t n, int heads, int half, int groups) {
-  int64_t rows = std::max<int64_t>(1, std::min<int64_t>({16, half ? kTable / half : 16, cdiv(4 * groups, heads)}));
+  int64_t rows = std::max<int64_t>(1, std::min<int64_t>({16, half ? kTable / half : 16, cdiv(32 * groups, heads)}));
   while (rows > 1 && cdiv(n, rows) < 1024) rows /= 2;
   return (int)rows;
 }
@@ -295,7 +344,7 @@ static int with_lanes(int lanes, F f) {
   return f(std::integral_constant<int, 64>());
 }
 
-static int fill_norm(NormRot &a, int64_t n, int hq, int hk, int dim, int turn, int interleaved,
+static int fill_norm(NormRot &a, int ve, int64_t n, int hq, int hk, int dim, int turn, int interleaved,
                      const int64_t *strides, const double *freqs, int pos_kind, const void *pos, const int32_t *ids,
                      const int32_t *starts, const void *wq, const void *wk, int w_f32, float eps) {
   KL_REQUIRE(n >= 0 && n < ((int64_t)1 << 31) - 256 && hq >= 0 && hk >= 0 && hq + hk <= 1 << 16,
@@ -311,7 +360,8 @@ static int fill_norm(NormRot &a, int64_t n, int hq, int hk, int dim, int turn, i
   a.hk = hk;
   a.dim = dim;
   a.half = turn / 2;
-  a.interleaved = interleaved ? 1 : 0;
+  const int h = turn / 2 / ve;  // lanes between partners
+  a.partner = interleaved ? OWN : turn / 2 % ve ? ANYWHERE : h == 8 ? AWAY_8 : h == 4 ? AWAY_4 : AWAY;
   a.eps = eps;
   a.freqs = freqs;
   a.pos_kind = pos_kind;
@@ -338,7 +388,7 @@ extern "C" int kl_norm_rotary_forward(kl_dtype dtype, int64_t num_rows, int q_he
                                       int pos_kind, const void *positions, const int32_t *ids, const int32_t *starts,
                                       float eps, void *out_q, void *out_k, kl_stream stream) {
   NormRot a;
-  KL_CHECK_RC(fill_norm(a, num_rows, q_heads, k_heads, dim, turn, interleaved, strides_host, freqs, pos_kind, positions,
+  KL_CHECK_RC(fill_norm(a, dtype == KL_F32 ? 4 : 8, num_rows, q_heads, k_heads, dim, turn, interleaved, strides_host, freqs, pos_kind, positions,
                         ids, starts, q_weight, k_weight, weight_f32, eps));
   if (num_rows == 0 || q_heads + k_heads == 0) return KL_OK;
   return with_type(dtype, "norm_rotary", [&](auto t) -> int {
@@ -364,7 +414,7 @@ extern "C" int kl_norm_rotary_backward(kl_dtype dtype, int64_t num_rows, int q_h
                                        void *grad_q, void *grad_k, void *grad_q_weight, void *grad_k_weight, void *ws,
                                        size_t ws_bytes, kl_stream stream) {
   NormRot a;
-  KL_CHECK_RC(fill_norm(a, num_rows, q_heads, k_heads, dim, turn, interleaved, strides_host, freqs, pos_kind, positions,
+  KL_CHECK_RC(fill_norm(a, dtype == KL_F32 ? 4 : 8, num_rows, q_heads, k_heads, dim, turn, interleaved, strides_host, freqs, pos_kind, positions,
                         ids, starts, q_weight, k_weight, weight_f32, eps));
   const bool weights = grad_q_weight || grad_k_weight;
   KL_REQUIRE(!weights || ws_bytes >= kl_norm_rotary_bwd_workspace_bytes(dim),

@@ -13,7 +13,9 @@
 // Bound by memory: a and b are read 1 + (share of 1) times and h is written once.  Step 3 takes the chunks in the
 // other order, so that it finds what 1 read last in the 256 MB cache.  One pass, with workgroups that publish and
 // await each other's (A, B), measured no faster: it reads less, but waits.
-// recur_rays_train's shapes (311,000 x 64, float, packs of 38): TBD
+// 311,000 rows of 64 columns, float, packs of 38 rows: forward 25 + 7 + 40 us (239 MB at least, 47 us at the rate of
+// a copy), backward 24 + 7 + 67 us (398 MB, 79 us); 131,074 x 1024, bf16, two packs: 69 + 11 + 71 and
+// 58 + 11 + 121 us (805 MB, 160 us, and 1342 MB, 267 us, with none of it found in the cache).
 //
 // States, A and B are in 32 bits (64 for double); outputs are rounded once.
 // Backward: g[t] = dh[t] + a[t+1] g[t+1] is the same recurrence in the other direction with the gate of the
