@@ -52,13 +52,20 @@ struct Stage {
   static_assert(ROWS * CH % 256 == 0, "whole pieces per thread");
   u32x4 w[PER];
 
-  // rows at or past `end` and columns at or past `dim` become zeros
+  // Columns at or past `dim` become zeros, rows at or past `end` zeros or, where rows overlap, some row's finite or
+  // other elements: nobody sees them.  The buffer ends with row end - 1, so no lane has to ask; base, row0 and end
+  // are the same for the whole workgroup.
   __device__ __forceinline__ void load(const T *__restrict__ base, int64_t stride, int row0, int end, int dim) {
+    static_assert(ROWS <= 64 && ROWS * sizeof(T) <= 128, "a tile's rows span less than 2^32 bytes (kMaxStride)");
+    constexpr uint32_t kNowhere = 0xfffffff0u;
+    const uint64_t bytes = ((uint64_t)(end - 1 - row0) * (uint64_t)stride + (uint64_t)dim) * sizeof(T);
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+        (void *)(base + row0 * stride), (short)0, (int)(uint32_t)min(bytes, (uint64_t)kNowhere), 0x00020000);
+    const uint32_t row = (uint32_t)stride * (uint32_t)sizeof(T), col = threadIdx.x % CH * E;
 #pragma unroll
     for (int i = 0; i < PER; i++) {
-      const int at = threadIdx.x + 256 * i, row = row0 + at / CH, col = at % CH * E;
-      w[i] = u32x4{0, 0, 0, 0};
-      if (row < end && col < dim) w[i] = *reinterpret_cast<const u32x4 *>(base + row * stride + col);
+      const uint32_t at = (threadIdx.x / CH + 256 / CH * i) * row + col * (uint32_t)sizeof(T);
+      w[i] = __builtin_amdgcn_raw_buffer_load_b128(rs, (int)((int)col < dim ? at : kNowhere), 0, 0);
     }
   }
   __device__ __forceinline__ void store(T *tile) const {
