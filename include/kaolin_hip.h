@@ -538,6 +538,10 @@ int kl_sum_reduce(kl_dtype dtype, int64_t num_feats, int64_t feat_dim, const voi
 size_t kl_pack_layout_workspace_bytes(int64_t num_rows);
 int kl_pack_layout(int64_t num_rows, const uint8_t *boundaries, int32_t *ids, int32_t *starts, void *workspace,
                    size_t workspace_bytes, kl_stream stream);
+/* The same for two masks at once; the workspace has the bytes of both. */
+int kl_pack_layout_pair(int64_t num_rows, const uint8_t *boundaries, int32_t *ids, int32_t *starts, int64_t num_rows2,
+                        const uint8_t *boundaries2, int32_t *ids2, int32_t *starts2, void *workspace,
+                        size_t workspace_bytes, kl_stream stream);
 
 /* out[i] = sum_j softmax_j(scale * q[i] . k[j]) v[j] over the keys j of the pack of keys that has the number
  * of i's pack of queries; causal: the last query of a pack sees all its keys, each one before it one key

@@ -211,60 +211,80 @@ __global__ void __launch_bounds__((64 * kWaves<T, DP>), (kDirect<T, DP> ? 3 : si
 }
 
 // The splits of one (key head, virtual row) joined: `lanes` threads of eight elements (a power of two), and
-// `shares` of them that take every shares-th split, for each of 256 / (lanes * shares) rows.
+// `shares` of them that take every shares-th split, for each of 256 / (lanes * shares) rows.  Every share has sums of
+// its own maximum; they are joined two by two, in an order that the sizes alone give.
 constexpr int kMaxSplits = 128;
 template <typename T>
 __global__ void __launch_bounds__(256) attend_join_kernel(Attend a, int splits, int lanes, int shares,
                                                         const float *__restrict__ part, const float2 *__restrict__ stat,
                                                         T *__restrict__ o, T *__restrict__ low,
                                                         float *__restrict__ lse) {
-  __shared__ float s_w[256 + kMaxSplits];  // weights of this workgroup's rows: rows * splits <= 256 or one row
-  __shared__ float s_sum[256 * 8];
+  constexpr int kEach = kMaxSplits * 16 / 256;  // splits of a share at most: 16 lanes, 16 shares
+  __shared__ float2 s_stat[64];
+  __shared__ float s_sum[64 * 8];
   const int64_t total = (int64_t)a.nq * a.group, rows = total * a.kv_heads;
   const int per = lanes * shares, here = 256 / per;
   const int mine = threadIdx.x / per, lane = threadIdx.x % lanes, share = threadIdx.x / lanes % shares;
   const int64_t at = (int64_t)blockIdx.x * here + mine;
   const int d = lane * 8;
   const bool live = at < rows;
+  float2 x[kEach];
   float top = -INFINITY, l = 0;
-  if (live) {
-    for (int s = threadIdx.x % per; s < splits; s += per) s_w[mine * splits + s] = stat[s * rows + at].x;
-  }
-  __syncthreads();
-  if (live) {
-    for (int s = 0; s < splits; s++) top = fmaxf(top, s_w[mine * splits + s]);
-  }
-  const float base = top == -INFINITY ? 0.f : top;
-  f32x8 sum = {};
-  if (live) {
-    for (int s = share; s < splits; s += shares) {
-      const float2 x = stat[s * rows + at];
-      if (x.x == -INFINITY && x.y == 0) continue;  // no key of the row in this split
-      const float w = exp2_fast(x.x - base);
-      l = fmaf(w, x.y, l);
-      if (d < a.dim) {
-        const f32x4 *p = reinterpret_cast<const f32x4 *>(part + (s * rows + at) * a.dim + d);
-        const f32x4 u0 = p[0], u1 = p[1];
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          sum[e] = fmaf(w, u0[e], sum[e]);
-          sum[4 + e] = fmaf(w, u1[e], sum[4 + e]);
-        }
+  for (int i = 0; i < kEach; i++) {
+    const int s = share + i * shares;
+    x[i] = live && s < splits ? stat[s * rows + at] : make_float2(-INFINITY, 0);
+    top = fmaxf(top, x[i].x);
+  }
+  f32x8 sum = {};
+#pragma unroll
+  for (int i = 0; i < kEach; i++) {
+    if (x[i].x == -INFINITY && x[i].y == 0) continue;  // no key of the row in this split
+    const float w = exp2_fast(x[i].x - (top == -INFINITY ? 0.f : top));
+    l = fmaf(w, x[i].y, l);
+    if (d < a.dim) {
+      const f32x4 *p = reinterpret_cast<const f32x4 *>(part + ((share + i * shares) * rows + at) * a.dim + d);
+      const f32x4 u0 = p[0], u1 = p[1];
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        sum[e] = fmaf(w, u0[e], sum[e]);
+        sum[4 + e] = fmaf(w, u1[e], sum[4 + e]);
       }
     }
   }
-  // the shares' sums, in their order
-  __syncthreads();
-  s_w[threadIdx.x] = l;
+  auto join = [&](float m, float n, const f32x8 &u) {
+    const float both = fmaxf(top, m), base = both == -INFINITY ? 0.f : both;
+    const float w = exp2_fast(top - base), v = exp2_fast(m - base);
+    top = both;
+    l = fmaf(l, w, n * v);
 #pragma unroll
-  for (int e = 0; e < 8; e++) s_sum[e * 256 + threadIdx.x] = sum[e];
-  __syncthreads();
-  if (!live || share > 0) return;
-  for (int s = 1; s < shares; s++) {
-    l += s_w[threadIdx.x + s * lanes];
+    for (int e = 0; e < 8; e++) sum[e] = fmaf(sum[e], w, u[e] * v);
+  };
+  for (int off = lanes; off < 64 && off < per; off *= 2) {
+    f32x8 u;
 #pragma unroll
-    for (int e = 0; e < 8; e++) sum[e] += s_sum[e * 256 + threadIdx.x + s * lanes];
+    for (int e = 0; e < 8; e++) u[e] = __shfl_xor(sum[e], off);
+    const float m = __shfl_xor(top, off), n = __shfl_xor(l, off);
+    join(m, n, u);
   }
+  if (per > 64) {  // then the waves'
+    const int wave = threadIdx.x >> 6, in = threadIdx.x & 63;
+    if (in < lanes) {
+      s_stat[wave * lanes + in] = make_float2(top, l);
+#pragma unroll
+      for (int e = 0; e < 8; e++) s_sum[(wave * lanes + in) * 8 + e] = sum[e];
+    }
+    __syncthreads();
+    if (share > 0) return;
+    for (int w = 1; w < per / 64; w++) {
+      const int from = (wave + w) * lanes + in;
+      f32x8 u;
+#pragma unroll
+      for (int e = 0; e < 8; e++) u[e] = s_sum[from * 8 + e];
+      join(s_stat[from].x, s_stat[from].y, u);
+    }
+  }
+  if (!live || share > 0) return;
   if (d >= a.dim) return;
   const int head = (int)(at / total);
   const int64_t m = at % total;

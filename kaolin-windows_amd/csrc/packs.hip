@@ -3,7 +3,8 @@
 //
 // A workgroup counts the marks of the rows before its own and of all rows, then writes its part.  Up to
 // kOneLaunchRows rows every workgroup counts the whole mask itself (one byte a row, from L2), in one
-// launch; past that a first launch leaves one count per workgroup.
+// launch; past that a first launch leaves one count per workgroup.  Two masks share their launches: each takes
+// some 4 us, whatever a small mask's few workgroups have to do.
 #include "seqcommon.h"
 
 namespace kl {
@@ -40,25 +41,39 @@ __device__ __forceinline__ int count_marks(const uint8_t *__restrict__ b, int64_
   return n;
 }
 
-__global__ void __launch_bounds__(256) pack_count_kernel(const uint8_t *__restrict__ b, int64_t n,
-                                                         int32_t *__restrict__ counts) {
+struct Mask {
+  const uint8_t *b;
+  int64_t n;
+  int blocks;               // 0: no mask
+  int32_t *counts;          // NULL: every workgroup counts
+  int32_t *ids, *starts;
+};
+
+__global__ void __launch_bounds__(256) pack_count_kernel(Mask one, Mask two) {
   __shared__ int s_wave[4];
-  const int64_t begin = (int64_t)blockIdx.x * kLayoutRows;
-  const int c = block_sum(count_marks(b, begin, min(n, begin + kLayoutRows)), s_wave);
-  if (threadIdx.x == 0) counts[blockIdx.x] = c;
+  const bool is_two = (int)blockIdx.x >= one.blocks;
+  const Mask m = is_two ? two : one;
+  const int block = (int)blockIdx.x - (is_two ? one.blocks : 0);
+  if (!m.counts) return;
+  const int64_t begin = (int64_t)block * kLayoutRows;
+  const int c = block_sum(count_marks(m.b, begin, min(m.n, begin + kLayoutRows)), s_wave);
+  if (threadIdx.x == 0) m.counts[block] = c;
 }
 
-__global__ void __launch_bounds__(256) pack_layout_kernel(const uint8_t *__restrict__ b, int64_t n,
-                                                          const int32_t *__restrict__ counts, int32_t *__restrict__ ids,
-                                                          int32_t *__restrict__ starts) {
+__global__ void __launch_bounds__(256) pack_layout_kernel(Mask one, Mask two) {
   __shared__ int s_wave[4];
-  const int64_t first = (int64_t)blockIdx.x * kLayoutRows;
+  const bool is_two = (int)blockIdx.x >= one.blocks;
+  const Mask m = is_two ? two : one;
+  const int block = (int)blockIdx.x - (is_two ? one.blocks : 0);
+  const uint8_t *b = m.b;
+  int32_t *ids = m.ids, *starts = m.starts;
+  const int64_t n = m.n, first = (int64_t)block * kLayoutRows;
   int before = 0, all = 0;
-  if (counts) {
-    for (int i = threadIdx.x; i < (int)gridDim.x; i += 256) {
-      const int c = counts[i];
+  if (m.counts) {
+    for (int i = threadIdx.x; i < m.blocks; i += 256) {
+      const int c = m.counts[i];
       all += c;
-      before += i < (int)blockIdx.x ? c : 0;
+      before += i < block ? c : 0;
     }
   } else {
     before = count_marks(b, 0, first);
@@ -83,7 +98,24 @@ __global__ void __launch_bounds__(256) pack_layout_kernel(const uint8_t *__restr
     if (mark[k]) starts[id] = (int32_t)(row + k);
     if (row + k >= all) starts[row + k] = (int32_t)n;  // past the last pack
   }
-  if (blockIdx.x == 0 && threadIdx.x == 0) starts[n] = (int32_t)n;
+  if (block == 0 && threadIdx.x == 0) starts[n] = (int32_t)n;
+}
+
+static int take_mask(Mask &m, const char *func, int64_t n, const uint8_t *b, int32_t *ids, int32_t *starts, char *ws) {
+  KL_REQUIRE(n >= 0 && n < (int64_t)1 << 31, std::string(func) + ": the number of rows is out of range");
+  m = {b, n, (int)std::max<int64_t>(1, cdiv(n, kLayoutRows)), n > kOneLaunchRows ? (int32_t *)ws : nullptr, ids, starts};
+  return KL_OK;
+}
+
+static int write_layouts(const Mask &one, const Mask &two, hipStream_t st) {
+  const dim3 blocks((unsigned)(one.blocks + two.blocks));
+  if (one.counts || two.counts) {
+    hipLaunchKernelGGL(pack_count_kernel, blocks, dim3(256), 0, st, one, two);
+    KL_CHECK_LAUNCH();
+  }
+  hipLaunchKernelGGL(pack_layout_kernel, blocks, dim3(256), 0, st, one, two);
+  KL_CHECK_LAUNCH();
+  return KL_OK;
 }
 
 }  // namespace kl
@@ -96,17 +128,20 @@ extern "C" size_t kl_pack_layout_workspace_bytes(int64_t num_rows) {
 
 extern "C" int kl_pack_layout(int64_t num_rows, const uint8_t *boundaries, int32_t *ids, int32_t *starts, void *ws,
                               size_t ws_bytes, kl_stream stream) {
-  KL_REQUIRE(num_rows >= 0 && num_rows < (int64_t)1 << 31, "pack_layout: the number of rows is out of range");
+  Mask one, none = {};
+  KL_CHECK_RC(take_mask(one, "pack_layout", num_rows, boundaries, ids, starts, (char *)ws));
   KL_REQUIRE(ws_bytes >= kl_pack_layout_workspace_bytes(num_rows), "pack_layout: the workspace is too small");
-  const unsigned blocks = (unsigned)std::max<int64_t>(1, cdiv(num_rows, kLayoutRows));
-  int32_t *counts = nullptr;
-  if (num_rows > kOneLaunchRows) {
-    counts = (int32_t *)ws;
-    hipLaunchKernelGGL(pack_count_kernel, dim3(blocks), dim3(256), 0, S(stream), boundaries, num_rows, counts);
-    KL_CHECK_LAUNCH();
-  }
-  hipLaunchKernelGGL(pack_layout_kernel, dim3(blocks), dim3(256), 0, S(stream), boundaries, num_rows, counts, ids,
-                     starts);
-  KL_CHECK_LAUNCH();
-  return KL_OK;
+  return write_layouts(one, none, S(stream));
+}
+
+extern "C" int kl_pack_layout_pair(int64_t num_rows, const uint8_t *boundaries, int32_t *ids, int32_t *starts,
+                                   int64_t num_rows2, const uint8_t *boundaries2, int32_t *ids2, int32_t *starts2,
+                                   void *ws, size_t ws_bytes, kl_stream stream) {
+  Mask one, two;
+  const size_t bytes = num_rows < 0 ? 0 : kl_pack_layout_workspace_bytes(num_rows);
+  KL_CHECK_RC(take_mask(one, "pack_layout_pair", num_rows, boundaries, ids, starts, (char *)ws));
+  KL_CHECK_RC(take_mask(two, "pack_layout_pair", num_rows2, boundaries2, ids2, starts2, (char *)ws + bytes));
+  KL_REQUIRE(ws_bytes >= bytes + kl_pack_layout_workspace_bytes(num_rows2),
+             "pack_layout_pair: the workspace is too small");
+  return write_layouts(one, two, S(stream));
 }

@@ -513,6 +513,19 @@ Layout make_layout(const at::Tensor &boundaries, int64_t stream) {
   return l;
 }
 
+// of two masks at once
+std::pair<Layout, Layout> make_layouts(const at::Tensor &one, const at::Tensor &two, int64_t stream) {
+  const int64_t n = one.size(0), m = two.size(0);
+  const auto ints = one.options().dtype(at::kInt);
+  const Layout a{at::empty({2 * n + 1}, ints)}, b{at::empty({2 * m + 1}, ints)};
+  const size_t bytes = kl_pack_layout_workspace_bytes(n) + kl_pack_layout_workspace_bytes(m);
+  at::Tensor ws = workspace(bytes, one.device(), stream);
+  check(kl_pack_layout_pair(n, (const uint8_t *)one.data_ptr(), a.ids(), a.starts(), m, (const uint8_t *)two.data_ptr(),
+                            b.ids(), b.starts(), ws.data_ptr(), bytes, (kl_stream)stream),
+        "pack_layout_pair");
+  return {a, b};
+}
+
 struct HeadStrides {
   int64_t v[6];
   HeadStrides(const at::Tensor &q, const at::Tensor &k, const at::Tensor &w)
@@ -594,7 +607,12 @@ c10::optional<at::Tensor> pack_attention(at::Tensor q, at::Tensor k, at::Tensor 
       !std::isfinite(scale) || !plain_mask(boundaries, k.size(0), dev) || !plain_mask(qb, q.size(0), dev))
     return c10::nullopt;
   const c10::DeviceGuard guard(dev);
-  const Layout lk = make_layout(boundaries, stream), lq = q_boundaries ? make_layout(qb, stream) : lk;
+  Layout lk, lq;
+  if (q_boundaries) {
+    std::tie(lk, lq) = make_layouts(boundaries, qb, stream);
+  } else {
+    lk = lq = make_layout(boundaries, stream);
+  }
   if (any_grad({&q, &k, &v})) return PackAttention::apply(q, k, v, lq.held, lk.held, scale, causal, stream)[0];
   return std::get<0>(attention_forward(q, k, v, lq, lk, scale, causal, false, stream));
 }

@@ -113,6 +113,7 @@ _SIGS = {
     'kl_sum_reduce': (_I, [_I, _I64, _I64, _P, _P, _I64, _P, _P]),
     'kl_pack_layout_workspace_bytes': (_SZ, [_I64]),
     'kl_pack_layout': (_I, [_I64, _P, _P, _P, _P, _SZ, _P]),
+    'kl_pack_layout_pair': (_I, [_I64, _P, _P, _P, _I64, _P, _P, _P, _P, _SZ, _P]),
     'kl_pack_attention_workspace_bytes': (_SZ, [_I, _I64, _I64, _I, _I, _I]),
     'kl_pack_attention_forward': (_I, [_I, _I64, _I64, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _F, _I, _P, _P, _P,
                                        _P, _SZ, _P]),

@@ -148,6 +148,14 @@ def test_library_refusals_without_gpu():
     assert lib.kl_pack_layout(1 << 31, None, None, None, None, 1 << 30, None) == -1
     assert lib.kl_pack_layout(70000, None, None, None, None, 0, None) == -1
     assert b'workspace' in lib.kl_last_error()
+    for n, m, ws in ((1 << 31, 1, 1 << 30), (1, -1, 1 << 30), (-1, 1, 1 << 30), (1, 1, 256), (70000, 70000, 300)):
+        assert lib.kl_pack_layout_pair(n, None, None, None, m, None, None, None, None, ws, None) == -1, (n, m)
+    for i in range(6):  # a tile's rows have to lie within 2^32 bytes, and forward
+        st[i] = -8
+        assert attend()[0] == -1 and b'negative stride' in lib.kl_last_error()
+        st[i] = 1 << 25
+        assert i % 2 or attend()[0] == -1 and b'too far apart' in lib.kl_last_error()
+        st[i] = 0
 
     def norm(dim=8, turn=8, eps=1e-6, kind=3, n=1):
         return lib.kl_norm_rotary_forward(0, n, 1, 1, dim, turn, 0, None, None, st, None, None, 0, None, kind, None, None,
@@ -231,6 +239,24 @@ def test_pack_layout(n, kind):
     want = torch.full((n + 1,), n, dtype=torch.int32)
     want[:len(rows)] = rows
     assert torch.equal(starts.cpu(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('n, m', [(1, 1), (0, 5), (1025, 3), (70001, 40), (40, 70001), (65537, 66000), (513, 0)])
+def test_pack_layout_pair(n, m):
+    import kaolin
+    from kaolin import _native as N
+    gen = torch.Generator().manual_seed(n + m)
+    masks = [(torch.rand(k, generator=gen) < 0.1).to(DEV) for k in (n, m)]
+    out = [(torch.full((k,), -7, dtype=torch.int32, device=DEV), torch.full((k + 1,), -7, dtype=torch.int32, device=DEV))
+           for k in (n, m)]
+    size = sum(N.size('kl_pack_layout_workspace_bytes', k) for k in (n, m))
+    ws = N.workspace(size, masks[0].device)
+    args = [x for k, mask, o in zip((n, m), masks, out) for x in (k, N.ptr(mask), N.ptr(o[0]), N.ptr(o[1]))]
+    N.check(N.lib().kl_pack_layout_pair(*args, N.ptr(ws), size, N.stream_of(masks[0].device)), 'pack_layout_pair')
+    for mask, o in zip(masks, out):
+        want = kaolin._C.render.spc.pack_layout_cuda(mask)
+        assert torch.equal(o[0], want[0]) and torch.equal(o[1], want[1])
 
 
 # ------------------------------------------------------------------------------- attention
