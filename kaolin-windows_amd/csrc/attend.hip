@@ -213,7 +213,7 @@ __global__ void __launch_bounds__((64 * kWaves<T, DP>), (kDirect<T, DP> ? 3 : si
 // The splits of one (key head, virtual row) joined: `lanes` threads of eight elements (a power of two), and
 // `shares` of them that take every shares-th split, for each of 256 / (lanes * shares) rows.  Every share has sums of
 // its own maximum; they are joined two by two, in an order that the sizes alone give.
-constexpr int kMaxSplits = 128;
+constexpr int kMaxSplits = 256;
 template <typename T>
 __global__ void __launch_bounds__(256) attend_join_kernel(Attend a, int splits, int lanes, int shares,
                                                         const float *__restrict__ part, const float2 *__restrict__ stat,
@@ -233,13 +233,13 @@ __global__ void __launch_bounds__(256) attend_join_kernel(Attend a, int splits, 
 #pragma unroll
   for (int i = 0; i < kEach; i++) {
     const int s = share + i * shares;
-    x[i] = live && s < splits ? stat[s * rows + at] : make_float2(-INFINITY, 0);
+    x[i] = i * shares < splits && live && s < splits ? stat[s * rows + at] : make_float2(-INFINITY, 0);
     top = fmaxf(top, x[i].x);
   }
   f32x8 sum = {};
 #pragma unroll
   for (int i = 0; i < kEach; i++) {
-    if (x[i].x == -INFINITY && x[i].y == 0) continue;  // no key of the row in this split
+    if (i * shares >= splits || (x[i].x == -INFINITY && x[i].y == 0)) continue;  // no key of the row in this split
     const float w = exp2_fast(x[i].x - (top == -INFINITY ? 0.f : top));
     l = fmaf(w, x[i].y, l);
     if (d < a.dim) {
