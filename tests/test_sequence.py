@@ -630,6 +630,33 @@ def test_recurrence_packs_do_not_touch(spc, reverse):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES + [torch.float64])
+@pytest.mark.parametrize('lens,lead', [([2], 0), ([63, 1], 0), ([64, 1], 0), ([1, 64], 5), ([100, 156], 0), ([256], 0),
+                                       ([250], 6), ([257], 0), ([1] * 200 + [56], 0), ([3, 190, 60], 3)])
+@pytest.mark.parametrize('reverse', [False, True])
+def test_recurrence_few_rows(spc, dtype, lens, lead, reverse):
+    """Rows that fit one workgroup, with an infinity and a NaN in the packs next to the one that is compared."""
+    b = marks(lens, lead)
+    n, dim = len(b), 16
+    a, x, g = (_normal(i, n, dim, scale=s, dtype=dtype) for i, s in enumerate((0.5, 1.0, 1.0)))
+    h0 = _normal(3, len(lens), dim, dtype=dtype)
+    outs, tols = recurrence(a, x, b, h0, reverse, grad=g, dtype=dtype)
+    which = lens.index(max(lens))
+    begin = lead + sum(lens[:which])
+    others = torch.ones(n, dtype=torch.bool)
+    others[begin:begin + lens[which]] = False
+    a, x = a.clone(), x.clone()
+    a[others & (torch.arange(n) % 2 == 0)] = math.nan
+    x[others] = math.inf
+    leaves = [_leaf(y) for y in (a, x, h0)]
+    h = spc.linear_recurrence(leaves[0], leaves[1], b.to(DEV), initial=leaves[2], reverse=reverse)
+    got = [h, *torch.autograd.grad(h, leaves, g.to(DEV))]
+    for name, y, want, tol in zip(('h', 'da', 'db', 'dinitial'), got, outs, tols):
+        rows = slice(which, which + 1) if name == 'dinitial' else ~others
+        check(name, y.cpu()[rows], want[rows], tol[rows])
+
+
+@pytest.mark.gpu
 def test_recurrence_is_cumsum_with_gates_of_one(spc):
     b = marks([30, 1, 300], lead=2).to(DEV)
     x = torch.randint(-8, 8, (333, 7), generator=torch.Generator().manual_seed(0)).float().to(DEV)
