@@ -135,9 +135,9 @@ template <typename T, int DP, bool CAREFUL>
 __device__ __forceinline__ bool fwd_rows(const Attend &a, const FwdArgs &p, FwdLds<T, DP> &lds) {
   constexpr int BM = FwdTile<T, DP>::BM, BN = FwdTile<T, DP>::BN;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
-  const int head = (int)blockIdx.x % a.kv_heads;
-  const int total = a.nq * a.group, tiles = (int)gridDim.x / a.kv_heads;  // virtual rows: under 2^31
-  const int m = (tiles - 1 - (int)blockIdx.x / a.kv_heads) * BM + wave * 32 + col;  // the last rows see most keys
+  const Place at_place = place(a, p.part != nullptr);
+  const int head = at_place.head, total = a.nq * a.group;  // virtual rows: under 2^31
+  const int m = (at_place.tiles - 1 - at_place.tile) * BM + wave * 32 + col;  // the last rows see most keys
   const bool live = m < total;
   const Row at_row = virtual_row(a, live ? m : 0);
   const int row = at_row.row, qhead = head * a.group + at_row.sub;
@@ -202,7 +202,7 @@ __device__ __forceinline__ bool fwd_rows(const Attend &a, const FwdArgs &p, FwdL
   return false;
 }
 
-// grid: (tiles * kv_heads, splits)
+// grid: places(tiles, splits)
 template <typename T, int DP>
 __global__ void __launch_bounds__((64 * kWaves<T, DP>), (kDirect<T, DP> ? 3 : sizeof(T) == 4 && DP == 128 ? 1 : 2))
     attend_fwd_kernel(Attend a, FwdArgs p) {
@@ -352,10 +352,10 @@ static int attend_forward(const Attend &a, const void *q, const void *k, const v
                           void *ws, hipStream_t st) {
   const int splits = attend_splits(sizeof(T) == 4 ? KL_F32 : KL_F16, a.nq, a.nk, a.kv_heads, a.group, a.dim);
   const int64_t total = (int64_t)a.nq * a.group, rows = total * a.kv_heads;
-  const unsigned blocks = (unsigned)(cdiv(total, FwdTile<T, DP>::BM) * a.kv_heads);
+  const int64_t tiles = cdiv(total, FwdTile<T, DP>::BM);
   float2 *stat = splits > 1 ? (float2 *)ws : nullptr;
   float *part = splits > 1 ? (float *)((char *)ws + al256((size_t)splits * rows * 8)) : nullptr;
-  hipLaunchKernelGGL((attend_fwd_kernel<T, DP>), dim3(blocks, splits), dim3(64 * kWaves<T, DP>), 0, st, a,
+  hipLaunchKernelGGL((attend_fwd_kernel<T, DP>), places(a, tiles, splits), dim3(64 * kWaves<T, DP>), 0, st, a,
                      FwdArgs{q, k, v, o, low, lse, part, stat});
   KL_CHECK_LAUNCH();
   if (splits > 1) {

@@ -364,8 +364,9 @@ template <typename T, int DP, bool CAREFUL>
 __device__ __forceinline__ bool dkv_keys(const Attend &a, const Grad &g, const GradArgs &p, DkvLds<T, DP> &lds) {
   constexpr int BQ = DkvTile<T, DP>::BQ, KEYS = DkvTile<T, DP>::KEYS;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
-  const int head = (int)blockIdx.x % a.kv_heads, heads = a.kv_heads * a.group;
-  const int j0 = (int)blockIdx.x / a.kv_heads * KEYS, key0 = j0 + wave * 32, key = key0 + col;
+  const Place at_place = place(a, p.part != nullptr);
+  const int head = at_place.head, heads = a.kv_heads * a.group;
+  const int j0 = at_place.tile * KEYS, key0 = j0 + wave * 32, key = key0 + col;
   const bool live = key < a.nk;
   Range rows = row_range(a, j0, min(j0 + KEYS, a.nk));
   rows = {uniform(rows.lo), uniform(rows.hi)};
@@ -421,9 +422,9 @@ __device__ __forceinline__ bool dkv_keys(const Attend &a, const Grad &g, const G
   return false;
 }
 
-// grid: (tiles of keys * kv_heads, splits of the rows)
+// grid: places(tiles of keys, splits of the rows)
 template <typename T, int DP>
-__global__ void __launch_bounds__((64 * kWaves<T, DP>), (DP == 128 ? 1 : 2))
+__global__ void __launch_bounds__((64 * kWaves<T, DP>), (DP == 128 ? 1 : kDirect<T, DP> ? 3 : 2))
     attend_dkv_kernel(Attend a, Grad g, GradArgs p) {
   __shared__ DkvLds<T, DP> lds;
   if (dkv_keys<T, DP, false>(a, g, p, lds)) dkv_keys<T, DP, true>(a, g, p, lds);
@@ -488,9 +489,8 @@ static int attend_backward(const Attend &a, const Grad &g, const void *q, const 
   }
   if (a.nk > 0 && dk) {
     constexpr int KEYS = DkvTile<T, DP>::KEYS, step = DkvTile<T, DP>::BQ;
-    const unsigned blocks = (unsigned)(cdiv(a.nk, KEYS) * a.kv_heads);
     const int splits = dkv_splits(sizeof(T) == 4 ? KL_F32 : KL_F16, a.nq, a.nk, a.kv_heads, a.group, a.dim);
-    hipLaunchKernelGGL((attend_dkv_kernel<T, DP>), dim3(blocks, splits), dim3(64 * kWaves<T, DP>), 0, st, a, g,
+    hipLaunchKernelGGL((attend_dkv_kernel<T, DP>), places(a, cdiv(a.nk, KEYS), splits), dim3(64 * kWaves<T, DP>), 0, st, a, g,
                        GradArgs{q, k, v, go, nullptr, dk, dv, splits > 1 ? part : nullptr});
     KL_CHECK_LAUNCH();
     if (splits > 1) {
