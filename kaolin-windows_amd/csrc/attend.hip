@@ -302,14 +302,14 @@ __global__ void __launch_bounds__(256) attend_join_kernel(Attend a, int splits, 
   if (lse && d == 0) lse[out] = l == 0 ? 0.f : top + log2_fast(l);
 }
 
-// Splits of the keys: enough waves for the chip's 1024 SIMDs where the rows alone give few, and at least two
-// tiles of keys for each of them if one pack held all keys.
+// Splits of the keys: two waves for each of the chip's 1024 SIMDs and no more, which is what runs at once (one more
+// workgroup waits for a whole round: attend_step with 43 splits 209 us, with 42 or 21 178), and at least two tiles of
+// keys for each of them if one pack held all keys.
 static int attend_splits(kl_dtype dtype, int64_t nq, int64_t nk, int kv_heads, int group, int dim) {
   const int waves = is_direct(dtype, dim) ? 1 : 4, step = dtype == KL_F32 ? 32 : 64;
   const int64_t all = cdiv(nq * group, 32 * waves) * kv_heads * waves;
-  if (all >= 2048) return 1;
   return (int)std::max<int64_t>(
-      1, std::min<int64_t>({cdiv(4096, std::max<int64_t>(all, 1)), cdiv(nk, 2 * step), kMaxSplits}));
+      1, std::min<int64_t>({2048 / std::max<int64_t>(all, 1), cdiv(nk, 2 * step), kMaxSplits}));
 }
 
 int fill_attend(Attend &a, const char *func, int64_t nq, int64_t nk, int heads, int kv_heads, int dim,
