@@ -213,13 +213,12 @@ __global__ void __launch_bounds__((64 * kWaves<T, DP>), (kDirect<T, DP> ? 3 : si
 // The splits of one (key head, virtual row) joined: `lanes` threads of eight elements (a power of two), and
 // `shares` of them that take every shares-th split, for each of 256 / (lanes * shares) rows.  Every share has sums of
 // its own maximum; they are joined two by two, in an order that the sizes alone give.
-constexpr int kMaxSplits = 256;
+constexpr int kMaxSplits = 256, kJoinEach = kMaxSplits * 16 / 256;  // splits of a share: 16 lanes, 16 shares
 template <typename T>
 __global__ void __launch_bounds__(256) attend_join_kernel(Attend a, int splits, int lanes, int shares,
                                                         const float *__restrict__ part, const float2 *__restrict__ stat,
                                                         T *__restrict__ o, T *__restrict__ low,
                                                         float *__restrict__ lse) {
-  constexpr int kEach = kMaxSplits * 16 / 256;  // splits of a share at most: 16 lanes, 16 shares
   __shared__ float2 s_stat[64];
   __shared__ float s_sum[64 * 8];
   const int64_t total = (int64_t)a.nq * a.group, rows = total * a.kv_heads;
@@ -228,17 +227,17 @@ __global__ void __launch_bounds__(256) attend_join_kernel(Attend a, int splits, 
   const int64_t at = (int64_t)blockIdx.x * here + mine;
   const int d = lane * 8;
   const bool live = at < rows;
-  float2 x[kEach];
+  float2 x[kJoinEach];
   float top = -INFINITY, l = 0;
 #pragma unroll
-  for (int i = 0; i < kEach; i++) {
+  for (int i = 0; i < kJoinEach; i++) {
     const int s = share + i * shares;
     x[i] = i * shares < splits && live && s < splits ? stat[s * rows + at] : make_float2(-INFINITY, 0);
     top = fmaxf(top, x[i].x);
   }
   f32x8 sum = {};
 #pragma unroll
-  for (int i = 0; i < kEach; i++) {
+  for (int i = 0; i < kJoinEach; i++) {
     if (i * shares >= splits || (x[i].x == -INFINITY && x[i].y == 0)) continue;  // no key of the row in this split
     const float w = exp2_fast(x[i].x - (top == -INFINITY ? 0.f : top));
     l = fmaf(w, x[i].y, l);
@@ -361,7 +360,8 @@ static int attend_forward(const Attend &a, const void *q, const void *k, const v
   if (splits > 1) {
     int lanes = 1, shares = 1;
     while (lanes * 8 < a.dim) lanes *= 2;
-    while (shares < splits && lanes * shares < 256) shares *= 2;
+    // many rows: a wave each (attend_step, 3072 rows of 21 splits, 10.4 us with a workgroup each, now 5.5)
+    while (shares < splits && (lanes * shares < (rows > 1024 ? 64 : 256) || shares * kJoinEach < splits)) shares *= 2;
     hipLaunchKernelGGL(attend_join_kernel<T>, dim3((unsigned)cdiv(rows, 256 / (lanes * shares))), dim3(256), 0, st, a,
                        splits, lanes, shares, part, stat, (T *)o, (T *)low, lse);
     KL_CHECK_LAUNCH();
