@@ -186,7 +186,8 @@ __device__ __forceinline__ bool fwd_rows(const Attend &a, const FwdArgs &p, FwdL
     return false;
   }
   const int64_t at = (int64_t)row * a.kv_heads * a.group + qhead;
-  const float w = l == 0 ? 0.f : 1.f / l;  // a row that sees no key: 0
+  const bool blind = mine.lo >= mine.hi;   // a row that sees no key: 0; one whose scores are all -inf: NaN
+  const float w = blind ? 0.f : 1.f / l;
   store_cols<T, DP>((T *)p.o + at * a.dim, acc, w, h, a.dim);
   if constexpr (sizeof(T) == 2) {
     if (p.low) {
@@ -198,7 +199,7 @@ __device__ __forceinline__ bool fwd_rows(const Attend &a, const FwdArgs &p, FwdL
       store_cols<T, DP>((T *)p.low + at * a.dim, acc, 1.f, h, a.dim);
     }
   }
-  if (p.lse && h == 0) p.lse[at] = l == 0 ? 0.f : st.m + log2_fast(l);
+  if (p.lse && h == 0) p.lse[at] = blind ? 0.f : st.m + log2_fast(l);
   return false;
 }
 
@@ -288,7 +289,12 @@ __global__ void __launch_bounds__(256) attend_join_kernel(Attend a, int splits, 
   const int head = (int)(at / total);
   const int64_t m = at % total;
   const int64_t out = m / a.group * a.kv_heads * a.group + head * a.group + m % a.group;
-  const float inv = l == 0 ? 0.f : 1.f / l;
+  bool blind = false;
+  if (l == 0) {
+    const Range r = key_range(a, (int)(m / a.group));
+    blind = r.lo >= r.hi;
+  }
+  const float inv = blind ? 0.f : 1.f / l;
 #pragma unroll
   for (int e = 0; e < 8; e++) sum[e] *= inv;
   const V8<T> y = __builtin_convertvector(sum, V8<T>);
@@ -298,7 +304,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(Attend a, int splits, 
     for (int e = 0; e < 8; e++) sum[e] -= (float)y[e];
     *reinterpret_cast<V8<T> *>(low + out * a.dim + d) = __builtin_convertvector(sum, V8<T>);
   }
-  if (lse && d == 0) lse[out] = l == 0 ? 0.f : top + log2_fast(l);
+  if (lse && d == 0) lse[out] = blind ? 0.f : top + log2_fast(l);
 }
 
 // Splits of the keys: two waves for each of the chip's 1024 SIMDs and no more, which is what runs at once (one more

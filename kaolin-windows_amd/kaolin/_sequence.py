@@ -91,8 +91,10 @@ def _attention_args(func, q, k, v, q_layout, k_layout, scale):
     return usable_heads(q), usable_heads(k), usable_heads(v)
 
 
-def _strides(q, k, v):
-    return (ctypes.c_int64 * 6)(q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1))
+def _strides(*tensors):
+    """Row and head strides; a single row's stride may be anything and is not used."""
+    s = [x for t in tensors for x in (t.stride(0) if t.shape[0] > 1 else 0, t.stride(1))]
+    return (ctypes.c_int64 * len(s))(*s)
 
 
 def pack_attention_forward_cuda(q, k, v, q_layout, k_layout, scale, causal, for_backward):
@@ -207,8 +209,7 @@ def _norm_args(func, q, k, q_weight, k_weight, freqs, layout, positions, eps):
             check_all_same_gpu(func, [aq, a])
             check_contiguous(func, [a])
     q, k = usable_heads(q), usable_heads(k)
-    strides = (ctypes.c_int64 * 4)(q.stride(0), q.stride(1), k.stride(0), k.stride(1))
-    return q, k, (strides, N.ptr(q_weight), N.ptr(k_weight), int(kinds == {torch.float32}), N.ptr(freqs), kind,
+    return q, k, (_strides(q, k), N.ptr(q_weight), N.ptr(k_weight), int(kinds == {torch.float32}), N.ptr(freqs), kind,
                   N.ptr(positions), N.ptr(ids), N.ptr(starts), eps)
 
 

@@ -393,6 +393,39 @@ def test_attention_seen_infinities(spc):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('lens,heads', [([5, 300], 1), ([5, 4096], 32)])  # with the keys split and not
+def test_attention_scores_all_minus_infinity(spc, dtype, lens, heads):
+    """A row whose keys all score -inf has no softmax (0 / 0), unlike one that sees no key, which is 0; the other
+    pack's rows have theirs."""
+    b = marks(lens, lead=2)
+    n = len(b)
+    q, k, v = (torch.ones(n, heads, 8, dtype=dtype) for _ in range(3))
+    k[2:7] = -math.inf
+    leaves = [_leaf(x) for x in (q, k, v)]
+    o = spc.pack_attention(*leaves, b.to(DEV))
+    dq, _, dv = torch.autograd.grad(o, leaves, torch.ones_like(o))
+    for x in (o, dq, dv):
+        assert not x[:2].any() and torch.isnan(x[2:7]).all()
+    assert torch.equal(o[7:], torch.ones_like(o[7:])) and torch.isfinite(dq[7:]).all()
+    one = spc.pack_attention(leaves[0][6:8].detach(), leaves[1].detach(), leaves[2].detach(), b.to(DEV),
+                             q_boundaries=torch.ones(2, dtype=torch.bool, device=DEV))
+    assert torch.isnan(one[0]).all() and torch.equal(one[1], torch.ones_like(one[1]))
+
+
+@pytest.mark.gpu
+def test_single_rows_of_any_stride(spc):
+    """The stride of a dimension of size one is whatever a view made it."""
+    x = _normal(0, 16).to(DEV)
+    far, b = x.as_strided((1, 2, 8), (1 << 40, 8, 1)), torch.ones(1, dtype=torch.bool, device=DEV)
+    near, f = x.view(1, 2, 8), torch.ones(4, dtype=torch.float64, device=DEV)
+    assert torch.equal(spc.pack_attention(far, far, far, b), spc.pack_attention(near, near, near, b))
+    for y, want in zip(spc.norm_rotary(far, far, None, None, f, boundaries=b),
+                       spc.norm_rotary(near, near, None, None, f, boundaries=b)):
+        assert torch.equal(y, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
 def test_attention_strides(spc, dtype):
     """Slices of one projection, heads in another order, expanded keys, a view that has to be copied: as the
     contiguous call."""
