@@ -281,9 +281,10 @@ int with_dim(int dim, F f) {
   if (dim <= 64) return f(std::integral_constant<int, 64>());
   return f(std::integral_constant<int, 128>());
 }
-// Checks an Attend's sizes and fills it.  dim: a multiple of 8 up to 128, so rows are whole 16-byte pieces.
-int fill_attend(Attend &a, const char *func, int64_t nq, int64_t nk, int heads, int kv_heads, int dim,
-                const int64_t *strides, const int32_t *qid, const int32_t *qstart, const int32_t *kid,
+// Checks an Attend's sizes and addresses and fills it.  dim: a multiple of 8 up to 128, so rows are whole 16-byte
+// pieces.
+int fill_attend(Attend &a, const char *func, kl_dtype dtype, int64_t nq, int64_t nk, int heads, int kv_heads, int dim,
+                const void *q, const void *k, const void *v, const int64_t *strides, const int32_t *qid, const int32_t *qstart, const int32_t *kid,
                 const int32_t *kstart, float scale, int causal);
 
 }  // namespace kl

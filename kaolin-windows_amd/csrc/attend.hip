@@ -317,8 +317,8 @@ static int attend_splits(kl_dtype dtype, int64_t nq, int64_t nk, int kv_heads, i
       1, std::min<int64_t>({2048 / std::max<int64_t>(all, 1), cdiv(nk, 2 * step), kMaxSplits}));
 }
 
-int fill_attend(Attend &a, const char *func, int64_t nq, int64_t nk, int heads, int kv_heads, int dim,
-                const int64_t *strides, const int32_t *qid, const int32_t *qstart, const int32_t *kid,
+int fill_attend(Attend &a, const char *func, kl_dtype dtype, int64_t nq, int64_t nk, int heads, int kv_heads, int dim,
+                const void *q, const void *k, const void *v, const int64_t *strides, const int32_t *qid, const int32_t *qstart, const int32_t *kid,
                 const int32_t *kstart, float scale, int causal) {
   const std::string f = std::string(func) + ": ";
   KL_REQUIRE(nq >= 0 && nk >= 0 && nq < (int64_t)1 << 31 && nk < (int64_t)1 << 31, f + "rows out of range");
@@ -337,6 +337,10 @@ int fill_attend(Attend &a, const char *func, int64_t nq, int64_t nk, int heads, 
   a.q = {strides[0], strides[1]};
   a.k = {strides[2], strides[3]};
   a.v = {strides[4], strides[5]};
+  const size_t esize = dtype == KL_F32 ? 4 : 2;
+  KL_REQUIRE(whole_pieces(q, nq, heads, a.q, esize) && whole_pieces(k, nk, kv_heads, a.k, esize) &&
+                 whole_pieces(v, nk, kv_heads, a.v, esize),
+             f + "rows do not start at multiples of 16 bytes");
   a.qid = qid;
   a.qstart = qstart;
   a.kid = kid;
@@ -394,8 +398,8 @@ extern "C" int kl_pack_attention_forward(kl_dtype dtype, int64_t num_q, int64_t 
                                          const int32_t *k_starts, float scale, int causal, void *out, void *out_low,
                                          float *lse, void *ws, size_t ws_bytes, kl_stream stream) {
   Attend a;
-  KL_CHECK_RC(fill_attend(a, "pack_attention", num_q, num_k, heads, kv_heads, dim, strides_host, q_ids, q_starts, k_ids,
-                          k_starts, scale, causal));
+  KL_CHECK_RC(fill_attend(a, "pack_attention", dtype, num_q, num_k, heads, kv_heads, dim, q, k, v, strides_host, q_ids,
+                          q_starts, k_ids, k_starts, scale, causal));
   KL_REQUIRE(ws_bytes >= kl_pack_attention_workspace_bytes(dtype, num_q, num_k, heads, kv_heads, dim),
              "pack_attention: the workspace is too small");
   if (num_q == 0) return KL_OK;

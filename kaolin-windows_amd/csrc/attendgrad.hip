@@ -522,8 +522,8 @@ extern "C" int kl_pack_attention_backward(kl_dtype dtype, int64_t num_q, int64_t
                                           const void *out_low, const float *lse, float scale, int causal, void *grad_q,
                                           void *grad_k, void *grad_v, void *ws, size_t ws_bytes, kl_stream stream) {
   Attend a;
-  KL_CHECK_RC(fill_attend(a, "pack_attention", num_q, num_k, heads, kv_heads, dim, strides_host, q_ids, q_starts, k_ids,
-                          k_starts, scale, causal));
+  KL_CHECK_RC(fill_attend(a, "pack_attention", dtype, num_q, num_k, heads, kv_heads, dim, q, k, v, strides_host, q_ids,
+                          q_starts, k_ids, k_starts, scale, causal));
   KL_REQUIRE(ws_bytes >= kl_pack_attention_bwd_workspace_bytes(dtype, num_q, num_k, heads, kv_heads, dim),
              "pack_attention: the workspace is too small");
   KL_REQUIRE((grad_k == nullptr) == (grad_v == nullptr), "pack_attention: grad_k and grad_v go together");

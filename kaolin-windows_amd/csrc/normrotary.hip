@@ -345,7 +345,7 @@ static int with_lanes(int lanes, F f) {
 }
 
 static int fill_norm(NormRot &a, int ve, int64_t n, int hq, int hk, int dim, int turn, int interleaved,
-                     const int64_t *strides, const double *freqs, int pos_kind, const void *pos, const int32_t *ids,
+                     const void *q, const void *k, const int64_t *strides, const double *freqs, int pos_kind, const void *pos, const int32_t *ids,
                      const int32_t *starts, const void *wq, const void *wk, int w_f32, float eps) {
   KL_REQUIRE(n >= 0 && n < ((int64_t)1 << 31) - 256 && hq >= 0 && hk >= 0 && hq + hk <= 1 << 16,
              "norm_rotary: sizes out of range");
@@ -355,6 +355,8 @@ static int fill_norm(NormRot &a, int ve, int64_t n, int hq, int hk, int dim, int
   KL_REQUIRE(pos_kind >= POS_PACK && pos_kind <= POS_F32, "norm_rotary: unknown kind of positions");
   a.q = {strides[0], strides[1]};
   a.k = {strides[2], strides[3]};
+  KL_REQUIRE(whole_pieces(q, n, hq, a.q, 16 / ve) && whole_pieces(k, n, hk, a.k, 16 / ve),
+             "norm_rotary: rows do not start at multiples of 16 bytes");
   a.n = n;
   a.hq = hq;
   a.hk = hk;
@@ -388,8 +390,8 @@ extern "C" int kl_norm_rotary_forward(kl_dtype dtype, int64_t num_rows, int q_he
                                       int pos_kind, const void *positions, const int32_t *ids, const int32_t *starts,
                                       float eps, void *out_q, void *out_k, kl_stream stream) {
   NormRot a;
-  KL_CHECK_RC(fill_norm(a, dtype == KL_F32 ? 4 : 8, num_rows, q_heads, k_heads, dim, turn, interleaved, strides_host, freqs, pos_kind, positions,
-                        ids, starts, q_weight, k_weight, weight_f32, eps));
+  KL_CHECK_RC(fill_norm(a, dtype == KL_F32 ? 4 : 8, num_rows, q_heads, k_heads, dim, turn, interleaved, q, k, strides_host,
+                        freqs, pos_kind, positions, ids, starts, q_weight, k_weight, weight_f32, eps));
   if (num_rows == 0 || q_heads + k_heads == 0) return KL_OK;
   return with_type(dtype, "norm_rotary", [&](auto t) -> int {
     using T = decltype(t);
@@ -414,8 +416,8 @@ extern "C" int kl_norm_rotary_backward(kl_dtype dtype, int64_t num_rows, int q_h
                                        void *grad_q, void *grad_k, void *grad_q_weight, void *grad_k_weight, void *ws,
                                        size_t ws_bytes, kl_stream stream) {
   NormRot a;
-  KL_CHECK_RC(fill_norm(a, dtype == KL_F32 ? 4 : 8, num_rows, q_heads, k_heads, dim, turn, interleaved, strides_host, freqs, pos_kind, positions,
-                        ids, starts, q_weight, k_weight, weight_f32, eps));
+  KL_CHECK_RC(fill_norm(a, dtype == KL_F32 ? 4 : 8, num_rows, q_heads, k_heads, dim, turn, interleaved, q, k, strides_host,
+                        freqs, pos_kind, positions, ids, starts, q_weight, k_weight, weight_f32, eps));
   const bool weights = grad_q_weight || grad_k_weight;
   KL_REQUIRE(!weights || ws_bytes >= kl_norm_rotary_bwd_workspace_bytes(dim),
              "norm_rotary: the workspace is too small");

@@ -14,8 +14,8 @@
 // other order, so that it finds what 1 read last in the 256 MB cache.  One pass, with workgroups that publish and
 // await each other's (A, B), measured no faster: it reads less, but waits.
 // 311,000 rows of 64 columns, float, packs of 38 rows: forward 25 + 7 + 40 us (239 MB at least, 47 us at the rate of
-// a copy), backward 24 + 7 + 67 us (398 MB, 79 us); 131,074 x 1024, bf16, two packs: 69 + 11 + 71 and
-// 58 + 11 + 121 us (805 MB, 160 us, and 1342 MB, 267 us, with none of it found in the cache).
+// a copy), backward 24 + 7 + 67 us (397 MB, 79 us); 65,537 x 1024, bf16, two packs: 68 + 11 + 70 and
+// 58 + 11 + 121 us (403 MB, 80 us, and 671 MB, 133 us).
 //
 // States, A and B are in 32 bits (64 for double); outputs are rounded once.
 // Backward: g[t] = dh[t] + a[t+1] g[t+1] is the same recurrence in the other direction with the gate of the

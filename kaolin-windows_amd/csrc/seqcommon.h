@@ -157,6 +157,11 @@ __device__ __forceinline__ float half_max(float v) {
 struct Heads {
   int64_t row, head;
 };
+// (rows, heads, dim) whose rows of a head all start at multiples of 16 bytes
+inline bool whole_pieces(const void *p, int64_t rows, int64_t heads, Heads st, size_t esize) {
+  return rows == 0 || heads == 0 ||
+         ((uintptr_t)p % 16 == 0 && (rows == 1 || st.row * esize % 16 == 0) && (heads == 1 || st.head * esize % 16 == 0));
+}
 
 // any element of a 16-byte piece that is an infinity or a NaN
 template <typename T>

@@ -156,6 +156,16 @@ def test_library_refusals_without_gpu():
         st[i] = 1 << 25
         assert i % 2 or attend()[0] == -1 and b'too far apart' in lib.kl_last_error()
         st[i] = 0
+    p16 = ctypes.c_void_p(16)
+    for i, at in ((0, 24), (1, 16), (2, 24)):  # an address, a row's stride, a head's stride
+        st[0], st[1] = (60, 16) if i == 1 else (64, 12 if i == 2 else 16)
+        rc = lib.kl_pack_attention_forward(2, 2, 2, 2, 2, 16, ctypes.c_void_p(at), p16, p16, st, None, None, None, None,
+                                           1.0, 0, None, None, None, None, 1 << 30, None)
+        assert rc == -1 and b'multiples of 16 bytes' in lib.kl_last_error(), (i, lib.kl_last_error())
+        rc = lib.kl_norm_rotary_forward(2, 2, 2, 2, 16, 8, 0, ctypes.c_void_p(at), p16, st, None, None, 0, None, 3, None,
+                                        None, None, 1e-6, None, None, None)
+        assert rc == -1 and b'multiples of 16 bytes' in lib.kl_last_error(), (i, lib.kl_last_error())
+    st[0] = st[1] = 0
 
     def norm(dim=8, turn=8, eps=1e-6, kind=3, n=1):
         return lib.kl_norm_rotary_forward(0, n, 1, 1, dim, turn, 0, None, None, st, None, None, 0, None, kind, None, None,
