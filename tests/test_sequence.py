@@ -532,6 +532,29 @@ def test_attention_offsets_past_32_bits(spc):
         assert torch.equal(x, y)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype,n,dim', [(torch.float16, 130, 64), (torch.float32, 70, 64), (torch.float32, 70, 32)])
+def test_attention_rows_as_far_apart_as_allowed(spc, dtype, n, dim):
+    """A tile's rows span all but 2^32 bytes; rows further apart than that are copied first."""
+    stride = (1 << 25) - 8
+    held = torch.empty((n - 1) * stride + 3 * dim, dtype=dtype, device=DEV)
+    far = [held.as_strided((n, 1, dim), (stride, dim, 1), i * dim) for i in range(3)]
+    near = [_normal(i, n, 1, dim, dtype=dtype).to(DEV) for i in range(3)]
+    for x, y in zip(far, near):
+        x.copy_(y)
+    b, g = marks([3, n - 7, 4]).to(DEV), _normal(5, n, 1, dim, dtype=dtype).to(DEV)
+    got = []
+    for xs in (far, near):
+        leaves = [x.detach().requires_grad_() for x in xs]
+        o = spc.pack_attention(*leaves, b, causal=True)
+        got.append([o, *torch.autograd.grad(o, leaves, g)])
+    for x, y in zip(*got):
+        assert torch.equal(x, y)
+    further = held.as_strided((9, 1, dim), (6 * stride, dim, 1))
+    assert torch.equal(spc.pack_attention(further, further, further, b[:9]),
+                       spc.pack_attention(further.contiguous(), further.contiguous(), further.contiguous(), b[:9]))
+
+
 # ------------------------------------------------------------------------------- norm and rotation
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', TYPES)
