@@ -4,7 +4,7 @@
 // Steps compose: rows t0 .. t1 take a state s to A s + B.  The rows are cut into chunks, one a thread and piece
 // of columns:
 //   1. every chunk's (A, B), from the start of its last pack on: what lies before has no effect past the chunk;
-//   2. within segments of kSegment chunks, the (A, B) of what lies before each chunk, and each segment's own;
+//   2. within segments of chunks, the (A, B) of what lies before each chunk, and each segment's own;
 //   3. every chunk's state before it from those, back to the nearest segment with a pack's start; then it is
 //      walked and written.
 // A chunk in which a pack starts (`reset`) has A = 0, and that is never multiplied with the state before it, which
@@ -41,6 +41,8 @@ struct alignas(sizeof(T) * V) Pack {
 struct Recur {
   int n, chunk, chunks, packs, down;  // chunk: rows of one; packs: rows of initial; down: rows descend
   int64_t dim, cols;                  // cols: pieces across
+  int segment, few;                   // log2 of a segment's chunks; few: the number of segments if one wave holds them
+  int wide;                           // log2 of a workgroup's pieces across, where steps 1 and 2 are one
   const int32_t *ids, *starts;
   // rows are numbered in the order they are walked
   __device__ __forceinline__ int64_t row(int64_t i) const { return down ? n - 1 - i : i; }
@@ -57,7 +59,9 @@ struct Recur {
 constexpr int kAhead = 8;       // rows whose loads are in flight together in step 1
 constexpr int kAheadWrite = 4;  // and in step 3, which keeps more of each
 constexpr int kRunChunks = 4;   // chunks of a thread of step 2
-constexpr int kSegment = 64 * kRunChunks;
+constexpr int kSegmentLog = 8, kSegment = 64 * kRunChunks;
+static_assert(kSegment == 1 << kSegmentLog, "a segment of step 2");
+constexpr int kFewSegments = 64;  // what a wave's lanes can look through at once
 
 // (A, B) of chunks and segments: a and b (count, dim), resets (count)
 template <typename S>
@@ -198,6 +202,73 @@ __global__ void __launch_bounds__(1024) recur_scan_kernel(Recur r, Composed<S> c
   }
 }
 
+// Steps 1 and 2 in one, where segments of 256 / 2^wide chunks are few: a workgroup takes one, 2^wide pieces across,
+// and step 3 folds the segments before a chunk from the last one with a pack's start.  With the pack arrays, every row a
+// pack / one pack: 4096 rows of 64 columns, float, 11.4 / 17.4 us, in three launches 14.7 / 16.9; 8192 rows of 1024, bf16,
+// 20.7 / 36.8, in three launches 29.7 / 34.7.
+template <typename T, int V, bool GRAD>
+__global__ void __launch_bounds__(256) recur_segment_kernel(Recur r, const T *__restrict__ a, const T *__restrict__ x,
+                                                          const T *__restrict__ init,
+                                                          Composed<typename StateOf<T>::S> chunks,
+                                                          int32_t *__restrict__ before,
+                                                          Composed<typename StateOf<T>::S> segments) {
+  using S = typename StateOf<T>::S;
+  __shared__ Pack<S, V> s_a[256], s_b[256];
+  __shared__ int s_reset[256];
+  const int me = threadIdx.x, w = 1 << r.wide;
+  const int64_t c = (int64_t)blockIdx.y * (256 >> r.wide) + (me >> r.wide);
+  const int64_t piece = (int64_t)blockIdx.x * w + (me & (w - 1)), col = piece * V;
+  const bool live = c < r.chunks && piece < r.cols;
+  Pack<S, V> ga, gb;
+#pragma unroll
+  for (int v = 0; v < V; v++) {
+    ga.v[v] = 1;
+    gb.v[v] = 0;
+  }
+  int reset = 0;
+  if (live) {
+    const int64_t begin = c * r.chunk, end = min((int64_t)r.n, begin + r.chunk);
+    reset = recur_compose<T, V, GRAD>(r, a, x, init, begin, end, col, ga.v, gb.v);
+  }
+  // inclusive over the chunks in doubling steps; nothing to do where every chunk has a reset
+  if (__syncthreads_or(live && !reset)) {
+    for (int off = w; off < 256; off *= 2) {
+      s_a[me] = ga;
+      s_b[me] = gb;
+      s_reset[me] = reset;
+      __syncthreads();
+      if (me >= off && !reset) {
+        const Pack<S, V> pa = s_a[me - off], pb = s_b[me - off];
+        reset = s_reset[me - off];
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+          gb.v[v] = fma(ga.v[v], pb.v[v], gb.v[v]);
+          ga.v[v] = reset ? (S)0 : ga.v[v] * pa.v[v];
+        }
+      }
+      __syncthreads();
+    }
+  }
+  s_a[me] = ga;
+  s_b[me] = gb;
+  s_reset[me] = reset;
+  __syncthreads();
+  if (piece < r.cols && me >= 256 - w) {
+    *reinterpret_cast<Pack<S, V> *>(segments.a + (int64_t)blockIdx.y * r.dim + col) = ga;
+    *reinterpret_cast<Pack<S, V> *>(segments.b + (int64_t)blockIdx.y * r.dim + col) = gb;
+    if (piece == 0) segments.resets[blockIdx.y] = reset;
+  }
+  if (!live) return;
+#pragma unroll
+  for (int v = 0; v < V; v++) {
+    ga.v[v] = me >= w ? s_a[me - w].v[v] : (S)1;
+    gb.v[v] = me >= w ? s_b[me - w].v[v] : (S)0;
+  }
+  *reinterpret_cast<Pack<S, V> *>(chunks.a + c * r.dim + col) = ga;
+  *reinterpret_cast<Pack<S, V> *>(chunks.b + c * r.dim + col) = gb;
+  if (piece == 0) before[c] = me >= w ? s_reset[me - w] : 0;
+}
+
 // Rows [begin, end) of a piece of columns walked and written, from the state before them where it is `carried`
 template <typename T, int V, bool GRAD>
 __device__ __forceinline__ void recur_walk(const Recur &r, const T *__restrict__ a, const T *__restrict__ x,
@@ -288,6 +359,8 @@ __global__ void __launch_bounds__(256) recur_write_kernel(Recur r, const T *__re
   using S = typename StateOf<T>::S;
   const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x, place = t / r.cols, col = (t - place * r.cols) * V;
   const int64_t c = r.chunks - 1 - place;
+  const int lane = threadIdx.x & 63;
+  const uint64_t marks = ballot(lane < r.few && segments.resets[lane] != 0);
   if (c < 0) {
     const int64_t p = -1 - c;
     if (dinit && p < r.packs && (p >= r.n || r.starts[p] >= r.n))
@@ -308,9 +381,34 @@ __global__ void __launch_bounds__(256) recur_write_kernel(Recur r, const T *__re
     };
     const bool here = chunk_before[c] != 0;
     if (!here) {
-      int64_t k = c / kSegment - 1;
-      while (k > 0 && !segments.resets[k]) k--;
-      for (; k >= 0 && k < c / kSegment; k++) step(segments, k, segments.resets[k] != 0);
+      const int64_t mine = c >> r.segment;
+      int64_t k = mine - 1;
+      if (r.few) {
+        const uint64_t left = marks & (((uint64_t)1 << mine) - 1);
+        k = left ? 63 - __clzll(left) : 0;
+        constexpr int kFold = V >= 4 ? 4 : 8;  // loads in flight together
+        for (; k < mine; k += kFold) {
+          Pack<S, V> ka[kFold], kb[kFold];
+#pragma unroll
+          for (int u = 0; u < kFold; u++) {
+            const int64_t at = min(k + u, mine - 1) * r.dim + col;
+            ka[u] = *reinterpret_cast<const Pack<S, V> *>(segments.a + at);
+            kb[u] = *reinterpret_cast<const Pack<S, V> *>(segments.b + at);
+          }
+#pragma unroll
+          for (int u = 0; u < kFold; u++) {
+            const bool in = k + u < mine, reset = marks >> ((k + u) & 63) & 1;
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+              const S with = fma(ka[u].v[v], state[v], kb[u].v[v]);
+              state[v] = !in ? state[v] : reset ? kb[u].v[v] : with;
+            }
+          }
+        }
+      } else {
+        while (k > 0 && !segments.resets[k]) k--;
+        for (; k >= 0 && k < mine; k++) step(segments, k, segments.resets[k] != 0);
+      }
     }
     step(chunks, c, here);
   }
@@ -416,7 +514,7 @@ struct RecurSpace {
       bytes += al256(n);
       return p;
     };
-    const int64_t num = cdiv(num_chunks, kSegment);
+    const int64_t num = std::max(cdiv(num_chunks, kSegment), std::min<int64_t>(cdiv(num_chunks, 16), kFewSegments));
     chunks.a = (S *)take(num_chunks * dim * sizeof(S));
     chunks.b = (S *)take(num_chunks * dim * sizeof(S));
     segments.a = (S *)take(num * dim * sizeof(S));
@@ -439,7 +537,19 @@ static int recur_run(Recur r, const void *a, const void *x, const void *h, const
     return KL_OK;
   }
   const RecurSpace<S> m((char *)ws, r.chunks, r.dim);
-  if (r.chunks > 1) {
+  r.segment = kSegmentLog;
+  while (r.wide < 4 && 1 << r.wide < r.cols) r.wide++;
+  const int64_t segments = cdiv(r.chunks, 256 >> r.wide);
+  if (r.chunks > 1 && segments <= kFewSegments) {
+    r.segment = 8 - r.wide;
+    r.few = (int)segments;
+    hipLaunchKernelGGL((recur_segment_kernel<T, V, GRAD>),
+                       dim3((unsigned)cdiv(r.cols, 1 << r.wide), (unsigned)segments), dim3(256), 0, st, r, (const T *)a,
+                       (const T *)x, (const T *)init, m.chunks, m.before, m.segments);
+    KL_CHECK_LAUNCH();
+  } else if (r.chunks > 1) {
+    const int64_t all = cdiv(r.chunks, kSegment);
+    r.few = all <= kFewSegments ? (int)all : 0;
     hipLaunchKernelGGL((recur_chunk_kernel<T, V, GRAD>), dim3((unsigned)cdiv(r.chunks * r.cols, 256)), dim3(256), 0, st,
                        r, (const T *)a, (const T *)x, (const T *)init, m.chunks);
     KL_CHECK_LAUNCH();

@@ -732,7 +732,8 @@ def test_recurrence_is_cumsum_with_gates_of_one(spc):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize('n,dim', [(70001, 8), (33000, 72), (9000, 260)])
+@pytest.mark.parametrize('n,dim', [(70001, 8), (33000, 72), (9000, 260), (900, 64), (4001, 72), (6000, 260), (30000, 8),
+                                   (2500, 5)])
 def test_recurrence_long(spc, dtype, n, dim):
     """Sizes at which chunks are many and long, against the same rows as many short calls would give them."""
     b = torch.zeros(n, dtype=torch.bool)
