@@ -237,18 +237,31 @@ __global__ void __launch_bounds__(256) attend_join_kernel(Attend a, int splits, 
     top = fmaxf(top, x[i].x);
   }
   f32x8 sum = {};
+  constexpr int kAhead = 4;  // splits whose loads are in flight together
 #pragma unroll
-  for (int i = 0; i < kJoinEach; i++) {
-    if (i * shares >= splits || (x[i].x == -INFINITY && x[i].y == 0)) continue;  // no key of the row in this split
-    const float w = exp2_fast(x[i].x - (top == -INFINITY ? 0.f : top));
-    l = fmaf(w, x[i].y, l);
-    if (d < a.dim) {
-      const f32x4 *p = reinterpret_cast<const f32x4 *>(part + ((share + i * shares) * rows + at) * a.dim + d);
-      const f32x4 u0 = p[0], u1 = p[1];
+  for (int i0 = 0; i0 < kJoinEach; i0 += kAhead) {
+    if (i0 * shares >= splits) break;
+    f32x4 u0[kAhead], u1[kAhead];
+    bool full[kAhead];  // the row has keys in this split
+#pragma unroll
+    for (int j = 0; j < kAhead; j++) {
+      const int i = i0 + j;
+      full[j] = x[i].x != -INFINITY || x[i].y != 0;
+      u0[j] = u1[j] = f32x4{0, 0, 0, 0};
+      if (full[j] && d < a.dim) {
+        const f32x4 *p = reinterpret_cast<const f32x4 *>(part + ((share + i * shares) * rows + at) * a.dim + d);
+        u0[j] = p[0];
+        u1[j] = p[1];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; j++) {
+      const float w = full[j] ? exp2_fast(x[i0 + j].x - (top == -INFINITY ? 0.f : top)) : 0.f;
+      l = fmaf(w, x[i0 + j].y, l);
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        sum[e] = fmaf(w, u0[e], sum[e]);
-        sum[4 + e] = fmaf(w, u1[e], sum[4 + e]);
+        sum[e] = fmaf(w, u0[j][e], sum[e]);
+        sum[4 + e] = fmaf(w, u1[j][e], sum[4 + e]);
       }
     }
   }
