@@ -24,7 +24,8 @@ struct Grad {
   int parts;
 };
 
-// D, the key ranges and the maxima of |do|: LANES lanes per (row, head), kItems of those a group at once.
+// D, the key ranges and the maxima of |do|: LANES lanes per (row, head), kItems of those a group at once.  (float with
+// heads up to 32: the kernel of dq does it, which has do at hand: attend_rays_train 60 + 352 us, now 392.)
 constexpr int kItems = 4;
 template <typename T, int LANES>
 __global__ void __launch_bounds__(256) attend_prep_kernel(Attend a, const T *__restrict__ o, const T *__restrict__ low,
@@ -164,6 +165,10 @@ struct GradArgs {
   const void *q, *k, *v, *go;
   void *dq, *dk, *dv;
   float *part;  // dk, dv: the splits' sums (NULL without splits)
+  const void *out;  // dq, kDirect: what the first kernel takes and writes
+  const float *lse;
+  float2 *ld;
+  int2 *range;
 };
 
 template <typename T, int DP>
@@ -187,11 +192,9 @@ __device__ __forceinline__ bool dq_rows(const Attend &a, const Grad &g, const Gr
   const Row at_row = virtual_row(a, live ? m : 0);
   const int row = at_row.row, qhead = head * a.group + at_row.sub;
   const Range none = no_keys();
-  const int2 mine = live ? g.range[row] : make_int2(none.lo, none.hi);
   const int64_t at = (int64_t)row * heads + qhead;
-  const float2 ld = live ? g.ld[at] : make_float2(0, 0);
-  const int wlo = min_over(mine.x), whi = max_over(mine.y);
-  const int full_lo = max_over(mine.x), full_hi = min_over(mine.y);
+  int2 mine = make_int2(none.lo, none.hi);
+  float2 ld = make_float2(0, 0);
   V8<T> qf[DP / 16], gf[DP / 16];
   const T *qrow = (const T *)p.q + row * a.q.row + qhead * a.q.head, *grow = (const T *)p.go + at * a.dim;
 #pragma unroll
@@ -199,6 +202,34 @@ __device__ __forceinline__ bool dq_rows(const Attend &a, const Grad &g, const Gr
     qf[i] = global_frag(qrow, live, 16 * i + 8 * h, a.dim);
     gf[i] = global_frag(grow, live, 16 * i + 8 * h, a.dim);
   }
+  if constexpr (kDirect<T, DP>) {  // the first kernel's work, where do is in registers anyway
+    const T *orow = (const T *)p.out + at * a.dim;
+    float sum[2] = {0, 0};  // in that kernel's order: pieces of four, then pieces 4, 2 and 1 apart
+#pragma unroll
+    for (int i = 0; i < DP / 16; i++) {
+      const V8<T> x = global_frag(orow, live, 16 * i + 8 * h, a.dim);
+#pragma unroll
+      for (int b = 0; b < 2; b++) {
+        float d = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) d = fmaf(x[4 * b + e], gf[i][4 * b + e], d);
+        sum[b] += d;
+      }
+    }
+    const float d = half_sum(sum[0]) + half_sum(sum[1]);
+    if (live) {
+      const Range r = key_range(a, row);
+      mine = make_int2(r.lo, r.hi);
+      ld = make_float2(p.lse[at], d);
+      if (h == 0) p.ld[at] = ld;
+      if (h == 0 && qhead == 0) p.range[row] = mine;
+    }
+  } else if (live) {
+    mine = g.range[row];
+    ld = g.ld[at];
+  }
+  const int wlo = min_over(mine.x), whi = max_over(mine.y);
+  const int full_lo = max_over(mine.x), full_hi = min_over(mine.y);
   const T *kh = (const T *)p.k + head * a.k.head, *vh = (const T *)p.v + head * a.v.head;
   f32x16 acc[DP / 32] = {};
   float gs = 1;
@@ -480,18 +511,18 @@ static int with_prep_lanes(int lanes, F f) {
 
 template <typename T, int DP>
 static int attend_backward(const Attend &a, const Grad &g, const void *q, const void *k, const void *v, const void *go,
-                           void *dq, void *dk, void *dv, float *part, hipStream_t st) {
+                           void *dq, void *dk, void *dv, float *part, const void *out, const float *lse, hipStream_t st) {
   if (a.nq > 0 && dq) {
     const unsigned blocks = (unsigned)(cdiv((int64_t)a.nq * a.group, 32 * kWaves<T, DP>) * a.kv_heads);
     hipLaunchKernelGGL((attend_dq_kernel<T, DP>), dim3(blocks), dim3(64 * kWaves<T, DP>), 0, st, a, g,
-                       GradArgs{q, k, v, go, dq, nullptr, nullptr, nullptr});
+                       GradArgs{q, k, v, go, dq, nullptr, nullptr, nullptr, out, lse, (float2 *)g.ld, (int2 *)g.range});
     KL_CHECK_LAUNCH();
   }
   if (a.nk > 0 && dk) {
     constexpr int KEYS = DkvTile<T, DP>::KEYS, step = DkvTile<T, DP>::BQ;
     const int splits = dkv_splits(sizeof(T) == 4 ? KL_F32 : KL_F16, a.nq, a.nk, a.kv_heads, a.group, a.dim);
     hipLaunchKernelGGL((attend_dkv_kernel<T, DP>), places(a, cdiv(a.nk, KEYS), splits), dim3(64 * kWaves<T, DP>), 0, st, a, g,
-                       GradArgs{q, k, v, go, nullptr, dk, dv, splits > 1 ? part : nullptr});
+                       GradArgs{q, k, v, go, nullptr, dk, dv, splits > 1 ? part : nullptr, nullptr, nullptr, nullptr, nullptr});
     KL_CHECK_LAUNCH();
     if (splits > 1) {
       const int64_t pieces = (int64_t)a.nk * a.kv_heads * a.dim / 4;
@@ -533,7 +564,7 @@ extern "C" int kl_pack_attention_backward(kl_dtype dtype, int64_t num_q, int64_t
   const Grad g = {ld, range, amax, num_q > 0 ? (int)prep_blocks(dtype, num_q, heads, dim) : 0};
   return with_type(dtype, "pack_attention", [&](auto t) -> int {
     using T = decltype(t);
-    if (num_q > 0) {
+    if (num_q > 0 && !(is_direct(dtype, dim) && grad_q)) {
       KL_CHECK_RC(with_prep_lanes(prep_lanes(dtype, dim), [&](auto lanes) -> int {
         hipLaunchKernelGGL((attend_prep_kernel<T, decltype(lanes)::value>), dim3(g.parts), dim3(256), 0, S(stream), a,
                            (const T *)out, sizeof(T) == 2 ? (const T *)out_low : (const T *)nullptr,
@@ -544,7 +575,7 @@ extern "C" int kl_pack_attention_backward(kl_dtype dtype, int64_t num_q, int64_t
     }
     return with_dim(dim, [&](auto dp) {
       return attend_backward<T, decltype(dp)::value>(a, g, q, k, v, grad_out, grad_q, grad_k, grad_v, amax + kMaxParts,
-                                                     S(stream));
+                                                     out, lse, S(stream));
     });
   });
 }
