@@ -11,6 +11,8 @@
 // in 32 bits.  float16 has no exponents for small gradients: there ds is multiplied by a power of two that
 // puts the largest |do| into [16, 32), and the result by its inverse, both exact.
 // Masked places that hold infinities or NaN: as in attend.hip.
+// Bound by issue and by the longest rows: 8191 rows in 4 packs, causal, 16 / 4 heads of 64, bf16: dq 178 us, dk and dv
+// in four splits of the rows 265 and 14 for their join, with the matrix units busy in 35 to 40 % of the cycles.
 #include "attend32.h"
 
 namespace kl {

@@ -4,7 +4,7 @@
 // A workgroup counts the marks of the rows before its own and of all rows, then writes its part.  Up to
 // kOneLaunchRows rows every workgroup counts the whole mask itself (one byte a row, from L2), in one
 // launch; past that a first launch leaves one count per workgroup.  Two masks share their launches: each takes
-// some 4 us, whatever a small mask's few workgroups have to do.
+// some 4 us, whatever a small mask's few workgroups have to do (16,385 rows 5.6 us, 311,094 rows 5 + 6).
 #include "seqcommon.h"
 
 namespace kl {

@@ -416,11 +416,11 @@ __global__ void __launch_bounds__(256) recur_write_kernel(Recur r, const T *__re
 }
 
 // All three steps in one launch, for up to kShortRows rows (one step of a batch of sequences): a workgroup takes one
-// piece of columns, each thread a row of it.  256 rows of 1024 columns, bf16, with the pack arrays: 7.0 us if every row
-// is a pack and 12.6 us if one pack has them all, 14.2 and 15.7 in three launches.  Rows of one piece lie in different
-// lines of memory: with four rows a thread 1024 rows took 19 and 32 us, in three launches 15 and 17, and 256 rows of 512
-// pieces (2048 columns, float) 12 and 19 us, in three launches 14 and 15.
-constexpr int kShortRows = 256, kShortPieces = 256;
+// piece of columns, each thread a row of it.  256 rows of 1024 columns, bf16, with the pack arrays: 7.1 us if every row
+// is a pack and 12.6 us if one pack has them all, 11.5 and 16.1 in two launches.  Rows of one piece lie in different
+// lines of memory: with four rows a thread 1024 rows took 19 and 32 us, in two launches 12 and 17, and 256 rows of 512
+// pieces (2048 columns, float) 12 and 19 us, in two launches 11 and 14 (64 rows of them 6.5 and 9 us, 10 and 13).
+constexpr int kShortRows = 256, kShortPieces = 1 << 16;  // pieces: of all rows
 template <typename T, int V, bool GRAD>
 __global__ void __launch_bounds__(kShortRows) recur_short_kernel(Recur r, const T *__restrict__ a, const T *__restrict__ x,
                                                          const T *__restrict__ h, const T *__restrict__ init,
@@ -487,7 +487,7 @@ __global__ void __launch_bounds__(kShortRows) recur_short_kernel(Recur r, const 
   }
   if (live) recur_walk<T, V, GRAD>(r, a, x, h, init, begin, end, col, carried, state, out, da, dinit);
   if (dinit) {
-    for (int64_t p = threadIdx.x; p < r.packs; p += kShortRows) {
+    for (int64_t p = threadIdx.x; p < r.packs; p += blockDim.x) {
       if (p >= r.n || r.starts[p] >= r.n) *reinterpret_cast<Pack<T, V> *>(dinit + p * r.dim + col) = Pack<T, V>{};
     }
   }
@@ -530,8 +530,8 @@ static int recur_run(Recur r, const void *a, const void *x, const void *h, const
                      void *dinit, void *ws, hipStream_t st) {
   using S = typename StateOf<T>::S;
   r.cols = r.dim / V;
-  if (r.n > 1 && r.n <= kShortRows && r.cols <= kShortPieces) {
-    hipLaunchKernelGGL((recur_short_kernel<T, V, GRAD>), dim3((unsigned)r.cols), dim3(kShortRows), 0, st, r, (const T *)a,
+  if (r.n > 1 && r.n <= kShortRows && r.n * r.cols <= kShortPieces) {
+    hipLaunchKernelGGL((recur_short_kernel<T, V, GRAD>), dim3((unsigned)r.cols), dim3((unsigned)cdiv(r.n, 64) * 64), 0, st, r, (const T *)a,
                        (const T *)x, (const T *)h, (const T *)init, (T *)out, (T *)da, (T *)dinit);
     KL_CHECK_LAUNCH();
     return KL_OK;
