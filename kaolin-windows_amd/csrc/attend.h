@@ -42,6 +42,13 @@ __device__ __forceinline__ Range key_range(const Attend &a, int row) {
   return hi > lo ? Range{lo, hi} : no_keys();
 }
 
+// The part of keys [begin, end) that split `y` of `n` takes, in whole steps
+__device__ __forceinline__ void take_split(int &begin, int &end, int y, int n, int step) {
+  const int steps = (end - begin + step - 1) / step, share = (steps + n - 1) / n * step;
+  begin = (int)min((int64_t)end, begin + (int64_t)share * y);
+  end = (int)min((int64_t)end, (int64_t)begin + share);
+}
+
 // Where a workgroup is.  Splits of one tile run side by side, so that tiles with much to do start first whichever
 // their splits are (a split of all tiles after the other: attend_long_train's dk and dv 322 us, now 263).
 struct Place {

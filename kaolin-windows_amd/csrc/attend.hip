@@ -110,13 +110,6 @@ __device__ __forceinline__ void fwd_walk(const Attend &a, const T *__restrict__ 
       });
 }
 
-// The part of keys [begin, end) that split `y` of `n` takes, in whole steps
-__device__ __forceinline__ void take_split(int &begin, int &end, int y, int n, int step) {
-  const int steps = (end - begin + step - 1) / step, share = (steps + n - 1) / n * step;
-  begin = (int)min((int64_t)end, begin + (int64_t)share * y);
-  end = (int)min((int64_t)end, (int64_t)begin + share);
-}
-
 // What a workgroup keeps in LDS
 template <typename T, int DP>
 struct FwdLds {

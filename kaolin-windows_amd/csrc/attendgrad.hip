@@ -171,7 +171,18 @@ struct GradArgs {
   const float *lse;
   float2 *ld;
   int2 *range;
+  int *used;        // dq: splits of each tile that have keys
 };
+
+// This workgroup's split of the keys [begin, end) of its tile; false: none are left for it, and nobody asks for it.  The
+// first leaves the number of those that have some.
+__device__ __forceinline__ bool dq_split(const GradArgs &p, int &begin, int &end, int step) {
+  const int steps = (end - begin + step - 1) / step, share = (steps + (int)gridDim.y - 1) / (int)gridDim.y;
+  if (blockIdx.y == 0 && threadIdx.x == 0)
+    p.used[blockIdx.z * gridDim.x + blockIdx.x] = share ? (steps + share - 1) / share : 0;
+  take_split(begin, end, blockIdx.y, gridDim.y, step);
+  return begin < end;
+}
 
 template <typename T, int DP>
 struct DqLds {
@@ -187,9 +198,9 @@ struct DqLds {
 template <typename T, int DP, bool CAREFUL>
 __device__ __forceinline__ bool dq_rows(const Attend &a, const Grad &g, const GradArgs &p, DqLds<T, DP> &lds) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
-  const int head = (int)blockIdx.x % a.kv_heads, heads = a.kv_heads * a.group;
-  const int total = a.nq * a.group, tiles = (int)gridDim.x / a.kv_heads;  // virtual rows: under 2^31
-  const int m = (tiles - 1 - (int)blockIdx.x / a.kv_heads) * (32 * kWaves<T, DP>) + wave * 32 + col;
+  const Place at_place = place(a, p.part != nullptr);
+  const int head = at_place.head, heads = a.kv_heads * a.group, total = a.nq * a.group;  // virtual rows: under 2^31
+  const int m = (at_place.tiles - 1 - at_place.tile) * (32 * kWaves<T, DP>) + wave * 32 + col;
   const bool live = m < total;
   const Row at_row = virtual_row(a, live ? m : 0);
   const int row = at_row.row, qhead = head * a.group + at_row.sub;
@@ -223,8 +234,10 @@ __device__ __forceinline__ bool dq_rows(const Attend &a, const Grad &g, const Gr
       const Range r = key_range(a, row);
       mine = make_int2(r.lo, r.hi);
       ld = make_float2(p.lse[at], d);
-      if (h == 0) p.ld[at] = ld;
-      if (h == 0 && qhead == 0) p.range[row] = mine;
+      if (h == 0 && blockIdx.y == 0) {
+        p.ld[at] = ld;
+        if (qhead == 0) p.range[row] = mine;
+      }
     }
   } else if (live) {
     mine = g.range[row];
@@ -236,7 +249,10 @@ __device__ __forceinline__ bool dq_rows(const Attend &a, const Grad &g, const Gr
   f32x16 acc[DP / 32] = {};
   float gs = 1;
   if constexpr (kDirect<T, DP>) {
-    dq_walk32<DP, CAREFUL>(a, kh, vh, wlo, whi, mine, ld, full_lo, full_hi, qf, gf, lds.ks, lds.vs, acc);
+    int begin = wlo, end = whi;
+    if (begin >= end) begin = end = 0;
+    if (p.part && !dq_split(p, begin, end, DqTile<T, DP>::BN)) return false;
+    dq_walk32<DP, CAREFUL>(a, kh, vh, begin, end, mine, ld, full_lo, full_hi, qf, gf, lds.ks, lds.vs, acc);
     if (!CAREFUL && __any(!all_finite(acc))) return true;
   } else {
     if (lane == 0) {
@@ -250,6 +266,7 @@ __device__ __forceinline__ bool dq_rows(const Attend &a, const Grad &g, const Gr
     int begin = uniform(min(min(lds.lo[0], lds.lo[1]), min(lds.lo[2], lds.lo[3])));
     int end = uniform(max(max(lds.hi[0], lds.hi[1]), max(lds.hi[2], lds.hi[3])));
     if (begin >= end) begin = end = 0;
+    if (p.part && !dq_split(p, begin, end, DqTile<T, DP>::BN)) return false;
     dq_walk<T, DP, CAREFUL>(a, kh, vh, begin, end, mine, ld, gs, wlo, whi, full_lo, full_hi, qf, gf, lds.ks, lds.vs,
                             lds.bad, acc);
     if (!CAREFUL) {
@@ -258,15 +275,39 @@ __device__ __forceinline__ bool dq_rows(const Attend &a, const Grad &g, const Gr
       if (lds.redo) return true;
     }
   }
-  if (live) store_cols<T, DP>((T *)p.dq + at * a.dim, acc, a.scale / gs, h, a.dim);
+  if (!live) return false;
+  if (p.part) {
+    const int64_t all = (int64_t)a.nq * heads;
+    store_cols<float, DP>(p.part + (blockIdx.y * all + at) * a.dim, acc, a.scale / gs, h, a.dim);
+  } else {
+    store_cols<T, DP>((T *)p.dq + at * a.dim, acc, a.scale / gs, h, a.dim);
+  }
   return false;
 }
 
+// grid: places(tiles, splits of the keys)
 template <typename T, int DP>
 __global__ void __launch_bounds__((64 * kWaves<T, DP>), (kDirect<T, DP> ? 3 : sizeof(T) == 4 && DP == 128 ? 1 : 2))
     attend_dq_kernel(Attend a, Grad g, GradArgs p) {
   __shared__ DqLds<T, DP> lds;
   if (dq_rows<T, DP, false>(a, g, p, lds)) dq_rows<T, DP, true>(a, g, p, lds);
+}
+
+// The splits of dq added in their order: four elements a thread.
+template <typename T>
+__global__ void __launch_bounds__(256) attend_dq_join_kernel(Attend a, int tile_rows, int tiles, const int *__restrict__ used,
+                                                           const float *__restrict__ part, T *__restrict__ dq) {
+  const int64_t all = (int64_t)a.nq * a.kv_heads * a.group * a.dim, at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (at >= all) return;
+  const int heads = a.kv_heads * a.group;
+  const int64_t line = at / a.dim;
+  const int row = (int)(line / heads), qhead = (int)(line % heads);
+  const int tile = tiles - 1 - (row * a.group + qhead % a.group) / tile_rows;  // as the workgroups were numbered
+  const int splits = used[tile * a.kv_heads + qhead / a.group];
+  f32x4 sum = {};
+#pragma unroll 4
+  for (int s = 0; s < splits; s++) sum += *reinterpret_cast<const f32x4 *>(part + s * all + at);
+  *reinterpret_cast<V4<T> *>(dq + at) = __builtin_convertvector(sum, V4<T>);
 }
 
 template <typename T, int DP>
@@ -485,6 +526,14 @@ __global__ void __launch_bounds__(256) attend_dkv_join_kernel(Attend a, int spli
   *reinterpret_cast<V4<T> *>(dv + at) = __builtin_convertvector(v, V4<T>);
 }
 
+// Splits of the keys that a tile of rows walks for dq: two waves for each of the 1024 SIMDs (forward and backward of
+// 2264 rows in 4 packs, 3 heads of 32 that share one key head, float: 171 us without, 111 with)
+static int dq_splits(kl_dtype dtype, int64_t nq, int64_t nk, int kv_heads, int group, int dim) {
+  const int waves = is_direct(dtype, dim) ? 1 : 4, step = dtype == KL_F32 ? 32 : 64;
+  const int64_t all = cdiv(nq * group, 32 * waves) * kv_heads * waves;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({2048 / std::max<int64_t>(all, 1), cdiv(nk, 2 * step), 16}));
+}
+
 // Splits of the rows that stream past a tile of keys: four waves for each of the 1024 SIMDs
 static int dkv_splits(kl_dtype dtype, int64_t nq, int64_t nk, int kv_heads, int group, int dim) {
   const int waves = is_direct(dtype, dim) ? 1 : 4, step = dtype == KL_F32 ? 32 : 64;
@@ -515,16 +564,27 @@ template <typename T, int DP>
 static int attend_backward(const Attend &a, const Grad &g, const void *q, const void *k, const void *v, const void *go,
                            void *dq, void *dk, void *dv, float *part, const void *out, const float *lse, hipStream_t st) {
   if (a.nq > 0 && dq) {
-    const unsigned blocks = (unsigned)(cdiv((int64_t)a.nq * a.group, 32 * kWaves<T, DP>) * a.kv_heads);
-    hipLaunchKernelGGL((attend_dq_kernel<T, DP>), dim3(blocks), dim3(64 * kWaves<T, DP>), 0, st, a, g,
-                       GradArgs{q, k, v, go, dq, nullptr, nullptr, nullptr, out, lse, (float2 *)g.ld, (int2 *)g.range});
+    const int splits = dq_splits(sizeof(T) == 4 ? KL_F32 : KL_F16, a.nq, a.nk, a.kv_heads, a.group, a.dim);
+    constexpr int ROWS = 32 * kWaves<T, DP>;
+    const int64_t tiles = cdiv((int64_t)a.nq * a.group, ROWS), all = (int64_t)a.nq * a.kv_heads * a.group * a.dim;
+    int *used = (int *)(part + splits * all);
+    hipLaunchKernelGGL((attend_dq_kernel<T, DP>), places(a, tiles, splits), dim3(64 * kWaves<T, DP>), 0, st, a, g,
+                       GradArgs{q, k, v, go, dq, nullptr, nullptr, splits > 1 ? part : nullptr, out, lse,
+                                (float2 *)g.ld, (int2 *)g.range, used});
     KL_CHECK_LAUNCH();
+    if (splits > 1) {
+      hipLaunchKernelGGL(attend_dq_join_kernel<T>, dim3((unsigned)cdiv(all / 4, 256)), dim3(256), 0, st, a, ROWS,
+                         (int)tiles, used, part, (T *)dq);
+      KL_CHECK_LAUNCH();
+    }
   }
   if (a.nk > 0 && dk) {
     constexpr int KEYS = DkvTile<T, DP>::KEYS, step = DkvTile<T, DP>::BQ;
     const int splits = dkv_splits(sizeof(T) == 4 ? KL_F32 : KL_F16, a.nq, a.nk, a.kv_heads, a.group, a.dim);
-    hipLaunchKernelGGL((attend_dkv_kernel<T, DP>), places(a, cdiv(a.nk, KEYS), splits), dim3(64 * kWaves<T, DP>), 0, st, a, g,
-                       GradArgs{q, k, v, go, nullptr, dk, dv, splits > 1 ? part : nullptr, nullptr, nullptr, nullptr, nullptr});
+    hipLaunchKernelGGL((attend_dkv_kernel<T, DP>), places(a, cdiv(a.nk, KEYS), splits), dim3(64 * kWaves<T, DP>), 0, st,
+                       a, g,
+                       GradArgs{q, k, v, go, nullptr, dk, dv, splits > 1 ? part : nullptr, nullptr, nullptr, nullptr,
+                                nullptr, nullptr});
     KL_CHECK_LAUNCH();
     if (splits > 1) {
       const int64_t pieces = (int64_t)a.nk * a.kv_heads * a.dim / 4;
@@ -544,8 +604,10 @@ extern "C" size_t kl_pack_attention_bwd_workspace_bytes(kl_dtype dtype, int64_t 
                                                         int kv_heads, int dim) {
   if (num_q < 0 || num_k < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || dim <= 0) return 256;
   const int splits = dkv_splits(dtype, num_q, num_k, kv_heads, heads / kv_heads, dim);
+  const int dq = dq_splits(dtype, num_q, num_k, kv_heads, heads / kv_heads, dim);
   return al256((size_t)num_q * heads * 8) + al256((size_t)num_q * 8) + kMaxParts * 4 +
-         (splits > 1 ? (size_t)2 * splits * num_k * kv_heads * dim * 4 : 0);
+         std::max(splits > 1 ? (size_t)2 * splits * num_k * kv_heads * dim * 4 : 0,
+                  dq > 1 ? (size_t)dq * num_q * heads * dim * 4 + (size_t)cdiv(num_q * (heads / kv_heads), 32) * kv_heads * 4 : 0);
 }
 
 extern "C" int kl_pack_attention_backward(kl_dtype dtype, int64_t num_q, int64_t num_k, int heads, int kv_heads,
