@@ -723,6 +723,43 @@ def test_recurrence_few_rows(spc, dtype, lens, lead, reverse):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('dtype,dim', [(torch.float32, 131), (torch.float16, 269), (torch.bfloat16, 268),
+                                       (torch.float64, 67)])
+@pytest.mark.parametrize('reverse', [False, True])
+def test_recurrence_rows_of_odd_length(spc, dtype, dim, reverse):
+    """Enough rows for pieces of 16 bytes where a row is not a whole number of them."""
+    b = marks([1500, 1, 2400, 99], lead=30)
+    n = len(b)
+    a = torch.sigmoid(_normal(0, n, dim, scale=3.0) + 2).to(dtype)
+    x, g, h0 = _normal(1, n, dim, dtype=dtype), _normal(2, n, dim, dtype=dtype), _normal(3, 4, dim, dtype=dtype)
+    outs, tols = recurrence(a, x, b, h0, reverse, grad=g, dtype=dtype)
+    leaves = [_leaf(y) for y in (a, x, h0)]
+    h = spc.linear_recurrence(leaves[0], leaves[1], b.to(DEV), initial=leaves[2], reverse=reverse)
+    got = [h, *torch.autograd.grad(h, leaves, g.to(DEV))]
+    for name, y, want, tol in zip(('h', 'da', 'db', 'dinitial'), got, outs, tols):
+        check(name, y, want, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('n,dim', [(40, 16), (300, 24), (5000, 269)])
+def test_recurrence_at_any_address(spc, dtype, n, dim):
+    b = marks([n // 3, n - n // 3]).to(DEV)
+    near = [_normal(i, n, dim, dtype=dtype).to(DEV) for i in range(3)]
+    odd = []
+    for x in near:
+        odd.append(torch.empty(n * dim + 1, dtype=dtype, device=DEV)[1:].view(n, dim))
+        odd[-1].copy_(x)
+    got = []
+    for a, x, g in (near, odd):
+        leaves = [a.detach().requires_grad_(), x.detach().requires_grad_()]
+        h = spc.linear_recurrence(*leaves, b)
+        got.append([h, *torch.autograd.grad(h, leaves, g)])
+    for y, z in zip(*got):
+        assert torch.equal(y, z)
+
+
+@pytest.mark.gpu
 def test_recurrence_is_cumsum_with_gates_of_one(spc):
     b = marks([30, 1, 300], lead=2).to(DEV)
     x = torch.randint(-8, 8, (333, 7), generator=torch.Generator().manual_seed(0)).float().to(DEV)
