@@ -105,7 +105,7 @@ template <int LANES>
 __device__ __forceinline__ float lanes_sum(float v) {
   v += dpp<0xb1>(v);   // lanes 1 away
   v += dpp<0x4e>(v);   // 2 away
-  v += dpp<0x141>(v);  // the other half of 8
+  if constexpr (LANES >= 8) v += dpp<0x141>(v);   // the other half of 8
   if constexpr (LANES >= 16) v += dpp<0x140>(v);  // of 16
   if constexpr (LANES >= 32) v += __shfl_xor(v, 16);
   if constexpr (LANES >= 64) v = half_sum(v);
@@ -329,15 +329,18 @@ __global__ void __launch_bounds__(256) norm_weight_grad_kernel(int dim, int part
 }
 
 // Rows of a workgroup: its table holds them, and each group of lanes gets some 32 heads (at the size above 4 take
-// 110 us, 8 take 93 and 32 take 81: the table and its barrier come first), unless that leaves too few workgroups.
+// 110 us, 8 take 93 and 32 take 81: the table and its barrier come first), unless that leaves too few workgroups; but
+// no fewer rows than the lanes take at once (1721 rows of 1 + 1 heads of 128, bf16, forward and backward: 14 + 20 us
+// one by one, 7 + 9 by eights).
 static int norm_rows(int64_t n, int heads, int half, int groups) {
   int64_t rows = std::max<int64_t>(1, std::min<int64_t>({16, half ? kTable / half : 16, cdiv(32 * groups, heads)}));
-  while (rows > 1 && cdiv(n, rows) < 1024) rows /= 2;
+  while (rows > 1 && cdiv(n, rows) < 1024 && (rows * heads > groups || rows * half > 256)) rows /= 2;
   return (int)rows;
 }
 
 template <typename F>
 static int with_lanes(int lanes, F f) {
+  if (lanes <= 4) return f(std::integral_constant<int, 4>());
   if (lanes <= 8) return f(std::integral_constant<int, 8>());
   if (lanes <= 16) return f(std::integral_constant<int, 16>());
   if (lanes <= 32) return f(std::integral_constant<int, 32>());
