@@ -8,8 +8,8 @@
 // memory took the L1 cache one line for each lane).
 //
 // Bound by the matrix units and waits for them, 45 to 49 % busy: tiles of 32 rows meet 1.8 times the keys that their
-// rows see.  311,094 rows in 8192 packs of 38 on average, 4 heads of 32: forward 265 us, dq with the sums of do . o 392,
-// dk and dv 496, where the bytes alone take 379 us.  Three waves a SIMD: with two, 303, 347 (without the sums) and 549;
+// rows see.  311,094 rows in 8192 packs of 38 on average, 4 heads of 32: forward 262 us, dq with the sums of do . o 370,
+// dk and dv 470, where the bytes alone take 379 us.  Three waves a SIMD: with two, 303, 347 (without the sums) and 549;
 // with four, whose registers spill, 315, 402 and 797.
 //
 // Rows past the end are copies of the last one: their scores are masked.  Rows with infinities or NaN: as in
