@@ -545,7 +545,7 @@ int kl_pack_layout_pair(int64_t num_rows, const uint8_t *boundaries, int32_t *id
 
 /* out[i] = sum_j softmax_j(scale * q[i] . k[j]) v[j] over the keys j of the pack of keys that has the number
  * of i's pack of queries; causal: the last query of a pack sees all its keys, each one before it one key
- * fewer.  A row that sees no key is 0.  q (num_q, heads, dim), k and v (num_k, kv_heads, dim), heads a
+ * fewer.  A row that sees no key is 0, one whose scores are all -inf NaN.  q (num_q, heads, dim), k and v (num_k, kv_heads, dim), heads a
  * multiple of kv_heads (query head h reads key head h / (heads / kv_heads)), dim a multiple of 8 up to 128;
  * f16 / bf16 / f32.  strides_host: the row and head strides of q, k, v in elements (q row, q head, k row, k
  * head, v row, v head); every row of a head starts at a multiple of 16 bytes.  out (num_q, heads, dim) and
@@ -558,17 +558,17 @@ int kl_pack_attention_forward(kl_dtype dtype, int64_t num_q, int64_t num_k, int 
                               const int32_t *q_ids, const int32_t *q_starts, const int32_t *k_ids,
                               const int32_t *k_starts, float scale, int causal, void *out, void *out_low,
                               float *lse, void *workspace, size_t workspace_bytes, kl_stream stream);
-/* Its gradients: grad_out, out, out_low (num_q, heads, dim; out_low may be NULL) contiguous and 16-byte aligned; grad_q as q and grad_k,
- * grad_v as k and v, contiguous, fully written (grad_q, or grad_k with grad_v, may be NULL).  Every sum has a
- * fixed order. */
+/* Its gradients: grad_out, out, out_low (num_q, heads, dim; out_low may be NULL) contiguous and 16-byte aligned;
+ * grad_q as q and grad_k, grad_v as k and v, contiguous, fully written (grad_q, or grad_k with grad_v, may be
+ * NULL).  Every sum has a fixed order. */
 size_t kl_pack_attention_bwd_workspace_bytes(kl_dtype dtype, int64_t num_q, int64_t num_k, int heads, int kv_heads,
                                              int dim);
 int kl_pack_attention_backward(kl_dtype dtype, int64_t num_q, int64_t num_k, int heads, int kv_heads, int dim,
                                const void *grad_out, const void *q, const void *k, const void *v,
                                const int64_t *strides_host, const int32_t *q_ids, const int32_t *q_starts,
                                const int32_t *k_ids, const int32_t *k_starts, const void *out, const void *out_low,
-                               const float *lse, float scale, int causal, void *grad_q, void *grad_k, void *grad_v, void *workspace,
-                               size_t workspace_bytes, kl_stream stream);
+                               const float *lse, float scale, int causal, void *grad_q, void *grad_k, void *grad_v,
+                               void *workspace, size_t workspace_bytes, kl_stream stream);
 
 /* RMS norm of each head of q (num_rows, q_heads, dim) and k (num_rows, k_heads, dim), then the rotation of the
  * first `turn` elements of each by angle positions[row] * freqs[pair] (freqs: turn / 2 doubles; pairs (2 i,

@@ -1,6 +1,6 @@
 """``_C.render.spc`` entries of the sequence operators over packs (csrc/packs.hip, attend.hip,
-attendgrad.hip, normrotary.hip, recurrence.hip): argument checks, outputs and one library call each.  The reference has none of
-these; they follow its packed ray ops' conventions (rows grouped by a boundary mask)."""
+attendgrad.hip, normrotary.hip, recurrence.hip): argument checks, outputs and one library call each.  The reference has
+none of these; they follow its packed ray ops' conventions (rows grouped by a boundary mask)."""
 import ctypes
 import math
 

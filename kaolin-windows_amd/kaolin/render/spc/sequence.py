@@ -1,5 +1,5 @@
-"""Learned operators along packs: attention, norm with rotation, and the gated linear recurrence.  They take packs as the packed ray ops do (raytrace.py):
-rows grouped by a boundary mask, and read nothing back to the host.
+"""Learned operators along packs: attention, norm with rotation, and the gated linear recurrence.  They take packs as
+the packed ray ops do (raytrace.py): rows grouped by a boundary mask, and read nothing back to the host.
 
 A plain call (types, sizes and strides that the kernels read as they are) runs as a compiled autograd node
 (csrc/torch_ops.cpp); the nodes here take every other one, copy what has to be copied, and refuse what is
@@ -56,7 +56,8 @@ def pack_attention(q, k, v, boundaries, q_boundaries=None, causal=False, scale=N
 
     Returns:
         (Tensor): (num_q, heads, dim).  Rows that see no key (before the first pack, of a pack that has no
-        keys, or masked altogether) are 0, and their gradients are 0.
+        keys, or masked altogether) are 0, and their gradients are 0.  A row whose scores are all -inf has no
+        softmax and is NaN.
 
     Rows of q, k and v may be strided, such as the slices of one projection's output; a last dimension
     that is not contiguous, or rows that do not start at multiples of 16 bytes, are copied first.  Keys that
