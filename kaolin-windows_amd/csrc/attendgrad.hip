@@ -8,8 +8,8 @@
 // accumulators of the first in place (seqcommon.h, acc_frag); the streamed tiles are read from LDS along
 // rows for the first products and along columns for the second.
 // Rounding: p and ds are rounded to the inputs' type for the second products, half a step each; sums stay
-// in 32 bits.  float16 has no exponents for small gradients: there ds is multiplied by a power of two that
-// puts the largest |do| into [16, 32), and the result by its inverse, both exact.
+// in 32 bits.  float16 has few exponents: there ds is multiplied by a power of two of its column (fit_column), and the
+// result by its inverse, both exact.
 // Masked places that hold infinities or NaN: as in attend.hip.
 // Bound by issue and by the longest rows: 8191 rows in 4 packs, causal, 16 / 4 heads of 64, bf16: dq 178 us, dk and dv
 // in four splits of the rows 265 and 14 for their join, with the matrix units busy in 35 to 40 % of the cycles.
@@ -17,23 +17,18 @@
 
 namespace kl {
 
-constexpr int kMaxParts = 1024;  // workgroups of the first kernel: partial maxima of |do|
-
 struct Grad {
   const float2 *ld;    // (lse, D) of each (row, head)
   const int2 *range;   // keys of each row
-  const float *amax;   // partial maxima of |do| (f16)
-  int parts;
 };
 
-// D, the key ranges and the maxima of |do|: LANES lanes per (row, head), kItems of those a group at once.  (float with
-// heads up to 32: the kernel of dq does it, which has do at hand: attend_rays_train 60 + 352 us, now 392.)
+// D and the key ranges: LANES lanes per (row, head), kItems of those a group at once.  (float with heads up to 32: the
+// kernel of dq does it, which has do at hand: attend_rays_train 60 + 352 us, now 392.)
 constexpr int kItems = 4;
 template <typename T, int LANES>
 __global__ void __launch_bounds__(256) attend_prep_kernel(Attend a, const T *__restrict__ o, const T *__restrict__ low,
                                                         const T *__restrict__ go, const float *__restrict__ lse,
-                                                        float2 *__restrict__ ld, int2 *__restrict__ range,
-                                                        float *__restrict__ amax) {
+                                                        float2 *__restrict__ ld, int2 *__restrict__ range) {
   constexpr int E = 16 / (int)sizeof(T), GROUPS = 256 / LANES;
   union Piece {
     u32x4 w;
@@ -41,7 +36,6 @@ __global__ void __launch_bounds__(256) attend_prep_kernel(Attend a, const T *__r
   };
   const int64_t rows = (int64_t)a.nq * a.kv_heads * a.group;
   const int sub = threadIdx.x % LANES, c = sub * E;
-  float big = 0;
   for (int64_t at0 = ((int64_t)blockIdx.x * GROUPS + threadIdx.x / LANES) * kItems; at0 < rows;
        at0 += (int64_t)gridDim.x * GROUPS * kItems) {
     Piece x[kItems], y[kItems], z[kItems];
@@ -61,10 +55,7 @@ __global__ void __launch_bounds__(256) attend_prep_kernel(Attend a, const T *__r
     for (int i = 0; i < kItems; i++) {
       float d = 0;
 #pragma unroll
-      for (int e = 0; e < E; e++) {
-        d = fmaf((float)x[i].v[e] + (float)z[i].v[e], (float)y[i].v[e], d);
-        big = fmaxf(big, fabsf((float)y[i].v[e]));
-      }
+      for (int e = 0; e < E; e++) d = fmaf((float)x[i].v[e] + (float)z[i].v[e], (float)y[i].v[e], d);
 #pragma unroll
       for (int s = LANES / 2; s > 0; s >>= 1) d += __shfl_xor(d, s);
       if (sub == 0 && at0 + i < rows) ld[at0 + i] = make_float2(ls[i], d);
@@ -74,27 +65,39 @@ __global__ void __launch_bounds__(256) attend_prep_kernel(Attend a, const T *__r
     const Range r = key_range(a, (int)row);
     range[row] = make_int2(r.lo, r.hi);
   }
-  if constexpr (std::is_same<T, f16_t>::value) {
-    __shared__ float s_max[4];
-    big = wave_max(big);
-    if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = big;
-    __syncthreads();
-    if (threadIdx.x == 0) amax[blockIdx.x] = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
-  }
 }
 
-// the power of two that puts the largest |do| into [16, 32); 1 where there is none.  Every thread calls it.
+// What is rounded to float16 for a second product is first multiplied by a power of two of its column (this lane and the
+// other half's; a row of q in dq, a key in dk), `up`, and the product divided by it in the end, both exact.  It starts
+// at kMostUp and falls, the sums so far with it, where a column's largest number would pass 2^15: that one then lies
+// in [2^11, 2^12), and smaller ones keep their bits down to 2^-25 of it.  So neither overflows, nor do large
+// numbers of another row, key or pack cost bits here.  (One power for all, from the largest |do|: ds overflowed where v is
+// large, and a pack of small gradients lost its bits to one of large ones.  Forward and backward of 8191 rows in 4 packs,
+// causal, 16 / 4 heads, f16: 602 us with that, 609 now, for heads of 64; 1317 and 1290 for heads of 128.)
 template <typename T>
-__device__ __forceinline__ float grad_scale(const Grad &g, float *s_max) {
-  if constexpr (!std::is_same<T, f16_t>::value) return 1.f;
-  float big = 0;
-  for (int i = threadIdx.x; i < g.parts; i += 256) big = fmaxf(big, g.amax[i]);
-  big = wave_max(big);
-  if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = big;
-  __syncthreads();
-  big = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
-  if (!(big > 0) || !finite(big)) return 1.f;
-  return __uint_as_float((uint32_t)(127 + 4 + 127 - (int)(__float_as_uint(big) >> 23)) << 23);
+constexpr bool kFitted = std::is_same<T, f16_t>::value;
+constexpr float kMostUp = 0x1p60f;  // leaves room for sums of 2^31 products of two of the largest float16 numbers
+
+template <int N>
+__device__ __forceinline__ void fit_column(f32x16 &x, float &up, f32x16 (&acc)[N]) {
+  float top = 0;
+#pragma unroll
+  for (int r = 0; r < 16; r++) top = fmaxf(top, fabsf(x[r]));
+  top = half_max(top);
+  const bool over = top * up > 0x1p15f;
+  if (__any(over)) {
+    // top = m 2^e, m in [0.5, 1).  An infinity stays one.
+    const float fit = over && finite(top) ? __builtin_amdgcn_ldexpf(1.f, 12 - __builtin_amdgcn_frexp_expf(top)) : up;
+    const float keep = fit / up;
+    up = fit;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+#pragma unroll
+      for (int r = 0; r < 16; r++) acc[i][r] *= keep;
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < 16; r++) x[r] *= up;
 }
 
 template <typename T, int DP>
@@ -104,7 +107,7 @@ struct DqTile {
 
 template <typename T, int DP, bool CAREFUL>
 __device__ __forceinline__ void dq_walk(const Attend &a, const T *__restrict__ k, const T *__restrict__ v, int first,
-                                        int end, int2 mine, float2 ld, float gs, int wlo, int whi, int full_lo,
+                                        int end, int2 mine, float2 ld, float &up, int wlo, int whi, int full_lo,
                                         int full_hi, const V8<T> (&qf)[DP / 16], const V8<T> (&gf)[DP / 16], T *ks,
                                         T *vs, uint32_t *bad, f32x16 (&acc)[DP / 32]) {
   constexpr int BN = DqTile<T, DP>::BN;
@@ -133,7 +136,7 @@ __device__ __forceinline__ void dq_walk(const Attend &a, const T *__restrict__ k
             dp = mma(L::row_frag(vb, 32 * b + col, 16 * i + 8 * h), gf[i], dp);
           }
 #pragma unroll
-          for (int r = 0; r < 16; r++) s[r] = exp2_fast(fmaf(s[r], a.c, -ld.x)) * ((dp[r] - ld.y) * gs);
+          for (int r = 0; r < 16; r++) s[r] = exp2_fast(fmaf(s[r], a.c, -ld.x)) * (dp[r] - ld.y);
           if (!whole) {
 #pragma unroll
             for (int r = 0; r < 16; r++) {
@@ -143,6 +146,7 @@ __device__ __forceinline__ void dq_walk(const Attend &a, const T *__restrict__ k
               s[r] = in ? s[r] : 0.f;
             }
           }
+          if constexpr (kFitted<T>) fit_column(s, up, acc);
 #pragma unroll
           for (int i = 0; i < 2; i++) {
             const V8<T> ds = acc_frag<T>(s, i);
@@ -157,7 +161,7 @@ __device__ __forceinline__ void dq_walk(const Attend &a, const T *__restrict__ k
             const float t = frag_dot<T, DP>(qf, ks + SIZE, r, h) * a.c;
             const float dp = frag_dot<T, DP>(gf, vs + SIZE, r, h);
             if (key >= mine.x && key < mine.y)
-              add_row<T, DP>(acc, exp2_fast(t - ld.x) * (dp - ld.y) * gs, ks + SIZE, r, h);
+              add_row<T, DP>(acc, exp2_fast(t - ld.x) * (dp - ld.y) * up, ks + SIZE, r, h);
           }
         }
       });
@@ -191,7 +195,6 @@ struct DqLds {
   alignas(16) T vs[N];
   uint32_t bad[2];
   int lo[4], hi[4], redo;
-  float max[4];
 };
 
 // One workgroup's rows.  True: something was not finite, and nothing was stored.
@@ -247,7 +250,7 @@ __device__ __forceinline__ bool dq_rows(const Attend &a, const Grad &g, const Gr
   const int full_lo = max_over(mine.x), full_hi = min_over(mine.y);
   const T *kh = (const T *)p.k + head * a.k.head, *vh = (const T *)p.v + head * a.v.head;
   f32x16 acc[DP / 32] = {};
-  float gs = 1;
+  float up = kFitted<T> ? kMostUp : 1.f;
   if constexpr (kDirect<T, DP>) {
     int begin = wlo, end = whi;
     if (begin >= end) begin = end = 0;
@@ -261,13 +264,12 @@ __device__ __forceinline__ bool dq_rows(const Attend &a, const Grad &g, const Gr
     }
     if (CAREFUL) __syncthreads();  // everyone has read lds.redo
     if (threadIdx.x == 0) lds.redo = 0;
-    gs = grad_scale<T>(g, lds.max);
     __syncthreads();
     int begin = uniform(min(min(lds.lo[0], lds.lo[1]), min(lds.lo[2], lds.lo[3])));
     int end = uniform(max(max(lds.hi[0], lds.hi[1]), max(lds.hi[2], lds.hi[3])));
     if (begin >= end) begin = end = 0;
     if (p.part && !dq_split(p, begin, end, DqTile<T, DP>::BN)) return false;
-    dq_walk<T, DP, CAREFUL>(a, kh, vh, begin, end, mine, ld, gs, wlo, whi, full_lo, full_hi, qf, gf, lds.ks, lds.vs,
+    dq_walk<T, DP, CAREFUL>(a, kh, vh, begin, end, mine, ld, up, wlo, whi, full_lo, full_hi, qf, gf, lds.ks, lds.vs,
                             lds.bad, acc);
     if (!CAREFUL) {
       if (!all_finite(acc)) lds.redo = 1;
@@ -278,9 +280,9 @@ __device__ __forceinline__ bool dq_rows(const Attend &a, const Grad &g, const Gr
   if (!live) return false;
   if (p.part) {
     const int64_t all = (int64_t)a.nq * heads;
-    store_cols<float, DP>(p.part + (blockIdx.y * all + at) * a.dim, acc, a.scale / gs, h, a.dim);
+    store_cols<float, DP>(p.part + (blockIdx.y * all + at) * a.dim, acc, a.scale / up, h, a.dim);
   } else {
-    store_cols<T, DP>((T *)p.dq + at * a.dim, acc, a.scale / gs, h, a.dim);
+    store_cols<T, DP>((T *)p.dq + at * a.dim, acc, a.scale / up, h, a.dim);
   }
   return false;
 }
@@ -319,7 +321,7 @@ struct DkvTile {
 template <typename T, int DP, bool CAREFUL>
 __device__ __forceinline__ void dkv_walk(const Attend &a, const Grad &g, const T *__restrict__ q, Heads gst,
                                          const T *__restrict__ go, int head, int begin, int end, Range rows,
-                                         int tiles, int key0, float gs,
+                                         int tiles, int key0, float &up_k,
                                          const V8<T> (&kf)[DP / 16], const V8<T> (&vf)[DP / 16], T *qs, T *os,
                                          float2 *s_ld, int2 *s_range, uint32_t *bad, f32x16 (&dk)[DP / 32],
                                          f32x16 (&dv)[DP / 32]) {
@@ -368,7 +370,7 @@ __device__ __forceinline__ void dkv_walk(const Attend &a, const Grad &g, const T
           for (int r = 0; r < 16; r++) {
             const float2 x = s_ld[slot + 32 * b + acc_row(r, h)];
             s[r] = exp2_fast(fmaf(s[r], a.c, -x.x));
-            dp[r] = s[r] * ((dp[r] - x.y) * gs);
+            dp[r] = s[r] * (dp[r] - x.y);
           }
           if (!whole) {
 #pragma unroll
@@ -380,6 +382,7 @@ __device__ __forceinline__ void dkv_walk(const Attend &a, const Grad &g, const T
               dp[r] = in ? dp[r] : 0.f;
             }
           }
+          if constexpr (kFitted<T>) fit_column(dp, up_k, dk);
 #pragma unroll
           for (int i = 0; i < 2; i++) {
             const V8<T> p = acc_frag<T>(s, i), ds = acc_frag<T>(dp, i);
@@ -399,7 +402,7 @@ __device__ __forceinline__ void dkv_walk(const Attend &a, const Grad &g, const T
             if (key >= kr.x && key < kr.y) {
               const float p = exp2_fast(t - x.x);
               add_row<T, DP>(dv, p, os + SIZE, r, h);
-              add_row<T, DP>(dk, p * (dpx - x.y) * gs, qs + SIZE, r, h);
+              add_row<T, DP>(dk, p * (dpx - x.y) * up_k, qs + SIZE, r, h);
             }
           }
         }
@@ -430,7 +433,6 @@ struct DkvLds {
   int2 range[2 * BQ];
   uint32_t bad[2];
   int redo;
-  float max[4];
 };
 
 // One workgroup's keys.  True: something was not finite, and nothing was stored.
@@ -464,7 +466,7 @@ __device__ __forceinline__ bool dkv_keys(const Attend &a, const Grad &g, const G
     vf[i] = global_frag(vrow, live, 16 * i + 8 * h, a.dim);
   }
   f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
-  float gs = 1;
+  float up_k = kFitted<T> ? kMostUp : 1.f;
   if constexpr (kDirect<T, DP>) {
     const float2 *ld = g.ld + head * a.group;
     dkv_walk32<DP, CAREFUL>(a, qh, gst, gh, ld, heads, g.range, begin, end, rows, tiles, key0, kf, vf, lds.qs, lds.os,
@@ -473,9 +475,8 @@ __device__ __forceinline__ bool dkv_keys(const Attend &a, const Grad &g, const G
   } else {
     if (CAREFUL) __syncthreads();  // everyone has read lds.redo
     if (threadIdx.x == 0) lds.redo = 0;
-    gs = grad_scale<T>(g, lds.max);
     __syncthreads();
-    dkv_walk<T, DP, CAREFUL>(a, g, qh, gst, gh, head, begin, end, rows, tiles, key0, gs, kf, vf, lds.qs, lds.os, lds.ld,
+    dkv_walk<T, DP, CAREFUL>(a, g, qh, gst, gh, head, begin, end, rows, tiles, key0, up_k, kf, vf, lds.qs, lds.os, lds.ld,
                              lds.range, lds.bad, dk, dv);
     if (!CAREFUL) {
       if (!(all_finite(dk) && all_finite(dv))) lds.redo = 1;
@@ -487,11 +488,11 @@ __device__ __forceinline__ bool dkv_keys(const Attend &a, const Grad &g, const G
   const int64_t at = ((int64_t)key * a.kv_heads + head) * a.dim;
   if (p.part) {
     const int64_t all = (int64_t)a.nk * a.kv_heads * a.dim;
-    store_cols<float, DP>(p.part + 2 * blockIdx.y * all + at, dk, a.scale / gs, h, a.dim);
+    store_cols<float, DP>(p.part + 2 * blockIdx.y * all + at, dk, a.scale / up_k, h, a.dim);
     store_cols<float, DP>(p.part + (2 * blockIdx.y + 1) * all + at, dv, 1.f, h, a.dim);
     return false;
   }
-  store_cols<T, DP>((T *)p.dk + at, dk, a.scale / gs, h, a.dim);
+  store_cols<T, DP>((T *)p.dk + at, dk, a.scale / up_k, h, a.dim);
   store_cols<T, DP>((T *)p.dv + at, dv, 1.f, h, a.dim);
   return false;
 }
@@ -548,11 +549,10 @@ static int dkv_splits(kl_dtype dtype, int64_t nq, int64_t nk, int kv_heads, int 
 // lanes per (row, head) of the first kernel: 16 bytes each
 static int prep_lanes(kl_dtype dtype, int dim) { return dim * (dtype == KL_F32 ? 4 : 2) / 16; }
 
-// Its workgroups: one per kItems * groups (row, head)s; f16: at most kMaxParts partial maxima
+// Its workgroups: one per kItems * groups (row, head)s
 static unsigned prep_blocks(kl_dtype dtype, int64_t num_q, int heads, int dim) {
   const int lanes = prep_lanes(dtype, dim), pow2 = lanes <= 4 ? 4 : lanes <= 8 ? 8 : lanes <= 16 ? 16 : 32;
-  const int64_t blocks = cdiv(num_q * heads, (int64_t)kItems * (256 / pow2));
-  return (unsigned)std::max<int64_t>(1, dtype == KL_F16 ? std::min<int64_t>(blocks, kMaxParts) : blocks);
+  return (unsigned)std::max<int64_t>(1, cdiv(num_q * heads, (int64_t)kItems * (256 / pow2)));
 }
 
 template <typename F>
@@ -608,7 +608,7 @@ extern "C" size_t kl_pack_attention_bwd_workspace_bytes(kl_dtype dtype, int64_t 
   if (num_q < 0 || num_k < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || dim <= 0) return 256;
   const int splits = dkv_splits(dtype, num_q, num_k, kv_heads, heads / kv_heads, dim);
   const int dq = dq_splits(dtype, num_q, num_k, kv_heads, heads / kv_heads, dim);
-  return al256((size_t)num_q * heads * 8) + al256((size_t)num_q * 8) + kMaxParts * 4 +
+  return al256((size_t)num_q * heads * 8) + al256((size_t)num_q * 8) +
          std::max(splits > 1 ? (size_t)2 * splits * num_k * kv_heads * dim * 4 : 0,
                   dq > 1 ? (size_t)dq * num_q * heads * dim * 4 + (size_t)cdiv(num_q * (heads / kv_heads), 32) * kv_heads * 4 : 0);
 }
@@ -627,22 +627,22 @@ extern "C" int kl_pack_attention_backward(kl_dtype dtype, int64_t num_q, int64_t
   KL_REQUIRE((grad_k == nullptr) == (grad_v == nullptr), "pack_attention: grad_k and grad_v go together");
   float2 *ld = (float2 *)ws;
   int2 *range = (int2 *)((char *)ws + al256((size_t)num_q * heads * 8));
-  float *amax = (float *)((char *)range + al256((size_t)num_q * 8));
-  const Grad g = {ld, range, amax, num_q > 0 ? (int)prep_blocks(dtype, num_q, heads, dim) : 0};
+  float *part = (float *)((char *)range + al256((size_t)num_q * 8));
+  const Grad g = {ld, range};
   return with_type(dtype, "pack_attention", [&](auto t) -> int {
     using T = decltype(t);
     if (num_q > 0 && !(is_direct(dtype, dim) && grad_q)) {
       KL_CHECK_RC(with_prep_lanes(prep_lanes(dtype, dim), [&](auto lanes) -> int {
-        hipLaunchKernelGGL((attend_prep_kernel<T, decltype(lanes)::value>), dim3(g.parts), dim3(256), 0, S(stream), a,
-                           (const T *)out, sizeof(T) == 2 ? (const T *)out_low : (const T *)nullptr,
-                           (const T *)grad_out, lse, ld, range, amax);
+        hipLaunchKernelGGL((attend_prep_kernel<T, decltype(lanes)::value>),
+                           dim3(prep_blocks(dtype, num_q, heads, dim)), dim3(256), 0, S(stream), a, (const T *)out,
+                           sizeof(T) == 2 ? (const T *)out_low : (const T *)nullptr, (const T *)grad_out, lse, ld, range);
         KL_CHECK_LAUNCH();
         return KL_OK;
       }));
     }
     return with_dim(dim, [&](auto dp) {
-      return attend_backward<T, decltype(dp)::value>(a, g, q, k, v, grad_out, grad_q, grad_k, grad_v, amax + kMaxParts,
-                                                     out, lse, S(stream));
+      return attend_backward<T, decltype(dp)::value>(a, g, q, k, v, grad_out, grad_q, grad_k, grad_v, part, out, lse,
+                                                     S(stream));
     });
   });
 }
