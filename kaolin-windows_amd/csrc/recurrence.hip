@@ -13,11 +13,13 @@
 // Bound by memory: a and b are read 1 + (share of 1) times and h is written once.  Step 3 takes the chunks in the
 // other order, so that it finds what 1 read last in the 256 MB cache.  One pass, with workgroups that publish and
 // await each other's (A, B), measured no faster: it reads less, but waits.
-// 311,000 rows of 64 columns, float, packs of 38 rows: forward 25 + 7 + 40 us (239 MB at least, 47 us at the rate of
-// a copy), backward 24 + 7 + 67 us (397 MB, 79 us); 65,537 x 1024, bf16, two packs: 68 + 11 + 70 and
-// 58 + 11 + 121 us (403 MB, 80 us, and 671 MB, 133 us).
+// 311,000 rows of 64 columns, float, packs of 38 rows: forward 24 + 9 + 40 us (239 MB at least, 47 us at the rate of
+// a copy), backward 26 + 9 + 67 us (397 MB, 79 us); 65,537 x 1024, bf16, two packs: 68 + 13 + 72 and
+// 60 + 13 + 124 us (403 MB, 80 us, and 671 MB, 133 us).
 //
-// States, A and B are in 32 bits (64 for double); outputs are rounded once.
+// States, A and B are in 32 bits (64 for double); outputs are rounded once.  A is a product of gates alone, and may pass a
+// float's range both ways where the states that it meets do not (they are 0, or small, or other gates undo it): it has
+// an exponent of its own (Gain).
 // Backward: g[t] = dh[t] + a[t+1] g[t+1] is the same recurrence in the other direction with the gate of the
 // row walked before; db = g, da[t] = g[t] h[t-1] with h as it was rounded, dinitial = a g at the first row.
 #include "seqcommon.h"
@@ -51,6 +53,36 @@ __device__ __forceinline__ void store_pack(T *p, const Pack<T, V> &x) {
   __builtin_memcpy(p, x.v, sizeof(T) * V);
 }
 
+// A = m 2^e with |m| in [0.5, 1), 0 or not finite; stored with 16 bits of exponent (near_exponent).  Against products in
+// a float: the scan of 65,537 x 1024 in bf16 13 us for 10.4, the whole of it 358 for 351; 8192 rows of one pack, which
+// fold up to 64 segments, 46 for 39.
+__device__ __forceinline__ float mantissa(float x) { return __builtin_amdgcn_frexp_mantf(x); }
+__device__ __forceinline__ double mantissa(double x) { return __builtin_amdgcn_frexp_mant(x); }
+__device__ __forceinline__ int exponent(float x) { return __builtin_amdgcn_frexp_expf(x); }
+__device__ __forceinline__ int exponent(double x) { return __builtin_amdgcn_frexp_exp(x); }
+__device__ __forceinline__ float times_two_to(float x, int e) { return __builtin_amdgcn_ldexpf(x, e); }
+__device__ __forceinline__ double times_two_to(double x, int e) { return __builtin_amdgcn_ldexp(x, e); }
+template <typename S>
+struct Gain {
+  S m;
+  int e;
+  __device__ __forceinline__ void take(S gate) {  // up to 64 gates, then settle(): m stays over 2^-65
+    m *= mantissa(gate);
+    e += exponent(gate);
+  }
+  __device__ __forceinline__ void settle() {
+    e += exponent(m);
+    m = mantissa(m);
+  }
+  // the gains of rows before this one's as well
+  __device__ __forceinline__ Gain after(const Gain &before) const {
+    Gain g = {m * before.m, e + before.e};
+    g.settle();
+    return g;
+  }
+  __device__ __forceinline__ S of(S state, S add) const { return times_two_to(m * state, e) + add; }
+};
+
 struct Recur {
   int n, chunk, chunks, packs, down;  // chunk: rows of one; packs: rows of initial; down: rows descend
   int64_t dim, cols;                  // cols: pieces across
@@ -78,19 +110,44 @@ constexpr int kSegmentLog = 8, kSegment = 64 * kRunChunks;
 static_assert(kSegment == 1 << kSegmentLog, "a segment of step 2");
 constexpr int kFewSegments = 64;  // what a wave's lanes can look through at once
 
-// (A, B) of chunks and segments: a and b (count, dim), resets (count)
+// (A, B) of chunks and segments: A = a 2^e and b (count, dim), resets (count)
 template <typename S>
 struct Composed {
   S *a, *b;
+  int16_t *e;
   int32_t *resets;
 };
+template <typename S>
+struct ComposedIn {
+  const S *a, *b;
+  const int16_t *e;
+  const int32_t *resets;
+};
+
+// No state but 0 comes through a gain that far, either way, and stays in its type's range: exponents stop there.
+constexpr int kFarExponent = 1 << 14;
+__device__ __forceinline__ int16_t near_exponent(int e) { return (int16_t)min(max(e, -kFarExponent), kFarExponent); }
+
+template <int V, typename S>
+__device__ __forceinline__ void store_gains(const Composed<S> &m, int64_t at, const Gain<S> (&g)[V]) {
+  Pack<S, V> a;
+  Pack<int16_t, V> e;
+#pragma unroll
+  for (int v = 0; v < V; v++) {
+    a.v[v] = g[v].m;
+    e.v[v] = near_exponent(g[v].e);
+  }
+  store_pack<V>(m.a + at, a);
+  store_pack<V>(m.e + at, e);
+}
 
 // (A, B) of rows [begin, end) of a piece of columns from the start of their last pack on, or of all of them.  True: a
 // pack (or rows of none) starts there.
 template <typename T, int V, bool GRAD>
 __device__ __forceinline__ bool recur_compose(const Recur &r, const T *__restrict__ a, const T *__restrict__ x,
                                               const T *__restrict__ init, int64_t begin, int64_t end, int64_t col,
-                                              typename StateOf<T>::S (&gain)[V], typename StateOf<T>::S (&state)[V]) {
+                                              Gain<typename StateOf<T>::S> (&gain)[V],
+                                              typename StateOf<T>::S (&state)[V]) {
   using S = typename StateOf<T>::S;
   using P = Pack<T, V>;
   auto at = [&](const T *p, int64_t i) { return load_pack<V>(p + r.row(i) * r.dim + col); };
@@ -99,7 +156,7 @@ __device__ __forceinline__ bool recur_compose(const Recur &r, const T *__restric
   const bool reset = start >= begin;
 #pragma unroll
   for (int v = 0; v < V; v++) {
-    gain[v] = reset ? 0 : 1;
+    gain[v] = {(S)(reset ? 0 : 1), 0};
     state[v] = 0;
   }
   int64_t i = max(begin, start);
@@ -129,10 +186,12 @@ __device__ __forceinline__ bool recur_compose(const Recur &r, const T *__restric
       for (int v = 0; v < V; v++) {
         const S g = (S)av[u].v[v], next = fma(g, state[v], (S)xv[u].v[v]);
         state[v] = in ? next : state[v];
-        gain[v] = in && !reset ? gain[v] * g : gain[v];
+        gain[v].take(in ? g : (S)1);
       }
     }
   }
+#pragma unroll
+  for (int v = 0; v < V; v++) gain[v].settle();
   return reset;
 }
 
@@ -145,9 +204,10 @@ __global__ void __launch_bounds__(256) recur_chunk_kernel(Recur r, const T *__re
   const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x, c = t / r.cols, piece = t - c * r.cols, col = r.column<V>(piece);
   if (c >= r.chunks) return;
   const int64_t begin = c * r.chunk, end = min((int64_t)r.n, begin + r.chunk);
-  Pack<S, V> gain, state;
-  const bool reset = recur_compose<T, V, GRAD>(r, a, x, init, begin, end, col, gain.v, state.v);
-  store_pack<V>(chunks.a + c * r.dim + col, gain);
+  Gain<S> gain[V];
+  Pack<S, V> state;
+  const bool reset = recur_compose<T, V, GRAD>(r, a, x, init, begin, end, col, gain, state.v);
+  store_gains<V>(chunks, c * r.dim + col, gain);
   store_pack<V>(chunks.b + c * r.dim + col, state);
   if (piece == 0) chunks.resets[c] = reset;
 }
@@ -157,27 +217,31 @@ __global__ void __launch_bounds__(256) recur_chunk_kernel(Recur r, const T *__re
 template <typename S>
 __global__ void __launch_bounds__(1024) recur_scan_kernel(Recur r, Composed<S> chunks, int32_t *__restrict__ before,
                                                         Composed<S> segments) {
-  __shared__ S s_a[1024], s_b[1024];
+  __shared__ S s_b[1024];
+  __shared__ Gain<S> s_a[1024];
   __shared__ int s_reset[1024];
   const int me = threadIdx.x;
   const int64_t col = (int64_t)blockIdx.x * 16 + me % 16, at = min(col, r.dim - 1);
   const int c0 = blockIdx.y * kSegment + me / 16 * kRunChunks;
-  S a[kRunChunks], b[kRunChunks], ga = 1, gb = 0;
+  const Gain<S> one = {1, 0}, none = {0, 0};
+  Gain<S> a[kRunChunks], ga = one;
+  S b[kRunChunks], gb = 0;
   int z[kRunChunks], reset = 0;
 #pragma unroll
   for (int k = 0; k < kRunChunks; k++) {
     const bool in = c0 + k < r.chunks;
     const int64_t from = (int64_t)(in ? c0 + k : 0) * r.dim + at;
-    a[k] = in ? chunks.a[from] : (S)1;
+    a[k] = in ? Gain<S>{chunks.a[from], chunks.e[from]} : one;
     b[k] = in ? chunks.b[from] : (S)0;
     z[k] = in ? chunks.resets[c0 + k] : 0;
   }
-#pragma unroll
-  for (int k = 0; k < kRunChunks; k++) {
-    gb = z[k] ? b[k] : fma(a[k], gb, b[k]);
-    ga = z[k] ? (S)0 : ga * a[k];
+  auto step = [&](int k) {
+    gb = z[k] ? b[k] : a[k].of(gb, b[k]);
+    ga = z[k] ? none : a[k].after(ga);
     reset |= z[k];
-  }
+  };
+#pragma unroll
+  for (int k = 0; k < kRunChunks; k++) step(k);
   // inclusive over the runs in doubling steps
   for (int off = 16; off < 1024; off *= 2) {
     s_a[me] = ga;
@@ -185,9 +249,9 @@ __global__ void __launch_bounds__(1024) recur_scan_kernel(Recur r, Composed<S> c
     s_reset[me] = reset;
     __syncthreads();
     if (me >= off && !reset) {
-      gb = fma(ga, s_b[me - off], gb);
+      gb = ga.of(s_b[me - off], gb);
       reset = s_reset[me - off];
-      ga = reset ? (S)0 : ga * s_a[me - off];
+      ga = reset ? none : ga.after(s_a[me - off]);
     }
     __syncthreads();
   }
@@ -196,11 +260,13 @@ __global__ void __launch_bounds__(1024) recur_scan_kernel(Recur r, Composed<S> c
   s_reset[me] = reset;
   __syncthreads();
   if (col < r.dim && me >= 1008) {
-    segments.a[(int64_t)blockIdx.y * r.dim + col] = ga;
-    segments.b[(int64_t)blockIdx.y * r.dim + col] = gb;
+    const int64_t to = (int64_t)blockIdx.y * r.dim + col;
+    segments.a[to] = ga.m;
+    segments.e[to] = near_exponent(ga.e);
+    segments.b[to] = gb;
     if (col == 0) segments.resets[blockIdx.y] = reset;
   }
-  ga = me >= 16 ? s_a[me - 16] : (S)1;
+  ga = me >= 16 ? s_a[me - 16] : one;
   gb = me >= 16 ? s_b[me - 16] : (S)0;
   reset = me >= 16 ? s_reset[me - 16] : 0;
   if (col >= r.dim) return;
@@ -208,12 +274,11 @@ __global__ void __launch_bounds__(1024) recur_scan_kernel(Recur r, Composed<S> c
   for (int k = 0; k < kRunChunks; k++) {
     if (c0 + k >= r.chunks) break;
     const int64_t to = (int64_t)(c0 + k) * r.dim + col;
-    chunks.a[to] = ga;
+    chunks.a[to] = ga.m;
+    chunks.e[to] = near_exponent(ga.e);
     chunks.b[to] = gb;
     if (col == 0) before[c0 + k] = reset;
-    gb = z[k] ? b[k] : fma(a[k], gb, b[k]);
-    ga = z[k] ? (S)0 : ga * a[k];
-    reset |= z[k];
+    step(k);
   }
 }
 
@@ -228,16 +293,21 @@ __global__ void __launch_bounds__(256) recur_segment_kernel(Recur r, const T *__
                                                           int32_t *__restrict__ before,
                                                           Composed<typename StateOf<T>::S> segments) {
   using S = typename StateOf<T>::S;
-  __shared__ Pack<S, V> s_a[256], s_b[256];
+  struct Gains {
+    Gain<S> v[V];
+  };
+  __shared__ Gains s_a[256];
+  __shared__ Pack<S, V> s_b[256];
   __shared__ int s_reset[256];
   const int me = threadIdx.x, w = 1 << r.wide;
   const int64_t c = (int64_t)blockIdx.y * (256 >> r.wide) + (me >> r.wide);
   const int64_t piece = (int64_t)blockIdx.x * w + (me & (w - 1)), col = r.column<V>(piece);
   const bool live = c < r.chunks && piece < r.cols;
-  Pack<S, V> ga, gb;
+  Gains ga;
+  Pack<S, V> gb;
 #pragma unroll
   for (int v = 0; v < V; v++) {
-    ga.v[v] = 1;
+    ga.v[v] = {1, 0};
     gb.v[v] = 0;
   }
   int reset = 0;
@@ -253,12 +323,13 @@ __global__ void __launch_bounds__(256) recur_segment_kernel(Recur r, const T *__
       s_reset[me] = reset;
       __syncthreads();
       if (me >= off && !reset) {
-        const Pack<S, V> pa = s_a[me - off], pb = s_b[me - off];
+        const Gains pa = s_a[me - off];
+        const Pack<S, V> pb = s_b[me - off];
         reset = s_reset[me - off];
 #pragma unroll
         for (int v = 0; v < V; v++) {
-          gb.v[v] = fma(ga.v[v], pb.v[v], gb.v[v]);
-          ga.v[v] = reset ? (S)0 : ga.v[v] * pa.v[v];
+          gb.v[v] = ga.v[v].of(pb.v[v], gb.v[v]);
+          ga.v[v] = reset ? Gain<S>{0, 0} : ga.v[v].after(pa.v[v]);
         }
       }
       __syncthreads();
@@ -269,17 +340,17 @@ __global__ void __launch_bounds__(256) recur_segment_kernel(Recur r, const T *__
   s_reset[me] = reset;
   __syncthreads();
   if (piece < r.cols && me >= 256 - w) {
-    store_pack<V>(segments.a + (int64_t)blockIdx.y * r.dim + col, ga);
+    store_gains<V>(segments, (int64_t)blockIdx.y * r.dim + col, ga.v);
     store_pack<V>(segments.b + (int64_t)blockIdx.y * r.dim + col, gb);
     if (piece == 0) segments.resets[blockIdx.y] = reset;
   }
   if (!live) return;
 #pragma unroll
   for (int v = 0; v < V; v++) {
-    ga.v[v] = me >= w ? s_a[me - w].v[v] : (S)1;
+    ga.v[v] = me >= w ? s_a[me - w].v[v] : Gain<S>{1, 0};
     gb.v[v] = me >= w ? s_b[me - w].v[v] : (S)0;
   }
-  store_pack<V>(chunks.a + c * r.dim + col, ga);
+  store_gains<V>(chunks, c * r.dim + col, ga.v);
   store_pack<V>(chunks.b + c * r.dim + col, gb);
   if (piece == 0) before[c] = me >= w ? s_reset[me - w] : 0;
 }
@@ -366,9 +437,9 @@ __device__ __forceinline__ void recur_walk(const Recur &r, const T *__restrict__
 template <typename T, int V, bool GRAD>
 __global__ void __launch_bounds__(256) recur_write_kernel(Recur r, const T *__restrict__ a, const T *__restrict__ x,
                                                         const T *__restrict__ h, const T *__restrict__ init,
-                                                        Composed<const typename StateOf<T>::S> chunks,
+                                                        ComposedIn<typename StateOf<T>::S> chunks,
                                                         const int32_t *__restrict__ chunk_before,
-                                                        Composed<const typename StateOf<T>::S> segments,
+                                                        ComposedIn<typename StateOf<T>::S> segments,
                                                         T *__restrict__ out, T *__restrict__ da,
                                                         T *__restrict__ dinit) {
   using S = typename StateOf<T>::S;
@@ -388,11 +459,14 @@ __global__ void __launch_bounds__(256) recur_write_kernel(Recur r, const T *__re
 #pragma unroll
   for (int v = 0; v < V; v++) state[v] = 0;
   if (carried) {
-    auto step = [&](const Composed<const S> &m, int64_t k, bool reset) {
-      const Pack<S, V> ka = load_pack<V>(m.a + k * r.dim + col);
-      const Pack<S, V> kb = load_pack<V>(m.b + k * r.dim + col);
+    auto step = [&](const ComposedIn<S> &m, int64_t k, bool reset) {
+      const Pack<S, V> ka = load_pack<V>(m.a + k * r.dim + col), kb = load_pack<V>(m.b + k * r.dim + col);
+      const Pack<int16_t, V> ke = load_pack<V>(m.e + k * r.dim + col);
 #pragma unroll
-      for (int v = 0; v < V; v++) state[v] = reset ? kb.v[v] : fma(ka.v[v], state[v], kb.v[v]);
+      for (int v = 0; v < V; v++) {
+        const S with = Gain<S>{ka.v[v], ke.v[v]}.of(state[v], kb.v[v]);
+        state[v] = reset ? kb.v[v] : with;
+      }
     };
     const bool here = chunk_before[c] != 0;
     if (!here) {
@@ -404,10 +478,12 @@ __global__ void __launch_bounds__(256) recur_write_kernel(Recur r, const T *__re
         constexpr int kFold = V >= 4 ? 4 : 8;  // loads in flight together
         for (; k < mine; k += kFold) {
           Pack<S, V> ka[kFold], kb[kFold];
+          Pack<int16_t, V> ke[kFold];
 #pragma unroll
           for (int u = 0; u < kFold; u++) {
             const int64_t at = min(k + u, mine - 1) * r.dim + col;
             ka[u] = load_pack<V>(segments.a + at);
+            ke[u] = load_pack<V>(segments.e + at);
             kb[u] = load_pack<V>(segments.b + at);
           }
 #pragma unroll
@@ -415,7 +491,7 @@ __global__ void __launch_bounds__(256) recur_write_kernel(Recur r, const T *__re
             const bool in = k + u < mine, reset = marks >> ((k + u) & 63) & 1;
 #pragma unroll
             for (int v = 0; v < V; v++) {
-              const S with = fma(ka[u].v[v], state[v], kb[u].v[v]);
+              const S with = Gain<S>{ka[u].v[v], ke[u].v[v]}.of(state[v], kb[u].v[v]);
               state[v] = !in ? state[v] : reset ? kb[u].v[v] : with;
             }
           }
@@ -443,18 +519,21 @@ __global__ void __launch_bounds__(kShortRows) recur_short_kernel(Recur r, const 
                                                          T *__restrict__ dinit) {
   using S = typename StateOf<T>::S;
   constexpr int kWaves = kShortRows / 64;
-  __shared__ S s_a[kWaves][V], s_b[kWaves][V];
+  __shared__ Gain<S> s_a[kWaves][V];
+  __shared__ S s_b[kWaves][V];
   __shared__ int s_reset[kWaves];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int64_t col = r.column<V>(blockIdx.x);
   const int64_t begin = threadIdx.x, end = begin + 1;
   const bool live = begin < r.n, carried = live && r.carried(begin);
-  S ga[V], gb[V];
+  Gain<S> ga[V];
+  S gb[V];
 #pragma unroll
   for (int v = 0; v < V; v++) {
-    ga[v] = 1;
+    ga[v] = {1, 0};
     gb[v] = 0;
   }
+  auto shifted = [](const Gain<S> &g, int off) { return Gain<S>{__shfl_up(g.m, off), __shfl_up(g.e, off)}; };
   int reset = 0;
   if (live) reset = recur_compose<T, V, GRAD>(r, a, x, init, begin, end, col, ga, gb);
   const bool needed = __any(carried);  // a thread whose state is not carried has a reset
@@ -465,9 +544,10 @@ __global__ void __launch_bounds__(kShortRows) recur_short_kernel(Recur r, const 
       const bool in = lane >= off && !reset;
 #pragma unroll
       for (int v = 0; v < V; v++) {
-        const S pa = __shfl_up(ga[v], off), pb = __shfl_up(gb[v], off);
-        gb[v] = in ? fma(ga[v], pb, gb[v]) : gb[v];
-        ga[v] = in ? (before ? (S)0 : ga[v] * pa) : ga[v];
+        const Gain<S> pa = shifted(ga[v], off);
+        const S pb = __shfl_up(gb[v], off);
+        gb[v] = in ? ga[v].of(pb, gb[v]) : gb[v];
+        ga[v] = in ? (before ? Gain<S>{0, 0} : ga[v].after(pa)) : ga[v];
       }
       reset = in ? before : reset;
     }
@@ -487,12 +567,13 @@ __global__ void __launch_bounds__(kShortRows) recur_short_kernel(Recur r, const 
   if (needed) {
     for (int w = 0; w < wave; w++) {
 #pragma unroll
-      for (int v = 0; v < V; v++) state[v] = s_reset[w] ? s_b[w][v] : fma(s_a[w][v], state[v], s_b[w][v]);
+      for (int v = 0; v < V; v++) state[v] = s_reset[w] ? s_b[w][v] : s_a[w][v].of(state[v], s_b[w][v]);
     }
     const int before = __shfl_up(reset, 1);
 #pragma unroll
     for (int v = 0; v < V; v++) {
-      const S pa = __shfl_up(ga[v], 1), pb = __shfl_up(gb[v], 1), with = before ? pb : fma(pa, state[v], pb);
+      const Gain<S> pa = shifted(ga[v], 1);
+      const S pb = __shfl_up(gb[v], 1), with = before ? pb : pa.of(state[v], pb);
       state[v] = lane > 0 ? with : state[v];
     }
   }
@@ -539,6 +620,8 @@ struct RecurSpace {
     chunks.b = (S *)take(num_chunks * dim * sizeof(S));
     segments.a = (S *)take(num * dim * sizeof(S));
     segments.b = (S *)take(num * dim * sizeof(S));
+    chunks.e = (int16_t *)take(num_chunks * dim * 2);
+    segments.e = (int16_t *)take(num * dim * 2);
     chunks.resets = (int32_t *)take(num_chunks * 4);
     before = (int32_t *)take(num_chunks * 4);
     segments.resets = (int32_t *)take(num * 4);
@@ -579,9 +662,9 @@ static int recur_run(Recur r, const void *a, const void *x, const void *h, const
   }
   const dim3 grid((unsigned)cdiv((r.chunks + (dinit ? (int64_t)r.packs : 0)) * r.cols, 256));
   hipLaunchKernelGGL((recur_write_kernel<T, V, GRAD>), grid, dim3(256), 0, st, r, (const T *)a, (const T *)x,
-                     (const T *)h, (const T *)init, Composed<const S>{m.chunks.a, m.chunks.b, m.chunks.resets},
-                     m.before, Composed<const S>{m.segments.a, m.segments.b, m.segments.resets}, (T *)out, (T *)da,
-                     (T *)dinit);
+                     (const T *)h, (const T *)init, ComposedIn<S>{m.chunks.a, m.chunks.b, m.chunks.e, m.chunks.resets},
+                     m.before, ComposedIn<S>{m.segments.a, m.segments.b, m.segments.e, m.segments.resets}, (T *)out,
+                     (T *)da, (T *)dinit);
   KL_CHECK_LAUNCH();
   return KL_OK;
 }

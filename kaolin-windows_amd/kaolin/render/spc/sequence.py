@@ -200,7 +200,9 @@ def linear_recurrence(gates, feats, boundaries, initial=None, reverse=False):
         (Tensor): the states h (num_rows, dim).  Rows before the first pack are 0, and so are their gradients.
 
     States are carried in 32 bits (64 for f64) and rounded once each; a pack is never touched by another's
-    values.  Differentiable once, with respect to gates, feats and initial; the gradient of the gates takes the
+    values.  Gates may be any numbers: a state is off by some roundings of the recurrence of the magnitudes,
+    ``s[t] = |gates[t]| * s[t-1] + |feats[t]|``, and finite where that is.  From a row with an infinite gate on, a pack's
+    states are infinite or NaN.  Differentiable once, with respect to gates, feats and initial; the gradient of the gates takes the
     states as they were rounded.
     """
     ext = _ext.get() if gates.is_cuda else None

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from seq_util import attention, check, marks
+from seq_util import attention, check, marks, recurrence
 from seq_wide_util import attention_heads
 from test_sequence import DEV, TYPES, _leaf, _normal, spc  # noqa: F401
 
@@ -91,3 +91,67 @@ def test_attention_gradients_of_very_different_packs(spc, dtype, causal):
         check(name, x[clean], want[clean], tol[clean])
         if name != 'o':
             assert not torch.isfinite(x[~clean]).all()
+
+
+def _recurrence(spc, a, x, b, first=None, reverse=False, grad=None):
+    outs, tols = recurrence(a, x, b, first, reverse, grad=grad, dtype=a.dtype)
+    leaves = [_leaf(y) for y in (a, x, first)]
+    h = spc.linear_recurrence(leaves[0], leaves[1], b.to(DEV), initial=leaves[2], reverse=reverse)
+    got = [h, *torch.autograd.grad(h, [y for y in leaves if y is not None], grad.to(DEV))]
+    for name, y, want, tol in zip(('h', 'da', 'db', 'dinitial'), got, outs, tols):
+        assert torch.isfinite(want).all() and torch.isfinite(y).all(), name
+        check(name, y, want, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float64])
+@pytest.mark.parametrize('n,dim', [(200, 3), (700, 8), (3000, 40), (9000, 260)])  # one launch, segments, three launches
+@pytest.mark.parametrize('reverse', [False, True])
+def test_recurrence_gates_above_one_over_zeros(spc, dtype, n, dim, reverse):
+    """States that are exactly 0 stay so however long gates of 2 run over them, and so do the gradients that are 0."""
+    lens = [n // 2, n - n // 2]
+    b = marks(lens)
+    a, x, g = torch.full((n, dim), 2.0), torch.zeros(n, dim), torch.zeros(n, dim)
+    for at, m in zip((0, n // 2), lens):
+        rows = list(range(at, at + m))[::-1 if reverse else 1]
+        for i in range(6):  # features in the last rows that the states walk, gradients in the last that theirs do (the
+            x[rows[-6 + i]] = 0.5 + i  # first): 2^6 each, where from the other end they would grow to 2^m
+            g[rows[i]] = 1.0 - 0.25 * i
+    _recurrence(spc, a.to(dtype), x.to(dtype), b, None, reverse, g.to(dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype,step,low', [(torch.float32, 2.0 ** 12, 2.0 ** -100), (torch.bfloat16, 2.0 ** 12, 2.0 ** -100),
+                                            (torch.float64, 2.0 ** 100, 2.0 ** -800)])
+@pytest.mark.parametrize('n,dim', [(100, 3), (256, 8), (1500, 40), (9000, 260)])
+@pytest.mark.parametrize('reverse', [False, True])
+def test_recurrence_gates_that_take_turns(spc, dtype, step, low, n, dim, reverse):
+    """16 rows whose gates are large, then 16 that undo them: their products pass the type's range, the states, between
+    `low` and low * step ** 16, do not."""
+    walked = torch.arange(n).flip(0) if reverse else torch.arange(n)
+    up, few = walked // 16 % 2 == 0, walked % 32 == 0  # few: where states are smallest
+    a = torch.where(up[:, None], step, 1 / step).to(torch.float64).expand(n, dim)
+    x = torch.where(few[:, None], _normal(0, n, dim).double() * low * 2.0 ** -10, 0.0)
+    g, first = _normal(1, n, dim).double() * low, _normal(2, 1, dim).double() * low
+    _recurrence(spc, a.to(dtype), x.to(dtype), marks([n]), first.to(dtype), reverse, g.to(dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('n,dim', [(200, 3), (700, 8), (9000, 260)])
+def test_recurrence_infinite_gates_and_features(spc, n, dim):
+    """A pack with an infinite gate is not finite from that row on, one with an infinite feature infinite up to the
+    next gate of 0; rows before it and other packs are as without them."""
+    lens = [n // 2, n - n // 2]
+    b = marks(lens)
+    a, x = torch.sigmoid(_normal(0, n, dim) + 2), _normal(1, n, dim)
+    (want, *_), (tol, *_) = recurrence(a, x, b, dtype=torch.float32)
+    for where in (a, x):
+        keep = where[20].clone()
+        where[20] = math.inf
+        h = spc.linear_recurrence(a.to(DEV), x.to(DEV), b.to(DEV)).cpu()
+        check('h', h[:20], want[:20], tol[:20])
+        check('h', h[n // 2:], want[n // 2:], tol[n // 2:])
+        assert not torch.isfinite(h[20:n // 2]).any()
+        if where is x:
+            assert (h[20:n // 2] == math.inf).all()
+        where[20] = keep
