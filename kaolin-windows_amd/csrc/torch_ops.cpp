@@ -465,6 +465,13 @@ kl_dtype seq_code(at::ScalarType t) {
   return t == at::kFloat ? KL_F32 : t == at::kHalf ? KL_F16 : t == at::kBFloat16 ? KL_BF16 : KL_F64;
 }
 
+// Scratch of one call alone, from the allocator's pool of the call's stream.  Kernels of a call hand each other numbers
+// through it (counts that bound loops among them), and another host thread may launch on the same stream between
+// them: a backward runs on the engine's thread.
+at::Tensor scratch(size_t bytes, const at::Device &dev) {
+  return at::empty({(int64_t)std::max<size_t>(bytes, 16)}, at::TensorOptions().dtype(at::kByte).device(dev));
+}
+
 bool seq_float(const at::Tensor &t) {
   return t.scalar_type() == at::kFloat || t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16;
 }
@@ -506,7 +513,7 @@ Layout make_layout(const at::Tensor &boundaries, int64_t stream) {
   const int64_t n = boundaries.size(0);
   Layout l{at::empty({2 * n + 1}, boundaries.options().dtype(at::kInt))};
   const size_t bytes = kl_pack_layout_workspace_bytes(n);
-  at::Tensor ws = workspace(bytes, boundaries.device(), stream);
+  at::Tensor ws = scratch(bytes, boundaries.device());
   check(kl_pack_layout(n, (const uint8_t *)boundaries.data_ptr(), l.ids(), l.starts(), ws.data_ptr(), bytes,
                        (kl_stream)stream),
         "pack_layout");
@@ -519,7 +526,7 @@ std::pair<Layout, Layout> make_layouts(const at::Tensor &one, const at::Tensor &
   const auto ints = one.options().dtype(at::kInt);
   const Layout a{at::empty({2 * n + 1}, ints)}, b{at::empty({2 * m + 1}, ints)};
   const size_t bytes = kl_pack_layout_workspace_bytes(n) + kl_pack_layout_workspace_bytes(m);
-  at::Tensor ws = workspace(bytes, one.device(), stream);
+  at::Tensor ws = scratch(bytes, one.device());
   check(kl_pack_layout_pair(n, (const uint8_t *)one.data_ptr(), a.ids(), a.starts(), m, (const uint8_t *)two.data_ptr(),
                             b.ids(), b.starts(), ws.data_ptr(), bytes, (kl_stream)stream),
         "pack_layout_pair");
@@ -544,7 +551,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_forward(const at::Tenso
   }
   const int heads = (int)q.size(1), kv = (int)k.size(1), dim = (int)q.size(2);
   const size_t bytes = kl_pack_attention_workspace_bytes(code, q.size(0), k.size(0), heads, kv, dim);
-  at::Tensor ws = workspace(bytes, q.device(), stream);
+  at::Tensor ws = scratch(bytes, q.device());
   const HeadStrides st(q, k, v);
   check(kl_pack_attention_forward(code, q.size(0), k.size(0), heads, kv, dim, ptr(q), ptr(k), ptr(v), st.v, lq.ids(),
                                   lq.starts(), lk.ids(), lk.starts(), (float)scale, causal, ptr(out), ptr(low),
@@ -579,7 +586,7 @@ struct PackAttention : public torch::autograd::Function<PackAttention> {
     const kl_dtype code = seq_code(q.scalar_type());
     const int heads = (int)q.size(1), kv = (int)k.size(1), dim = (int)q.size(2);
     const size_t bytes = kl_pack_attention_bwd_workspace_bytes(code, q.size(0), k.size(0), heads, kv, dim);
-    at::Tensor ws = workspace(bytes, q.device(), stream);
+    at::Tensor ws = scratch(bytes, q.device());
     const HeadStrides st(q, k, v);
     const Layout lq{s[6]}, lk{s[7]};
     check(kl_pack_attention_backward(code, q.size(0), k.size(0), heads, kv, dim, ptr(g), ptr(q), ptr(k), ptr(v), st.v,
@@ -674,7 +681,7 @@ struct NormRotary : public torch::autograd::Function<NormRotary> {
     at::Tensor dwk = a.wk.defined() && ctx->needs_input_grad(a.wq.defined() ? 3 : 2) ? at::empty_like(a.wk)
                                                                                      : at::Tensor();
     const size_t bytes = kl_norm_rotary_bwd_workspace_bytes((int)q.size(2));
-    at::Tensor ws = workspace(bytes, q.device(), a.stream);
+    at::Tensor ws = scratch(bytes, q.device());
     const HeadStrides st(q, k, k);
     check(kl_norm_rotary_backward(seq_code(q.scalar_type()), q.size(0), (int)q.size(1), (int)k.size(1), (int)q.size(2),
                                   2 * (int)a.freqs.size(0), a.interleaved, ptr(gq), ptr(gk), ptr(q), ptr(k), st.v,
@@ -736,7 +743,7 @@ at::Tensor recurrence_forward(const at::Tensor &gates, const at::Tensor &feats, 
   const int64_t n = gates.size(0), dim = gates.size(1);
   at::Tensor out = at::empty(gates.sizes(), gates.options());
   const size_t bytes = kl_linear_recurrence_workspace_bytes(code, n, dim);
-  at::Tensor ws = workspace(bytes, gates.device(), stream);
+  at::Tensor ws = scratch(bytes, gates.device());
   check(kl_linear_recurrence_forward(code, n, dim, ptr(gates), ptr(feats), ptr(initial),
                                      initial.defined() ? initial.size(0) : 0, l.ids(), l.starts(), reverse, ptr(out),
                                      ptr(ws), bytes, (kl_stream)stream),
@@ -768,7 +775,7 @@ struct LinearRecurrence : public torch::autograd::Function<LinearRecurrence> {
     at::Tensor di = initial.defined() ? at::empty(initial.sizes(), initial.options()) : at::Tensor();
     const kl_dtype code = seq_code(gates.scalar_type());
     const size_t bytes = kl_linear_recurrence_workspace_bytes(code, n, dim);
-    at::Tensor ws = workspace(bytes, gates.device(), stream);
+    at::Tensor ws = scratch(bytes, gates.device());
     check(kl_linear_recurrence_backward(code, n, dim, ptr(g), ptr(gates), ptr(s[1]), ptr(initial),
                                         initial.defined() ? initial.size(0) : 0, l.ids(), l.starts(),
                                         ctx->saved_data["reverse"].toBool(), ptr(da), ptr(db), ptr(di), ptr(ws), bytes,

@@ -249,6 +249,13 @@ def workspace(nbytes, device):
     return t
 
 
+def scratch(nbytes, device):
+    """Scratch of one call alone, for entries whose kernels hand each other numbers through it (counts that bound
+    loops among them): another host thread may launch on the same stream between them (ctypes calls and
+    backwards run without the interpreter's lock).  From the allocator's pool of the current stream."""
+    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
+
+
 _ZK = {}
 
 

@@ -46,7 +46,7 @@ def pack_layout_cuda(boundaries):
     starts = torch.empty((n + 1,), dtype=torch.int32, device=dev)
     with N.on_device(dev):
         ws_bytes = N.size('kl_pack_layout_workspace_bytes', n)
-        ws = N.workspace(ws_bytes, dev)
+        ws = N.scratch(ws_bytes, dev)
         N.check(N.lib().kl_pack_layout(n, N.ptr(boundaries), N.ptr(ids), N.ptr(starts), N.ptr(ws), ws_bytes,
                                        N.stream_of(dev)), func)
     return ids, starts
@@ -111,7 +111,7 @@ def pack_attention_forward_cuda(q, k, v, q_layout, k_layout, scale, causal, for_
     with N.on_device(dev):
         ws_bytes = N.size('kl_pack_attention_workspace_bytes', code, q.shape[0], k.shape[0], q.shape[1], k.shape[1],
                           q.shape[2])
-        ws = N.workspace(ws_bytes, dev)
+        ws = N.scratch(ws_bytes, dev)
         N.check(N.lib().kl_pack_attention_forward(
             code, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2], N.ptr(q), N.ptr(k), N.ptr(v),
             _strides(q, k, v), N.ptr(q_layout[0]), N.ptr(q_layout[1]), N.ptr(k_layout[0]), N.ptr(k_layout[1]),
@@ -145,7 +145,7 @@ def pack_attention_backward_cuda(grad_out, q, k, v, q_layout, k_layout, out, lse
     with N.on_device(dev):
         ws_bytes = N.size('kl_pack_attention_bwd_workspace_bytes', _CODES[q.dtype], q.shape[0], k.shape[0], q.shape[1],
                           k.shape[1], q.shape[2])
-        ws = N.workspace(ws_bytes, dev)
+        ws = N.scratch(ws_bytes, dev)
         N.check(N.lib().kl_pack_attention_backward(
             _CODES[q.dtype], q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2], N.ptr(grad_out),
             N.ptr(q), N.ptr(k), N.ptr(v), _strides(q, k, v), N.ptr(q_layout[0]), N.ptr(q_layout[1]),
@@ -241,7 +241,7 @@ def norm_rotary_backward_cuda(grad_q_out, grad_k_out, q, k, q_weight, k_weight, 
     dqw, dkw = (torch.empty_like(w) if w is not None and need_weights else None for w in (q_weight, k_weight))
     with N.on_device(dev):
         ws_bytes = N.size('kl_norm_rotary_bwd_workspace_bytes', q.shape[2])
-        ws = N.workspace(ws_bytes, dev)
+        ws = N.scratch(ws_bytes, dev)
         N.check(N.lib().kl_norm_rotary_backward(
             _CODES[q.dtype], q.shape[0], q.shape[1], k.shape[1], q.shape[2], 2 * freqs.shape[0], int(interleaved),
             N.ptr(gq), N.ptr(gk), N.ptr(q), N.ptr(k), *rest, N.ptr(dq), N.ptr(dk), N.ptr(dqw), N.ptr(dkw), N.ptr(ws),
@@ -284,7 +284,7 @@ def linear_recurrence_forward_cuda(gates, feats, layout, initial, reverse):
     out = torch.empty_like(gates)
     with N.on_device(dev):
         ws_bytes = N.size('kl_linear_recurrence_workspace_bytes', code, n, dim)
-        ws = N.workspace(ws_bytes, dev)
+        ws = N.scratch(ws_bytes, dev)
         N.check(N.lib().kl_linear_recurrence_forward(
             code, n, dim, N.ptr(gates), N.ptr(feats), N.ptr(initial), 0 if initial is None else initial.shape[0],
             N.ptr(layout[0]), N.ptr(layout[1]), int(reverse), N.ptr(out), N.ptr(ws), ws_bytes, N.stream_of(dev)), func)
@@ -301,7 +301,7 @@ def linear_recurrence_backward_cuda(grad_out, gates, out, layout, initial, rever
     di = torch.empty_like(initial) if initial is not None else None
     with N.on_device(dev):
         ws_bytes = N.size('kl_linear_recurrence_workspace_bytes', code, n, dim)
-        ws = N.workspace(ws_bytes, dev)
+        ws = N.scratch(ws_bytes, dev)
         N.check(N.lib().kl_linear_recurrence_backward(
             code, n, dim, N.ptr(grad_out), N.ptr(gates), N.ptr(out), N.ptr(initial),
             0 if initial is None else initial.shape[0], N.ptr(layout[0]), N.ptr(layout[1]), int(reverse), N.ptr(da),
