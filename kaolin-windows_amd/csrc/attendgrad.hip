@@ -8,8 +8,8 @@
 // accumulators of the first in place (seqcommon.h, acc_frag); the streamed tiles are read from LDS along
 // rows for the first products and along columns for the second.
 // Rounding: p and ds are rounded to the inputs' type for the second products, half a step each; sums stay
-// in 32 bits.  float16 has few exponents: there ds is multiplied by a power of two of its column (fit_column), and the
-// result by its inverse, both exact.
+// in 32 bits.  float16 has few exponents: there ds, and p for dv, are multiplied by a power of two of their column
+// (fit_column), and the result by its inverse, both exact.
 // Masked places that hold infinities or NaN: as in attend.hip.
 // Bound by issue and by the longest rows: 8191 rows in 4 packs, causal, 16 / 4 heads of 64, bf16: dq 178 us, dk and dv
 // in four splits of the rows 265 and 14 for their join, with the matrix units busy in 35 to 40 % of the cycles.
@@ -68,12 +68,13 @@ __global__ void __launch_bounds__(256) attend_prep_kernel(Attend a, const T *__r
 }
 
 // What is rounded to float16 for a second product is first multiplied by a power of two of its column (this lane and the
-// other half's; a row of q in dq, a key in dk), `up`, and the product divided by it in the end, both exact.  It starts
-// at kMostUp and falls, the sums so far with it, where a column's largest number would pass 2^15: that one then lies
-// in [2^11, 2^12), and smaller ones keep their bits down to 2^-25 of it.  So neither overflows, nor do large
-// numbers of another row, key or pack cost bits here.  (One power for all, from the largest |do|: ds overflowed where v is
-// large, and a pack of small gradients lost its bits to one of large ones.  Forward and backward of 8191 rows in 4 packs,
-// causal, 16 / 4 heads, f16: 602 us with that, 609 now, for heads of 64; 1317 and 1290 for heads of 128.)
+// other half's; a row of q in dq, a key in dk and dv), `up`, and the product divided by it in the end, both exact.  It
+// starts at kMostUp and falls, the sums so far with it, where a column's largest number would pass 2^15: that one
+// then lies in [2^11, 2^12), and smaller ones keep their bits down to 2^-25 of it.  So neither overflows, nor do large
+// numbers of another row, key or pack cost bits here, nor long packs those of the weights.  (One power for all, from the
+// largest |do|: ds overflowed where v is large, and a pack of small gradients lost its bits to one of large ones.  Weights
+// as they are: under 2^-14 dv lost bits, at 2^-25 all.  Forward and backward of 8191 rows in 4 packs, causal, 16 / 4
+// heads: 611 us with those, 631 now, for heads of 64; 1333 and 1321 for 128; 458 and 492 for 32.)
 template <typename T>
 constexpr bool kFitted = std::is_same<T, f16_t>::value;
 constexpr float kMostUp = 0x1p60f;  // leaves room for sums of 2^31 products of two of the largest float16 numbers
@@ -321,7 +322,7 @@ struct DkvTile {
 template <typename T, int DP, bool CAREFUL>
 __device__ __forceinline__ void dkv_walk(const Attend &a, const Grad &g, const T *__restrict__ q, Heads gst,
                                          const T *__restrict__ go, int head, int begin, int end, Range rows,
-                                         int tiles, int key0, float &up_k,
+                                         int tiles, int key0, float &up_k, float &up_v,
                                          const V8<T> (&kf)[DP / 16], const V8<T> (&vf)[DP / 16], T *qs, T *os,
                                          float2 *s_ld, int2 *s_range, uint32_t *bad, f32x16 (&dk)[DP / 32],
                                          f32x16 (&dv)[DP / 32]) {
@@ -382,7 +383,10 @@ __device__ __forceinline__ void dkv_walk(const Attend &a, const Grad &g, const T
               dp[r] = in ? dp[r] : 0.f;
             }
           }
-          if constexpr (kFitted<T>) fit_column(dp, up_k, dk);
+          if constexpr (kFitted<T>) {
+            fit_column(dp, up_k, dk);
+            fit_column(s, up_v, dv);
+          }
 #pragma unroll
           for (int i = 0; i < 2; i++) {
             const V8<T> p = acc_frag<T>(s, i), ds = acc_frag<T>(dp, i);
@@ -401,7 +405,7 @@ __device__ __forceinline__ void dkv_walk(const Attend &a, const Grad &g, const T
             const float t = frag_dot<T, DP>(kf, qs + SIZE, r, h) * a.c, dpx = frag_dot<T, DP>(vf, os + SIZE, r, h);
             if (key >= kr.x && key < kr.y) {
               const float p = exp2_fast(t - x.x);
-              add_row<T, DP>(dv, p, os + SIZE, r, h);
+              add_row<T, DP>(dv, p * up_v, os + SIZE, r, h);
               add_row<T, DP>(dk, p * (dpx - x.y) * up_k, qs + SIZE, r, h);
             }
           }
@@ -466,7 +470,7 @@ __device__ __forceinline__ bool dkv_keys(const Attend &a, const Grad &g, const G
     vf[i] = global_frag(vrow, live, 16 * i + 8 * h, a.dim);
   }
   f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
-  float up_k = kFitted<T> ? kMostUp : 1.f;
+  float up_k = kFitted<T> ? kMostUp : 1.f, up_v = up_k;
   if constexpr (kDirect<T, DP>) {
     const float2 *ld = g.ld + head * a.group;
     dkv_walk32<DP, CAREFUL>(a, qh, gst, gh, ld, heads, g.range, begin, end, rows, tiles, key0, kf, vf, lds.qs, lds.os,
@@ -476,8 +480,8 @@ __device__ __forceinline__ bool dkv_keys(const Attend &a, const Grad &g, const G
     if (CAREFUL) __syncthreads();  // everyone has read lds.redo
     if (threadIdx.x == 0) lds.redo = 0;
     __syncthreads();
-    dkv_walk<T, DP, CAREFUL>(a, g, qh, gst, gh, head, begin, end, rows, tiles, key0, up_k, kf, vf, lds.qs, lds.os, lds.ld,
-                             lds.range, lds.bad, dk, dv);
+    dkv_walk<T, DP, CAREFUL>(a, g, qh, gst, gh, head, begin, end, rows, tiles, key0, up_k, up_v, kf, vf, lds.qs, lds.os,
+                             lds.ld, lds.range, lds.bad, dk, dv);
     if (!CAREFUL) {
       if (!(all_finite(dk) && all_finite(dv))) lds.redo = 1;
       __syncthreads();
@@ -489,11 +493,11 @@ __device__ __forceinline__ bool dkv_keys(const Attend &a, const Grad &g, const G
   if (p.part) {
     const int64_t all = (int64_t)a.nk * a.kv_heads * a.dim;
     store_cols<float, DP>(p.part + 2 * blockIdx.y * all + at, dk, a.scale / up_k, h, a.dim);
-    store_cols<float, DP>(p.part + (2 * blockIdx.y + 1) * all + at, dv, 1.f, h, a.dim);
+    store_cols<float, DP>(p.part + (2 * blockIdx.y + 1) * all + at, dv, 1.f / up_v, h, a.dim);
     return false;
   }
   store_cols<T, DP>((T *)p.dk + at, dk, a.scale / up_k, h, a.dim);
-  store_cols<T, DP>((T *)p.dv + at, dv, 1.f, h, a.dim);
+  store_cols<T, DP>((T *)p.dv + at, dv, 1.f / up_v, h, a.dim);
   return false;
 }
 

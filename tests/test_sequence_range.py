@@ -93,6 +93,23 @@ def test_attention_gradients_of_very_different_packs(spc, dtype, causal):
             assert not torch.isfinite(x[~clean]).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('rows,sharp', [(131072, 3.0), (4096, 0.0)])
+def test_attention_gradients_of_small_weights(spc, dtype, rows, sharp):
+    """The values' gradients of one query over many keys, of weights down to 2^-24 and less: a long pack, and one whose first
+    key has nearly all the weight."""
+    dim = 64
+    q, k, v, g = (_normal(i, m, 1, dim, dtype=dtype) for i, m in enumerate((1, rows, rows, 1)))
+    if sharp:
+        k = (k.float() * sharp).to(dtype)
+    else:  # scores of 0 and some -14.6: weights of 1 and 2^-21
+        k = torch.where(torch.arange(rows)[:, None, None] == 0, 0.0, -117 / dim + 0.01 * k.float()).to(dtype)
+        q = torch.ones_like(q)
+    g = (1000 * g.float()).to(dtype)
+    _compare(spc, (q, k, v), g, marks([rows]), q_boundaries=marks([1]))
+
+
 def _recurrence(spc, a, x, b, first=None, reverse=False, grad=None):
     outs, tols = recurrence(a, x, b, first, reverse, grad=grad, dtype=a.dtype)
     leaves = [_leaf(y) for y in (a, x, first)]
