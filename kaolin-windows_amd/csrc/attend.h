@@ -269,6 +269,11 @@ struct RowState {
   __device__ __forceinline__ float base() const { return m == -INFINITY ? 0.f : m; }
 };
 constexpr float kLag = 8;
+// float16's weights are 2^kLift times larger, so that 2^kLag * 2^kLift = 2^15 is in its range and those down to 2^-32
+// of the largest are: without it 131,072 keys of weights 2^-25 of another's, a 256th of it together, were lost.  A
+// row's sum is of the same weights, so the result has no factor.
+template <typename T>
+constexpr float kLift = std::is_same<T, f16_t>::value ? 7.f : 0.f;
 
 template <int N>
 __device__ __forceinline__ void rescale(RowState &st, float m, f32x16 (&acc)[N]) {

@@ -12,9 +12,9 @@
 // 175 us, 4.8 TB/s, and 5 us for the join.
 // low (training, 16-bit types): what the rounding of o left out, so that the backward's sums over do . o,
 // which cancel against other terms, have o to twice its bits.
-// Rounding: weights, at most 2^kLag, are rounded to the inputs' type for the second product (each off by half a
-// step at most, whatever their size; float stays float); the sum they are divided by is taken before the rounding,
-// in 32 bits.
+// Rounding: weights, at most 2^kLag (float16: times 2^kLift), are rounded to the inputs' type for the second product (each
+// off by half a step at most, whatever their size; float stays float); the sum they are divided by is taken before the
+// rounding, in 32 bits.
 //
 // A key outside a row's range has weight 0, but 0 * inf and 0 * NaN would still reach the row through the
 // product.  Nothing in the main walk guards against that: if an accumulator ends up not finite, the
@@ -79,7 +79,7 @@ __device__ __forceinline__ void fwd_walk(const Attend &a, const T *__restrict__ 
         }
         top = half_max(top) * a.c;
         if (__any(top > st.m + kLag)) rescale(st, fmaxf(st.m, top), acc);
-        const float base = st.base();
+        const float base = st.base() - kLift<T>;
 #pragma unroll
         for (int b = 0; b < BN / 32; b++) {
 #pragma unroll
@@ -101,7 +101,7 @@ __device__ __forceinline__ void fwd_walk(const Attend &a, const T *__restrict__ 
             const float t = frag_dot<T, DP>(qf, ks + SIZE, r, h) * a.c;
             if (key >= mine.lo && key < mine.hi) {
               rescale(st, fmaxf(st.m, t), acc);
-              const float p = exp2_fast(t - st.base());
+              const float p = exp2_fast(t - (st.base() - kLift<T>));
               st.l += h == 0 ? p : 0.f;
               add_row<T, DP>(acc, p, vs + SIZE, r, h);
             }
@@ -196,7 +196,7 @@ __device__ __forceinline__ bool fwd_rows(const Attend &a, const FwdArgs &p, FwdL
       store_cols<T, DP>((T *)p.low + at * a.dim, acc, 1.f, h, a.dim);
     }
   }
-  if (p.lse && h == 0) p.lse[at] = blind ? 0.f : st.m + log2_fast(l);
+  if (p.lse && h == 0) p.lse[at] = blind ? 0.f : st.m - kLift<T> + log2_fast(l);
   return false;
 }
 
@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(Attend a, int splits, 
     for (int e = 0; e < 8; e++) sum[e] -= (float)y[e];
     *reinterpret_cast<V8<T> *>(low + out * a.dim + d) = __builtin_convertvector(sum, V8<T>);
   }
-  if (lse && d == 0) lse[out] = blind ? 0.f : top + log2_fast(l);
+  if (lse && d == 0) lse[out] = blind ? 0.f : top - kLift<T> + log2_fast(l);
 }
 
 // Splits of the keys: two waves for each of the chip's 1024 SIMDs and no more, which is what runs at once (one more

@@ -110,6 +110,21 @@ def test_attention_gradients_of_small_weights(spc, dtype, rows, sharp):
     _compare(spc, (q, k, v), g, marks([rows]), q_boundaries=marks([1]))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
+def test_attention_many_small_weights(spc, dtype):
+    """131,071 keys of weights 2^-25.5 of the first one's, whose sum counts: enough rows that their keys are not split."""
+    n, rows, heads, dim = 131072, 4096, 16, 8
+    k, v = torch.full((n, heads, dim), -6.25), torch.ones(n, heads, dim)
+    k[0], v[0] = 0, 0
+    q, k, v = torch.ones(rows, heads, dim).to(dtype), k.to(dtype), v.to(dtype)
+    b = marks([n])
+    (want,), (tol,) = attention_heads(q[:1], k, v, b, marks([1]))
+    assert (want > 2e-3).all() and (tol < 0.05 * want).all()
+    o = spc.pack_attention(q.to(DEV), k.to(DEV), v.to(DEV), b.to(DEV), q_boundaries=marks([rows]).to(DEV))
+    check('o', o, want.expand(rows, heads, dim), tol.expand(rows, heads, dim))
+
+
 def _recurrence(spc, a, x, b, first=None, reverse=False, grad=None):
     outs, tols = recurrence(a, x, b, first, reverse, grad=grad, dtype=a.dtype)
     leaves = [_leaf(y) for y in (a, x, first)]
