@@ -497,6 +497,13 @@ bool any_grad(std::initializer_list<const at::Tensor *> ts) {
   return false;
 }
 
+// a forward-mode derivative: the Python nodes refuse it, the bare kernels would drop it
+bool any_tangent(std::initializer_list<const at::Tensor *> ts) {
+  for (const at::Tensor *t : ts)
+    if (t->defined() && t->_fw_grad(/*level=*/0).defined()) return true;
+  return false;
+}
+
 at::Tensor contiguous16(const at::Tensor &t) {
   const at::Tensor c = t.contiguous();
   return c.numel() && (uintptr_t)c.data_ptr() % 16 ? c.clone() : c;
@@ -611,7 +618,8 @@ c10::optional<at::Tensor> pack_attention(at::Tensor q, at::Tensor k, at::Tensor 
       v.scalar_type() != q.scalar_type() || !plain_heads(q) || !plain_heads(k) || !plain_heads(v) ||
       k.sizes() != v.sizes() || k.size(2) != q.size(2) || q.size(2) % 8 || q.size(2) < 8 || q.size(2) > 128 ||
       k.size(1) == 0 || q.size(1) == 0 || q.size(1) % k.size(1) || q.size(1) > 4096 || !(scale > 0) ||
-      !std::isfinite(scale) || !plain_mask(boundaries, k.size(0), dev) || !plain_mask(qb, q.size(0), dev))
+      !std::isfinite(scale) || !plain_mask(boundaries, k.size(0), dev) || !plain_mask(qb, q.size(0), dev) ||
+      any_tangent({&q, &k, &v}))
     return c10::nullopt;
   const c10::DeviceGuard guard(dev);
   Layout lk, lq;
@@ -715,7 +723,7 @@ c10::optional<std::tuple<at::Tensor, at::Tensor>> norm_rotary(at::Tensor q, at::
       !plain_weight(wk) || (wq.defined() && wk.defined() && wq.scalar_type() != wk.scalar_type()) ||
       freqs.device() != dev || freqs.scalar_type() != at::kDouble || freqs.dim() != 1 || !freqs.is_contiguous() ||
       freqs.requires_grad() || 2 * freqs.size(0) > q.size(2) || !(eps >= 0) || !std::isfinite(eps) ||
-      boundaries.has_value() == positions.defined())
+      boundaries.has_value() == positions.defined() || any_tangent({&q, &k, &wq, &wk, &freqs, &positions}))
     return c10::nullopt;
   if (positions.defined()) {
     const auto t = positions.scalar_type();
@@ -798,7 +806,8 @@ c10::optional<at::Tensor> linear_recurrence(at::Tensor gates, at::Tensor feats, 
   if (!gates.is_cuda() || (!seq_float(gates) && gates.scalar_type() != at::kDouble) || !plain(gates) || !plain(feats) ||
       gates.sizes() != feats.sizes() || gates.size(1) >= 1 << 24 || !plain_mask(boundaries, gates.size(0), dev) ||
       (initial.defined() && (!plain(initial) || initial.size(1) != gates.size(1) ||
-                             initial.size(0) >= (int64_t)1 << 31)))
+                             initial.size(0) >= (int64_t)1 << 31)) ||
+      any_tangent({&gates, &feats, &initial}))
     return c10::nullopt;
   const c10::DeviceGuard guard(dev);
   const Layout l = make_layout(boundaries, stream);

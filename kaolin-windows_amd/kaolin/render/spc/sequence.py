@@ -63,7 +63,7 @@ def pack_attention(q, k, v, boundaries, q_boundaries=None, causal=False, scale=N
     that is not contiguous, or rows that do not start at multiples of 16 bytes, are copied first.  Keys that
     a row does not see have no effect on it whatever they hold (infinities and NaN too).  Scores and sums are
     in 32 bits; f16 and bf16 weights are rounded to the type for the product with ``v``.  Results are the same
-    on every run.  Differentiable once, with respect to q, k and v.
+    on every run.  Differentiable once, backwards, with respect to q, k and v.
     """
     scale = (max(q.shape[-1], 1) if q.dim() else 1) ** -0.5 if scale is None else float(scale)
     ext = _ext.get() if q.is_cuda else None
@@ -121,8 +121,8 @@ def norm_rotary(q, k, q_weight, k_weight, freqs, boundaries=None, positions=None
     Returns:
         (Tensor, Tensor): the new q and k, contiguous.
 
-    Angles are formed in 64 bits, the rest in 32, and the outputs are rounded once.  Differentiable once, with
-    respect to q, k and the weights; the sums for the weights have a fixed order.  Strides: as
+    Angles are formed in 64 bits, the rest in 32, and the outputs are rounded once.  Differentiable once,
+    backwards, with respect to q, k and the weights; the sums for the weights have a fixed order.  Strides: as
     :func:`pack_attention`.
     """
     ext = _ext.get() if q.is_cuda else None
@@ -202,8 +202,8 @@ def linear_recurrence(gates, feats, boundaries, initial=None, reverse=False):
     States are carried in 32 bits (64 for f64) and rounded once each; a pack is never touched by another's
     values.  Gates may be any numbers: a state is off by some roundings of the recurrence of the magnitudes,
     ``s[t] = |gates[t]| * s[t-1] + |feats[t]|``, and finite where that is.  From a row with an infinite gate on, a pack's
-    states are infinite or NaN.  Differentiable once, with respect to gates, feats and initial; the gradient of the gates takes the
-    states as they were rounded.
+    states are infinite or NaN.  Differentiable once, backwards, with respect to gates, feats and initial; the
+    gradient of the gates takes the states as they were rounded.
     """
     ext = _ext.get() if gates.is_cuda else None
     if ext is not None:
