@@ -121,9 +121,9 @@ def norm_rotary(q, k, q_weight, k_weight, freqs, boundaries=None, positions=None
     Returns:
         (Tensor, Tensor): the new q and k, contiguous.
 
-    Angles are formed in 64 bits, the rest in 32, and the outputs are rounded once.  Differentiable once,
-    backwards, with respect to q, k and the weights; the sums for the weights have a fixed order.  Strides: as
-    :func:`pack_attention`.
+    Angles are formed in 64 bits, the rest in 32 (heads whose squares would leave a float's range are scaled first), and the
+    outputs are rounded once.  Differentiable once, backwards, with respect to q, k and the weights; the sums for the
+    weights have a fixed order.  Strides: as :func:`pack_attention`.
     """
     ext = _ext.get() if q.is_cuda else None
     if ext is not None:

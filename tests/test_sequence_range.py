@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from seq_util import attention, check, marks, recurrence
+from seq_util import attention, check, marks, norm_rotary, recurrence
 from seq_wide_util import attention_heads
 from test_sequence import DEV, TYPES, _leaf, _normal, spc  # noqa: F401
 
@@ -187,3 +187,32 @@ def test_recurrence_infinite_gates_and_features(spc, n, dim):
         if where is x:
             assert (h[20:n // 2] == math.inf).all()
         where[20] = keep
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('size,eps', [(1e25, 1e-6), (1e37, 0.0), (1e-25, 0.0), (1e-25, 1e-6), (1e-30, 1e-38), (1.0, 1e38),
+                                      (1e-20, 1e-35)])
+@pytest.mark.parametrize('heads,kv,dim,turn,interleaved', [(3, 1, 128, 128, False), (2, 2, 40, 8, True), (1, 5, 256, 64, False)])
+def test_norm_of_heads_far_from_one(spc, dtype, size, eps, heads, kv, dim, turn, interleaved):
+    """Heads whose squares, or eps, leave a float's range, beside ones of order 1 and one of zeros in the same rows."""
+    n = 37
+    x = {'q': _normal(0, n, heads, dim), 'k': _normal(1, n, kv, dim)}
+    for y in x.values():
+        y[::2] *= size
+        y[5:7, :1] = 0
+    if eps == 0:  # a head of zeros has no norm then
+        for y in x.values():
+            y[5:7, :1] = 1
+    x = {m: y.to(dtype) for m, y in x.items()}
+    w = {m: (1 + _normal(2 + i, dim, scale=0.3)).to(dtype) for i, m in enumerate('qk')}
+    g = {m: _normal(4 + i, *x[m].shape, dtype=dtype) for i, m in enumerate('qk')}
+    f = 100.0 ** (-torch.arange(turn // 2).double() * 2 / turn)
+    leaves = [_leaf(y) for y in (x['q'], x['k'], w['q'], w['k'])]
+    y = spc.norm_rotary(*leaves, f.to(DEV), positions=torch.arange(n, device=DEV), eps=eps, interleaved=interleaved)
+    grads = torch.autograd.grad(y, leaves, [g[m].to(DEV) for m in 'qk'])
+    eps = float(torch.tensor(eps, dtype=torch.float32))
+    for i, m in enumerate('qk'):
+        outs, tols = norm_rotary(x[m], w[m], f, torch.arange(n), eps, interleaved, grad=g[m], dtype=dtype)
+        for name, got, want, tol in zip(('y', 'dx', 'dw'), (y[i], grads[i], grads[2 + i]), outs, tols):
+            check(f'{name} of {m}', got, want, tol)
