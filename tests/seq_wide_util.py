@@ -78,3 +78,70 @@ def attention_heads(q, k, v, boundaries, q_boundaries=None, causal=False, scale=
         tols[2][k0:k1] = 2 * (u * dk.abs() + floor + shared(scale * times(tk.transpose(1, 2), qq.abs())))
         tols[3][k0:k1] = 2 * (u * dv.abs() + floor + shared(times(tv.transpose(1, 2), g.abs())))
     return [x.cpu() for x in outs], [x.cpu() for x in tols]
+
+
+def _scan(a, b, starts, longest):
+    """h[t] = a[t] h[t - 1] + b[t] down dimension 0, a[starts] taken as 0, in doubling steps."""
+    a, b = a.clone(), b.clone()
+    a[starts] = 0
+    step = 1
+    while step < longest:
+        b[step:] += a[step:] * b[:-step]
+        a[step:] = a[step:] * torch.cat((torch.zeros_like(a[:step]), a[:-step]))[step:]
+        step *= 2
+    return b
+
+
+def recurrence_scan(a, b, boundaries, initial=None, reverse=False, grad=None):
+    """As seq_util.recurrence for many rows: h, the gradients of a, b (and initial, with a row for every pack) where `grad`
+    is given, bounds.
+
+    Bounds: whatever the order of products and sums, what enters at row r is off by one rounding for each row that it is
+    carried over and each sum, so h[t] by E (scan(|a|, size) + 16 size) for the recurrence of magnitudes `size`."""
+    dtype = b.dtype
+    u, floor, e = HALF_STEP[dtype], FLOOR[dtype], 2.0 ** -53 if dtype == torch.float64 else E
+    a, b = a.detach().double(), b.detach().double()
+    n = len(b)
+    starts = torch.nonzero(boundaries)[:, 0]
+    lead = int(starts[0]) if len(starts) else n
+    first = initial.detach().double() if initial is not None else torch.zeros(len(starts), b.shape[1], dtype=torch.float64)
+    ends = torch.cat((starts[1:], starts.new_tensor([n]))) - 1
+    longest = int((ends - starts).max()) + 1
+    out_rows = torch.ones(n, 1, dtype=torch.float64)
+    out_rows[:lead] = 0
+    if reverse:
+        a, b, out_rows = a.flip(0), b.flip(0), out_rows.flip(0)
+        starts, ends, first = (n - 1 - ends).flip(0), (n - 1 - starts).flip(0), first.flip(0)
+    a, b = a * out_rows, b * out_rows
+
+    def walk(a, x, s0, starts):
+        x = x.clone()
+        x[starts] += a[starts] * s0
+        return _scan(a, x, starts, longest)
+    h, size = walk(a, b, first, starts), walk(a.abs(), b.abs(), first.abs(), starts)
+    zero = torch.zeros_like(first)
+    eh = e * (walk(a.abs(), size, zero, starts) + 16 * size)
+    res = [('h', h, u * h.abs() + eh)]
+    if grad is not None:
+        g = grad.double().flip(0) if reverse else grad.double()
+        g = g * out_rows
+        after = torch.cat((a[1:], torch.zeros_like(a[:1]))) * out_rows
+        ends_up = (n - 1 - ends).flip(0)
+
+        def back(gates, x):
+            return _scan(gates.flip(0), x.flip(0), ends_up, longest).flip(0)
+        db, ga = back(after, g), back(after.abs(), g.abs())
+        eg = e * (back(after.abs(), ga) + 16 * ga)
+
+        def before(x, s0):
+            y = torch.cat((torch.zeros_like(x[:1]), x[:-1]))
+            y[starts] = s0
+            return y * out_rows
+        hb, ehb = before(h, first), before(eh, zero)
+        da = db * hb
+        res += [('da', da, u * da.abs() + (eg + 2 * e * ga) * hb.abs() + ga * (u * hb.abs() + ehb)),
+                ('db', db, u * db.abs() + eg)]
+        if initial is not None:
+            di = a[starts] * db[starts]
+            res.append(('dinitial', di, u * di.abs() + a[starts].abs() * (eg + 2 * e * ga)[starts]))
+    return [(name, x.flip(0) if reverse else x, 2 * ((t.flip(0) if reverse else t) + floor)) for name, x, t in res]
