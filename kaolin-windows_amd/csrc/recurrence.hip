@@ -13,8 +13,8 @@
 // Bound by memory: a and b are read 1 + (share of 1) times and h is written once.  Step 3 takes the chunks in the
 // other order, so that it finds what 1 read last in the 256 MB cache.  One pass, with workgroups that publish and
 // await each other's (A, B), measured no faster: it reads less, but waits.
-// 311,000 rows of 64 columns, float, packs of 38 rows: forward 24 + 9 + 40 us (239 MB at least, 47 us at the rate of
-// a copy), backward 26 + 9 + 67 us (397 MB, 79 us); 65,537 x 1024, bf16, two packs: 68 + 13 + 72 and
+// 311,000 rows of 64 columns, float, packs of 38 rows: forward 24 + 8 + 40 us (239 MB at least, 47 us at the rate of
+// a copy), backward 26 + 8 + 67 us (397 MB, 79 us); 65,537 x 1024, bf16, two packs: 70 + 13 + 72 and
 // 60 + 13 + 124 us (403 MB, 80 us, and 671 MB, 133 us).
 //
 // States, A and B are in 32 bits (64 for double); outputs are rounded once.  A is a product of gates alone, and may pass a
@@ -53,9 +53,10 @@ __device__ __forceinline__ void store_pack(T *p, const Pack<T, V> &x) {
   __builtin_memcpy(p, x.v, sizeof(T) * V);
 }
 
-// A = m 2^e with |m| in [0.5, 1), 0 or not finite; stored with 16 bits of exponent (near_exponent).  Against products in
-// a float: the scan of 65,537 x 1024 in bf16 13 us for 10.4, the whole of it 358 for 351; 8192 rows of one pack, which
-// fold up to 64 segments, 46 for 39.
+// A = m 2^e with |m| in [0.5, 1), 0 or not finite.  Exponents are whole: a segment's are under 256 chunks * 64 rows * 1074
+// (saturated at 2^+-16384, in 16 bits, a double's state came back to life behind 20 gates of 2^-1000 and 16 of 2^1000).
+// Against products in a float: 65,537 x 1024 in bf16, training, 360 us for 351; 8192 rows of one pack, which fold up to
+// 64 segments with three operations for one, 47 for 39.
 __device__ __forceinline__ float mantissa(float x) { return __builtin_amdgcn_frexp_mantf(x); }
 __device__ __forceinline__ double mantissa(double x) { return __builtin_amdgcn_frexp_mant(x); }
 __device__ __forceinline__ int exponent(float x) { return __builtin_amdgcn_frexp_expf(x); }
@@ -114,28 +115,22 @@ constexpr int kFewSegments = 64;  // what a wave's lanes can look through at onc
 template <typename S>
 struct Composed {
   S *a, *b;
-  int16_t *e;
-  int32_t *resets;
+  int32_t *e, *resets;
 };
 template <typename S>
 struct ComposedIn {
   const S *a, *b;
-  const int16_t *e;
-  const int32_t *resets;
+  const int32_t *e, *resets;
 };
-
-// No state but 0 comes through a gain that far, either way, and stays in its type's range: exponents stop there.
-constexpr int kFarExponent = 1 << 14;
-__device__ __forceinline__ int16_t near_exponent(int e) { return (int16_t)min(max(e, -kFarExponent), kFarExponent); }
 
 template <int V, typename S>
 __device__ __forceinline__ void store_gains(const Composed<S> &m, int64_t at, const Gain<S> (&g)[V]) {
   Pack<S, V> a;
-  Pack<int16_t, V> e;
+  Pack<int32_t, V> e;
 #pragma unroll
   for (int v = 0; v < V; v++) {
     a.v[v] = g[v].m;
-    e.v[v] = near_exponent(g[v].e);
+    e.v[v] = g[v].e;
   }
   store_pack<V>(m.a + at, a);
   store_pack<V>(m.e + at, e);
@@ -262,7 +257,7 @@ __global__ void __launch_bounds__(1024) recur_scan_kernel(Recur r, Composed<S> c
   if (col < r.dim && me >= 1008) {
     const int64_t to = (int64_t)blockIdx.y * r.dim + col;
     segments.a[to] = ga.m;
-    segments.e[to] = near_exponent(ga.e);
+    segments.e[to] = ga.e;
     segments.b[to] = gb;
     if (col == 0) segments.resets[blockIdx.y] = reset;
   }
@@ -275,7 +270,7 @@ __global__ void __launch_bounds__(1024) recur_scan_kernel(Recur r, Composed<S> c
     if (c0 + k >= r.chunks) break;
     const int64_t to = (int64_t)(c0 + k) * r.dim + col;
     chunks.a[to] = ga.m;
-    chunks.e[to] = near_exponent(ga.e);
+    chunks.e[to] = ga.e;
     chunks.b[to] = gb;
     if (col == 0) before[c0 + k] = reset;
     step(k);
@@ -284,8 +279,8 @@ __global__ void __launch_bounds__(1024) recur_scan_kernel(Recur r, Composed<S> c
 
 // Steps 1 and 2 in one, where segments of 256 / 2^wide chunks are few: a workgroup takes one, 2^wide pieces across,
 // and step 3 folds the segments before a chunk from the last one with a pack's start.  With the pack arrays, every row a
-// pack / one pack: 4096 rows of 64 columns, float, 11.4 / 17.4 us, in three launches 14.7 / 16.9; 8192 rows of 1024, bf16,
-// 20.7 / 36.8, in three launches 29.7 / 34.7.
+// pack / one pack: 4096 rows of 64 columns, float, 11.5 / 18.9 us, in three launches 15.6 / 17.9; 8192 rows of 1024, bf16,
+// 22.5 / 44.8, in three launches 33.5 / 39.9.
 template <typename T, int V, bool GRAD>
 __global__ void __launch_bounds__(256) recur_segment_kernel(Recur r, const T *__restrict__ a, const T *__restrict__ x,
                                                           const T *__restrict__ init,
@@ -293,64 +288,62 @@ __global__ void __launch_bounds__(256) recur_segment_kernel(Recur r, const T *__
                                                           int32_t *__restrict__ before,
                                                           Composed<typename StateOf<T>::S> segments) {
   using S = typename StateOf<T>::S;
-  struct Gains {
-    Gain<S> v[V];
-  };
-  __shared__ Gains s_a[256];
-  __shared__ Pack<S, V> s_b[256];
-  __shared__ int s_reset[256];
+  __shared__ S s_m[V][256], s_b[V][256];  // a column's, side by side: no bank conflicts
+  __shared__ int s_e[V][256], s_reset[256];
   const int me = threadIdx.x, w = 1 << r.wide;
   const int64_t c = (int64_t)blockIdx.y * (256 >> r.wide) + (me >> r.wide);
   const int64_t piece = (int64_t)blockIdx.x * w + (me & (w - 1)), col = r.column<V>(piece);
   const bool live = c < r.chunks && piece < r.cols;
-  Gains ga;
+  Gain<S> ga[V];
   Pack<S, V> gb;
 #pragma unroll
   for (int v = 0; v < V; v++) {
-    ga.v[v] = {1, 0};
+    ga[v] = {1, 0};
     gb.v[v] = 0;
   }
   int reset = 0;
   if (live) {
     const int64_t begin = c * r.chunk, end = min((int64_t)r.n, begin + r.chunk);
-    reset = recur_compose<T, V, GRAD>(r, a, x, init, begin, end, col, ga.v, gb.v);
+    reset = recur_compose<T, V, GRAD>(r, a, x, init, begin, end, col, ga, gb.v);
   }
+  auto publish = [&]() {
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+      s_m[v][me] = ga[v].m;
+      s_e[v][me] = ga[v].e;
+      s_b[v][me] = gb.v[v];
+    }
+    s_reset[me] = reset;
+    __syncthreads();
+  };
   // inclusive over the chunks in doubling steps; nothing to do where every chunk has a reset
   if (__syncthreads_or(live && !reset)) {
     for (int off = w; off < 256; off *= 2) {
-      s_a[me] = ga;
-      s_b[me] = gb;
-      s_reset[me] = reset;
-      __syncthreads();
+      publish();
       if (me >= off && !reset) {
-        const Gains pa = s_a[me - off];
-        const Pack<S, V> pb = s_b[me - off];
         reset = s_reset[me - off];
 #pragma unroll
         for (int v = 0; v < V; v++) {
-          gb.v[v] = ga.v[v].of(pb.v[v], gb.v[v]);
-          ga.v[v] = reset ? Gain<S>{0, 0} : ga.v[v].after(pa.v[v]);
+          gb.v[v] = ga[v].of(s_b[v][me - off], gb.v[v]);
+          ga[v] = reset ? Gain<S>{0, 0} : ga[v].after({s_m[v][me - off], s_e[v][me - off]});
         }
       }
       __syncthreads();
     }
   }
-  s_a[me] = ga;
-  s_b[me] = gb;
-  s_reset[me] = reset;
-  __syncthreads();
+  publish();
   if (piece < r.cols && me >= 256 - w) {
-    store_gains<V>(segments, (int64_t)blockIdx.y * r.dim + col, ga.v);
+    store_gains<V>(segments, (int64_t)blockIdx.y * r.dim + col, ga);
     store_pack<V>(segments.b + (int64_t)blockIdx.y * r.dim + col, gb);
     if (piece == 0) segments.resets[blockIdx.y] = reset;
   }
   if (!live) return;
 #pragma unroll
   for (int v = 0; v < V; v++) {
-    ga.v[v] = me >= w ? s_a[me - w].v[v] : Gain<S>{1, 0};
-    gb.v[v] = me >= w ? s_b[me - w].v[v] : (S)0;
+    ga[v] = me >= w ? Gain<S>{s_m[v][me - w], s_e[v][me - w]} : Gain<S>{1, 0};
+    gb.v[v] = me >= w ? s_b[v][me - w] : (S)0;
   }
-  store_gains<V>(chunks, c * r.dim + col, ga.v);
+  store_gains<V>(chunks, c * r.dim + col, ga);
   store_pack<V>(chunks.b + c * r.dim + col, gb);
   if (piece == 0) before[c] = me >= w ? s_reset[me - w] : 0;
 }
@@ -461,7 +454,7 @@ __global__ void __launch_bounds__(256) recur_write_kernel(Recur r, const T *__re
   if (carried) {
     auto step = [&](const ComposedIn<S> &m, int64_t k, bool reset) {
       const Pack<S, V> ka = load_pack<V>(m.a + k * r.dim + col), kb = load_pack<V>(m.b + k * r.dim + col);
-      const Pack<int16_t, V> ke = load_pack<V>(m.e + k * r.dim + col);
+      const Pack<int32_t, V> ke = load_pack<V>(m.e + k * r.dim + col);
 #pragma unroll
       for (int v = 0; v < V; v++) {
         const S with = Gain<S>{ka.v[v], ke.v[v]}.of(state[v], kb.v[v]);
@@ -478,7 +471,7 @@ __global__ void __launch_bounds__(256) recur_write_kernel(Recur r, const T *__re
         constexpr int kFold = V >= 4 ? 4 : 8;  // loads in flight together
         for (; k < mine; k += kFold) {
           Pack<S, V> ka[kFold], kb[kFold];
-          Pack<int16_t, V> ke[kFold];
+          Pack<int32_t, V> ke[kFold];
 #pragma unroll
           for (int u = 0; u < kFold; u++) {
             const int64_t at = min(k + u, mine - 1) * r.dim + col;
@@ -507,10 +500,10 @@ __global__ void __launch_bounds__(256) recur_write_kernel(Recur r, const T *__re
 }
 
 // All three steps in one launch, for up to kShortRows rows (one step of a batch of sequences): a workgroup takes one
-// piece of columns, each thread a row of it.  256 rows of 1024 columns, bf16, with the pack arrays: 7.1 us if every row
-// is a pack and 12.6 us if one pack has them all, 11.5 and 16.1 in two launches.  Rows of one piece lie in different
+// piece of columns, each thread a row of it.  256 rows of 1024 columns, bf16, with the pack arrays: 7.0 us if every row
+// is a pack and 13.8 us if one pack has them all, 11.3 and 17.3 in two launches.  Rows of one piece lie in different
 // lines of memory: with four rows a thread 1024 rows took 19 and 32 us, in two launches 12 and 17, and 256 rows of 512
-// pieces (2048 columns, float) 12 and 19 us, in two launches 11 and 14 (64 rows of them 6.5 and 9 us, 10 and 13).
+// pieces (2048 columns, float) 12 and 19 us, in two launches 11 and 15 (64 rows of them 6.4 and 9.4 us, 10 and 13).
 constexpr int kShortRows = 256, kShortPieces = 1 << 16;  // pieces: of all rows
 template <typename T, int V, bool GRAD>
 __global__ void __launch_bounds__(kShortRows) recur_short_kernel(Recur r, const T *__restrict__ a, const T *__restrict__ x,
@@ -620,8 +613,8 @@ struct RecurSpace {
     chunks.b = (S *)take(num_chunks * dim * sizeof(S));
     segments.a = (S *)take(num * dim * sizeof(S));
     segments.b = (S *)take(num * dim * sizeof(S));
-    chunks.e = (int16_t *)take(num_chunks * dim * 2);
-    segments.e = (int16_t *)take(num * dim * 2);
+    chunks.e = (int32_t *)take(num_chunks * dim * 4);
+    segments.e = (int32_t *)take(num * dim * 4);
     chunks.resets = (int32_t *)take(num_chunks * 4);
     before = (int32_t *)take(num_chunks * 4);
     segments.resets = (int32_t *)take(num * 4);

@@ -216,3 +216,23 @@ def test_norm_of_heads_far_from_one(spc, dtype, size, eps, heads, kv, dim, turn,
         outs, tols = norm_rotary(x[m], w[m], f, torch.arange(n), eps, interleaved, grad=g[m], dtype=dtype)
         for name, got, want, tol in zip(('y', 'dx', 'dw'), (y[i], grads[i], grads[2 + i]), outs, tols):
             check(f'{name} of {m}', got, want, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('rows,at', [(26200, 2000), (26200, 8000), (3000, 2000)])  # chunks of 20 rows and a scan, of 8
+@pytest.mark.parametrize('reverse', [False, True])
+def test_recurrence_states_that_left_the_range(spc, rows, at, reverse):
+    """20 gates of 2^-1000 take a state to 0, and 16 of 2^1000 do not bring it back; 20 of 2^1000 take it to infinity, and
+    16 of 2^-1000 do not bring it back either; a state of 0 stays 0."""
+    h0 = torch.tensor([2.0 ** 500, -2.0 ** 500, 0.0], dtype=torch.float64)[None].repeat(1, 67)[:, :200]
+    for first, then, left in ((-1000, 1000, 0.0), (1000, -1000, math.inf)):
+        a = torch.ones(rows, 200, dtype=torch.float64)
+        a[at:at + 20], a[at + 20:at + 36] = 2.0 ** first, 2.0 ** then
+        x = torch.zeros_like(a)
+        if reverse:
+            a = a.flip(0).contiguous()
+        h = spc.linear_recurrence(a.to(DEV), x.to(DEV), marks([rows]).to(DEV), initial=h0.to(DEV), reverse=reverse).cpu()
+        h = h.flip(0) if reverse else h
+        assert torch.equal(h[:at], h0.expand(at, 200))
+        want = torch.where(h0 == 0, 0.0, torch.where(h0 < 0, -left, left))
+        assert torch.equal(h[at + 19:], want.expand(rows - at - 19, 200))
