@@ -6,8 +6,9 @@
 // bits.  Scores are computed transposed, S^T = K Q^T, so a lane holds one row's scores: the softmax is lane-local but
 // for one exchange with the other half, and the weights are the second product's operand (O^T = V^T P^T) where
 // they lie, without a trip through LDS (seqcommon.h, acc_frag).
-// Bound by issue where rows are many: 16,385 rows in 6 packs, causal, 32 / 8 heads of 128, bf16: 515 us, 837 TFLOP/s,
-// with the matrix units busy in 41 % of the cycles, the vector units in 43 % and LDS in 31 %, without bank conflicts.
+// Bound by issue where rows are many: 16,385 rows in 6 packs, causal, 32 / 8 heads of 128, bf16: 526 us a call among others,
+// 819 TFLOP/s (565 to 614 us a kernel under a profiler, which lets each end before the next), with the matrix units busy
+// in 41 % of the cycles, the vector units in 43 % and LDS in 31 %, without bank conflicts.
 // Bound by memory where they are few: one row for each of 96 sequences (205,153 keys of 8 heads of 128, f16, 842 MB):
 // 175 us, 4.8 TB/s, and 5 us for the join.
 // low (training, 16-bit types): what the rounding of o left out, so that the backward's sums over do . o,

@@ -8,9 +8,9 @@
 // memory took the L1 cache one line for each lane).
 //
 // Bound by the matrix units and waits for them, 45 to 49 % busy: tiles of 32 rows meet 1.8 times the keys that their
-// rows see.  311,094 rows in 8192 packs of 38 on average, 4 heads of 32: forward 262 us, dq with the sums of do . o 370,
-// dk and dv 470, where the bytes alone take 379 us.  Three waves a SIMD: with two, 303, 347 (without the sums) and 549;
-// with four, whose registers spill, 315, 402 and 797.
+// rows see.  311,094 rows in 8192 packs of 38 on average, 4 heads of 32: forward 258 us, dq with the sums of do . o 341,
+// dk and dv 428 (kernels under a profiler), where the bytes alone take 379 us.  Three waves a SIMD: with two, 303, 347
+// (without the sums) and 549; with four, whose registers spill, 315, 402 and 797, where three took 260, 346 and 496.
 //
 // Rows past the end are copies of the last one: their scores are masked.  Rows with infinities or NaN: as in
 // attend.hip; the careful walk finds a tile's bad rows in its registers, zeroes them and adds them one by one.

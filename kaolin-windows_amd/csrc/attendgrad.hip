@@ -11,8 +11,9 @@
 // in 32 bits.  float16 has few exponents: there ds, and p for dv, are multiplied by a power of two of their column
 // (fit_column), and the result by its inverse, both exact.
 // Masked places that hold infinities or NaN: as in attend.hip.
-// Bound by issue and by the longest rows: 8191 rows in 4 packs, causal, 16 / 4 heads of 64, bf16: dq 178 us, dk and dv
-// in four splits of the rows 265 and 14 for their join, with the matrix units busy in 35 to 40 % of the cycles.
+// Bound by issue and by the longest rows: 8191 rows in 4 packs, causal, 16 / 4 heads of 64, bf16: dq 165 us, dk and dv
+// in four splits of the rows 243 and 14 for their join (f16: 188, 273 and 14), with the matrix units busy in 35 to 40 % of
+// the cycles.
 #include "attend32.h"
 
 namespace kl {

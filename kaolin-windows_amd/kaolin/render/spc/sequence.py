@@ -46,7 +46,8 @@ def pack_attention(q, k, v, boundaries, q_boundaries=None, causal=False, scale=N
         k, v (Tensor): (num_k, kv_heads, dim) of the same type.  ``heads`` is a multiple of ``kv_heads``:
             query head ``h`` reads key head ``h // (heads // kv_heads)``.
         boundaries (Tensor): (num_k,) bool, True at the first row of each pack of ``k`` and ``v``
-            (:func:`mark_pack_boundaries`).
+            (:func:`mark_pack_boundaries`).  Packs lie one behind the other: of a cache with spare rows, gather those
+            that count first.
         q_boundaries (Tensor): (num_q,) bool, the packs of ``q``; pack p of ``q`` attends to pack p of ``k``.
             Default: ``boundaries`` (rows attend to rows of their own pack).  With one row per pack, all
             True: one query reads out each pack, or the newest row of each attends to those before it.
